@@ -386,6 +386,121 @@ int32_t mx_sgd_momentum_clip(void* handle, float* params, const float* grads, fl
                              float max_grad_norm, const float* norm_sq, void* stream);
 
 /* ---------------------------------------------------------------------- */
+/* A pre-norm gated feed-forward block: layer norm, the gated linear layer, */
+/* AdamW                                                                     */
+/* ---------------------------------------------------------------------- */
+/* New; the reference's layers are Linear and ReLU, its optimizer on this path
+ * momentum SGD.  These take float32 (MX_F32) or bfloat16 (MX_BF16) tensors of
+ * the caller, allocate nothing, and keep nothing between calls but what the
+ * caller owns: calls on different streams may overlap when their outputs and
+ * scratch do.  Outputs must not overlap inputs unless said otherwise.  They
+ * are not part of the NpArray mode (the reference has no CPU path to match);
+ * on such a context the gated layer's float32 products run in NpArray order. */
+#define MX_F32 0
+#define MX_BF16 1
+
+/* y = (x - mean) * rstd * weight + bias over the last dimension, with
+ * mean = sum(x) / cols and rstd = 1 / sqrt(sum((x - mean)^2) / cols + eps).
+ * x, y: dtype, rows of ldx / ldy elements; weight, bias: float32[cols] or NULL
+ * (1 and 0).  mean, rstd: float32[rows] for the backward pass, or NULL. */
+int32_t mx_layer_norm_fwd(void* handle, int32_t dtype, const void* x, int64_t ldx,
+                          const float* weight, const float* bias, void* y, int64_t ldy,
+                          float* mean, float* rstd, int32_t rows, int32_t cols, float eps,
+                          void* stream);
+
+/* The gradients of mx_layer_norm_fwd: dx (dtype, rows of lddx), dweight and
+ * dbias (float32[cols], sums over the rows in a fixed order).  Any of the
+ * three may be NULL.  scratch: mx_layer_norm_bwd_scratch_bytes(handle, rows,
+ * cols) bytes, 16-byte aligned, when dweight or dbias is wanted. */
+int32_t mx_layer_norm_bwd(void* handle, int32_t dtype, const void* dy, int64_t lddy,
+                          const void* x, int64_t ldx, const float* weight, const float* mean,
+                          const float* rstd, void* dx, int64_t lddx, float* dweight,
+                          float* dbias, int32_t rows, int32_t cols, void* scratch,
+                          uint64_t scratch_bytes, void* stream);
+uint64_t mx_layer_norm_bwd_scratch_bytes(void* handle, int32_t rows, int32_t cols);
+
+/* Activations of the gated layer: z * sigmoid(z), z * Phi(z) (erf), its tanh
+ * form, max(z, 0) (a NaN gives 0, as in this library's ReLU), sigmoid(z). */
+#define MX_ACT_SILU 0
+#define MX_ACT_GELU 1
+#define MX_ACT_GELU_TANH 2
+#define MX_ACT_RELU 3
+#define MX_ACT_SIGMOID 4
+
+/* The gated linear layer: with [g | u] = x[M,K] op(w) + bias[2F],
+ * h[M,F] = act(g) * u.  transpose_w = 0: w stored [K,2F]; 1: [2F,K]; the
+ * gate's F columns (rows) come first, then the other projection's.  x, w,
+ * bias, h: dtype, packed.  bias may be NULL.  pre (may be NULL) receives
+ * [g | u] as float32[M,2F] for the backward pass: kept in 32 bits so that the
+ * gradients are rounded once.  float32 products are float32-class (relative
+ * error below 1e-6 of the terms' size), on tensor cores where the shape is
+ * large; MX_PREC_FP32 on the context or here keeps them on the exact SIMT
+ * kernels.  An infinite x or w gives NaN where it meets a float32 tensor-core
+ * product.  workspace: mx_gated_linear_workspace_bytes(...) bytes, 256-byte
+ * aligned, not shared with an overlapping call. */
+int32_t mx_gated_linear_fwd(void* handle, int32_t dtype, const void* x, const void* w,
+                            const void* bias, void* h, float* pre, int32_t M, int32_t K,
+                            int32_t F, int32_t transpose_w, int32_t act, int32_t precision,
+                            void* workspace, uint64_t workspace_bytes, void* stream);
+
+/* The gradients of mx_gated_linear_fwd from dh[M,F] and the saved pre:
+ * dpre = [dh * u * act'(g) | dh * act(g)], dx = dpre op(w)^T, dw = the
+ * gradient of w in w's layout, dbias = the sums of dpre over the rows.  Any of
+ * the three may be NULL.  For bfloat16 tensors dpre is rounded to bfloat16
+ * once before the two products (dbias is summed before that). */
+int32_t mx_gated_linear_bwd(void* handle, int32_t dtype, const void* dh, const float* pre,
+                            const void* x, const void* w, void* dx, void* dw, void* dbias,
+                            int32_t M, int32_t K, int32_t F, int32_t transpose_w, int32_t act,
+                            int32_t precision, void* workspace, uint64_t workspace_bytes,
+                            void* stream);
+/* Workspace of the forward (backward = 0) or backward (1) call of a shape. */
+uint64_t mx_gated_linear_workspace_bytes(void* handle, int32_t dtype, int32_t M, int32_t K,
+                                         int32_t F, int32_t transpose_w, int32_t precision,
+                                         int32_t backward);
+
+/* One tensor of mx_adamw_step.  param: float32, updated in place; grad:
+ * float32 or bfloat16 (grad_type); m, v: the moments, float32[n], or with
+ * 8-bit states int8[n] and uint8[n] with one float32 scale for each 256
+ * values in m_scale and v_scale (ceil(n / 256) floats each; zeros are a fresh
+ * state).  copy_bf16 (may be NULL) receives the new values as bfloat16. */
+typedef struct mx_adamw_tensor {
+  float* param;
+  const void* grad;
+  void* m;
+  void* v;
+  float* m_scale;
+  float* v_scale;
+  void* copy_bf16;
+  int64_t n;
+  double weight_decay;
+  int32_t grad_type;
+} mx_adamw_tensor;
+
+/* One AdamW step over `count` tensors (host array) in one launch:
+ *   g' = clip * g,  m = beta1 m + (1 - beta1) g',  v = beta2 v + (1 - beta2) g'^2,
+ *   p = (1 - lr weight_decay) p
+ *       - lr / (1 - beta1^t) m / (sqrt(v) / sqrt(1 - beta2^t) + eps).
+ * state_bits: 32 or 8.  t = step (>= 1), or, with step_dev (device int32), the
+ * incremented *step_dev, so that a captured call counts its replays.
+ * max_grad_norm > 0 clips by the norm over all the tensors' gradients as
+ * mx_sgd_momentum_autoclip does (norm_out, device, may be NULL, receives it).
+ * 8-bit codes: c stands for sign(c) (c / 127)^2 scale (m) and
+ * sqrt(v) = (c / 255)^2 scale; the scale is the largest magnitude of its 256
+ * values, NaN if one of them is not finite.  The tensors must not overlap.
+ * scratch: mx_adamw_scratch_bytes(count, max_grad_norm > 0) bytes, 16-byte
+ * aligned (may be NULL without clipping and step_dev). */
+int32_t mx_adamw_step(void* handle, const mx_adamw_tensor* tensors, int32_t count,
+                      int32_t state_bits, double lr, double beta1, double beta2, double eps,
+                      int64_t step, int32_t* step_dev, double max_grad_norm, float* norm_out,
+                      void* scratch, uint64_t scratch_bytes, void* stream);
+uint64_t mx_adamw_scratch_bytes(int32_t count, int32_t clip);
+
+/* The moments that 8-bit codes stand for, as bfloat16[n]: m from int8 codes
+ * (second = 0), v from uint8 codes (second = 1). */
+int32_t mx_adamw_state_values(void* handle, const void* codes, const float* scale, int64_t n,
+                              int32_t second, void* out_bf16, void* stream);
+
+/* ---------------------------------------------------------------------- */
 /* Data-parallel collectives (NCCL over NVLink / NVSwitch)                  */
 /* ---------------------------------------------------------------------- */
 /* The reference has no collectives: its only host loop, run_gpu

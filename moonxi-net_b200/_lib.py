@@ -34,10 +34,17 @@ PREC_NPARRAY = 5
 PRECISIONS = {"default": PREC_DEFAULT, "auto": PREC_AUTO, "fp32": PREC_FP32,
               "3xtf32": PREC_3XTF32, "tf32": PREC_TF32, "nparray": PREC_NPARRAY}
 
+# element types and activations of the layer norm, gated layer and AdamW calls
+F32 = 0
+BF16 = 1
+ACTIVATIONS = {"silu": 0, "gelu": 1, "gelu_tanh": 2, "relu": 3, "sigmoid": 4}
+
 _vp = ctypes.c_void_p
 _i32 = ctypes.c_int32
 _i64 = ctypes.c_int64
 _f32 = ctypes.c_float
+_f64 = ctypes.c_double
+_u64 = ctypes.c_uint64
 
 
 
@@ -49,6 +56,13 @@ class SplitGemm(ctypes.Structure):
                 ("M", _i32), ("K", _i32), ("N", _i32), ("alpha", _f32), ("beta", _f32),
                 ("bias", _vp), ("relu", _i32), ("mask", _vp), ("ldm", _i64), ("flags", _i32),
                 ("colsum", _vp), ("colsum_scratch", _vp), ("colsum_scratch_bytes", ctypes.c_uint64)]
+
+
+class AdamWTensor(ctypes.Structure):
+    """mx_adamw_tensor: one tensor of mx_adamw_step (include/mx_matmul.h)."""
+    _fields_ = [("param", _vp), ("grad", _vp), ("m", _vp), ("v", _vp), ("m_scale", _vp),
+                ("v_scale", _vp), ("copy_bf16", _vp), ("n", _i64), ("weight_decay", _f64),
+                ("grad_type", _i32)]
 
 
 # name -> (restype, argtypes); mirrors include/mx_matmul.h
@@ -108,6 +122,20 @@ SIGNATURES = {
                                         _vp]),
     "mx_sum_squares": (_i32, [_vp, _vp, _i64, _vp, _i32, _vp]),
     "mx_sgd_momentum_clip": (_i32, [_vp, _vp, _vp, _vp, _i64, _f32, _f32, _f32, _f32, _vp, _vp]),
+    "mx_layer_norm_fwd": (_i32, [_vp, _i32, _vp, _i64, _vp, _vp, _vp, _i64, _vp, _vp, _i32, _i32,
+                                 _f32, _vp]),
+    "mx_layer_norm_bwd": (_i32, [_vp, _i32, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _vp,
+                                 _vp, _i32, _i32, _vp, _u64, _vp]),
+    "mx_layer_norm_bwd_scratch_bytes": (_u64, [_vp, _i32, _i32]),
+    "mx_gated_linear_fwd": (_i32, [_vp, _i32, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32,
+                                   _i32, _i32, _vp, _u64, _vp]),
+    "mx_gated_linear_bwd": (_i32, [_vp, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32,
+                                   _i32, _i32, _i32, _i32, _vp, _u64, _vp]),
+    "mx_gated_linear_workspace_bytes": (_u64, [_vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32]),
+    "mx_adamw_step": (_i32, [_vp, ctypes.POINTER(AdamWTensor), _i32, _i32, _f64, _f64, _f64,
+                             _f64, _i64, _vp, _f64, _vp, _vp, _u64, _vp]),
+    "mx_adamw_scratch_bytes": (_u64, [_i32, _i32]),
+    "mx_adamw_state_values": (_i32, [_vp, _vp, _vp, _i64, _i32, _vp, _vp]),
     "moonbit_nccl_version": (_i32, []),
     "moonbit_nccl_get_unique_id": (_i32, [_vp]),
     "moonbit_nccl_init": (_vp, [_vp, _i32, _i32, _i32]),

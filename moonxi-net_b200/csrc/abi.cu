@@ -783,3 +783,164 @@ MX_EXPORT int32_t mx_sgd_momentum_autoclip(void* handle, float* params, const fl
                                       max_grad_norm, norm_out, s),
                 s);
 }
+
+// ------------------------- layer norm, the gated linear layer, AdamW
+namespace {
+bool known_type(int32_t dtype) { return dtype == MX_F32 || dtype == MX_BF16; }
+}  // namespace
+
+MX_EXPORT int32_t mx_layer_norm_fwd(void* handle, int32_t dtype, const void* x, int64_t ldx,
+                                    const float* weight, const float* bias, void* y, int64_t ldy,
+                                    float* mean, float* rstd, int32_t rows, int32_t cols,
+                                    float eps, void* stream) {
+  Scoped scope(handle);
+  Context* c = scope.c;
+  if (!c) return MX_ERR_NO_DEVICE;
+  if (!known_type(dtype) || rows < 0 || cols < 1 || ldx < cols || ldy < cols || !(eps >= 0.0f))
+    return MX_ERR_INVALID;
+  if (rows > 0 && (!x || !y)) return MX_ERR_INVALID;
+  cudaStream_t s = pick_stream(c, stream);
+  return finish(c, layer_norm_fwd(c, dtype, x, ldx, weight, bias, y, ldy, mean, rstd, rows, cols,
+                                  eps, s), s);
+}
+
+MX_EXPORT int32_t mx_layer_norm_bwd(void* handle, int32_t dtype, const void* dy, int64_t lddy,
+                                    const void* x, int64_t ldx, const float* weight,
+                                    const float* mean, const float* rstd, void* dx, int64_t lddx,
+                                    float* dweight, float* dbias, int32_t rows, int32_t cols,
+                                    void* scratch, uint64_t scratch_bytes, void* stream) {
+  Scoped scope(handle);
+  Context* c = scope.c;
+  if (!c) return MX_ERR_NO_DEVICE;
+  if (!known_type(dtype) || rows < 0 || cols < 1 || ldx < cols || lddy < cols ||
+      (dx && lddx < cols))
+    return MX_ERR_INVALID;
+  if (rows > 0 && (!dy || !x || !mean || !rstd)) return MX_ERR_INVALID;
+  cudaStream_t s = pick_stream(c, stream);
+  return finish(c, layer_norm_bwd(c, dtype, dy, lddy, x, ldx, weight, mean, rstd, dx, lddx,
+                                  dweight, dbias, rows, cols, scratch, scratch_bytes, s), s);
+}
+
+MX_EXPORT uint64_t mx_layer_norm_bwd_scratch_bytes(void* handle, int32_t rows, int32_t cols) {
+  Scoped scope(handle);
+  return scope.c ? layer_norm_bwd_scratch_bytes(scope.c, rows, cols) : 0;
+}
+
+namespace {
+// The products' part of a gated call; kOk or MX_ERR_INVALID.
+int gated_args(Context* c, int32_t dtype, int32_t M, int32_t K, int32_t F, int32_t transpose_w,
+               int32_t act, int32_t precision, GatedArgs& a) {
+  a = GatedArgs{};
+  if (!known_type(dtype) || M < 0 || K < 0 || F < 0 || F > 0x3fffffff) return MX_ERR_INVALID;
+  if (act < MX_ACT_SILU || act > MX_ACT_SIGMOID) return MX_ERR_INVALID;
+  if (precision < MX_PREC_DEFAULT || precision > MX_PREC_NPARRAY) return MX_ERR_INVALID;
+  const int p = precision == MX_PREC_DEFAULT ? c->precision : precision;
+  a.dtype = dtype;
+  a.M = M; a.K = K; a.F = F;
+  a.tw = transpose_w ? 1 : 0;
+  a.act = act;
+  a.strict = p == MX_PREC_NPARRAY;
+  a.exact = p == MX_PREC_FP32 || a.strict;
+  return kOk;
+}
+}  // namespace
+
+MX_EXPORT int32_t mx_gated_linear_fwd(void* handle, int32_t dtype, const void* x, const void* w,
+                                      const void* bias, void* h, float* pre, int32_t M, int32_t K,
+                                      int32_t F, int32_t transpose_w, int32_t act,
+                                      int32_t precision, void* workspace,
+                                      uint64_t workspace_bytes, void* stream) {
+  Scoped scope(handle);
+  Context* c = scope.c;
+  if (!c) return MX_ERR_NO_DEVICE;
+  GatedArgs a;
+  const int rc = gated_args(c, dtype, M, K, F, transpose_w, act, precision, a);
+  if (rc != kOk) return rc;
+  if (M == 0 || F == 0) return MX_OK;
+  if (!h || (K > 0 && (!x || !w))) return MX_ERR_INVALID;
+  a.x = x; a.w = w; a.bias = bias; a.h = h; a.pre = pre;
+  a.ws = workspace; a.ws_bytes = workspace_bytes;
+  const size_t need = gated_workspace_bytes(c, a, false);
+  if (need > 0 && (!workspace || workspace_bytes < need)) return MX_ERR_INVALID;
+  cudaStream_t s = pick_stream(c, stream);
+  return finish(c, gated_fwd(c, a, s), s);
+}
+
+MX_EXPORT int32_t mx_gated_linear_bwd(void* handle, int32_t dtype, const void* dh,
+                                      const float* pre, const void* x, const void* w, void* dx,
+                                      void* dw, void* dbias, int32_t M, int32_t K, int32_t F,
+                                      int32_t transpose_w, int32_t act, int32_t precision,
+                                      void* workspace, uint64_t workspace_bytes, void* stream) {
+  Scoped scope(handle);
+  Context* c = scope.c;
+  if (!c) return MX_ERR_NO_DEVICE;
+  GatedArgs a;
+  const int rc = gated_args(c, dtype, M, K, F, transpose_w, act, precision, a);
+  if (rc != kOk) return rc;
+  cudaStream_t s = pick_stream(c, stream);
+  const size_t b = dtype == MX_BF16 ? 2 : 4;
+  if (M == 0 || F == 0 || K == 0) {  // empty sums are zero
+    cudaError_t e = cudaSuccess;
+    if (dx && M > 0 && K > 0) e = cudaMemsetAsync(dx, 0, b * M * K, s);
+    if (e == cudaSuccess && dw && K > 0 && F > 0) e = cudaMemsetAsync(dw, 0, b * 2 * K * F, s);
+    if (e == cudaSuccess && dbias && F > 0 && M == 0) e = cudaMemsetAsync(dbias, 0, b * 2 * F, s);
+    if (e != cudaSuccess) return cuda_status(e);
+    if (M == 0 || F == 0 || !dbias) return MX_OK;
+    dx = dw = nullptr;  // K == 0: the bias alone has a gradient
+  }
+  if (!dh || !pre || (dx && !w) || (dw && !x)) return MX_ERR_INVALID;
+  a.x = x; a.w = w; a.dh = dh; a.pre = const_cast<float*>(pre);
+  a.dx = dx; a.dw = dw; a.dbias = dbias;
+  a.ws = workspace; a.ws_bytes = workspace_bytes;
+  const size_t need = gated_workspace_bytes(c, a, true);
+  if (need > 0 && (!workspace || workspace_bytes < need)) return MX_ERR_INVALID;
+  return finish(c, gated_bwd(c, a, s), s);
+}
+
+MX_EXPORT uint64_t mx_gated_linear_workspace_bytes(void* handle, int32_t dtype, int32_t M,
+                                                   int32_t K, int32_t F, int32_t transpose_w,
+                                                   int32_t precision, int32_t backward) {
+  Scoped scope(handle);
+  Context* c = scope.c;
+  GatedArgs a;
+  if (!c || gated_args(c, dtype, M, K, F, transpose_w, MX_ACT_SILU, precision, a) != kOk) return 0;
+  if (M == 0 || F == 0) return 0;
+  return gated_workspace_bytes(c, a, backward != 0);
+}
+
+MX_EXPORT int32_t mx_adamw_step(void* handle, const mx_adamw_tensor* tensors, int32_t count,
+                                int32_t state_bits, double lr, double beta1, double beta2,
+                                double eps, int64_t step, int32_t* step_dev,
+                                double max_grad_norm, float* norm_out, void* scratch,
+                                uint64_t scratch_bytes, void* stream) {
+  Scoped scope(handle);
+  Context* c = scope.c;
+  if (!c) return MX_ERR_NO_DEVICE;
+  if (count < 0 || (count > 0 && !tensors) || (state_bits != 32 && state_bits != 8))
+    return MX_ERR_INVALID;
+  if (!(beta1 >= 0.0 && beta1 < 1.0) || !(beta2 >= 0.0 && beta2 < 1.0) || !(eps >= 0.0))
+    return MX_ERR_INVALID;
+  if ((!step_dev && step < 1) || !(max_grad_norm >= 0.0)) return MX_ERR_INVALID;
+  const bool clip = max_grad_norm > 0.0;
+  if ((clip || step_dev) && (!scratch || scratch_bytes < adamw_scratch_bytes(count, clip)))
+    return MX_ERR_INVALID;
+  const int rc = adamw_check(tensors, count, state_bits);
+  if (rc != kOk) return rc;
+  cudaStream_t s = pick_stream(c, stream);
+  return finish(c, adamw_step(tensors, count, state_bits, lr, beta1, beta2, eps, step, step_dev,
+                              max_grad_norm, norm_out, scratch, s), s);
+}
+
+MX_EXPORT uint64_t mx_adamw_scratch_bytes(int32_t count, int32_t clip) {
+  return adamw_scratch_bytes(count, clip);
+}
+
+MX_EXPORT int32_t mx_adamw_state_values(void* handle, const void* codes, const float* scale,
+                                        int64_t n, int32_t second, void* out_bf16, void* stream) {
+  Scoped scope(handle);
+  Context* c = scope.c;
+  if (!c) return MX_ERR_NO_DEVICE;
+  if (n < 0 || (n > 0 && (!codes || !scale || !out_bf16))) return MX_ERR_INVALID;
+  cudaStream_t s = pick_stream(c, stream);
+  return finish(c, adamw_state_values(codes, scale, n, second == 0, out_bf16, s), s);
+}

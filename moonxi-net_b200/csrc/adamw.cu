@@ -1,0 +1,491 @@
+// adamw.cu -- one AdamW step over many tensors in one launch, its two moments
+// held in float32 or in 8 bits.
+//
+//   g' = clip * g                         clip = max_norm / ||g|| when above it
+//   m  = b1 m + (1 - b1) g',   v = b2 v + (1 - b2) g'^2
+//   p  = (1 - lr wd) p - (lr / (1 - b1^t)) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+//
+// 8-bit states: 256 consecutive values of a tensor share one float32, the
+// largest magnitude among them (top, at least 2^-120).  The first moment is
+// held as signed codes c for (c / 127)^2 top with c's sign, the second as
+// unsigned codes c for sqrt(v) = (c / 255)^2 top; the code is the nearest one
+// in the root.  The square gives values near the largest fine steps (0.8 % of
+// sqrt(v)) and still reaches 1.5e-5 of it; holding sqrt(v) halves the range of
+// exponents that v spans.  A sqrt(v) above zero keeps a code above zero (a
+// vanished v would blow the step up), and since `top` itself is not rounded,
+// moments that decay together decay exactly.  What is lost is a change of one
+// value against its block's largest by less than half a step.  The step itself
+// uses this step's float32 moments, before they are rounded.  A moment that is
+// not finite makes its block's scale, and so the whole block, NaN.
+//
+// Each multiply and add is rounded by itself (no fused multiply-add): the
+// step is then the same arithmetic as its elementwise form, and a code next to
+// the border between two of its neighbours falls on the same side.
+//
+// Bound by the bytes: 28 B a value with float32 gradients and states, 16 B
+// with 8-bit states (14 B with bf16 gradients).  A warp takes 256 values,
+// 8 a lane in 16-byte accesses, so an 8-bit block is one warp's and its
+// maximum five shuffles.
+#include <algorithm>
+#include <cmath>
+
+#include <cuda_bf16.h>
+
+#include "../../include/mx_matmul.h"
+#include "mx_internal.h"
+#include "mx_ptx.cuh"
+
+namespace mx {
+namespace {
+
+constexpr int kQBlock = 256;           // values of one scale, of one warp
+constexpr int kWarps = 8;
+constexpr int kChunk = kWarps * kQBlock;  // values of one block
+
+enum : uint32_t { kGradBf16 = 1, kVec = 2 };
+
+struct Tensor {
+  float* p;
+  const void* g;
+  void* m;
+  void* v;
+  float* ms;            // 8-bit states: the blocks' scales
+  float* vs;
+  __nv_bfloat16* copy;  // bf16 copy of the new values, or null
+  int64_t n;
+  float keep;           // 1 - lr * weight_decay
+  uint32_t flags;
+};
+
+// The tensors of one launch, by value: nothing to upload, and a captured
+// launch holds its own table.  first[i]: the first chunk of tensor i.
+template <int CAP>
+struct Table {
+  Tensor t[CAP];
+  int64_t first[CAP + 1];
+  int count;
+};
+
+struct Hyper {
+  float b1, omb1, b2, omb2, eps, step_size, inv_root;  // see adamw_one
+  const float* scalars;   // device: {step_size, inv_root} instead, or null
+  const float* norm;      // device: the gradients' norm, or null (no clipping)
+  float max_norm;
+};
+
+template <int CAP>
+__device__ __forceinline__ int find_tensor(const Table<CAP>& tb, int64_t chunk) {
+  int lo = 0, hi = tb.count - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (tb.first[mid] <= chunk) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
+// The new m, v and p of one value; returns sqrt(v).
+__device__ __forceinline__ float adamw_one(float& p, float g, float& m, float& v, float keep,
+                                           const Hyper& h) {
+  m = __fadd_rn(__fmul_rn(m, h.b1), __fmul_rn(g, h.omb1));
+  v = __fadd_rn(__fmul_rn(v, h.b2), __fmul_rn(__fmul_rn(g, g), h.omb2));
+  const float root = __fsqrt_rn(v);
+  const float denom = __fadd_rn(__fmul_rn(root, h.inv_root), h.eps);
+  p = __fsub_rn(__fmul_rn(p, keep), __fdiv_rn(__fmul_rn(m, h.step_size), denom));
+  return root;
+}
+
+// 8 values of a lane, those past `left` not touched.
+__device__ __forceinline__ void load8(const float* p, bool vec, int left, float (&x)[8]) {
+  if (vec && left >= 8) {
+    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = i < left ? p[i] : 0.0f;
+  }
+}
+__device__ __forceinline__ void store8(float* p, bool vec, int left, const float (&x)[8]) {
+  if (vec && left >= 8) {
+    *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+    *reinterpret_cast<float4*>(p + 4) = make_float4(x[4], x[5], x[6], x[7]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < left) p[i] = x[i];
+  }
+}
+__device__ __forceinline__ void load8(const __nv_bfloat16* p, bool vec, int left, float (&x)[8]) {
+  if (vec && left >= 8) {
+    const uint4 r = *reinterpret_cast<const uint4*>(p);
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[2 * i] = __uint_as_float(w[i] << 16);
+      x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = i < left ? __bfloat162float(p[i]) : 0.0f;
+  }
+}
+__device__ __forceinline__ void store8(__nv_bfloat16* p, bool vec, int left, const float (&x)[8]) {
+  if (vec && left >= 8) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < left) p[i] = __float2bfloat16_rn(x[i]);
+  }
+}
+
+// What 8 codes of a block with the largest magnitude `top` stand for.
+template <bool SIGNED>
+__device__ __forceinline__ void decode8(const uint8_t* q, float top, bool vec, int left,
+                                        float (&x)[8]) {
+  uint32_t w[2] = {0, 0};
+  if (vec && left >= 8) {
+    const uint2 r = *reinterpret_cast<const uint2*>(q);
+    w[0] = r.x;
+    w[1] = r.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < left) w[i >> 2] |= static_cast<uint32_t>(q[i]) << (8 * (i & 3));
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t byte = (w[i >> 2] >> (8 * (i & 3))) & 255u;
+    const float c = SIGNED ? static_cast<float>(static_cast<int8_t>(byte)) : static_cast<float>(byte);
+    const float r = __fmul_rn(c, SIGNED ? 1.0f / 127.0f : 1.0f / 255.0f);
+    x[i] = __fmul_rn(__fmul_rn(r, fabsf(r)), top);
+  }
+}
+// The warp's largest magnitude, at least 2^-120; NaN if a value is not finite.
+__device__ __forceinline__ float block_top(const float (&x)[8]) {
+  float top = 7.52316384526264e-37f;  // 2^-120
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float a = fabsf(x[i]);
+    bad |= !(a <= 3.4028234663852886e38f);
+    top = fmaxf(top, a);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  return __any_sync(0xffffffffu, bad) ? __int_as_float(0x7fc00000) : top;
+}
+template <bool SIGNED>
+__device__ __forceinline__ void encode8(uint8_t* q, float top, bool vec, int left,
+                                        const float (&x)[8]) {
+  const float inv = __fdiv_rn(1.0f, top);
+  uint32_t w[2] = {0, 0};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float r = __fsqrt_rn(__fmul_rn(fabsf(x[i]), inv));
+    int c = __float2int_rn(__fmul_rn(r, SIGNED ? 127.0f : 255.0f));  // NaN: 0, in a NaN block
+    if (SIGNED) c = x[i] < 0.0f ? -c : c;
+    else c = x[i] > 0.0f ? max(c, 1) : c;
+    w[i >> 2] |= (static_cast<uint32_t>(c) & 255u) << (8 * (i & 3));
+  }
+  if (vec && left >= 8) {
+    *reinterpret_cast<uint2*>(q) = make_uint2(w[0], w[1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < left) q[i] = static_cast<uint8_t>(w[i >> 2] >> (8 * (i & 3)));
+  }
+}
+
+template <int CAP, bool Q8>
+__global__ void __launch_bounds__(32 * kWarps) adamw_kernel(const __grid_constant__ Table<CAP> tb,
+                                                            const Hyper hy) {
+  const int ti = find_tensor(tb, blockIdx.x);
+  const Tensor& t = tb.t[ti];
+  const int lane = threadIdx.x & 31;
+  const int64_t block = (blockIdx.x - tb.first[ti]) * kWarps + (threadIdx.x >> 5);
+  const int64_t at = block * kQBlock + lane * 8;
+  if (block * kQBlock >= t.n) return;  // the whole warp
+  Hyper h = hy;
+  if (h.scalars) {
+    h.step_size = h.scalars[0];
+    h.inv_root = h.scalars[1];
+  }
+  float clip = 1.0f;
+  if (h.norm) {
+    const float nv = *h.norm;
+    if (nv > h.max_norm) clip = __fdiv_rn(h.max_norm, nv);
+  }
+  const int64_t rest = t.n - at;
+  const int left = rest >= 8 ? 8 : rest > 0 ? static_cast<int>(rest) : 0;
+  const bool vec = t.flags & kVec;
+  float p[8], g[8], m[8], v[8];
+  load8(t.p + at, vec, left, p);
+  if (t.flags & kGradBf16) load8(static_cast<const __nv_bfloat16*>(t.g) + at, vec, left, g);
+  else load8(static_cast<const float*>(t.g) + at, vec, left, g);
+  if (Q8) {
+    decode8<true>(static_cast<const uint8_t*>(t.m) + at, t.ms[block], vec, left, m);
+    decode8<false>(static_cast<const uint8_t*>(t.v) + at, t.vs[block], vec, left, v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = __fmul_rn(v[i], v[i]);
+  } else {
+    load8(static_cast<const float*>(t.m) + at, vec, left, m);
+    load8(static_cast<const float*>(t.v) + at, vec, left, v);
+  }
+  float root[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if (h.norm) g[i] = __fmul_rn(g[i], clip);
+    root[i] = adamw_one(p[i], g[i], m[i], v[i], t.keep, h);
+  }
+  store8(t.p + at, vec, left, p);
+  if (t.copy) store8(t.copy + at, vec, left, p);
+  if (Q8) {
+    const float sm = block_top(m), sv = block_top(root);
+    encode8<true>(static_cast<uint8_t*>(t.m) + at, sm, vec, left, m);
+    encode8<false>(static_cast<uint8_t*>(t.v) + at, sv, vec, left, root);
+    __syncwarp();  // every lane has read the old scales
+    if (lane == 0) {
+      t.ms[block] = sm;
+      t.vs[block] = sv;
+    }
+  } else {
+    store8(static_cast<float*>(t.m) + at, vec, left, m);
+    store8(static_cast<float*>(t.v) + at, vec, left, v);
+  }
+}
+
+// The values that 8-bit codes stand for, rounded to bf16: the first moment, or
+// (SIGNED false) the second.
+template <bool SIGNED>
+__global__ void __launch_bounds__(32 * kWarps) adamw_values_kernel(const uint8_t* q,
+                                                                   const float* scale, int64_t n,
+                                                                   __nv_bfloat16* out, bool vec) {
+  const int64_t block = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
+  const int64_t at = block * kQBlock + (threadIdx.x & 31) * 8;
+  if (at >= n) return;
+  const int left = n - at >= 8 ? 8 : static_cast<int>(n - at);
+  float x[8];
+  decode8<SIGNED>(q + at, scale[block], vec, left, x);
+  if (!SIGNED)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = __fmul_rn(x[i], x[i]);
+  store8(out + at, vec, left, x);
+}
+
+// Sum of squares of the gradients of one launch's tensors: block b's sum of
+// its chunks goes to part[b]; the order is fixed.
+template <int CAP>
+__global__ void __launch_bounds__(32 * kWarps) grad_norm_kernel(const __grid_constant__ Table<CAP> tb,
+                                                                float* part) {
+  __shared__ float sh[kWarps];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  float s = 0.0f;
+  for (int64_t c = blockIdx.x; c < tb.first[tb.count]; c += gridDim.x) {
+    const int ti = find_tensor(tb, c);
+    const Tensor& t = tb.t[ti];
+    const int64_t at = (c - tb.first[ti]) * kChunk + threadIdx.x * 8;
+    const int64_t rest = t.n - at;
+    const int left = rest >= 8 ? 8 : rest > 0 ? static_cast<int>(rest) : 0;
+    float g[8];
+    if (t.flags & kGradBf16)
+      load8(static_cast<const __nv_bfloat16*>(t.g) + at, t.flags & kVec, left, g);
+    else
+      load8(static_cast<const float*>(t.g) + at, t.flags & kVec, left, g);
+    float q = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) q += g[i] * g[i];
+    s += q;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if (lane == 0) sh[warp] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < kWarps; ++i) s += sh[i];
+    part[blockIdx.x] = s;
+  }
+}
+
+// One block: the norm of `n` partial sums of squares, and the step's scalars
+// from a step number on the device.  Either may be off.
+__global__ void __launch_bounds__(256) adamw_prelude_kernel(const float* part, int n, float* norm,
+                                                            float* norm_out, int32_t* step,
+                                                            float* scalars, double lr, double b1,
+                                                            double b2) {
+  __shared__ float sh[256];
+  if (norm) {
+    float s = 0.0f;
+    for (int i = threadIdx.x; i < n; i += 256) s += part[i];
+    sh[threadIdx.x] = s;
+    __syncthreads();
+    for (int o = 128; o > 0; o >>= 1) {
+      if (threadIdx.x < o) sh[threadIdx.x] += sh[threadIdx.x + o];
+      __syncthreads();
+    }
+    if (threadIdx.x == 0) {
+      *norm = sqrtf(sh[0]);
+      if (norm_out) *norm_out = *norm;
+    }
+  }
+  if (scalars && threadIdx.x == 32) {
+    const int32_t t = *step + 1;
+    *step = t;
+    scalars[0] = static_cast<float>(lr / (1.0 - pow(b1, static_cast<double>(t))));
+    scalars[1] = static_cast<float>(1.0 / sqrt(1.0 - pow(b2, static_cast<double>(t))));
+  }
+}
+
+constexpr int kNormBlocks = 592;  // partial sums of a launch: four blocks an SM
+
+int64_t chunks_of(int64_t n) { return (n + kChunk - 1) / kChunk; }
+
+bool aligned(const void* a, unsigned to) { return (reinterpret_cast<uintptr_t>(a) & (to - 1)) == 0; }
+
+template <int CAP>
+void fill(Table<CAP>& tb, const mx_adamw_tensor* ts, int count, int bits, double lr) {
+  tb.count = 0;
+  int64_t at = 0;
+  for (int i = 0; i < count; ++i) {
+    const mx_adamw_tensor& a = ts[i];
+    if (a.n == 0) continue;
+    Tensor& t = tb.t[tb.count];
+    t.p = a.param;
+    t.g = a.grad;
+    t.m = a.m;
+    t.v = a.v;
+    t.ms = a.m_scale;
+    t.vs = a.v_scale;
+    t.copy = static_cast<__nv_bfloat16*>(a.copy_bf16);
+    t.n = a.n;
+    t.keep = static_cast<float>(1.0 - lr * a.weight_decay);
+    const unsigned sa = bits == 8 ? 8 : 16;
+    t.flags = (a.grad_type == MX_BF16 ? kGradBf16 : 0u) |
+              (aligned(a.param, 16) && aligned(a.grad, 16) && aligned(a.m, sa) &&
+                       aligned(a.v, sa) && aligned(a.copy_bf16, 16)
+                   ? kVec : 0u);
+    tb.first[tb.count++] = at;
+    at += chunks_of(a.n);
+  }
+  tb.first[tb.count] = at;
+}
+
+template <int CAP>
+cudaError_t launch_norm(const mx_adamw_tensor* ts, int count, int bits, float* part, int* blocks,
+                        cudaStream_t s) {
+  Table<CAP> tb;
+  fill(tb, ts, count, bits, 0.0);
+  *blocks = static_cast<int>(std::min<int64_t>(tb.first[tb.count], kNormBlocks));
+  if (*blocks == 0) return cudaSuccess;
+  grad_norm_kernel<CAP><<<*blocks, 32 * kWarps, 0, s>>>(tb, part);
+  note_launches(1);
+  return cudaGetLastError();
+}
+
+template <int CAP>
+cudaError_t launch_step(const mx_adamw_tensor* ts, int count, int bits, double lr, const Hyper& h,
+                        cudaStream_t s) {
+  Table<CAP> tb;
+  fill(tb, ts, count, bits, lr);
+  const int64_t chunks = tb.first[tb.count];
+  if (chunks == 0) return cudaSuccess;
+  if (bits == 8)
+    adamw_kernel<CAP, true><<<static_cast<unsigned>(chunks), 32 * kWarps, 0, s>>>(tb, h);
+  else
+    adamw_kernel<CAP, false><<<static_cast<unsigned>(chunks), 32 * kWarps, 0, s>>>(tb, h);
+  note_launches(1);
+  return cudaGetLastError();
+}
+
+// Tensors of one launch.  A kernel's parameters hold up to 32 KB; the small
+// table keeps a call on a few tensors at a quarter of a page.
+constexpr int kSmallTable = 16, kLargeTable = 320;
+static_assert(sizeof(Table<kLargeTable>) + sizeof(Hyper) <= 32764, "kernel parameters");
+
+}  // namespace
+
+size_t adamw_scratch_bytes(int count, int clip) {
+  const int64_t launches = (std::max(count, 1) + kLargeTable - 1) / kLargeTable;
+  return (4 + (clip ? launches * kNormBlocks : 0)) * sizeof(float);
+}
+
+int adamw_check(const mx_adamw_tensor* ts, int count, int bits) {
+  int64_t chunks = 0;
+  for (int i = 0; i < count; ++i) {
+    const mx_adamw_tensor& a = ts[i];
+    if (a.n < 0 || (a.grad_type != MX_F32 && a.grad_type != MX_BF16)) return kErrInvalid;
+    if (a.n == 0) continue;
+    if (!a.param || !a.grad || !a.m || !a.v) return kErrInvalid;
+    if (bits == 8 && (!a.m_scale || !a.v_scale)) return kErrInvalid;
+    chunks = i % kLargeTable == 0 ? chunks_of(a.n) : chunks + chunks_of(a.n);
+    if (chunks > 0x7fffffff) return kErrUnsupported;  // blocks of one launch
+  }
+  return kOk;
+}
+
+int adamw_step(const mx_adamw_tensor* ts, int count, int bits, double lr, double b1, double b2,
+               double eps, int64_t step, int32_t* step_dev, double max_norm, float* norm_out,
+               void* scratch, cudaStream_t s) {
+  float* sc = static_cast<float*>(scratch);  // [0] norm, [1..2] scalars, [4..] partial sums
+  float* part = sc + 4;
+  const bool clip = max_norm > 0.0;
+  int parts = 0;
+  cudaError_t e = cudaSuccess;
+  if (clip)
+    for (int i = 0; i < count && e == cudaSuccess; i += kLargeTable) {
+      const int k = std::min(kLargeTable, count - i);
+      int blocks = 0;
+      e = k <= kSmallTable ? launch_norm<kSmallTable>(ts + i, k, bits, part + parts, &blocks, s)
+                           : launch_norm<kLargeTable>(ts + i, k, bits, part + parts, &blocks, s);
+      parts += blocks;
+    }
+  if (e == cudaSuccess && (clip || step_dev)) {
+    adamw_prelude_kernel<<<1, 256, 0, s>>>(part, parts, clip ? sc : nullptr, norm_out, step_dev,
+                                           step_dev ? sc + 1 : nullptr, lr, b1, b2);
+    note_launches(1);
+    e = cudaGetLastError();
+  }
+  Hyper h;
+  h.b1 = static_cast<float>(b1);
+  h.omb1 = static_cast<float>(1.0 - b1);
+  h.b2 = static_cast<float>(b2);
+  h.omb2 = static_cast<float>(1.0 - b2);
+  h.eps = static_cast<float>(eps);
+  const double t = static_cast<double>(step);
+  h.step_size = step_dev ? 0.0f : static_cast<float>(lr / (1.0 - std::pow(b1, t)));
+  h.inv_root = step_dev ? 0.0f : static_cast<float>(1.0 / std::sqrt(1.0 - std::pow(b2, t)));
+  h.scalars = step_dev ? sc + 1 : nullptr;
+  h.norm = clip ? sc : nullptr;
+  h.max_norm = static_cast<float>(max_norm);
+  for (int i = 0; i < count && e == cudaSuccess; i += kLargeTable) {
+    const int k = std::min(kLargeTable, count - i);
+    e = k <= kSmallTable ? launch_step<kSmallTable>(ts + i, k, bits, lr, h, s)
+                         : launch_step<kLargeTable>(ts + i, k, bits, lr, h, s);
+  }
+  return cuda_status(e);
+}
+
+int adamw_state_values(const void* q, const float* scale, int64_t n, int is_signed, void* out,
+                       cudaStream_t s) {
+  if (n <= 0) return kOk;
+  const int64_t blocks = chunks_of(n);
+  if (blocks > 0x7fffffff) return kErrUnsupported;
+  const bool vec = aligned(q, 8) && aligned(out, 16);
+  const uint8_t* c = static_cast<const uint8_t*>(q);
+  __nv_bfloat16* o = static_cast<__nv_bfloat16*>(out);
+  if (is_signed)
+    adamw_values_kernel<true><<<static_cast<unsigned>(blocks), 32 * kWarps, 0, s>>>(c, scale, n, o, vec);
+  else
+    adamw_values_kernel<false><<<static_cast<unsigned>(blocks), 32 * kWarps, 0, s>>>(c, scale, n, o, vec);
+  note_launches(1);
+  return cuda_status(cudaGetLastError());
+}
+
+}  // namespace mx

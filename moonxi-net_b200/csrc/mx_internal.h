@@ -8,6 +8,8 @@
 #include <cstddef>
 #include <cstdint>
 
+#include "../../include/mx_matmul.h"
+
 namespace mx {
 
 // Per-device execution context.  The reference passes an opaque handle to
@@ -204,6 +206,41 @@ int sum_squares(Context* ctx, const float* x, int64_t n, float* out, int accumul
 int sgd_momentum_clip(Context* ctx, float* p, const float* g, float* v, int64_t n, float lr,
                       float momentum, float wd, float max_norm, const float* norm_sq,
                       cudaStream_t s);
+
+// Layer norm (norm_ops.cu), the gated linear layer (gated.cu) and AdamW
+// (adamw.cu): include/mx_matmul.h has their arguments.  dtype: MX_F32 / MX_BF16.
+int layer_norm_fwd(Context* ctx, int dtype, const void* x, int64_t ldx, const float* w,
+                   const float* b, void* y, int64_t ldy, float* mean, float* rstd, int rows,
+                   int cols, float eps, cudaStream_t s);
+size_t layer_norm_bwd_scratch_bytes(const Context* ctx, int rows, int cols);
+int layer_norm_bwd(Context* ctx, int dtype, const void* dy, int64_t lddy, const void* x,
+                   int64_t ldx, const float* w, const float* mean, const float* rstd, void* dx,
+                   int64_t lddx, float* dw, float* db, int rows, int cols, void* scratch,
+                   size_t scratch_bytes, cudaStream_t s);
+struct GatedArgs {
+  int dtype, M, K, F, tw, act;
+  bool exact;   // float32 products on the SIMT kernels
+  bool strict;  // ... in NpArray order
+  const void* x;
+  const void* w;
+  const void* bias;
+  float* pre;
+  void* h;                              // forward
+  const void* dh;                       // backward
+  void *dx, *dw, *dbias;
+  void* ws;
+  size_t ws_bytes;
+};
+size_t gated_workspace_bytes(const Context* ctx, const GatedArgs& a, bool backward);
+int gated_fwd(Context* ctx, const GatedArgs& a, cudaStream_t s);
+int gated_bwd(Context* ctx, const GatedArgs& a, cudaStream_t s);
+size_t adamw_scratch_bytes(int count, int clip);
+int adamw_check(const mx_adamw_tensor* ts, int count, int bits);
+int adamw_step(const mx_adamw_tensor* ts, int count, int bits, double lr, double b1, double b2,
+               double eps, int64_t step, int32_t* step_dev, double max_norm, float* norm_out,
+               void* scratch, cudaStream_t s);
+int adamw_state_values(const void* q, const float* scale, int64_t n, int is_signed, void* out,
+                       cudaStream_t s);
 
 // cuTensorMapEncodeTiled through the runtime's driver entry point.
 bool make_tmap_2d(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer,

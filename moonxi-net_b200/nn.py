@@ -33,7 +33,7 @@ from __future__ import annotations
 import numpy as np
 import torch
 
-from . import ops
+from . import _lib, ops
 from .collectives import as_collectives
 
 _ALIGN = 64  # floats: every parameter block starts on a 256-byte boundary
@@ -758,3 +758,104 @@ class HostBatchPipeline:
         they hold collectives)."""
         self.graphs = None
         self.model.release_graph()
+
+
+class AdamW:
+    """AdamW over a list of tensors, one launch a step (mx_adamw_step).
+
+    params: contiguous float32 CUDA tensors of one device, updated in place.
+    Gradients may be float32 or bfloat16, tensor by tensor.  state_bits = 32
+    keeps both moments in float32, 8 in one byte each with a float32 scale for
+    every 256 values.  copies: bfloat16 tensors (or None) that receive the new
+    values, for layers that compute in bfloat16.  weight_decay: one number, or
+    one for each tensor (0 for norms and biases).  max_grad_norm > 0 clips by
+    the global norm, which `norm` then holds after a step.
+
+    device_step=True keeps the step number on the device, so that a captured
+    step counts its replays.  state, step_count: the moments and the number of
+    steps of an earlier run (`state`, `step_count`), taken over as they are.
+    """
+
+    def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
+                 weight_decay=0.01, max_grad_norm: float = 0.0, state_bits: int = 32, copies=None,
+                 device_step: bool = False, state=None, step_count: int = 0, ctx=None):
+        self.params = list(params)
+        if not self.params:
+            raise ValueError("AdamW needs at least one tensor")
+        if state_bits not in (8, 32):
+            raise ValueError(f"state_bits must be 8 or 32, got {state_bits}")
+        n = len(self.params)
+        first = self.params[0]
+        for i, p in enumerate(self.params):
+            ops._check_like(p, f"params[{i}]", first, torch.float32)
+        self.device = first.device
+        self.copies = [None] * n if copies is None else list(copies)
+        decay = [float(weight_decay)] * n if not isinstance(weight_decay, (list, tuple)) \
+            else [float(d) for d in weight_decay]
+        if len(self.copies) != n or len(decay) != n or (state is not None and len(state) != n):
+            raise ValueError("copies, weight_decay and state need one entry for each tensor")
+        for i, (c, p) in enumerate(zip(self.copies, self.params)):
+            if c is not None:
+                ops._check_like(c, f"copies[{i}]", first, torch.bfloat16, p.shape)
+        self.lr, self.betas, self.eps = float(lr), (float(betas[0]), float(betas[1])), float(eps)
+        self.max_grad_norm, self.state_bits = float(max_grad_norm), int(state_bits)
+        self.ctx = ctx
+        self.state = self._fresh_state() if state is None else [tuple(s) for s in state]
+        self._check_state()
+        self.step_count = int(step_count)
+        self.step_dev = torch.full((1,), self.step_count, dtype=torch.int32, device=self.device) \
+            if device_step else None
+        self.norm = torch.zeros(1, device=self.device)
+        self._table = (_lib.AdamWTensor * n)()
+        for t, p, c, s, d in zip(self._table, self.params, self.copies, self.state, decay):
+            t.param, t.n, t.weight_decay = p.data_ptr(), p.numel(), d
+            t.copy_bf16 = None if c is None else c.data_ptr()
+            if self.state_bits == 8:
+                t.m, t.m_scale, t.v, t.v_scale = (x.data_ptr() for x in s)
+            else:
+                t.m, t.v = (x.data_ptr() for x in s)
+        nb = _lib.lib().mx_adamw_scratch_bytes(n, int(self.max_grad_norm > 0))
+        self._scratch = torch.empty(nb, dtype=torch.uint8, device=self.device)
+
+    def _fresh_state(self):
+        def zeros(k, dtype):
+            return torch.zeros(k, dtype=dtype, device=self.device)
+
+        if self.state_bits == 32:
+            return [(zeros(p.numel(), torch.float32), zeros(p.numel(), torch.float32))
+                    for p in self.params]
+        return [(zeros(p.numel(), torch.int8), zeros(-(-p.numel() // 256), torch.float32),
+                 zeros(p.numel(), torch.uint8), zeros(-(-p.numel() // 256), torch.float32))
+                for p in self.params]
+
+    def _check_state(self):
+        f32 = torch.float32
+        names, types = (("m", "v"), (f32, f32)) if self.state_bits == 32 else \
+            (("m", "m_scale", "v", "v_scale"), (torch.int8, f32, torch.uint8, f32))
+        for i, (s, p) in enumerate(zip(self.state, self.params)):
+            if len(s) != len(names):
+                raise ValueError(f"state[{i}] needs {names}")
+            for x, name, dtype in zip(s, names, types):
+                ops._check_like(x, f"state[{i}].{name}", p, dtype)
+                k = -(-p.numel() // 256) if name.endswith("scale") else p.numel()
+                if x.numel() != k:
+                    raise ValueError(f"state[{i}].{name} has {x.numel()} elements, needs {k}")
+
+    def step(self, grads, stream=None) -> None:
+        """One update from `grads`, a tensor for each parameter."""
+        if len(grads) != len(self.params):
+            raise ValueError(f"{len(grads)} gradients for {len(self.params)} tensors")
+        for i, (t, g, p) in enumerate(zip(self._table, grads, self.params)):
+            kind = ops._check_type(g, f"grads[{i}]")
+            if g.numel() != p.numel() or g.device != p.device or not g.is_contiguous():
+                raise ValueError(f"grads[{i}] must be contiguous, of {p.numel()} elements on "
+                                 f"{p.device}")
+            t.grad, t.grad_type = g.data_ptr(), kind
+        s = ops._on(self.params[0], stream)
+        rc = _lib.lib().mx_adamw_step(
+            ops._handle(self.ctx, self.params[0]), self._table, len(self.params), self.state_bits,
+            self.lr, self.betas[0], self.betas[1], self.eps, self.step_count + 1,
+            ops._ptr(self.step_dev), self.max_grad_norm, self.norm.data_ptr(),
+            self._scratch.data_ptr(), self._scratch.numel(), s.cuda_stream)
+        ops.check(rc, "mx_adamw_step")
+        self.step_count += 1

@@ -1,12 +1,13 @@
 """Device ops of the matmul path, called through the C ABI.
 
 torch is used only for device memory and streams: every function here takes
-CUDA float32 tensors, passes their raw pointers and the current torch stream
+CUDA tensors (float32; the layer norm, gated layer and AdamW also bfloat16), passes their raw pointers and the current torch stream
 to ``libmxgemm.so`` and lets the library's kernels do the work.
 """
 from __future__ import annotations
 
 import ctypes
+import math
 
 import torch
 
@@ -364,6 +365,228 @@ def sgd_momentum_clip(params, grads, vels, lr, momentum, weight_decay, max_grad_
         float(lr), float(momentum), float(weight_decay), float(max_grad_norm),
         norm_sq.data_ptr(), _stream_ptr(stream))
     check(rc, "mx_sgd_momentum_clip")
+
+
+# ------------------------------ layer norm, the gated linear layer, AdamW
+_DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
+
+
+def _check_like(t: torch.Tensor, name: str, ref: torch.Tensor, dtype=None, shape=None):
+    """A contiguous CUDA tensor on ref's device, of ref's type unless given."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise TypeError(f"{name} must be a CUDA tensor")
+    dtype = ref.dtype if dtype is None else dtype
+    if t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    if t.device != ref.device:
+        raise ValueError(f"{name} is on {t.device}, not on {ref.device}")
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, needs {tuple(shape)}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+
+
+def _check_type(t: torch.Tensor, name: str) -> int:
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise TypeError(f"{name} must be a CUDA tensor")
+    if t.dtype not in _DTYPES:
+        raise TypeError(f"{name} must be float32 or bfloat16, got {t.dtype}")
+    return _DTYPES[t.dtype]
+
+
+def _on(t: torch.Tensor, stream):
+    """The stream of a call on t: the given one, else the current one of t's
+    device.  What the call allocates is allocated on it."""
+    return stream if stream is not None else torch.cuda.current_stream(t.device)
+
+
+def _empty(shape, dtype, t: torch.Tensor, stream):
+    with torch.cuda.stream(stream):
+        return torch.empty(shape, dtype=dtype, device=t.device)
+
+
+def _rows(t: torch.Tensor, name: str) -> tuple[int, int, int]:
+    """(rows, columns, row stride) of a tensor seen as rows of its last
+    dimension: contiguous, or 2-D with contiguous rows."""
+    if t.dim() < 1 or t.shape[-1] < 1:
+        raise ValueError(f"{name} needs a last dimension of at least 1")
+    cols = t.shape[-1]
+    rows = t.numel() // cols
+    if t.is_contiguous():
+        return rows, cols, cols
+    if t.dim() == 2 and t.stride(1) == 1 and t.stride(0) >= cols:
+        return rows, cols, t.stride(0)
+    raise ValueError(f"{name} must be contiguous, or 2-D with contiguous rows")
+
+
+def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None,
+               bias: torch.Tensor | None = None, eps: float = 1e-5, stats: bool = False,
+               out: torch.Tensor | None = None, stream=None, ctx=None):
+    """(y, mean, rstd) of layer norm over the last dimension
+    (mx_layer_norm_fwd).  x: float32 or bfloat16, contiguous or 2-D with
+    contiguous rows; weight, bias: float32.  mean and rstd (float32, one a row,
+    for layer_norm_backward) are None unless `stats`."""
+    dt = _check_type(x, "x")
+    rows, cols, ldx = _rows(x, "x")
+    for t, name in ((weight, "weight"), (bias, "bias")):
+        if t is not None:
+            _check_like(t, name, x, torch.float32, (cols,))
+    s = _on(x, stream)
+    if out is None:
+        out = _empty(x.shape, x.dtype, x, s)
+    elif out.shape != x.shape or out.dtype != x.dtype or out.device != x.device:
+        raise ValueError("out must be like x")
+    ldy = _rows(out, "out")[2]
+    mean = rstd = None
+    if stats:
+        mean, rstd = _empty((2, rows), torch.float32, x, s)
+    rc = _lib.lib().mx_layer_norm_fwd(
+        _handle(ctx, x), dt, x.data_ptr(), ldx, _ptr(weight), _ptr(bias), out.data_ptr(), ldy,
+        _ptr(mean), _ptr(rstd), rows, cols, float(eps), s.cuda_stream)
+    check(rc, "mx_layer_norm_fwd")
+    return out, mean, rstd
+
+
+def layer_norm_backward(grad_out: torch.Tensor, x: torch.Tensor, weight: torch.Tensor | None,
+                        mean: torch.Tensor, rstd: torch.Tensor, dx: torch.Tensor | None = None,
+                        dweight: torch.Tensor | None = None, dbias: torch.Tensor | None = None,
+                        stream=None, ctx=None):
+    """(dx, dweight, dbias) of layer_norm from its input and the mean and rstd
+    that it gave (mx_layer_norm_bwd).  dweight and dbias are float32, summed
+    over the rows in a fixed order."""
+    dt = _check_type(x, "x")
+    rows, cols, ldx = _rows(x, "x")
+    if grad_out.shape != x.shape or grad_out.dtype != x.dtype or grad_out.device != x.device:
+        raise ValueError("grad_out must be like x")
+    lddy = _rows(grad_out, "grad_out")[2]
+    if weight is not None:
+        _check_like(weight, "weight", x, torch.float32, (cols,))
+    _check_like(mean, "mean", x, torch.float32, (rows,))
+    _check_like(rstd, "rstd", x, torch.float32, (rows,))
+    s = _on(x, stream)
+    if dx is None:
+        dx = _empty(x.shape, x.dtype, x, s)
+    elif dx.shape != x.shape or dx.dtype != x.dtype or dx.device != x.device:
+        raise ValueError("dx must be like x")
+    lddx = _rows(dx, "dx")[2]
+    if dweight is None:
+        dweight = _empty((cols,), torch.float32, x, s)
+    if dbias is None:
+        dbias = _empty((cols,), torch.float32, x, s)
+    _check_like(dweight, "dweight", x, torch.float32, (cols,))
+    _check_like(dbias, "dbias", x, torch.float32, (cols,))
+    h = _handle(ctx, x)
+    nb = _lib.lib().mx_layer_norm_bwd_scratch_bytes(h, rows, cols)
+    scratch = _empty((nb,), torch.uint8, x, s)
+    rc = _lib.lib().mx_layer_norm_bwd(
+        h, dt, grad_out.data_ptr(), lddy, x.data_ptr(), ldx, _ptr(weight), mean.data_ptr(),
+        rstd.data_ptr(), dx.data_ptr(), lddx, dweight.data_ptr(), dbias.data_ptr(), rows, cols,
+        scratch.data_ptr(), nb, s.cuda_stream)
+    check(rc, "mx_layer_norm_bwd")
+    return dx, dweight, dbias
+
+
+def _gated_shape(x: torch.Tensor, w: torch.Tensor, transpose_w: bool, act: str):
+    dt = _check_type(x, "x")
+    if act not in _lib.ACTIVATIONS:
+        raise ValueError(f"act must be one of {sorted(_lib.ACTIVATIONS)}, got {act!r}")
+    if x.dim() < 1 or w.dim() != 2:
+        raise ValueError("x needs a last dimension, w two dimensions")
+    K = x.shape[-1]
+    M = x.numel() // K if K else math.prod(x.shape[:-1])
+    two_f = w.shape[0] if transpose_w else w.shape[1]
+    if two_f % 2 or w.shape[1 if transpose_w else 0] != K:
+        raise ValueError(f"w has shape {tuple(w.shape)}, needs "
+                         f"{('[2F, %d]' if transpose_w else '[%d, 2F]') % K}")
+    _check_like(x, "x", x)
+    _check_like(w, "w", x)
+    return dt, M, K, two_f // 2
+
+
+def gated_linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None,
+                 act: str = "silu", transpose_w: bool = False, save: bool = False,
+                 out: torch.Tensor | None = None, pre: torch.Tensor | None = None,
+                 precision="default", stream=None, ctx=None):
+    """(h, pre): h = act(g) * u with [g | u] = x op(w) + bias
+    (mx_gated_linear_fwd).  x: [..., K] float32 or bfloat16; w: [K, 2F]
+    (transpose_w=False) or [2F, K], the gate's half first; bias: [2F].  w, bias
+    and h are of x's type.  pre, [g | u] in float32 for
+    gated_linear_backward, is None unless `save` (or a buffer) is given."""
+    dt, M, K, F = _gated_shape(x, w, transpose_w, act)
+    if bias is not None:
+        _check_like(bias, "bias", x, None, (2 * F,))
+    s = _on(x, stream)
+    lead = tuple(x.shape[:-1])
+    if out is None:
+        out = _empty(lead + (F,), x.dtype, x, s)
+    _check_like(out, "out", x, None, lead + (F,))
+    if pre is None and save:
+        pre = _empty(lead + (2 * F,), torch.float32, x, s)
+    if pre is not None:
+        _check_like(pre, "pre", x, torch.float32, lead + (2 * F,))
+    h, p = _handle(ctx, x), _prec(precision)
+    nb = _lib.lib().mx_gated_linear_workspace_bytes(h, dt, M, K, F, int(transpose_w), p, 0)
+    ws = _empty((nb,), torch.uint8, x, s) if nb else None
+    rc = _lib.lib().mx_gated_linear_fwd(
+        h, dt, x.data_ptr(), w.data_ptr(), _ptr(bias), out.data_ptr(), _ptr(pre), M, K, F,
+        int(transpose_w), _lib.ACTIVATIONS[act], p, _ptr(ws), nb, s.cuda_stream)
+    check(rc, "mx_gated_linear_fwd")
+    return out, pre
+
+
+def gated_linear_backward(grad_out: torch.Tensor, pre: torch.Tensor, x: torch.Tensor,
+                          w: torch.Tensor, act: str = "silu", transpose_w: bool = False,
+                          want_bias: bool = True, dx: torch.Tensor | None = None,
+                          dw: torch.Tensor | None = None, dbias: torch.Tensor | None = None,
+                          precision="default", stream=None, ctx=None):
+    """(dx, dw, dbias) of gated_linear from the `pre` that it saved
+    (mx_gated_linear_bwd); dbias is None without `want_bias`."""
+    dt, M, K, F = _gated_shape(x, w, transpose_w, act)
+    lead = tuple(x.shape[:-1])
+    _check_like(grad_out, "grad_out", x, None, lead + (F,))
+    _check_like(pre, "pre", x, torch.float32, lead + (2 * F,))
+    s = _on(x, stream)
+    dx = _empty(x.shape, x.dtype, x, s) if dx is None else dx
+    dw = _empty(w.shape, x.dtype, x, s) if dw is None else dw
+    if dbias is None and want_bias:
+        dbias = _empty((2 * F,), x.dtype, x, s)
+    _check_like(dx, "dx", x, None, x.shape)
+    _check_like(dw, "dw", x, None, w.shape)
+    if dbias is not None:
+        _check_like(dbias, "dbias", x, None, (2 * F,))
+    h, p = _handle(ctx, x), _prec(precision)
+    nb = _lib.lib().mx_gated_linear_workspace_bytes(h, dt, M, K, F, int(transpose_w), p, 1)
+    ws = _empty((nb,), torch.uint8, x, s) if nb else None
+    rc = _lib.lib().mx_gated_linear_bwd(
+        h, dt, grad_out.data_ptr(), pre.data_ptr(), x.data_ptr(), w.data_ptr(), dx.data_ptr(),
+        dw.data_ptr(), _ptr(dbias), M, K, F, int(transpose_w), _lib.ACTIVATIONS[act], p,
+        _ptr(ws), nb, s.cuda_stream)
+    check(rc, "mx_gated_linear_bwd")
+    return dx, dw, dbias
+
+
+def adamw_state_values(codes: torch.Tensor, scale: torch.Tensor, out: torch.Tensor | None = None,
+                       stream=None, ctx=None) -> torch.Tensor:
+    """The moments that 8-bit AdamW states stand for, in bfloat16
+    (mx_adamw_state_values): the first moment from int8 codes, the second from
+    uint8 codes; scale holds one float32 for each 256 of them."""
+    if not isinstance(codes, torch.Tensor) or not codes.is_cuda:
+        raise TypeError("codes must be a CUDA tensor")
+    if codes.dtype not in (torch.int8, torch.uint8):
+        raise TypeError(f"codes must be int8 or uint8, got {codes.dtype}")
+    _check_like(codes, "codes", codes)
+    _check_like(scale, "scale", codes, torch.float32)
+    if scale.numel() != -(-codes.numel() // 256):
+        raise ValueError(f"scale has {scale.numel()} elements, needs {-(-codes.numel() // 256)}")
+    s = _on(codes, stream)
+    if out is None:
+        out = _empty(codes.shape, torch.bfloat16, codes, s)
+    _check_like(out, "out", codes, torch.bfloat16, codes.shape)
+    rc = _lib.lib().mx_adamw_state_values(
+        _handle(ctx, codes), codes.data_ptr(), scale.data_ptr(), codes.numel(),
+        int(codes.dtype == torch.uint8), out.data_ptr(), s.cuda_stream)
+    check(rc, "mx_adamw_state_values")
+    return out
 
 
 def status(device: int | None = None) -> tuple[int, int]:
