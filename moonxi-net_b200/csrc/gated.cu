@@ -3,189 +3,546 @@
 //   [g | u] = x op(w) + bias,  h = act(g) * u
 //   dpre = [dh * u * act'(g) | dh * act(g)],  dx = dpre op(w)^T,
 //   dw = x^T dpre (w stored [K,2F]) or dpre^T x ([2F,K]),  dbias = sum_rows dpre
+//
+// The products are those of gemm_bf16.cu (the forward one with the activation
+// in its epilogue), read in the layout in which x, w and dpre are stored; a
+// float32 tensor goes in as three bfloat16 copies, and a bfloat16 one whose
+// rows TMA cannot address (not a multiple of 16 bytes) as one padded copy.
+// Small float32 products stay on the exact SIMT kernels.  dpre is one pass over
+// dh and the saved [g | u] that also sums dbias; it is rounded to bfloat16 once
+// (bfloat16 tensors: half a step, 2^-9 of each value, as much as dx and dw
+// themselves are rounded by, and independent of it) or split in three.
 #include <algorithm>
 #include <cmath>
 
-#include <cuda_bf16.h>
-
+#include "gated_act.cuh"
 #include "mx_internal.h"
 #include "mx_ptx.cuh"
 
 namespace mx {
 namespace {
 
-__device__ __forceinline__ float to_f(float x) { return x; }
-__device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
-__device__ __forceinline__ void put(float* p, float x) { *p = x; }
-__device__ __forceinline__ void put(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
+using bf16 = __nv_bfloat16;
 
-// act(z) and, for the backward pass, act'(z).
-__device__ __forceinline__ float act_value(int act, float z) {
-  switch (act) {
-    case MX_ACT_SILU: return z / (1.0f + expf(-z));
-    case MX_ACT_GELU: return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
-    case MX_ACT_GELU_TANH:
-      return 0.5f * z * (1.0f + tanhf(0.79788456080286536f * (z + 0.044715f * z * z * z)));
-    case MX_ACT_RELU: return z > 0.0f ? z : 0.0f;
-    default: return 1.0f / (1.0f + expf(-z));
-  }
-}
-__device__ __forceinline__ void act_grad(int act, float z, float& a, float& da) {
-  switch (act) {
-    case MX_ACT_SILU: {
-      const float s = 1.0f / (1.0f + expf(-z));
-      a = z * s;
-      da = s * (1.0f + z * (1.0f - s));
-      return;
+// The bfloat16 copies (NC of them, see gemm_bf16.cu) of 8 values.
+template <int NC>
+__device__ __forceinline__ void store_copies(const float (&x)[8], bf16* dst, int64_t copy) {
+  float r[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r[i] = x[i];
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(r[2 * i], r[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+      if (c + 1 < NC) {  // exact: the difference has fewer bits than r
+        r[2 * i] -= __uint_as_float(w[i] << 16);
+        r[2 * i + 1] -= __uint_as_float(w[i] & 0xffff0000u);
+      }
     }
-    case MX_ACT_GELU: {
-      const float c = 0.5f * (1.0f + erff(z * 0.70710678118654752f));
-      a = z * c;
-      da = c + z * expf(-0.5f * z * z) * 0.39894228040143268f;
-      return;
-    }
-    case MX_ACT_GELU_TANH: {
-      const float k = 0.79788456080286536f;
-      const float t = tanhf(k * (z + 0.044715f * z * z * z));
-      a = 0.5f * z * (1.0f + t);
-      da = 0.5f * (1.0f + t) + 0.5f * z * (1.0f - t * t) * k * (1.0f + 0.134145f * z * z);
-      return;
-    }
-    case MX_ACT_RELU:
-      a = z > 0.0f ? z : 0.0f;
-      da = z > 0.0f ? 1.0f : 0.0f;
-      return;
-    default:
-      a = 1.0f / (1.0f + expf(-z));
-      da = a * (1.0f - a);
-  }
-}
-
-// One thread an output; 32 x 32 tiles of the operands in shared memory.
-// C(m, n) = sum_k A(m, k) B(k, n), any strides.
-template <typename TA, typename TB, typename TC, bool GATED>
-__global__ void __launch_bounds__(1024) tile_kernel(const TA* a, int64_t am, int64_t ak,
-                                                    const TB* b, int64_t bk, int64_t bn,
-                                                    const TB* bias, TC* c, float* pre, int M,
-                                                    int N, int K, int act) {
-  __shared__ float sa[32][33], sb[32][33], su[32][33];
-  const int tx = threadIdx.x, ty = threadIdx.y;
-  const int m = blockIdx.y * 32 + ty, n = blockIdx.x * 32 + tx;
-  float g = 0.0f, u = 0.0f;
-  for (int k0 = 0; k0 < K; k0 += 32) {
-    sa[ty][tx] = m < M && k0 + tx < K ? to_f(a[m * am + (k0 + tx) * ak]) : 0.0f;
-    sb[ty][tx] = n < N && k0 + ty < K ? to_f(b[(k0 + ty) * bk + n * bn]) : 0.0f;
-    if (GATED) su[ty][tx] = n < N && k0 + ty < K ? to_f(b[(k0 + ty) * bk + (n + N) * bn]) : 0.0f;
-    __syncthreads();
-    for (int k = 0; k < 32; ++k) {
-      g += sa[ty][k] * sb[k][tx];
-      if (GATED) u += sa[ty][k] * su[k][tx];
-    }
-    __syncthreads();
-  }
-  if (m >= M || n >= N) return;
-  if (GATED) {
-    if (bias) {
-      g += to_f(bias[n]);
-      u += to_f(bias[N + n]);
-    }
-    if (pre) {
-      pre[static_cast<int64_t>(m) * 2 * N + n] = g;
-      pre[static_cast<int64_t>(m) * 2 * N + N + n] = u;
-    }
-    g = act_value(act, g) * u;
-  }
-  put(c + static_cast<int64_t>(m) * N + n, g);
-}
-
-template <typename T>
-__global__ void __launch_bounds__(256) dpre_kernel(const T* dh, const float* pre, float* dpre,
-                                                   int64_t n, int F, int act) {
-  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
-    const int64_t m = i / F, f = i - m * F;
-    float a, da;
-    act_grad(act, pre[m * 2 * F + f], a, da);
-    const float d = to_f(dh[i]);
-    dpre[m * 2 * F + f] = d * pre[m * 2 * F + F + f] * da;
-    dpre[m * 2 * F + F + f] = d * a;
+    *reinterpret_cast<uint4*>(dst + c * copy) = make_uint4(w[0], w[1], w[2], w[3]);
   }
 }
 
 template <typename T>
-__global__ void __launch_bounds__(256) colsum_kernel(const float* x, T* out, int rows, int cols) {
+__device__ __forceinline__ void load8(const T* p, float (&x)[8]);
+template <>
+__device__ __forceinline__ void load8(const float* p, float (&x)[8]) {
+  const float4 a = __ldg(reinterpret_cast<const float4*>(p));
+  const float4 b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+  x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+  x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+}
+template <>
+__device__ __forceinline__ void load8(const bf16* p, float (&x)[8]) {
+  const uint4 r = __ldg(reinterpret_cast<const uint4*>(p));
+  const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x[2 * i] = __uint_as_float(w[i] << 16);
+    x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+}
+
+// Copies of a row-major [rows][cols] matrix with rows of ldd elements (a
+// multiple of 8): columns below `split` at 0, the others from `up` on, zeros
+// between.  A thread makes 8 columns.
+template <typename T, int NC, bool VEC>
+__global__ void __launch_bounds__(256) pack_kernel(const T* __restrict__ src, int64_t ld, int rows,
+                                                   int cols, int split, int up,
+                                                   bf16* __restrict__ dst, int64_t ldd,
+                                                   int64_t copy) {
+  const int64_t d = (blockIdx.x * 256ll + threadIdx.x) * 8;
+  if (d >= ldd) return;
+  for (int64_t r = blockIdx.y; r < rows; r += gridDim.y) {
+    float x[8];
+    if (VEC) {
+      load8(src + r * ld + d, x);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int64_t e = d + i;
+        const int64_t c = e < up ? (e < split ? e : cols) : split + (e - up);
+        x[i] = c < cols ? to_f(src[r * ld + c]) : 0.0f;
+      }
+    }
+    store_copies<NC>(x, dst + r * ldd + d, copy);
+  }
+}
+
+struct Dpre {
+  const void* dh;
+  const float* pre;
+  void* out;      // OUT 1, 3: bfloat16 copies; 0: float32
+  int64_t ldo, copy;
+  float* part;    // [row blocks][2F], or null
+  int rows, F, act, per;  // per: rows of a block
+};
+
+// A block: 32 * V columns of both halves, `per` rows, its eight warps a row at
+// a time.  V = 8: 16-byte accesses.  Bound by the bytes: with bfloat16 tensors
+// 10 read and 4 written a value of h.
+template <typename T, int OUT, int V>
+__global__ void __launch_bounds__(256) dpre_kernel(const Dpre p) {
+  __shared__ float sh[8][32 * V];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t f = (blockIdx.x * 32ll + lane) * V;
+  const int64_t r0 = blockIdx.y * static_cast<int64_t>(p.per);
+  const int64_t r1 = r0 + p.per < p.rows ? r0 + p.per : p.rows;
+  float sg[V], su[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) sg[i] = su[i] = 0.0f;
+  if (f < p.F) {
+    for (int64_t r = r0 + warp; r < r1; r += 8) {
+      const T* dh = static_cast<const T*>(p.dh) + r * p.F + f;
+      const float* pre = p.pre + r * 2 * p.F + f;
+      float d[V], g[V], u[V];
+      if constexpr (V == 8) {
+        load8(dh, d);
+        load8(pre, g);
+        load8(pre + p.F, u);
+      } else {
+        d[0] = to_f(*dh);
+        g[0] = pre[0];
+        u[0] = pre[p.F];
+      }
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        float a, da;
+        act_grad(p.act, g[i], a, da);
+        g[i] = d[i] * u[i] * da;
+        u[i] = d[i] * a;
+        sg[i] += g[i];
+        su[i] += u[i];
+      }
+      if constexpr (OUT == 0) {
+        float* out = static_cast<float*>(p.out) + r * p.ldo + f;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          out[i] = g[i];
+          out[p.F + i] = u[i];
+        }
+      } else if constexpr (V == 8) {
+        bf16* out = static_cast<bf16*>(p.out) + r * p.ldo + f;
+        store_copies<OUT>(g, out, p.copy);
+        store_copies<OUT>(u, out + p.F, p.copy);
+      } else {
+        bf16* out = static_cast<bf16*>(p.out) + r * p.ldo + f;
+        float x = g[0], y = u[0];
+#pragma unroll
+        for (int c = 0; c < OUT; ++c) {
+          const bf16 a = __float2bfloat16_rn(x), b = __float2bfloat16_rn(y);
+          out[c * p.copy] = a;
+          out[c * p.copy + p.F] = b;
+          x -= __bfloat162float(a);
+          y -= __bfloat162float(b);
+        }
+      }
+    }
+  }
+  if (!p.part) return;
+  float* part = p.part + blockIdx.y * 2ll * p.F;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {  // the eight warps' sums, in their order
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < V; ++i) sh[warp][lane * V + i] = h ? su[i] : sg[i];
+    __syncthreads();
+    const int64_t c = blockIdx.x * 32ll * V + threadIdx.x;
+    if (threadIdx.x < 32 * V && c < p.F) {
+      float s = 0.0f;
+#pragma unroll
+      for (int w = 0; w < 8; ++w) s += sh[w][threadIdx.x];
+      part[h * static_cast<int64_t>(p.F) + c] = s;
+    }
+  }
+}
+
+// dbias = the row blocks' sums, in a fixed order.
+template <typename T>
+__global__ void __launch_bounds__(256) dbias_kernel(const float* part, T* out, int blocks,
+                                                    int64_t width) {
   __shared__ float sh[8][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t c = blockIdx.x * 32ll + lane;
   float s = 0.0f;
-  if (c < cols)
-    for (int64_t r = warp; r < rows; r += 8) s += x[r * cols + c];
+  if (c < width)
+    for (int r = warp; r < blocks; r += 8) s += part[r * width + c];
   sh[warp][lane] = s;
   __syncthreads();
-  if (warp == 0 && c < cols) {
+  if (warp == 0 && c < width) {
     s = 0.0f;
     for (int i = 0; i < 8; ++i) s += sh[i][lane];
     put(out + c, s);
   }
 }
 
+// h from a complete [g | u] (the SIMT products); K = 0: [g | u] is the bias.
 template <typename T>
-int fwd(const GatedArgs& a, cudaStream_t s) {
-  const dim3 grid((a.F + 31) / 32, (a.M + 31) / 32);
-  const int64_t bk = a.tw ? 1 : 2ll * a.F, bn = a.tw ? a.K : 1;
-  tile_kernel<T, T, T, true><<<grid, dim3(32, 32), 0, s>>>(
-      static_cast<const T*>(a.x), a.K, 1, static_cast<const T*>(a.w), bk, bn,
-      static_cast<const T*>(a.bias), static_cast<T*>(a.h), a.pre, a.M, a.F, a.K, a.act);
+__global__ void __launch_bounds__(256) gate_kernel(const float* pre, T* h, int64_t n, int F,
+                                                   int act) {
+  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
+    const int64_t m = i / F, f = i - m * F;
+    put(h + i, act_value(act, pre[m * 2 * F + f]) * pre[m * 2 * F + F + f]);
+  }
+}
+template <typename T>
+__global__ void __launch_bounds__(256) bias_rows_kernel(const T* bias, float* pre, T* h, int64_t n,
+                                                        int F, int act) {
+  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
+    const int64_t m = i / F, f = i - m * F;
+    const float g = bias ? to_f(bias[f]) : 0.0f, u = bias ? to_f(bias[F + f]) : 0.0f;
+    if (pre) {
+      pre[m * 2 * F + f] = g;
+      pre[m * 2 * F + F + f] = u;
+    }
+    put(h + i, act_value(act, g) * u);
+  }
+}
+
+int64_t pad8(int64_t n) { return (n + 7) & ~7ll; }
+size_t align256(size_t x) { return (x + 255) & ~static_cast<size_t>(255); }
+bool aligned16(const void* a) { return (reinterpret_cast<uintptr_t>(a) & 15u) == 0; }
+unsigned grid_for(int64_t n, int num_sms) {
+  return static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>((n + 255) / 256, num_sms * 8)));
+}
+
+// Pieces of the workspace, 256-byte aligned.  With a null base it measures.
+struct Carver {
+  uint8_t* base;
+  size_t used = 0;
+  template <typename P>
+  P* take(size_t bytes) {
+    P* p = base ? reinterpret_cast<P*>(base + used) : nullptr;
+    used += align256(bytes);
+    return p;
+  }
+};
+
+// float32 products on the tensor cores: where they fill enough of the machine
+// to pay for the three copies of each operand.
+bool tensor_f32(const GatedArgs& a) {
+  return !a.exact && a.M >= 128 && a.K >= 64 && a.F >= 64 && 4.0 * a.M * a.K * a.F >= 1.0e9;
+}
+int copies_of(const GatedArgs& a) { return a.dtype == MX_BF16 ? 1 : 3; }
+bool tensor_path(const GatedArgs& a) { return a.dtype == MX_BF16 || tensor_f32(a); }
+
+// A packed copy of a [rows][cols] matrix, or (bfloat16 that TMA can address)
+// the matrix itself.  `halves`: columns from cols / 2 on start at a multiple
+// of 8.
+struct Packed {
+  bool direct;
+  int64_t ld, up, copy;
+};
+Packed packed_of(const GatedArgs& a, const void* src, int rows, int64_t cols, bool halves) {
+  Packed p;
+  const int64_t half = cols / 2;
+  p.direct = a.dtype == MX_BF16 && cols % 8 == 0 && aligned16(src) && (!halves || half % 8 == 0);
+  p.ld = halves ? 2 * pad8(half) : pad8(cols);
+  p.up = halves ? pad8(half) : p.ld;
+  p.copy = static_cast<int64_t>(rows) * p.ld;
+  return p;
+}
+size_t packed_bytes(const GatedArgs& a, const Packed& p) {
+  return p.direct ? 0 : static_cast<size_t>(copies_of(a)) * p.copy * 2;
+}
+// The operand of a matrix: packed into `dst` unless it is read as it is.
+cudaError_t pack(Context* ctx, const GatedArgs& a, const void* src, int rows, int64_t cols,
+                 const Packed& p, bool halves, bf16* dst, cudaStream_t s, Bf16Operand& o) {
+  o.copy = p.copy;
+  o.ld = p.ld;
+  o.base = p.direct ? src : dst;
+  if (p.direct) return cudaSuccess;
+  const int split = static_cast<int>(halves ? cols / 2 : cols);
+  const dim3 grid(static_cast<unsigned>((p.ld / 8 + 255) / 256),
+                  static_cast<unsigned>(std::min(rows, 32768)));
+  const bool vec = cols == p.ld && (!halves || p.up == split) && aligned16(src);
+  const int n = static_cast<int>(cols), up = static_cast<int>(p.up);
+  if (a.dtype == MX_BF16)
+    pack_kernel<bf16, 1, false><<<grid, 256, 0, s>>>(static_cast<const bf16*>(src), cols, rows, n,
+                                                     split, up, dst, p.ld, p.copy);
+  else if (vec)
+    pack_kernel<float, 3, true><<<grid, 256, 0, s>>>(static_cast<const float*>(src), cols, rows,
+                                                     n, split, up, dst, p.ld, p.copy);
+  else
+    pack_kernel<float, 3, false><<<grid, 256, 0, s>>>(static_cast<const float*>(src), cols, rows,
+                                                      n, split, up, dst, p.ld, p.copy);
   note_launches(1);
-  return cuda_status(cudaGetLastError());
+  return cudaGetLastError();
+}
+
+// An exact SIMT product on scratch of its own (no workspace or counters of the
+// context, so calls on different streams may overlap).
+GemmArgs simt_args(const GatedArgs& a, const void* x, const void* w, float* c, int M, int K, int N,
+                   int ta, int tb, const void* bias) {
+  GemmArgs g;
+  g.a = static_cast<const float*>(x);
+  g.b = static_cast<const float*>(w);
+  g.c = c;
+  g.M = M; g.K = K; g.N = N;
+  g.ta = ta; g.tb = tb;
+  g.lda = ta ? M : K;
+  g.ldb = tb ? K : N;
+  g.ldc = N;
+  g.bias = static_cast<const float*>(bias);
+  g.strict = a.strict ? 1 : 0;
+  return g;
+}
+size_t simt_scratch(const Context* ctx, GemmArgs g) {
+  size_t need = 0;
+  for (uintptr_t off : {0, 4}) {  // aligned and not: the plans differ
+    g.a = reinterpret_cast<const float*>(off);
+    g.b = reinterpret_cast<const float*>(off);
+    need = std::max(need, simt_gemm_scratch_bytes(ctx, g));
+  }
+  return need;
+}
+int simt_product(Context* ctx, const GemmArgs& g, void* scratch, size_t bytes, cudaStream_t s) {
+  Context local = *ctx;
+  local.counters = nullptr;  // arrival counters come from the scratch
+  return skinny_applies(g) ? skinny_gemm(&local, g, s, scratch, bytes)
+                           : simt_gemm_launch(&local, g, s, static_cast<float*>(scratch), bytes);
+}
+
+// The three products' workspaces, laid out alike for the size query and the
+// call.
+struct FwdWork {
+  Packed x, w;
+  bf16 *xp, *wp;
+  float* parts;
+  float* pre;       // SIMT: [g | u] when the caller saves none
+  void* scratch;
+  size_t scratch_bytes, bytes;
+};
+FwdWork fwd_work(const Context* ctx, const GatedArgs& a) {
+  FwdWork w{};
+  Carver c{static_cast<uint8_t*>(a.ws)};
+  if (tensor_path(a)) {
+    // a size query knows no pointers: room for copies of unaligned tensors
+    const bool asked = !a.x;
+    const void* off = reinterpret_cast<const void*>(uintptr_t{1});
+    w.x = packed_of(a, asked ? off : a.x, a.M, a.K, false);
+    w.w = a.tw ? packed_of(a, asked ? off : a.w, 2 * a.F, a.K, false)
+               : packed_of(a, asked ? off : a.w, a.K, 2ll * a.F, true);
+    w.xp = c.take<bf16>(packed_bytes(a, w.x));
+    w.wp = c.take<bf16>(packed_bytes(a, w.w));
+    w.parts = c.take<float>(bf16_gemm_scratch_bytes(ctx, a.M, a.F, a.K, true, copies_of(a)));
+  } else {
+    w.pre = a.pre ? a.pre : c.take<float>(static_cast<size_t>(a.M) * 2 * a.F * sizeof(float));
+    w.scratch_bytes = simt_scratch(
+        ctx, simt_args(a, nullptr, nullptr, nullptr, a.M, a.K, 2 * a.F, 0, a.tw, nullptr));
+    w.scratch = c.take<void>(w.scratch_bytes);
+  }
+  w.bytes = c.used;
+  return w;
+}
+
+template <typename T>
+int fwd(Context* ctx, const GatedArgs& a, cudaStream_t s) {
+  const int64_t n = static_cast<int64_t>(a.M) * a.F;
+  if (a.K == 0) {
+    bias_rows_kernel<T><<<grid_for(n, ctx->num_sms), 256, 0, s>>>(
+        static_cast<const T*>(a.bias), a.pre, static_cast<T*>(a.h), n, a.F, a.act);
+    note_launches(1);
+    return cuda_status(cudaGetLastError());
+  }
+  const FwdWork w = fwd_work(ctx, a);
+  if (w.bytes > a.ws_bytes) return kErrInvalid;
+  if (!tensor_path(a)) {
+    const GemmArgs g = simt_args(a, a.x, a.w, w.pre, a.M, a.K, 2 * a.F, 0, a.tw, a.bias);
+    const int rc = simt_product(ctx, g, w.scratch, w.scratch_bytes, s);
+    if (rc != kOk) return rc;
+    gate_kernel<T><<<grid_for(n, ctx->num_sms), 256, 0, s>>>(w.pre, static_cast<T*>(a.h), n, a.F,
+                                                             a.act);
+    note_launches(1);
+    return cuda_status(cudaGetLastError());
+  }
+  Bf16Gemm g;
+  cudaError_t e = pack(ctx, a, a.x, a.M, a.K, w.x, false, w.xp, s, g.a);
+  if (e == cudaSuccess)
+    e = a.tw ? pack(ctx, a, a.w, 2 * a.F, a.K, w.w, false, w.wp, s, g.b)
+             : pack(ctx, a, a.w, a.K, 2ll * a.F, w.w, true, w.wp, s, g.b);
+  if (e != cudaSuccess) return cuda_status(e);
+  g.a.kmajor = true;
+  g.b.kmajor = a.tw != 0;
+  g.b2 = g.b;
+  g.b2.base = static_cast<const bf16*>(g.b.base) + (a.tw ? a.F * g.b.ld : w.w.direct ? a.F : w.w.up);
+  g.gated = true;
+  g.copies = copies_of(a);
+  g.M = a.M; g.N = a.F; g.K = a.K;
+  g.out = a.h;
+  g.ldc = a.F;
+  g.bias = a.bias;
+  g.pre = a.pre;
+  g.act = a.act;
+  g.parts = w.parts;
+  return bf16_gemm(ctx, g, s);
+}
+
+struct BwdWork {
+  Packed x, w;
+  bf16 *xp, *wp;
+  void* dpre;
+  int64_t ldp, copy;
+  float* part;
+  int row_blocks, per;
+  float* parts;
+  void* scratch;
+  size_t scratch_bytes, bytes;
+};
+BwdWork bwd_work(const Context* ctx, const GatedArgs& a) {
+  BwdWork w{};
+  Carver c{static_cast<uint8_t*>(a.ws)};
+  // rows of a block of dpre_kernel: at least 16, and four blocks an SM at most
+  const int col_blocks = (a.F + 255) / 256;
+  const int want = std::max(1, 8 * ctx->num_sms / col_blocks);
+  w.per = std::max(16, (a.M + want - 1) / want);
+  w.row_blocks = (a.M + w.per - 1) / w.per;
+  w.part = c.take<float>(static_cast<size_t>(w.row_blocks) * 2 * a.F * sizeof(float));
+  if (tensor_path(a)) {
+    const int nc = copies_of(a);
+    w.ldp = pad8(2ll * a.F);
+    w.copy = w.ldp * a.M;
+    w.dpre = c.take<void>(static_cast<size_t>(nc) * w.copy * 2);
+    const bool asked = !a.pre;
+    const void* off = reinterpret_cast<const void*>(uintptr_t{1});
+    w.x = packed_of(a, asked ? off : a.x, a.M, a.K, false);
+    w.w = a.tw ? packed_of(a, asked ? off : a.w, 2 * a.F, a.K, false)
+               : packed_of(a, asked ? off : a.w, a.K, 2ll * a.F, false);
+    w.xp = c.take<bf16>(packed_bytes(a, w.x));
+    w.wp = c.take<bf16>(packed_bytes(a, w.w));
+    const int m2 = a.tw ? 2 * a.F : a.K, n2 = a.tw ? a.K : 2 * a.F;
+    w.parts = c.take<float>(std::max(bf16_gemm_scratch_bytes(ctx, a.M, a.K, 2 * a.F, false, nc),
+                                     bf16_gemm_scratch_bytes(ctx, m2, n2, a.M, false, nc)));
+  } else {
+    w.ldp = 2ll * a.F;
+    w.dpre = c.take<void>(static_cast<size_t>(a.M) * w.ldp * sizeof(float));
+    const GemmArgs dx = simt_args(a, nullptr, nullptr, nullptr, a.M, 2 * a.F, a.K, 0, !a.tw, nullptr);
+    const GemmArgs dw = a.tw ? simt_args(a, nullptr, nullptr, nullptr, 2 * a.F, a.M, a.K, 1, 0, nullptr)
+                             : simt_args(a, nullptr, nullptr, nullptr, a.K, a.M, 2 * a.F, 1, 0, nullptr);
+    w.scratch_bytes = std::max(simt_scratch(ctx, dx), simt_scratch(ctx, dw));
+    w.scratch = c.take<void>(w.scratch_bytes);
+  }
+  w.bytes = c.used;
+  return w;
+}
+
+template <typename T, int OUT>
+void launch_dpre(const Dpre& p, int row_blocks, cudaStream_t s) {
+  const bool vec = p.F % 8 == 0 && aligned16(p.dh) && aligned16(p.pre);
+  const int width = vec ? 256 : 32;
+  const dim3 grid((p.F + width - 1) / width, row_blocks);
+  if (vec) dpre_kernel<T, OUT, 8><<<grid, 256, 0, s>>>(p);
+  else dpre_kernel<T, OUT, 1><<<grid, 256, 0, s>>>(p);
+  note_launches(1);
 }
 
 template <typename T>
 int bwd(Context* ctx, const GatedArgs& a, cudaStream_t s) {
+  const BwdWork w = bwd_work(ctx, a);
+  if (w.bytes > a.ws_bytes) return kErrInvalid;
+  const bool tensor = tensor_path(a);
   const int F2 = 2 * a.F;
-  float* dpre = static_cast<float*>(a.ws);
-  const int64_t n = static_cast<int64_t>(a.M) * a.F;
-  dpre_kernel<T><<<static_cast<unsigned>(std::min<int64_t>((n + 255) / 256, ctx->num_sms * 8)), 256,
-                   0, s>>>(static_cast<const T*>(a.dh), a.pre, dpre, n, a.F, a.act);
-  const dim3 th(32, 32);
-  const T* w = static_cast<const T*>(a.w);
-  const T* x = static_cast<const T*>(a.x);
+  const Dpre p{a.dh, a.pre, w.dpre, w.ldp, w.copy, a.dbias ? w.part : nullptr, a.M, a.F, a.act, w.per};
+  if (a.dtype == MX_BF16) launch_dpre<bf16, 1>(p, w.row_blocks, s);
+  else if (tensor) launch_dpre<float, 3>(p, w.row_blocks, s);
+  else launch_dpre<float, 0>(p, w.row_blocks, s);
+  cudaError_t e = cudaGetLastError();
+  if (e == cudaSuccess && a.dbias) {
+    dbias_kernel<T><<<(F2 + 31) / 32, 256, 0, s>>>(w.part, static_cast<T*>(a.dbias), w.row_blocks, F2);
+    note_launches(1);
+    e = cudaGetLastError();
+  }
+  if (e != cudaSuccess) return cuda_status(e);
+  if (!tensor) {
+    int rc = kOk;
+    if (a.dx)
+      rc = simt_product(ctx, simt_args(a, w.dpre, a.w, static_cast<float*>(a.dx), a.M, F2, a.K, 0,
+                                       !a.tw, nullptr), w.scratch, w.scratch_bytes, s);
+    if (rc == kOk && a.dw)
+      rc = simt_product(ctx, a.tw ? simt_args(a, w.dpre, a.x, static_cast<float*>(a.dw), F2, a.M,
+                                              a.K, 1, 0, nullptr)
+                                  : simt_args(a, a.x, w.dpre, static_cast<float*>(a.dw), a.K, a.M,
+                                              F2, 1, 0, nullptr),
+                        w.scratch, w.scratch_bytes, s);
+    return rc;
+  }
+  Bf16Operand d;
+  d.base = w.dpre;
+  d.copy = w.copy;
+  d.ld = w.ldp;
+  Bf16Gemm g;
+  g.copies = copies_of(a);
+  g.parts = w.parts;
   if (a.dx) {
-    const dim3 grid((a.K + 31) / 32, (a.M + 31) / 32);
-    tile_kernel<float, T, T, false><<<grid, th, 0, s>>>(
-        dpre, F2, 1, w, a.tw ? a.K : 1, a.tw ? 1 : F2, nullptr, static_cast<T*>(a.dx), nullptr,
-        a.M, a.K, F2, 0);
+    e = a.tw ? pack(ctx, a, a.w, F2, a.K, w.w, false, w.wp, s, g.b)
+             : pack(ctx, a, a.w, a.K, F2, w.w, false, w.wp, s, g.b);
+    if (e != cudaSuccess) return cuda_status(e);
+    g.a = d;
+    g.a.kmajor = true;
+    g.b.kmajor = !a.tw;
+    g.M = a.M; g.N = a.K; g.K = F2;
+    g.out = a.dx;
+    g.ldc = a.K;
+    const int rc = bf16_gemm(ctx, g, s);
+    if (rc != kOk) return rc;
   }
-  if (a.dw && !a.tw) {
-    const dim3 grid((F2 + 31) / 32, (a.K + 31) / 32);
-    tile_kernel<T, float, T, false><<<grid, th, 0, s>>>(x, 1, a.K, dpre, F2, 1, nullptr,
-                                                       static_cast<T*>(a.dw), nullptr, a.K, F2,
-                                                       a.M, 0);
-  } else if (a.dw) {
-    const dim3 grid((a.K + 31) / 32, (F2 + 31) / 32);
-    tile_kernel<float, T, T, false><<<grid, th, 0, s>>>(dpre, 1, F2, x, a.K, 1, nullptr,
-                                                       static_cast<T*>(a.dw), nullptr, F2, a.K,
-                                                       a.M, 0);
+  if (a.dw) {
+    Bf16Operand x;
+    e = pack(ctx, a, a.x, a.M, a.K, w.x, false, w.xp, s, x);
+    if (e != cudaSuccess) return cuda_status(e);
+    g.a = a.tw ? d : x;
+    g.b = a.tw ? x : d;
+    g.a.kmajor = g.b.kmajor = false;
+    g.M = a.tw ? F2 : a.K;
+    g.N = a.tw ? a.K : F2;
+    g.K = a.M;
+    g.out = a.dw;
+    g.ldc = g.N;
+    return bf16_gemm(ctx, g, s);
   }
-  if (a.dbias)
-    colsum_kernel<T><<<(F2 + 31) / 32, 256, 0, s>>>(dpre, static_cast<T*>(a.dbias), a.M, F2);
-  note_launches(4);
-  return cuda_status(cudaGetLastError());
+  return kOk;
 }
 
 }  // namespace
 
 size_t gated_workspace_bytes(const Context* ctx, const GatedArgs& a, bool backward) {
-  (void)ctx;
-  return backward ? static_cast<size_t>(a.M) * 2 * a.F * sizeof(float) : 0;
+  GatedArgs q = a;
+  q.ws = nullptr;
+  q.x = q.w = nullptr;  // the size does not depend on the tensors' alignment
+  q.pre = nullptr;
+  if (!backward && a.K == 0) return 0;
+  return backward ? bwd_work(ctx, q).bytes : fwd_work(ctx, q).bytes;
 }
 
 int gated_fwd(Context* ctx, const GatedArgs& a, cudaStream_t s) {
-  (void)ctx;
-  return a.dtype == MX_BF16 ? fwd<__nv_bfloat16>(a, s) : fwd<float>(a, s);
+  return a.dtype == MX_BF16 ? fwd<bf16>(ctx, a, s) : fwd<float>(ctx, a, s);
 }
 
 int gated_bwd(Context* ctx, const GatedArgs& a, cudaStream_t s) {
-  return a.dtype == MX_BF16 ? bwd<__nv_bfloat16>(ctx, a, s) : bwd<float>(ctx, a, s);
+  return a.dtype == MX_BF16 ? bwd<bf16>(ctx, a, s) : bwd<float>(ctx, a, s);
 }
 
 }  // namespace mx

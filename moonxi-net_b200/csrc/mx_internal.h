@@ -217,6 +217,31 @@ int layer_norm_bwd(Context* ctx, int dtype, const void* dy, int64_t lddy, const 
                    int64_t ldx, const float* w, const float* mean, const float* rstd, void* dx,
                    int64_t lddx, float* dw, float* db, int rows, int cols, void* scratch,
                    size_t scratch_bytes, cudaStream_t s);
+// GEMM on bfloat16 operands (gemm_bf16.cu): one copy of each operand, or three
+// whose sum is a float32 operand.  Element (r, k) of copy i at
+// base[i * copy + r * ld + k] (kmajor) or base[i * copy + k * ld + r]; base
+// 16-byte aligned, ld and copy multiples of 8.
+struct Bf16Operand {
+  const void* base = nullptr;
+  int64_t copy = 0, ld = 0;
+  bool kmajor = true;
+};
+struct Bf16Gemm {
+  Bf16Operand a, b;
+  Bf16Operand b2;          // gated: the other projection's columns
+  bool gated = false;      // h = act(A B + bias) * (A B2 + bias2), N columns each
+  int copies = 1;          // 1: outputs bfloat16; 3: float32
+  int M = 0, N = 0, K = 0;
+  void* out = nullptr;     // [M][ldc]
+  int64_t ldc = 0;
+  const void* bias = nullptr;  // gated: [2N], of the output's type
+  float* pre = nullptr;        // gated: float32 [M][2N]
+  int act = 0;
+  float* parts = nullptr;  // scratch of bf16_gemm_scratch_bytes, 16-byte aligned
+};
+size_t bf16_gemm_scratch_bytes(const Context* ctx, int M, int N, int K, bool gated, int copies);
+int bf16_gemm(Context* ctx, const Bf16Gemm& g, cudaStream_t s);
+
 struct GatedArgs {
   int dtype, M, K, F, tw, act;
   bool exact;   // float32 products on the SIMT kernels
@@ -251,6 +276,10 @@ bool make_tmap_2d(CUtensorMap* map, const void* base, uint64_t inner, uint64_t o
 bool make_tmap_3d(CUtensorMap* map, const void* base, const uint64_t dims[3],
                   const uint64_t strides_bytes[2], const uint32_t box[3],
                   CUtensorMapSwizzle swizzle);
+
+// bfloat16, 128-byte swizzle: box_inner is 64 elements.
+bool make_tmap_bf16(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer,
+                    uint64_t row_stride_bytes, uint32_t box_inner, uint32_t box_outer);
 
 int cuda_status(cudaError_t e);
 
