@@ -128,12 +128,9 @@ __global__ void __launch_bounds__(256) dpre_kernel(const Dpre p) {
         g[0] = pre[0];
         u[0] = pre[p.F];
       }
+      gate_grad(p.act, d, g, u);
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        float a, da;
-        act_grad(p.act, g[i], a, da);
-        g[i] = d[i] * u[i] * da;
-        u[i] = d[i] * a;
         sg[i] += g[i];
         su[i] += u[i];
       }
@@ -205,7 +202,9 @@ __global__ void __launch_bounds__(256) gate_kernel(const float* pre, T* h, int64
                                                    int act) {
   for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
     const int64_t m = i / F, f = i - m * F;
-    put(h + i, act_value(act, pre[m * 2 * F + f]) * pre[m * 2 * F + F + f]);
+    float g[1] = {pre[m * 2 * F + f]}, u[1] = {pre[m * 2 * F + F + f]};
+    gate(act, g, u);
+    put(h + i, g[0]);
   }
 }
 template <typename T>
@@ -213,12 +212,13 @@ __global__ void __launch_bounds__(256) bias_rows_kernel(const T* bias, float* pr
                                                         int F, int act) {
   for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
     const int64_t m = i / F, f = i - m * F;
-    const float g = bias ? to_f(bias[f]) : 0.0f, u = bias ? to_f(bias[F + f]) : 0.0f;
+    float g[1] = {bias ? to_f(bias[f]) : 0.0f}, u[1] = {bias ? to_f(bias[F + f]) : 0.0f};
     if (pre) {
-      pre[m * 2 * F + f] = g;
-      pre[m * 2 * F + F + f] = u;
+      pre[m * 2 * F + f] = g[0];
+      pre[m * 2 * F + F + f] = u[0];
     }
-    put(h + i, act_value(act, g) * u);
+    gate(act, g, u);
+    put(h + i, g[0]);
   }
 }
 

@@ -9,9 +9,9 @@
 // The tensor core truncates its accumulator at every MMA, about 2e-8 of the
 // result each and always towards zero (measured: a 3xTF32 product of K = 1024
 // left in one accumulator is off by 7e-6).  So a stage's six products go from
-// the smallest to the largest, only the last four MMAs meet the full
-// accumulator, and after every 64 of K the epilogue warps add the accumulator
-// to float32 registers with rounding.
+// the smallest to the largest, only the last two MMAs meet the full
+// accumulator, and after every stage, 32 of K, the epilogue warps add the
+// accumulator to float32 registers with rounding.
 //
 // CTA pairs (cta_group::2): a pair computes a 256 x 256 tile, each CTA holding
 // 128 rows of A, 128 columns of B and its 128 x 256 half of the accumulator:
@@ -24,8 +24,12 @@
 // Persistent, 320 threads: warp 0 one lane issues TMA loads (128-byte swizzle,
 // both operands in their stored layout, K- or MN-major) into a ring of stages;
 // warp 1 of the even CTA one lane issues the MMAs for the pair; warps 2-9 read
-// the accumulator (32 lanes x 32 columns at a time), transpose through padded
-// shared memory and store whole rows.  Two accumulators: a tile's epilogue runs
+// the accumulator (32 lanes x 32 columns at a time) and store each thread's 32
+// columns of a row in 32-byte pieces, whole sectors.  They stay off the shared
+// memory, which the MMAs' operand reads and the TMA writes fill between them: a
+// transpose there took the forward product of 8192 x 4096 x 2 x 8192 from 0.81
+// to 1.6 ms.  Only where rows are not 32-byte aligned do they transpose through
+// padded shared memory, to store whole rows of odd width.  Two accumulators: a tile's epilogue runs
 // beside the next tile's (three copies: the next stage's) MMAs.
 // Few tiles and a long K: the K range is split over the pairs, fp32 partial
 // tiles go to scratch and a second kernel adds them in order.
@@ -42,15 +46,17 @@ namespace {
 
 constexpr int kTile = 256;             // rows and columns of a pair's tile
 constexpr int kHalf = 128;             // ... of one CTA's operand tiles
-constexpr int kBK = 64;                // 128 bytes of bf16
-constexpr int kOpBytes = kHalf * kBK * 2;
 constexpr int kThreads = 320;
 constexpr int kTmemCols = 512;
 constexpr int kTrFloats = 32 * 33;     // a warp's transpose buffer
 
+// A stage is 64 of K, three copies 32 (with 64 only two stages fit, and a
+// stage's loads have no more than the other stage's MMAs to hide behind).
 template <int NC>
 struct Cfg {
-  static constexpr int kStages = NC == 3 ? 2 : 6;
+  static constexpr int kBK = NC == 3 ? 32 : 64;
+  static constexpr int kOpBytes = kHalf * kBK * 2;  // one operand tile
+  static constexpr int kStages = NC == 3 ? 4 : 6;
   static constexpr int kStageBytes = 2 * NC * kOpBytes;
   static constexpr int kSmem = kStages * kStageBytes + 8 * kTrFloats * 4 + 256 + 1024;
 };
@@ -74,6 +80,7 @@ struct Params {
   int tiles_m, tiles_n, tiles;
   int splits, kb_per;  // k-blocks of a split
   int act;
+  int vec;             // 32-byte stores: rows and halves start on 32 bytes
 };
 
 // Bands of 8 tiles of rows, column by column inside a band: the pairs that run
@@ -87,26 +94,53 @@ __device__ __forceinline__ void tile_at(const Params& p, int t, int& tm, int& tn
   tn = r / gm;
 }
 
-// A 128 x 64 tile of one copy: one box of 64 k x 128 rows, or two of 64 rows x
-// 64 k.
-template <bool KMAJOR>
+// A 128 x BK tile of one copy: one box of BK k x 128 rows, or two of 64 rows x
+// BK k.
+template <bool KMAJOR, int BK>
 __device__ __forceinline__ void load_tile(uint8_t* dst, const CUtensorMap* map, uint32_t bar,
                                           int r0, int k0) {
   if (KMAJOR) {
     tma_load_2d_pair(dst, map, bar, k0, r0);
   } else {
     tma_load_2d_pair(dst, map, bar, r0, k0);
-    tma_load_2d_pair(dst + kOpBytes / 2, map, bar, r0 + 64, k0);
+    tma_load_2d_pair(dst + kHalf * BK, map, bar, r0 + 64, k0);
   }
 }
 
-// The 16-deep slice j of a tile.  K-major: 128-byte rows, groups of 8 rows
-// 1024 bytes apart, a slice 32 bytes on.  MN-major: chunks of 64 columns 8 KB
-// apart, groups of 8 k 1024 bytes apart, a slice two groups on.
-template <bool KMAJOR>
+// The 16-deep slice j of a tile.  K-major: rows of 2 BK bytes (swizzled over
+// that), groups of 8 rows 16 BK bytes apart, a slice 32 bytes on.  MN-major:
+// chunks of 64 columns 128 BK bytes apart, groups of 8 k 1024 bytes apart, a
+// slice two groups on.
+template <bool KMAJOR, int BK>
 __device__ __forceinline__ uint64_t slice_desc(uint32_t addr, int j) {
-  return KMAJOR ? sdesc_kmajor(addr + j * 32, 1024, 2)
-                : sdesc_mnmajor(addr + j * 2048, kOpBytes / 2, 1024, 2);
+  return KMAJOR ? sdesc_kmajor(addr + j * 32, 16 * BK, BK == 64 ? 2 : 4)
+                : sdesc_mnmajor(addr + j * 2048, 128 * BK, 1024, 2);
+}
+
+// 32 consecutive values of a row, in 32-byte stores; `left` columns remain (a
+// multiple of a store's).
+__device__ __forceinline__ void store_row(float* p, const float (&v)[32], int left) {
+#pragma unroll
+  for (int i = 0; i < 32; i += 8)
+    if (i < left) {
+      uint32_t r[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) r[j] = __float_as_uint(v[i + j]);
+      st_global_32b(p + i, r);
+    }
+}
+__device__ __forceinline__ void store_row(__nv_bfloat16* p, const float (&v)[32], int left) {
+#pragma unroll
+  for (int i = 0; i < 32; i += 16)
+    if (i < left) {
+      uint32_t r[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(v[i + 2 * j], v[i + 2 * j + 1]);
+        r[j] = *reinterpret_cast<const uint32_t*>(&h);
+      }
+      st_global_32b(p + i, r);
+    }
 }
 
 template <int NC, bool AK, bool BKM, bool GATED>
@@ -114,6 +148,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     bf16_gemm_kernel(const __grid_constant__ Maps<NC> maps, const Params p) {
   using T = typename std::conditional<NC == 1, __nv_bfloat16, float>::type;
   using C = Cfg<NC>;
+  constexpr int kBK = C::kBK, kOpBytes = C::kOpBytes;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -184,8 +219,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           const uint32_t bar = cluster_addr(&full[stage], 0);
 #pragma unroll
           for (int i = 0; i < NC; ++i) {
-            load_tile<AK>(base + i * kOpBytes, &maps.a[i], bar, m0, kb * kBK);
-            load_tile<BKM>(base + (NC + i) * kOpBytes, &maps.b[rank][i], bar, n0, kb * kBK);
+            load_tile<AK, kBK>(base + i * kOpBytes, &maps.a[i], bar, m0, kb * kBK);
+            load_tile<BKM, kBK>(base + (NC + i) * kOpBytes, &maps.b[rank][i], bar, n0, kb * kBK);
           }
           if (++stage == C::kStages) {
             stage = 0;
@@ -241,8 +276,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           const uint32_t d = tmem_base + (seg & 1) * kTile;
           if (NC == 1) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              mma_f16_pair(d, slice_desc<AK>(sa, k), slice_desc<BKM>(sb, k), idesc, accumulate);
+            for (int k = 0; k < kBK / 16; ++k) {
+              mma_f16_pair(d, slice_desc<AK, kBK>(sa, k), slice_desc<BKM, kBK>(sb, k), idesc, accumulate);
               accumulate = 1;
             }
           } else {
@@ -251,9 +286,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int q = 0; q < 6; ++q)
 #pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                mma_f16_pair(d, slice_desc<AK>(sa + pa[q] * kOpBytes, k),
-                             slice_desc<BKM>(sb + pb[q] * kOpBytes, k), idesc, accumulate);
+              for (int k = 0; k < kBK / 16; ++k) {
+                mma_f16_pair(d, slice_desc<AK, kBK>(sa + pa[q] * kOpBytes, k),
+                             slice_desc<BKM, kBK>(sb + pb[q] * kOpBytes, k), idesc, accumulate);
                 accumulate = 1;
               }
           }
@@ -344,6 +379,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         ok = wait_acc();
       }
       if (!ok) break;
+      // block q of this warp, lane = row
       auto block = [&](int q, float (&v)[32]) {
         if (NC == 3) {
 #pragma unroll
@@ -354,62 +390,88 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
         }
-        turn(v);
       };
       if constexpr (GATED) {
-#pragma unroll
+        // (one copy: rolled, the registers are loaded inside)
+#pragma unroll(NC == 3 ? 2 : 1)
         for (int q = 0; q < 4; q += 2) {
-          const int col = tn * kHalf + half * 64 + (q >> 1) * 32 + lane;
-          const bool in = col < p.N;
+          const int col0 = tn * kHalf + half * 64 + (q >> 1) * 32;
           float g[32], u[32];
           block(q, g);
           block(q + 1, u);
-          if (p.parts) {
-            float* dst = p.parts + (static_cast<int64_t>(split) * p.M + row0) * 2 * p.N + col;
+          const int64_t ld2 = 2ll * p.N;
+          float* pre = p.parts ? p.parts + static_cast<int64_t>(split) * p.M * ld2 : p.pre;
+          T* h = static_cast<T*>(p.out);
+          if (p.vec) {
+            const int64_t row = row0 + lane;
+            if (lane >= rows || col0 >= p.N) continue;
+            if (p.bias && !p.parts) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (in && i < rows) {
-                dst[static_cast<int64_t>(i) * 2 * p.N] = g[i];
-                dst[static_cast<int64_t>(i) * 2 * p.N + p.N] = u[i];
-              }
-            continue;
-          }
-          float bg = 0.0f, bu = 0.0f;
-          if (p.bias && in) {
-            bg = to_f(static_cast<const T*>(p.bias)[col]);
-            bu = to_f(static_cast<const T*>(p.bias)[p.N + col]);
-          }
-          T* h = static_cast<T*>(p.out) + static_cast<int64_t>(row0) * p.ldc + col;
-          float* pre = p.pre ? p.pre + static_cast<int64_t>(row0) * 2 * p.N + col : nullptr;
+              for (int i = 0; i < 32; ++i)
+                if (col0 + i < p.N) {
+                  g[i] += to_f(static_cast<const T*>(p.bias)[col0 + i]);
+                  u[i] += to_f(static_cast<const T*>(p.bias)[p.N + col0 + i]);
+                }
+            }
+            if (pre) {
+              store_row(pre + row * ld2 + col0, g, p.N - col0);
+              store_row(pre + row * ld2 + p.N + col0, u, p.N - col0);
+            }
+            if (!p.parts) {
+              gate(p.act, g, u);
+              store_row(h + row * p.ldc + col0, g, p.N - col0);
+            }
+          } else {
+            turn(g);
+            turn(u);
+            const int col = col0 + lane;
+            const bool in = col < p.N;
+            float bg = 0.0f, bu = 0.0f;
+            if (p.bias && in && !p.parts) {
+              bg = to_f(static_cast<const T*>(p.bias)[col]);
+              bu = to_f(static_cast<const T*>(p.bias)[p.N + col]);
+            }
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (in && i < rows) {
+            for (int i = 0; i < 32; ++i) {
+              const int64_t row = row0 + i;
               g[i] += bg;
               u[i] += bu;
-              if (pre) {
-                pre[static_cast<int64_t>(i) * 2 * p.N] = g[i];
-                pre[static_cast<int64_t>(i) * 2 * p.N + p.N] = u[i];
+              if (pre && in && i < rows) {
+                pre[row * ld2 + col] = g[i];
+                pre[row * ld2 + p.N + col] = u[i];
               }
-              put(h + static_cast<int64_t>(i) * p.ldc, act_value(p.act, g[i]) * u[i]);
             }
+            if (!p.parts) {
+              gate(p.act, g, u);
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (in && i < rows) put(h + (row0 + i) * p.ldc + col, g[i]);
+            }
+          }
         }
       } else {
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const int col = tn * kTile + col_of(q) + lane;
-          const bool in = col < p.N;
+          const int col0 = tn * kTile + col_of(q);
           float v[32];
           block(q, v);
-          if (p.parts) {
-            float* dst = p.parts + (static_cast<int64_t>(split) * p.M + row0) * p.N + col;
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (in && i < rows) dst[static_cast<int64_t>(i) * p.N] = v[i];
+          float* part = p.parts ? p.parts + static_cast<int64_t>(split) * p.M * p.N : nullptr;
+          T* out = static_cast<T*>(p.out);
+          if (p.vec) {
+            const int64_t row = row0 + lane;
+            if (lane >= rows || col0 >= p.N) continue;
+            if (part) store_row(part + row * p.N + col0, v, p.N - col0);
+            else store_row(out + row * p.ldc + col0, v, p.N - col0);
           } else {
-            T* dst = static_cast<T*>(p.out) + static_cast<int64_t>(row0) * p.ldc + col;
+            turn(v);
+            const int col = col0 + lane;
 #pragma unroll
             for (int i = 0; i < 32; ++i)
-              if (in && i < rows) put(dst + static_cast<int64_t>(i) * p.ldc, v[i]);
+              if (col < p.N && i < rows) {
+                const int64_t row = row0 + i;
+                if (part) part[row * p.N + col] = v[i];
+                else put(out + row * p.ldc + col, v[i]);
+              }
           }
         }
       }
@@ -447,7 +509,9 @@ __global__ void __launch_bounds__(256) join_kernel(const Params p) {
         p.pre[m * width + c] = g;
         p.pre[m * width + p.N + c] = u;
       }
-      g = act_value(p.act, g) * u;
+      float ga[1] = {g}, ua[1] = {u};
+      gate(p.act, ga, ua);
+      g = ga[0];
     }
     put(static_cast<T*>(p.out) + m * p.ldc + c, g);
   }
@@ -462,11 +526,12 @@ Plan plan_of(const Context* ctx, int M, int N, int K, bool gated, int copies) {
   q.tiles_m = (M + kTile - 1) / kTile;
   q.tiles_n = (N + width - 1) / width;
   q.tiles = q.tiles_m * q.tiles_n;
-  const int num_kb = std::max(1, (K + kBK - 1) / kBK);
+  const int bk = copies == 3 ? Cfg<3>::kBK : Cfg<1>::kBK;
+  const int num_kb = std::max(1, (K + bk - 1) / bk);
   const int pairs = std::max(1, ctx->tc_sms() / 2);
   // Split K when whole tiles leave more than half of the pairs idle, into
   // pieces of at least 512 of K (three copies: 128, six times the work).
-  const int least = copies == 3 ? 2 : 8;
+  const int least = copies == 3 ? 4 : 8;
   q.splits = 1;
   if (2 * q.tiles <= pairs) q.splits = std::max(1, std::min(pairs / q.tiles, num_kb / least));
   q.kb_per = (num_kb + q.splits - 1) / q.splits;
@@ -475,21 +540,22 @@ Plan plan_of(const Context* ctx, int M, int N, int K, bool gated, int copies) {
   return q;
 }
 
-bool operand_map(CUtensorMap* m, const Bf16Operand& o, int copy, int rows, int K) {
+bool operand_map(CUtensorMap* m, const Bf16Operand& o, int copy, int rows, int K, int bk) {
   const void* base = static_cast<const __nv_bfloat16*>(o.base) + copy * o.copy;
-  return o.kmajor ? make_tmap_bf16(m, base, K, rows, o.ld * 2, kBK, kHalf)
-                  : make_tmap_bf16(m, base, rows, K, o.ld * 2, 64, kBK);
+  return o.kmajor ? make_tmap_bf16(m, base, K, rows, o.ld * 2, bk, kHalf)
+                  : make_tmap_bf16(m, base, rows, K, o.ld * 2, 64, bk);
 }
 
 template <int NC, bool AK, bool BKM, bool GATED>
 int launch(Context* ctx, const Bf16Gemm& g, cudaStream_t s) {
   using T = typename std::conditional<NC == 1, __nv_bfloat16, float>::type;
   const Plan q = plan_of(ctx, g.M, g.N, g.K, GATED, NC);
+  constexpr int bk = Cfg<NC>::kBK;
   Maps<NC> maps;
   for (int i = 0; i < NC; ++i)
-    if (!operand_map(&maps.a[i], g.a, i, g.M, g.K) ||
-        !operand_map(&maps.b[0][i], g.b, i, g.N, g.K) ||
-        !operand_map(&maps.b[1][i], GATED ? g.b2 : g.b, i, g.N, g.K))
+    if (!operand_map(&maps.a[i], g.a, i, g.M, g.K, bk) ||
+        !operand_map(&maps.b[0][i], g.b, i, g.N, g.K, bk) ||
+        !operand_map(&maps.b[1][i], GATED ? g.b2 : g.b, i, g.N, g.K, bk))
       return kErrUnsupported;
   Params p{};
   p.out = g.out;
@@ -504,6 +570,9 @@ int launch(Context* ctx, const Bf16Gemm& g, cudaStream_t s) {
   p.splits = q.splits; p.kb_per = q.kb_per;
   p.act = g.act;
   if (q.splits > 1 && !g.parts) return kErrInvalid;
+  auto on32 = [](const void* a) { return (reinterpret_cast<uintptr_t>(a) & 31u) == 0; };
+  p.vec = g.N % (32 / sizeof(T)) == 0 && g.ldc % (32 / sizeof(T)) == 0 && on32(g.out) &&
+          on32(g.pre) && on32(p.parts);
   auto kern = bf16_gemm_kernel<NC, AK, BKM, GATED>;
   static SmemOptIn opt_in;
   cudaError_t e = opt_in.ensure(kern, Cfg<NC>::kSmem);

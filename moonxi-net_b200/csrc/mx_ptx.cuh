@@ -247,6 +247,13 @@ __host__ __device__ constexpr uint32_t idesc_tf32(int m, int n, bool a_mn = fals
          | (static_cast<uint32_t>(m >> 4) << 24);    // M / 16
 }
 
+// 32 bytes to a 32-byte aligned address: a whole sector from one thread.
+__device__ __forceinline__ void st_global_32b(void* p, const uint32_t (&r)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(r[0]),
+               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+
 // ------------------------------------------------- CTA pairs (cta_group::2)
 // Two CTAs of a cluster work on one tile: each holds half of A's rows and half
 // of B's columns in its shared memory and half of the accumulator's rows in

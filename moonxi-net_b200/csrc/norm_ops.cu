@@ -38,7 +38,7 @@ __device__ __forceinline__ void load_vec(const T* p, float (&v)[V]) {
   if constexpr (V == 1) {
     v[0] = to_f(*p);
   } else {
-    const uint4 raw = __ldg(reinterpret_cast<const uint4*>(p));
+    const uint4 raw = *reinterpret_cast<const uint4*>(p);
     if constexpr (sizeof(T) == 4) {
       v[0] = __uint_as_float(raw.x); v[1] = __uint_as_float(raw.y);
       v[2] = __uint_as_float(raw.z); v[3] = __uint_as_float(raw.w);
@@ -85,31 +85,59 @@ __device__ __forceinline__ void load_par(const float* p, int c, float (&v)[V], f
   }
 }
 
-// Sums of N values over the TPR threads of a row, given to all of them.  The
-// order is fixed.  TPR = 32: the row is a warp's.  Otherwise the block's, and
-// `buf` holds N floats a warp.
+// Sums of N values over the TPR threads of a row, given to all of them, in a
+// fixed order.  TPR = 32: the row is a warp's.  Otherwise the block's: `buf`
+// holds two sets of N floats a warp, used in turn, so that one barrier a sum is
+// enough (whoever writes a set again has passed the barrier of the sum between,
+// which its readers reach after reading).
 template <int TPR, int N>
-__device__ __forceinline__ void row_sum(float (&s)[N], float* buf) {
+__device__ __forceinline__ void row_sum(float (&s)[N], float* buf, int& turn) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1)
 #pragma unroll
     for (int i = 0; i < N; ++i) s[i] += __shfl_xor_sync(0xffffffffu, s[i], o);
   if constexpr (TPR > 32) {
     constexpr int W = TPR / 32;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    __syncthreads();  // the last sum's readers are done
-    if (lane == 0)
+    float* b = buf + turn * N * W;
+    turn ^= 1;
+    if ((threadIdx.x & 31) == 0)
 #pragma unroll
-      for (int i = 0; i < N; ++i) buf[i * W + warp] = s[i];
+      for (int i = 0; i < N; ++i) b[i * W + (threadIdx.x >> 5)] = s[i];
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      float t = lane < W ? buf[i * W + lane] : 0.0f;
+      float t = 0.0f;
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+      for (int w = 0; w < W; w += 4) {
+        const float4 q = *reinterpret_cast<const float4*>(b + i * W + w);
+        t += (q.x + q.y) + (q.z + q.w);
+      }
       s[i] = t;
     }
   }
+}
+
+// Rows in flight of a block: a thread copies its own 16-byte pieces of the next
+// rows to its own places in shared memory (no other thread reads them, so no
+// barrier), and takes them into registers when their turn comes.
+constexpr int kRingBytes = 200 * 1024;  // of an SM, over its blocks
+__host__ __device__ constexpr int block_threads(int tpr) { return tpr == 32 ? 128 : tpr; }
+// 1024 threads an SM, 64 registers each.
+__host__ __device__ constexpr int blocks_per_sm(int tpr) {
+  return 1024 / block_threads(tpr);
+}
+__host__ __device__ constexpr int ring_rows(int tpr, int e, int size, int tensors) {
+  const int d = kRingBytes / blocks_per_sm(tpr) / (block_threads(tpr) * e * size * tensors);
+  return d < 1 ? 1 : d > 4 ? 4 : d;
+}
+__host__ __device__ constexpr int ring_bytes(int tpr, int e, int size, int tensors, int v) {
+  return v == 1 ? 0 : ring_rows(tpr, e, size, tensors) * block_threads(tpr) * e * size * tensors;
+}
+__device__ __forceinline__ void copy16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                   static_cast<uint32_t>(__cvta_generic_to_shared(dst))),
+               "l"(src)
+               : "memory");
 }
 
 struct NormFwd {
@@ -125,61 +153,92 @@ struct NormFwd {
 };
 
 // Rows of up to TPR * E values, in registers: a thread holds E / V groups of V
-// consecutive columns.  TPR = 32: four rows a block, one a warp.
+// consecutive columns.  A block takes rows blockIdx.x, + gridDim.x, ...
+// (TPR = 32: four at a time, one a warp).
 template <typename T, int TPR, int E, int V>
-__global__ void __launch_bounds__(TPR == 32 ? 128 : TPR) norm_fwd_kernel(const NormFwd p) {
-  constexpr int NV = E / V;
-  __shared__ float buf[TPR > 32 ? 2 * TPR / 32 : 1];
+__global__ void __launch_bounds__(block_threads(TPR), blocks_per_sm(TPR)) norm_fwd_kernel(const NormFwd p) {
+  constexpr int NV = E / V, D = ring_rows(TPR, E, sizeof(T), 1), BLOCK = block_threads(TPR);
+  extern __shared__ uint4 ring[];  // [D][NV][BLOCK]
+  __shared__ __align__(16) float buf[TPR > 32 ? 2 * 2 * TPR / 32 : 1];
   const int t = TPR == 32 ? threadIdx.x & 31 : threadIdx.x;
-  const int64_t row = TPR == 32 ? blockIdx.x * 4ll + (threadIdx.x >> 5) : blockIdx.x;
-  if (row >= p.rows) return;
-  const T* x = static_cast<const T*>(p.x) + row * p.ldx;
-  float v[NV][V];
-  float s[1] = {0.0f};
+  const int64_t step = TPR == 32 ? gridDim.x * 4ll : gridDim.x;
+  int64_t row = TPR == 32 ? blockIdx.x * 4ll + (threadIdx.x >> 5) : blockIdx.x;
+  const float n = static_cast<float>(p.cols);
+  auto fetch = [&](int64_t r, int slot) {
+    if constexpr (V > 1) {
+      if (r < p.rows) {
+        const T* x = static_cast<const T*>(p.x) + r * p.ldx;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          const int c = (i * TPR + t) * V;
+          if (c < p.cols) copy16(ring + (slot * NV + i) * BLOCK + threadIdx.x, x + c);
+        }
+      }
+      cp_async_commit();
+    }
+  };
+#pragma unroll
+  for (int d = 0; d < D; ++d) fetch(row + d * step, d);
+  float w[NV][V], b[NV][V];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int c = (i * TPR + t) * V;
     if (c < p.cols) {
-      load_vec<T, V>(x + c, v[i]);
-#pragma unroll
-      for (int j = 0; j < V; ++j) s[0] += v[i][j];
+      load_par<V>(p.w, c, w[i], 1.0f);
+      load_par<V>(p.b, c, b[i], 0.0f);
     }
   }
-  row_sum<TPR>(s, buf);
-  const float n = static_cast<float>(p.cols);
-  const float mean = s[0] / n;
-  // The centred values' own mean is what rounding left of it: it is taken off
-  // the values and off the variance, so a mean far above the deviation costs
-  // no more than the rounding of x itself.
-  float q[2] = {0.0f, 0.0f};
+  int slot = 0, turn = 0;
+  for (; row < p.rows; row += step) {
+    float v[NV][V];
+    float s[1] = {0.0f};
+    if constexpr (V > 1) cp_async_wait<D - 1>();
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
-    if ((i * TPR + t) * V < p.cols)
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * TPR + t) * V;
+      if (c < p.cols) {
+        if constexpr (V > 1)
+          load_vec<T, V>(reinterpret_cast<const T*>(ring + (slot * NV + i) * BLOCK + threadIdx.x), v[i]);
+        else
+          load_vec<T, V>(static_cast<const T*>(p.x) + row * p.ldx + c, v[i]);
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        v[i][j] -= mean;
-        q[0] += v[i][j];
-        q[1] += v[i][j] * v[i][j];
+        for (int j = 0; j < V; ++j) s[0] += v[i][j];
       }
-  row_sum<TPR>(q, buf);
-  const float rest = q[0] / n;
-  const float var = q[1] / n - rest * rest;
-  const float rstd = 1.0f / sqrtf((var < 0.0f ? 0.0f : var) + p.eps);  // NaN stays NaN
-  if (t == 0) {
-    if (p.mean) p.mean[row] = mean + rest;
-    if (p.rstd) p.rstd[row] = rstd;
-  }
-  T* y = static_cast<T*>(p.y) + row * p.ldy;
+    }
+    fetch(row + D * step, slot);
+    slot = slot + 1 == D ? 0 : slot + 1;
+    row_sum<TPR>(s, buf, turn);
+    const float mean = s[0] / n;
+    // The centred values' own mean is what rounding left of it: it is taken off
+    // the values and off the variance, so a mean far above the deviation costs
+    // no more than the rounding of x itself.
+    float q[2] = {0.0f, 0.0f};
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int c = (i * TPR + t) * V;
-    if (c < p.cols) {
-      float w[V], b[V];
-      load_par<V>(p.w, c, w, 1.0f);
-      load_par<V>(p.b, c, b, 0.0f);
+    for (int i = 0; i < NV; ++i)
+      if ((i * TPR + t) * V < p.cols)
 #pragma unroll
-      for (int j = 0; j < V; ++j) v[i][j] = (v[i][j] - rest) * rstd * w[j] + b[j];
-      store_vec<T, V>(y + c, v[i]);
+        for (int j = 0; j < V; ++j) {
+          v[i][j] -= mean;
+          q[0] += v[i][j];
+          q[1] += v[i][j] * v[i][j];
+        }
+    row_sum<TPR>(q, buf, turn);
+    const float rest = q[0] / n;
+    const float var = q[1] / n - rest * rest;
+    const float rstd = 1.0f / sqrtf((var < 0.0f ? 0.0f : var) + p.eps);  // NaN stays NaN
+    if (t == 0) {
+      if (p.mean) p.mean[row] = mean + rest;
+      if (p.rstd) p.rstd[row] = rstd;
+    }
+    T* y = static_cast<T*>(p.y) + row * p.ldy;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * TPR + t) * V;
+      if (c < p.cols) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[i][j] = (v[i][j] - rest) * rstd * w[i][j] + b[i][j];
+        store_vec<T, V>(y + c, v[i]);
+      }
     }
   }
 }
@@ -188,12 +247,13 @@ __global__ void __launch_bounds__(TPR == 32 ? 128 : TPR) norm_fwd_kernel(const N
 // the second and third from the caches.
 template <typename T>
 __global__ void __launch_bounds__(1024) norm_fwd_long_kernel(const NormFwd p) {
-  __shared__ float buf[2 * 32];
+  __shared__ __align__(16) float buf[2 * 2 * 32];
+  int turn = 0;
   const int64_t row = blockIdx.x;
   const T* x = static_cast<const T*>(p.x) + row * p.ldx;
   float s[1] = {0.0f};
   for (int c = threadIdx.x; c < p.cols; c += 1024) s[0] += to_f(x[c]);
-  row_sum<1024>(s, buf);
+  row_sum<1024>(s, buf, turn);
   const float mean = s[0] / static_cast<float>(p.cols);
   float q[2] = {0.0f, 0.0f};
   for (int c = threadIdx.x; c < p.cols; c += 1024) {
@@ -201,7 +261,7 @@ __global__ void __launch_bounds__(1024) norm_fwd_long_kernel(const NormFwd p) {
     q[0] += d;
     q[1] += d * d;
   }
-  row_sum<1024>(q, buf);
+  row_sum<1024>(q, buf, turn);
   const float n = static_cast<float>(p.cols), rest = q[0] / n;
   const float var = q[1] / n - rest * rest;
   const float rstd = 1.0f / sqrtf((var < 0.0f ? 0.0f : var) + p.eps);  // NaN stays NaN
@@ -226,12 +286,13 @@ struct NormBwd {
   int rows, cols;
 };
 
-// A block takes rows blockIdx.x, + gridDim.x, ... (TPR = 32: four at a time,
-// one a warp, whose sums meet in shared memory at the end).
+// Rows as in norm_fwd_kernel; TPR = 32: the four warps' sums meet in shared
+// memory at the end.
 template <typename T, int TPR, int E, int V>
-__global__ void __launch_bounds__(TPR == 32 ? 128 : TPR) norm_bwd_kernel(const NormBwd p) {
-  constexpr int NV = E / V;
-  __shared__ float buf[TPR > 32 ? 2 * TPR / 32 : 4 * 32 * E];
+__global__ void __launch_bounds__(block_threads(TPR), blocks_per_sm(TPR)) norm_bwd_kernel(const NormBwd p) {
+  constexpr int NV = E / V, D = ring_rows(TPR, E, sizeof(T), 2), BLOCK = block_threads(TPR);
+  extern __shared__ uint4 ring[];  // [D][2][NV][BLOCK]
+  __shared__ __align__(16) float buf[TPR > 32 ? 2 * 2 * TPR / 32 : 4 * 32 * E];
   const int t = TPR == 32 ? threadIdx.x & 31 : threadIdx.x;
   const int warp = threadIdx.x >> 5;
   const float inv_c = 1.0f / static_cast<float>(p.cols);
@@ -244,20 +305,47 @@ __global__ void __launch_bounds__(TPR == 32 ? 128 : TPR) norm_bwd_kernel(const N
     if (c < p.cols) load_par<V>(p.w, c, w[i], 1.0f);
   }
   const int64_t step = TPR == 32 ? gridDim.x * 4ll : gridDim.x;
-  for (int64_t row = TPR == 32 ? blockIdx.x * 4ll + warp : blockIdx.x; row < p.rows; row += step) {
-    const T* x = static_cast<const T*>(p.x) + row * p.ldx;
-    const T* dy = static_cast<const T*>(p.dy) + row * p.lddy;
+  int64_t row = TPR == 32 ? blockIdx.x * 4ll + warp : blockIdx.x;
+  auto fetch = [&](int64_t r, int slot) {
+    if constexpr (V > 1) {
+      if (r < p.rows) {
+        const T* x = static_cast<const T*>(p.x) + r * p.ldx;
+        const T* dy = static_cast<const T*>(p.dy) + r * p.lddy;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          const int c = (i * TPR + t) * V;
+          if (c < p.cols) {
+            copy16(ring + (slot * 2 * NV + i) * BLOCK + threadIdx.x, x + c);
+            copy16(ring + (slot * 2 * NV + NV + i) * BLOCK + threadIdx.x, dy + c);
+          }
+        }
+      }
+      cp_async_commit();
+    }
+  };
+#pragma unroll
+  for (int d = 0; d < D; ++d) fetch(row + d * step, d);
+  int slot = 0, turn = 0;
+  for (; row < p.rows; row += step) {
     const float mean = __ldg(p.mean + row), rstd = __ldg(p.rstd + row);
     float xh[NV][V], a[NV][V];
     float s[2] = {0.0f, 0.0f};
+    if constexpr (V > 1) cp_async_wait<D - 1>();
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = (i * TPR + t) * V;
       if (c < p.cols) {
-        load_vec<T, V>(x + c, xh[i]);
-        load_vec<T, V>(dy + c, a[i]);
+        if constexpr (V > 1) {
+          load_vec<T, V>(reinterpret_cast<const T*>(ring + (slot * 2 * NV + i) * BLOCK + threadIdx.x), xh[i]);
+          load_vec<T, V>(reinterpret_cast<const T*>(ring + (slot * 2 * NV + NV + i) * BLOCK + threadIdx.x), a[i]);
+        } else {
+          load_vec<T, V>(static_cast<const T*>(p.x) + row * p.ldx + c, xh[i]);
+          load_vec<T, V>(static_cast<const T*>(p.dy) + row * p.lddy + c, a[i]);
+        }
       }
     }
+    fetch(row + D * step, slot);
+    slot = slot + 1 == D ? 0 : slot + 1;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
       if ((i * TPR + t) * V < p.cols)
@@ -270,7 +358,7 @@ __global__ void __launch_bounds__(TPR == 32 ? 128 : TPR) norm_bwd_kernel(const N
           s[0] += a[i][j];
           s[1] += a[i][j] * xh[i][j];
         }
-    row_sum<TPR>(s, buf);
+    row_sum<TPR>(s, buf, turn);
     const float c1 = s[0] * inv_c, c2 = s[1] * inv_c;
     if (p.dx) {
       T* dx = static_cast<T*>(p.dx) + row * p.lddx;
@@ -319,7 +407,8 @@ __global__ void __launch_bounds__(TPR == 32 ? 128 : TPR) norm_bwd_kernel(const N
 // their own (norm_cols_kernel), since no block holds a row's columns.
 template <typename T>
 __global__ void __launch_bounds__(1024) norm_bwd_long_kernel(const NormBwd p) {
-  __shared__ float buf[2 * 32];
+  __shared__ __align__(16) float buf[2 * 2 * 32];
+  int turn = 0;
   const int64_t row = blockIdx.x;
   const T* x = static_cast<const T*>(p.x) + row * p.ldx;
   const T* dy = static_cast<const T*>(p.dy) + row * p.lddy;
@@ -331,7 +420,7 @@ __global__ void __launch_bounds__(1024) norm_bwd_long_kernel(const NormBwd p) {
     s[0] += a;
     s[1] += a * ((to_f(x[c]) - mean) * rstd);
   }
-  row_sum<1024>(s, buf);
+  row_sum<1024>(s, buf, turn);
   const float inv_c = 1.0f / static_cast<float>(p.cols);
   const float c1 = s[0] * inv_c, c2 = s[1] * inv_c;
   for (int c = threadIdx.x; c < p.cols; c += 1024) {
@@ -393,37 +482,60 @@ __global__ void __launch_bounds__(256) norm_finish_kernel(const float* __restric
 // Columns up to which a row is held in registers.
 constexpr int kNormRegCols = 16384;
 
-template <typename T, int V>
-cudaError_t launch_fwd(const NormFwd& p, cudaStream_t s) {
-  const int c = p.cols;
-  if (c <= 256) norm_fwd_kernel<T, 32, 8, V><<<(p.rows + 3) / 4, 128, 0, s>>>(p);
-  else if (c <= 1024) norm_fwd_kernel<T, 32, 32, V><<<(p.rows + 3) / 4, 128, 0, s>>>(p);
-  else if (c <= 2048) norm_fwd_kernel<T, 128, 16, V><<<p.rows, 128, 0, s>>>(p);
-  else if (c <= 4096) norm_fwd_kernel<T, 256, 16, V><<<p.rows, 256, 0, s>>>(p);
-  else if (c <= 8192) norm_fwd_kernel<T, 512, 16, V><<<p.rows, 512, 0, s>>>(p);
-  else norm_fwd_kernel<T, 1024, 16, V><<<p.rows, 1024, 0, s>>>(p);
-  return cudaGetLastError();
+// Blocks of a pass over rows: as many as fit on the SMs at a time.
+int row_blocks(int rows, int cols, int per_sm, int num_sms) {
+  const int at_once = cols <= 256 ? 4 : 1;  // rows of a block
+  return std::max(1, std::min(per_sm * num_sms, (rows + at_once - 1) / at_once));
 }
 
+template <typename T, int TPR, int E, int V>
+cudaError_t run_fwd(const NormFwd& p, int num_sms, cudaStream_t s) {
+  constexpr int kBytes = ring_bytes(TPR, E, sizeof(T), 1, V);
+  auto kern = norm_fwd_kernel<T, TPR, E, V>;
+  static SmemOptIn opt_in;
+  cudaError_t e = kBytes > 32768 ? opt_in.ensure(kern, kBytes) : cudaSuccess;
+  if (e != cudaSuccess) return e;
+  kern<<<row_blocks(p.rows, p.cols, blocks_per_sm(TPR), num_sms), block_threads(TPR), kBytes,
+         s>>>(p);
+  return cudaGetLastError();
+}
+template <typename T, int V>
+cudaError_t launch_fwd(const NormFwd& p, int num_sms, cudaStream_t s) {
+  const int c = p.cols;
+  if (c <= 256) return run_fwd<T, 32, 8, V>(p, num_sms, s);
+  if (c <= 1024) return run_fwd<T, 128, 8, V>(p, num_sms, s);
+  if (c <= 2048) return run_fwd<T, 256, 8, V>(p, num_sms, s);
+  if (c <= 4096) return run_fwd<T, 512, 8, V>(p, num_sms, s);
+  if (c <= 8192) return run_fwd<T, 1024, 8, V>(p, num_sms, s);
+  return run_fwd<T, 1024, 16, V>(p, num_sms, s);
+}
+
+template <typename T, int TPR, int E, int V>
+cudaError_t run_bwd(const NormBwd& p, int blocks, cudaStream_t s) {
+  constexpr int kBytes = ring_bytes(TPR, E, sizeof(T), 2, V);
+  auto kern = norm_bwd_kernel<T, TPR, E, V>;
+  static SmemOptIn opt_in;
+  cudaError_t e = kBytes > 32768 ? opt_in.ensure(kern, kBytes) : cudaSuccess;
+  if (e != cudaSuccess) return e;
+  kern<<<blocks, block_threads(TPR), kBytes, s>>>(p);
+  return cudaGetLastError();
+}
 template <typename T, int V>
 cudaError_t launch_bwd(const NormBwd& p, int blocks, cudaStream_t s) {
   const int c = p.cols;
-  if (c <= 256) norm_bwd_kernel<T, 32, 8, V><<<blocks, 128, 0, s>>>(p);
-  else if (c <= 1024) norm_bwd_kernel<T, 32, 32, V><<<blocks, 128, 0, s>>>(p);
-  else if (c <= 2048) norm_bwd_kernel<T, 128, 16, V><<<blocks, 128, 0, s>>>(p);
-  else if (c <= 4096) norm_bwd_kernel<T, 256, 16, V><<<blocks, 256, 0, s>>>(p);
-  else if (c <= 8192) norm_bwd_kernel<T, 512, 16, V><<<blocks, 512, 0, s>>>(p);
-  else norm_bwd_kernel<T, 1024, 16, V><<<blocks, 1024, 0, s>>>(p);
-  return cudaGetLastError();
+  if (c <= 256) return run_bwd<T, 32, 8, V>(p, blocks, s);
+  if (c <= 1024) return run_bwd<T, 128, 8, V>(p, blocks, s);
+  if (c <= 2048) return run_bwd<T, 256, 8, V>(p, blocks, s);
+  if (c <= 4096) return run_bwd<T, 512, 8, V>(p, blocks, s);
+  if (c <= 8192) return run_bwd<T, 1024, 8, V>(p, blocks, s);
+  return run_bwd<T, 1024, 16, V>(p, blocks, s);
 }
 
 // Blocks of the backward pass (rows of partial sums).
 int bwd_blocks(int rows, int cols, int num_sms) {
   if (cols > kNormRegCols) return std::min(64, (rows + 63) / 64);  // row ranges of norm_cols
-  const int threads = cols <= 2048 ? 128 : cols <= 4096 ? 256 : cols <= 8192 ? 512 : 1024;
-  const int per_block = cols <= 1024 ? 4 : 1;  // rows at a time
-  const int fit = std::max(1, 512 / threads) * num_sms;
-  return std::max(1, std::min(fit, (rows + 2 * per_block - 1) / (2 * per_block)));
+  const int tpr = cols <= 1024 ? 128 : cols <= 2048 ? 256 : cols <= 4096 ? 512 : 1024;
+  return row_blocks((rows + 1) / 2, cols, blocks_per_sm(tpr), num_sms);
 }
 
 bool aligned16(const void* a) { return (reinterpret_cast<uintptr_t>(a) & 15u) == 0; }
@@ -438,8 +550,8 @@ size_t layer_norm_bwd_scratch_bytes(const Context* ctx, int rows, int cols) {
 int layer_norm_fwd(Context* ctx, int dtype, const void* x, int64_t ldx, const float* w,
                    const float* b, void* y, int64_t ldy, float* mean, float* rstd, int rows,
                    int cols, float eps, cudaStream_t s) {
-  (void)ctx;
   if (rows <= 0) return kOk;
+  const int n = ctx->num_sms;
   const NormFwd p{x, w, b, y, mean, rstd, ldx, ldy, rows, cols, eps};
   const int vec = dtype == MX_BF16 ? 8 : 4;
   const bool v16 = cols % vec == 0 && ldx % vec == 0 && ldy % vec == 0 && aligned16(x) &&
@@ -450,9 +562,9 @@ int layer_norm_fwd(Context* ctx, int dtype, const void* x, int64_t ldx, const fl
     else norm_fwd_long_kernel<float><<<rows, 1024, 0, s>>>(p);
     e = cudaGetLastError();
   } else if (dtype == MX_BF16) {
-    e = v16 ? launch_fwd<__nv_bfloat16, 8>(p, s) : launch_fwd<__nv_bfloat16, 1>(p, s);
+    e = v16 ? launch_fwd<__nv_bfloat16, 8>(p, n, s) : launch_fwd<__nv_bfloat16, 1>(p, n, s);
   } else {
-    e = v16 ? launch_fwd<float, 4>(p, s) : launch_fwd<float, 1>(p, s);
+    e = v16 ? launch_fwd<float, 4>(p, n, s) : launch_fwd<float, 1>(p, n, s);
   }
   note_launches(1);
   return cuda_status(e);

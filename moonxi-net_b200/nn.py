@@ -785,10 +785,11 @@ class AdamW:
         if state_bits not in (8, 32):
             raise ValueError(f"state_bits must be 8 or 32, got {state_bits}")
         n = len(self.params)
-        first = self.params[0]
+        ops._check_type(self.params[0], "params[0]")
+        self.device = self.params[0].device
+        self._dev = dev = self.params[0].get_device()
         for i, p in enumerate(self.params):
-            ops._check_like(p, f"params[{i}]", first, torch.float32)
-        self.device = first.device
+            ops._check_like(p, f"params[{i}]", dev, torch.float32)
         self.copies = [None] * n if copies is None else list(copies)
         decay = [float(weight_decay)] * n if not isinstance(weight_decay, (list, tuple)) \
             else [float(d) for d in weight_decay]
@@ -796,7 +797,7 @@ class AdamW:
             raise ValueError("copies, weight_decay and state need one entry for each tensor")
         for i, (c, p) in enumerate(zip(self.copies, self.params)):
             if c is not None:
-                ops._check_like(c, f"copies[{i}]", first, torch.bfloat16, p.shape)
+                ops._check_like(c, f"copies[{i}]", dev, torch.bfloat16, p.shape)
         self.lr, self.betas, self.eps = float(lr), (float(betas[0]), float(betas[1])), float(eps)
         self.max_grad_norm, self.state_bits = float(max_grad_norm), int(state_bits)
         self.ctx = ctx
@@ -836,7 +837,7 @@ class AdamW:
             if len(s) != len(names):
                 raise ValueError(f"state[{i}] needs {names}")
             for x, name, dtype in zip(s, names, types):
-                ops._check_like(x, f"state[{i}].{name}", p, dtype)
+                ops._check_like(x, f"state[{i}].{name}", self._dev, dtype)
                 k = -(-p.numel() // 256) if name.endswith("scale") else p.numel()
                 if x.numel() != k:
                     raise ValueError(f"state[{i}].{name} has {x.numel()} elements, needs {k}")
@@ -845,17 +846,17 @@ class AdamW:
         """One update from `grads`, a tensor for each parameter."""
         if len(grads) != len(self.params):
             raise ValueError(f"{len(grads)} gradients for {len(self.params)} tensors")
-        for i, (t, g, p) in enumerate(zip(self._table, grads, self.params)):
+        for i, (t, g) in enumerate(zip(self._table, grads)):
             kind = ops._check_type(g, f"grads[{i}]")
-            if g.numel() != p.numel() or g.device != p.device or not g.is_contiguous():
-                raise ValueError(f"grads[{i}] must be contiguous, of {p.numel()} elements on "
-                                 f"{p.device}")
+            if g.numel() != t.n or g.get_device() != self._dev or not g.is_contiguous():
+                raise ValueError(f"grads[{i}] must be contiguous, of {t.n} elements on "
+                                 f"{self.device}")
             t.grad, t.grad_type = g.data_ptr(), kind
-        s = ops._on(self.params[0], stream)
         rc = _lib.lib().mx_adamw_step(
             ops._handle(self.ctx, self.params[0]), self._table, len(self.params), self.state_bits,
             self.lr, self.betas[0], self.betas[1], self.eps, self.step_count + 1,
             ops._ptr(self.step_dev), self.max_grad_norm, self.norm.data_ptr(),
-            self._scratch.data_ptr(), self._scratch.numel(), s.cuda_stream)
+            self._scratch.data_ptr(), self._scratch.numel(),
+            ops._launch_stream(self._dev, stream))
         ops.check(rc, "mx_adamw_step")
         self.step_count += 1

@@ -371,16 +371,15 @@ def sgd_momentum_clip(params, grads, vels, lr, momentum, weight_decay, max_grad_
 _DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
 
 
-def _check_like(t: torch.Tensor, name: str, ref: torch.Tensor, dtype=None, shape=None):
-    """A contiguous CUDA tensor on ref's device, of ref's type unless given."""
+def _check_like(t: torch.Tensor, name: str, device: int, dtype, shape=None):
+    """A contiguous CUDA tensor on the device `device`, of the given type."""
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise TypeError(f"{name} must be a CUDA tensor")
-    dtype = ref.dtype if dtype is None else dtype
-    if t.dtype != dtype:
+    if t.dtype is not dtype:
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
-    if t.device != ref.device:
-        raise ValueError(f"{name} is on {t.device}, not on {ref.device}")
-    if shape is not None and tuple(t.shape) != tuple(shape):
+    if t.get_device() != device:
+        raise ValueError(f"{name} is on cuda:{t.get_device()}, not on cuda:{device}")
+    if shape is not None and t.shape != shape:
         raise ValueError(f"{name} has shape {tuple(t.shape)}, needs {tuple(shape)}")
     if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
@@ -389,20 +388,25 @@ def _check_like(t: torch.Tensor, name: str, ref: torch.Tensor, dtype=None, shape
 def _check_type(t: torch.Tensor, name: str) -> int:
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise TypeError(f"{name} must be a CUDA tensor")
-    if t.dtype not in _DTYPES:
+    dt = _DTYPES.get(t.dtype)
+    if dt is None:
         raise TypeError(f"{name} must be float32 or bfloat16, got {t.dtype}")
-    return _DTYPES[t.dtype]
+    return dt
 
 
-def _on(t: torch.Tensor, stream):
-    """The stream of a call on t: the given one, else the current one of t's
-    device.  What the call allocates is allocated on it."""
-    return stream if stream is not None else torch.cuda.current_stream(t.device)
+def _launch_stream(device: int, stream) -> int:
+    """The raw stream of a call: the given one, else the device's current one."""
+    return stream.cuda_stream if stream is not None else \
+        torch._C._cuda_getCurrentRawStream(device)
 
 
-def _empty(shape, dtype, t: torch.Tensor, stream):
+def _empty(shape, dtype, device, stream):
+    """Memory for a call on `stream` (None: the current one), allocated on that
+    stream, so that it is not handed on before the call is done with it."""
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
     with torch.cuda.stream(stream):
-        return torch.empty(shape, dtype=dtype, device=t.device)
+        return torch.empty(shape, dtype=dtype, device=device)
 
 
 def _rows(t: torch.Tensor, name: str) -> tuple[int, int, int]:
@@ -411,12 +415,19 @@ def _rows(t: torch.Tensor, name: str) -> tuple[int, int, int]:
     if t.dim() < 1 or t.shape[-1] < 1:
         raise ValueError(f"{name} needs a last dimension of at least 1")
     cols = t.shape[-1]
-    rows = t.numel() // cols
     if t.is_contiguous():
-        return rows, cols, cols
+        return t.numel() // cols, cols, cols
     if t.dim() == 2 and t.stride(1) == 1 and t.stride(0) >= cols:
-        return rows, cols, t.stride(0)
+        return t.shape[0], cols, t.stride(0)
     raise ValueError(f"{name} must be contiguous, or 2-D with contiguous rows")
+
+
+def _like_rows(t: torch.Tensor, name: str, x: torch.Tensor, of: str) -> int:
+    """The row stride of a tensor of x's shape, type and device."""
+    if not isinstance(t, torch.Tensor) or t.shape != x.shape or t.dtype is not x.dtype or \
+            t.device != x.device:
+        raise ValueError(f"{name} must have the shape, type and device of {of}")
+    return _rows(t, name)[2]
 
 
 def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None,
@@ -428,21 +439,21 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None,
     for layer_norm_backward) are None unless `stats`."""
     dt = _check_type(x, "x")
     rows, cols, ldx = _rows(x, "x")
+    dev = x.get_device()
     for t, name in ((weight, "weight"), (bias, "bias")):
         if t is not None:
-            _check_like(t, name, x, torch.float32, (cols,))
-    s = _on(x, stream)
+            _check_like(t, name, dev, torch.float32, (cols,))
     if out is None:
-        out = _empty(x.shape, x.dtype, x, s)
-    elif out.shape != x.shape or out.dtype != x.dtype or out.device != x.device:
-        raise ValueError("out must be like x")
-    ldy = _rows(out, "out")[2]
+        out, ldy = _empty(x.shape, x.dtype, x.device, stream), cols
+    else:
+        ldy = _like_rows(out, "out", x, "x")
     mean = rstd = None
     if stats:
-        mean, rstd = _empty((2, rows), torch.float32, x, s)
+        mean = _empty(rows, torch.float32, x.device, stream)
+        rstd = _empty(rows, torch.float32, x.device, stream)
     rc = _lib.lib().mx_layer_norm_fwd(
         _handle(ctx, x), dt, x.data_ptr(), ldx, _ptr(weight), _ptr(bias), out.data_ptr(), ldy,
-        _ptr(mean), _ptr(rstd), rows, cols, float(eps), s.cuda_stream)
+        _ptr(mean), _ptr(rstd), rows, cols, eps, _launch_stream(dev, stream))
     check(rc, "mx_layer_norm_fwd")
     return out, mean, rstd
 
@@ -456,32 +467,31 @@ def layer_norm_backward(grad_out: torch.Tensor, x: torch.Tensor, weight: torch.T
     over the rows in a fixed order."""
     dt = _check_type(x, "x")
     rows, cols, ldx = _rows(x, "x")
-    if grad_out.shape != x.shape or grad_out.dtype != x.dtype or grad_out.device != x.device:
-        raise ValueError("grad_out must be like x")
-    lddy = _rows(grad_out, "grad_out")[2]
+    dev, f32 = x.get_device(), torch.float32
+    lddy = _like_rows(grad_out, "grad_out", x, "x")
     if weight is not None:
-        _check_like(weight, "weight", x, torch.float32, (cols,))
-    _check_like(mean, "mean", x, torch.float32, (rows,))
-    _check_like(rstd, "rstd", x, torch.float32, (rows,))
-    s = _on(x, stream)
+        _check_like(weight, "weight", dev, f32, (cols,))
+    _check_like(mean, "mean", dev, f32, (rows,))
+    _check_like(rstd, "rstd", dev, f32, (rows,))
     if dx is None:
-        dx = _empty(x.shape, x.dtype, x, s)
-    elif dx.shape != x.shape or dx.dtype != x.dtype or dx.device != x.device:
-        raise ValueError("dx must be like x")
-    lddx = _rows(dx, "dx")[2]
+        dx, lddx = _empty(x.shape, x.dtype, x.device, stream), cols
+    else:
+        lddx = _like_rows(dx, "dx", x, "x")
     if dweight is None:
-        dweight = _empty((cols,), torch.float32, x, s)
+        dweight = _empty(cols, f32, x.device, stream)
+    else:
+        _check_like(dweight, "dweight", dev, f32, (cols,))
     if dbias is None:
-        dbias = _empty((cols,), torch.float32, x, s)
-    _check_like(dweight, "dweight", x, torch.float32, (cols,))
-    _check_like(dbias, "dbias", x, torch.float32, (cols,))
+        dbias = _empty(cols, f32, x.device, stream)
+    else:
+        _check_like(dbias, "dbias", dev, f32, (cols,))
     h = _handle(ctx, x)
     nb = _lib.lib().mx_layer_norm_bwd_scratch_bytes(h, rows, cols)
-    scratch = _empty((nb,), torch.uint8, x, s)
+    scratch = _empty(nb, torch.uint8, x.device, stream)
     rc = _lib.lib().mx_layer_norm_bwd(
         h, dt, grad_out.data_ptr(), lddy, x.data_ptr(), ldx, _ptr(weight), mean.data_ptr(),
         rstd.data_ptr(), dx.data_ptr(), lddx, dweight.data_ptr(), dbias.data_ptr(), rows, cols,
-        scratch.data_ptr(), nb, s.cuda_stream)
+        scratch.data_ptr(), nb, _launch_stream(dev, stream))
     check(rc, "mx_layer_norm_bwd")
     return dx, dweight, dbias
 
@@ -490,6 +500,9 @@ def _gated_shape(x: torch.Tensor, w: torch.Tensor, transpose_w: bool, act: str):
     dt = _check_type(x, "x")
     if act not in _lib.ACTIVATIONS:
         raise ValueError(f"act must be one of {sorted(_lib.ACTIVATIONS)}, got {act!r}")
+    dev = x.get_device()
+    _check_like(x, "x", dev, x.dtype)
+    _check_like(w, "w", dev, x.dtype)
     if x.dim() < 1 or w.dim() != 2:
         raise ValueError("x needs a last dimension, w two dimensions")
     K = x.shape[-1]
@@ -498,9 +511,7 @@ def _gated_shape(x: torch.Tensor, w: torch.Tensor, transpose_w: bool, act: str):
     if two_f % 2 or w.shape[1 if transpose_w else 0] != K:
         raise ValueError(f"w has shape {tuple(w.shape)}, needs "
                          f"{('[2F, %d]' if transpose_w else '[%d, 2F]') % K}")
-    _check_like(x, "x", x)
-    _check_like(w, "w", x)
-    return dt, M, K, two_f // 2
+    return dt, dev, M, K, two_f // 2, x.shape[:-1]
 
 
 def gated_linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None,
@@ -512,24 +523,23 @@ def gated_linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = N
     (transpose_w=False) or [2F, K], the gate's half first; bias: [2F].  w, bias
     and h are of x's type.  pre, [g | u] in float32 for
     gated_linear_backward, is None unless `save` (or a buffer) is given."""
-    dt, M, K, F = _gated_shape(x, w, transpose_w, act)
+    dt, dev, M, K, F, lead = _gated_shape(x, w, transpose_w, act)
     if bias is not None:
-        _check_like(bias, "bias", x, None, (2 * F,))
-    s = _on(x, stream)
-    lead = tuple(x.shape[:-1])
+        _check_like(bias, "bias", dev, x.dtype, (2 * F,))
     if out is None:
-        out = _empty(lead + (F,), x.dtype, x, s)
-    _check_like(out, "out", x, None, lead + (F,))
-    if pre is None and save:
-        pre = _empty(lead + (2 * F,), torch.float32, x, s)
+        out = _empty(lead + (F,), x.dtype, x.device, stream)
+    else:
+        _check_like(out, "out", dev, x.dtype, lead + (F,))
     if pre is not None:
-        _check_like(pre, "pre", x, torch.float32, lead + (2 * F,))
-    h, p = _handle(ctx, x), _prec(precision)
-    nb = _lib.lib().mx_gated_linear_workspace_bytes(h, dt, M, K, F, int(transpose_w), p, 0)
-    ws = _empty((nb,), torch.uint8, x, s) if nb else None
-    rc = _lib.lib().mx_gated_linear_fwd(
+        _check_like(pre, "pre", dev, torch.float32, lead + (2 * F,))
+    elif save:
+        pre = _empty(lead + (2 * F,), torch.float32, x.device, stream)
+    L, h, p = _lib.lib(), _handle(ctx, x), _prec(precision)
+    nb = L.mx_gated_linear_workspace_bytes(h, dt, M, K, F, transpose_w, p, 0)
+    ws = _empty(nb, torch.uint8, x.device, stream) if nb else None
+    rc = L.mx_gated_linear_fwd(
         h, dt, x.data_ptr(), w.data_ptr(), _ptr(bias), out.data_ptr(), _ptr(pre), M, K, F,
-        int(transpose_w), _lib.ACTIVATIONS[act], p, _ptr(ws), nb, s.cuda_stream)
+        transpose_w, _lib.ACTIVATIONS[act], p, _ptr(ws), nb, _launch_stream(dev, stream))
     check(rc, "mx_gated_linear_fwd")
     return out, pre
 
@@ -541,26 +551,28 @@ def gated_linear_backward(grad_out: torch.Tensor, pre: torch.Tensor, x: torch.Te
                           precision="default", stream=None, ctx=None):
     """(dx, dw, dbias) of gated_linear from the `pre` that it saved
     (mx_gated_linear_bwd); dbias is None without `want_bias`."""
-    dt, M, K, F = _gated_shape(x, w, transpose_w, act)
-    lead = tuple(x.shape[:-1])
-    _check_like(grad_out, "grad_out", x, None, lead + (F,))
-    _check_like(pre, "pre", x, torch.float32, lead + (2 * F,))
-    s = _on(x, stream)
-    dx = _empty(x.shape, x.dtype, x, s) if dx is None else dx
-    dw = _empty(w.shape, x.dtype, x, s) if dw is None else dw
-    if dbias is None and want_bias:
-        dbias = _empty((2 * F,), x.dtype, x, s)
-    _check_like(dx, "dx", x, None, x.shape)
-    _check_like(dw, "dw", x, None, w.shape)
+    dt, dev, M, K, F, lead = _gated_shape(x, w, transpose_w, act)
+    _check_like(grad_out, "grad_out", dev, x.dtype, lead + (F,))
+    _check_like(pre, "pre", dev, torch.float32, lead + (2 * F,))
+    if dx is None:
+        dx = _empty(x.shape, x.dtype, x.device, stream)
+    else:
+        _check_like(dx, "dx", dev, x.dtype, x.shape)
+    if dw is None:
+        dw = _empty(w.shape, x.dtype, x.device, stream)
+    else:
+        _check_like(dw, "dw", dev, x.dtype, w.shape)
     if dbias is not None:
-        _check_like(dbias, "dbias", x, None, (2 * F,))
-    h, p = _handle(ctx, x), _prec(precision)
-    nb = _lib.lib().mx_gated_linear_workspace_bytes(h, dt, M, K, F, int(transpose_w), p, 1)
-    ws = _empty((nb,), torch.uint8, x, s) if nb else None
-    rc = _lib.lib().mx_gated_linear_bwd(
+        _check_like(dbias, "dbias", dev, x.dtype, (2 * F,))
+    elif want_bias:
+        dbias = _empty(2 * F, x.dtype, x.device, stream)
+    L, h, p = _lib.lib(), _handle(ctx, x), _prec(precision)
+    nb = L.mx_gated_linear_workspace_bytes(h, dt, M, K, F, transpose_w, p, 1)
+    ws = _empty(nb, torch.uint8, x.device, stream) if nb else None
+    rc = L.mx_gated_linear_bwd(
         h, dt, grad_out.data_ptr(), pre.data_ptr(), x.data_ptr(), w.data_ptr(), dx.data_ptr(),
-        dw.data_ptr(), _ptr(dbias), M, K, F, int(transpose_w), _lib.ACTIVATIONS[act], p,
-        _ptr(ws), nb, s.cuda_stream)
+        dw.data_ptr(), _ptr(dbias), M, K, F, transpose_w, _lib.ACTIVATIONS[act], p, _ptr(ws), nb,
+        _launch_stream(dev, stream))
     check(rc, "mx_gated_linear_bwd")
     return dx, dw, dbias
 
@@ -574,17 +586,16 @@ def adamw_state_values(codes: torch.Tensor, scale: torch.Tensor, out: torch.Tens
         raise TypeError("codes must be a CUDA tensor")
     if codes.dtype not in (torch.int8, torch.uint8):
         raise TypeError(f"codes must be int8 or uint8, got {codes.dtype}")
-    _check_like(codes, "codes", codes)
-    _check_like(scale, "scale", codes, torch.float32)
-    if scale.numel() != -(-codes.numel() // 256):
-        raise ValueError(f"scale has {scale.numel()} elements, needs {-(-codes.numel() // 256)}")
-    s = _on(codes, stream)
+    dev, n = codes.get_device(), codes.numel()
+    _check_like(codes, "codes", dev, codes.dtype)
+    _check_like(scale, "scale", dev, torch.float32, (-(-n // 256),))
     if out is None:
-        out = _empty(codes.shape, torch.bfloat16, codes, s)
-    _check_like(out, "out", codes, torch.bfloat16, codes.shape)
+        out = _empty(codes.shape, torch.bfloat16, codes.device, stream)
+    else:
+        _check_like(out, "out", dev, torch.bfloat16, codes.shape)
     rc = _lib.lib().mx_adamw_state_values(
-        _handle(ctx, codes), codes.data_ptr(), scale.data_ptr(), codes.numel(),
-        int(codes.dtype == torch.uint8), out.data_ptr(), s.cuda_stream)
+        _handle(ctx, codes), codes.data_ptr(), scale.data_ptr(), n, codes.dtype is torch.uint8,
+        out.data_ptr(), _launch_stream(dev, stream))
     check(rc, "mx_adamw_state_values")
     return out
 
