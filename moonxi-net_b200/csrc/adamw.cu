@@ -36,7 +36,8 @@ namespace {
 
 constexpr int kQBlock = 256;           // values of one scale, of one warp
 constexpr int kWarps = 8;
-constexpr int kChunk = kWarps * kQBlock;  // values of one block
+constexpr int kPerWarp = 1;            // 256-value blocks of a warp
+constexpr int kChunk = kPerWarp * kWarps * kQBlock;  // values of one block
 
 enum : uint32_t { kGradBf16 = 1, kVec = 2 };
 
@@ -80,6 +81,18 @@ __device__ __forceinline__ int find_tensor(const Table<CAP>& tb, int64_t chunk) 
   return lo;
 }
 
+// To 2 units in the last place, values below 2^-126 as zeros.
+__device__ __forceinline__ float fast_sqrt(float x) {
+  float r;
+  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float fast_rcp(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
 // The new m, v and p of one value; returns sqrt(v).  32-bit moments: every
 // operation rounded by itself, as the elementwise form of the step computes
 // it.  8-bit moments: fused, with the approximate root and quotient (2 units in
@@ -91,9 +104,8 @@ __device__ __forceinline__ float adamw_one(float& p, float g, float& m, float& v
   if constexpr (Q8) {
     m = fmaf(m, h.b1, g * h.omb1);
     v = fmaf(v, h.b2, g * g * h.omb2);
-    float root;
-    asm("sqrt.approx.f32 %0, %1;" : "=f"(root) : "f"(v));
-    p = fmaf(p, keep, -__fdividef(m * h.step_size, fmaf(root, h.inv_root, h.eps)));
+    const float root = fast_sqrt(v);
+    p = fmaf(p, keep, -(m * h.step_size) * fast_rcp(fmaf(root, h.inv_root, h.eps)));
     return root;
   }
   m = __fadd_rn(__fmul_rn(m, h.b1), __fmul_rn(g, h.omb1));
@@ -182,30 +194,28 @@ __device__ __forceinline__ void decode8(const uint8_t* q, float top, bool vec, i
 }
 // The warp's largest magnitude, at least 2^-120; NaN if a value is not finite.
 // As integers, magnitudes keep their order, with infinity and NaN above all.
+template <bool SIGNED>
 __device__ __forceinline__ float block_top(const float (&x)[8]) {
   uint32_t top = 0x03800000u;  // 2^-120
 #pragma unroll
-  for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+  for (int i = 0; i < 8; ++i)
+    top = max(top, SIGNED ? __float_as_uint(x[i]) & 0x7fffffffu : __float_as_uint(x[i]));
   top = __reduce_max_sync(0xffffffffu, top);
   return __uint_as_float(top >= 0x7f800000u ? 0x7fc00000u : top);
 }
-// The codes: c = round(most * sqrt(|x| / top)), rounded by adding 1.5 * 2^23,
+// The codes: c = round(sqrt(|x| most^2 / top)), rounded by adding 1.5 * 2^23,
 // which leaves it in the low byte.  The root's last bit does not matter here.
 template <bool SIGNED>
 __device__ __forceinline__ void encode8(uint8_t* q, float top, bool vec, int left,
                                         const float (&x)[8]) {
-  const float inv = __fdiv_rn(1.0f, top);
+  const float scale = __fdiv_rn(SIGNED ? 16129.0f : 65025.0f, top);
   uint32_t b[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    float r = fabsf(x[i]) * inv;
-    asm("sqrt.approx.f32 %0, %0;" : "+f"(r));
-    if (SIGNED) {
-      b[i] = __float_as_uint(fmaf(copysignf(r, x[i]), 127.0f, 12582912.0f));
-    } else {
-      const float c = fmaxf(r * 255.0f, x[i] > 0.0f ? 1.0f : 0.0f);
-      b[i] = __float_as_uint(c + 12582912.0f);
-    }
+    float c = fast_sqrt(fabsf(x[i]) * scale);
+    if (SIGNED) c = copysignf(c, x[i]);
+    else if (x[i] > 0.0f) c = fmaxf(c, 1.0f);
+    b[i] = __float_as_uint(c + 12582912.0f);
   }
   uint32_t w[2];
 #pragma unroll
@@ -221,15 +231,57 @@ __device__ __forceinline__ void encode8(uint8_t* q, float top, bool vec, int lef
   }
 }
 
+// The step of 256 values, a warp's; VEC: all of them are there, 16-byte
+// aligned (8-bit states 8-byte).
+template <bool Q8, bool VEC>
+__device__ __forceinline__ void adamw_block(const Tensor& t, const Hyper& h, float clip,
+                                            int64_t block) {
+  const int lane = threadIdx.x & 31;
+  const int64_t at = block * kQBlock + lane * 8;
+  const int64_t rest = t.n - at;
+  const int left = VEC ? 8 : rest >= 8 ? 8 : rest > 0 ? static_cast<int>(rest) : 0;
+  float p[8], g[8], m[8], v[8];
+  load8(t.p + at, VEC, left, p);
+  if (t.flags & kGradBf16) load8(static_cast<const __nv_bfloat16*>(t.g) + at, VEC, left, g);
+  else load8(static_cast<const float*>(t.g) + at, VEC, left, g);
+  if (Q8) {
+    decode8<true>(static_cast<const uint8_t*>(t.m) + at, t.ms[block], VEC, left, m);
+    decode8<false>(static_cast<const uint8_t*>(t.v) + at, t.vs[block], VEC, left, v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = __fmul_rn(v[i], v[i]);
+  } else {
+    load8(static_cast<const float*>(t.m) + at, VEC, left, m);
+    load8(static_cast<const float*>(t.v) + at, VEC, left, v);
+  }
+  if (h.norm) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) g[i] = __fmul_rn(g[i], clip);
+  }
+  float root[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) root[i] = adamw_one<Q8>(p[i], g[i], m[i], v[i], t.keep, h);
+  store8(t.p + at, VEC, left, p);
+  if (t.copy) store8(t.copy + at, VEC, left, p);
+  if (Q8) {
+    const float sm = block_top<true>(m), sv = block_top<false>(root);
+    encode8<true>(static_cast<uint8_t*>(t.m) + at, sm, VEC, left, m);
+    encode8<false>(static_cast<uint8_t*>(t.v) + at, sv, VEC, left, root);
+    __syncwarp();  // every lane has read the old scales
+    if (lane == 0) {
+      t.ms[block] = sm;
+      t.vs[block] = sv;
+    }
+  } else {
+    store8(static_cast<float*>(t.m) + at, VEC, left, m);
+    store8(static_cast<float*>(t.v) + at, VEC, left, v);
+  }
+}
+
 template <int CAP, bool Q8>
 __global__ void __launch_bounds__(32 * kWarps) adamw_kernel(const __grid_constant__ Table<CAP> tb,
                                                             const Hyper hy) {
   const int ti = find_tensor(tb, blockIdx.x);
-  const Tensor& t = tb.t[ti];
-  const int lane = threadIdx.x & 31;
-  const int64_t block = (blockIdx.x - tb.first[ti]) * kWarps + (threadIdx.x >> 5);
-  const int64_t at = block * kQBlock + lane * 8;
-  if (block * kQBlock >= t.n) return;  // the whole warp
+  const Tensor t = tb.t[ti];
   Hyper h = hy;
   if (h.scalars) {
     h.step_size = h.scalars[0];
@@ -240,42 +292,13 @@ __global__ void __launch_bounds__(32 * kWarps) adamw_kernel(const __grid_constan
     const float nv = *h.norm;
     if (nv > h.max_norm) clip = __fdiv_rn(h.max_norm, nv);
   }
-  const int64_t rest = t.n - at;
-  const int left = rest >= 8 ? 8 : rest > 0 ? static_cast<int>(rest) : 0;
-  const bool vec = t.flags & kVec;
-  float p[8], g[8], m[8], v[8];
-  load8(t.p + at, vec, left, p);
-  if (t.flags & kGradBf16) load8(static_cast<const __nv_bfloat16*>(t.g) + at, vec, left, g);
-  else load8(static_cast<const float*>(t.g) + at, vec, left, g);
-  if (Q8) {
-    decode8<true>(static_cast<const uint8_t*>(t.m) + at, t.ms[block], vec, left, m);
-    decode8<false>(static_cast<const uint8_t*>(t.v) + at, t.vs[block], vec, left, v);
+  const int64_t first = (blockIdx.x - tb.first[ti]) * (kChunk / kQBlock) + (threadIdx.x >> 5);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = __fmul_rn(v[i], v[i]);
-  } else {
-    load8(static_cast<const float*>(t.m) + at, vec, left, m);
-    load8(static_cast<const float*>(t.v) + at, vec, left, v);
-  }
-  float root[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    if (h.norm) g[i] = __fmul_rn(g[i], clip);
-    root[i] = adamw_one<Q8>(p[i], g[i], m[i], v[i], t.keep, h);
-  }
-  store8(t.p + at, vec, left, p);
-  if (t.copy) store8(t.copy + at, vec, left, p);
-  if (Q8) {
-    const float sm = block_top(m), sv = block_top(root);
-    encode8<true>(static_cast<uint8_t*>(t.m) + at, sm, vec, left, m);
-    encode8<false>(static_cast<uint8_t*>(t.v) + at, sv, vec, left, root);
-    __syncwarp();  // every lane has read the old scales
-    if (lane == 0) {
-      t.ms[block] = sm;
-      t.vs[block] = sv;
-    }
-  } else {
-    store8(static_cast<float*>(t.m) + at, vec, left, m);
-    store8(static_cast<float*>(t.v) + at, vec, left, v);
+  for (int k = 0; k < kPerWarp; ++k) {
+    const int64_t block = first + k * kWarps;
+    if (block * kQBlock >= t.n) return;  // the whole warp
+    if ((t.flags & kVec) && (block + 1) * kQBlock <= t.n) adamw_block<Q8, true>(t, h, clip, block);
+    else adamw_block<Q8, false>(t, h, clip, block);
   }
 }
 
@@ -308,18 +331,21 @@ __global__ void __launch_bounds__(32 * kWarps) grad_norm_kernel(const __grid_con
   for (int64_t c = blockIdx.x; c < tb.first[tb.count]; c += gridDim.x) {
     const int ti = find_tensor(tb, c);
     const Tensor& t = tb.t[ti];
-    const int64_t at = (c - tb.first[ti]) * kChunk + threadIdx.x * 8;
-    const int64_t rest = t.n - at;
-    const int left = rest >= 8 ? 8 : rest > 0 ? static_cast<int>(rest) : 0;
-    float g[8];
-    if (t.flags & kGradBf16)
-      load8(static_cast<const __nv_bfloat16*>(t.g) + at, t.flags & kVec, left, g);
-    else
-      load8(static_cast<const float*>(t.g) + at, t.flags & kVec, left, g);
-    float q = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) q += g[i] * g[i];
-    s += q;
+    for (int k = 0; k < kPerWarp; ++k) {
+      const int64_t at = (c - tb.first[ti]) * kChunk + (k * 32 * kWarps + threadIdx.x) * 8;
+      const int64_t rest = t.n - at;
+      const int left = rest >= 8 ? 8 : rest > 0 ? static_cast<int>(rest) : 0;
+      float g[8];
+      if (t.flags & kGradBf16)
+        load8(static_cast<const __nv_bfloat16*>(t.g) + at, t.flags & kVec, left, g);
+      else
+        load8(static_cast<const float*>(t.g) + at, t.flags & kVec, left, g);
+      float q = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) q += g[i] * g[i];
+      s += q;
+    }
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
@@ -492,7 +518,7 @@ int adamw_step(const mx_adamw_tensor* ts, int count, int bits, double lr, double
 int adamw_state_values(const void* q, const float* scale, int64_t n, int is_signed, void* out,
                        cudaStream_t s) {
   if (n <= 0) return kOk;
-  const int64_t blocks = chunks_of(n);
+  const int64_t blocks = (n + kWarps * kQBlock - 1) / (kWarps * kQBlock);
   if (blocks > 0x7fffffff) return kErrUnsupported;
   const bool vec = aligned(q, 8) && aligned(out, 16);
   const uint8_t* c = static_cast<const uint8_t*>(q);

@@ -9,9 +9,11 @@
 // The tensor core truncates its accumulator at every MMA, about 2e-8 of the
 // result each and always towards zero (measured: a 3xTF32 product of K = 1024
 // left in one accumulator is off by 7e-6).  So a stage's six products go from
-// the smallest to the largest, only the last two MMAs meet the full
-// accumulator, and after every stage, 32 of K, the epilogue warps add the
-// accumulator to float32 registers with rounding.
+// the smallest to the largest, few MMAs meet a full accumulator, and after
+// every stage, 64 of K, the epilogue warps add the accumulator to float32
+// registers with rounding: 2e-7 for 512 x 1024 x 8192 where SGEMM has 9e-7.
+// (Four stages of 32 of K: 60 us for that product against 45 when every stage
+// is added up, the epilogue's rate, and 48 us and 6e-7 when every second is.)
 //
 // CTA pairs (cta_group::2): a pair computes a 256 x 256 tile, each CTA holding
 // 128 rows of A, 128 columns of B and its 128 x 256 half of the accumulator:
@@ -46,17 +48,15 @@ namespace {
 
 constexpr int kTile = 256;             // rows and columns of a pair's tile
 constexpr int kHalf = 128;             // ... of one CTA's operand tiles
+constexpr int kBK = 64;                // a stage's depth: 128 bytes of bf16
+constexpr int kOpBytes = kHalf * kBK * 2;  // an operand tile
 constexpr int kThreads = 320;
 constexpr int kTmemCols = 512;
 constexpr int kTrFloats = 32 * 33;     // a warp's transpose buffer
 
-// A stage is 64 of K, three copies 32 (with 64 only two stages fit, and a
-// stage's loads have no more than the other stage's MMAs to hide behind).
 template <int NC>
 struct Cfg {
-  static constexpr int kBK = NC == 3 ? 32 : 64;
-  static constexpr int kOpBytes = kHalf * kBK * 2;  // one operand tile
-  static constexpr int kStages = NC == 3 ? 4 : 6;
+  static constexpr int kStages = NC == 3 ? 2 : 6;
   static constexpr int kStageBytes = 2 * NC * kOpBytes;
   static constexpr int kSmem = kStages * kStageBytes + 8 * kTrFloats * 4 + 256 + 1024;
 };
@@ -94,27 +94,26 @@ __device__ __forceinline__ void tile_at(const Params& p, int t, int& tm, int& tn
   tn = r / gm;
 }
 
-// A 128 x BK tile of one copy: one box of BK k x 128 rows, or two of 64 rows x
-// BK k.
-template <bool KMAJOR, int BK>
+// A 128 x 64 tile of one copy: one box of 64 k x 128 rows, or two of 64 rows x
+// 64 k.
+template <bool KMAJOR>
 __device__ __forceinline__ void load_tile(uint8_t* dst, const CUtensorMap* map, uint32_t bar,
                                           int r0, int k0) {
   if (KMAJOR) {
     tma_load_2d_pair(dst, map, bar, k0, r0);
   } else {
     tma_load_2d_pair(dst, map, bar, r0, k0);
-    tma_load_2d_pair(dst + kHalf * BK, map, bar, r0 + 64, k0);
+    tma_load_2d_pair(dst + kOpBytes / 2, map, bar, r0 + 64, k0);
   }
 }
 
-// The 16-deep slice j of a tile.  K-major: rows of 2 BK bytes (swizzled over
-// that), groups of 8 rows 16 BK bytes apart, a slice 32 bytes on.  MN-major:
-// chunks of 64 columns 128 BK bytes apart, groups of 8 k 1024 bytes apart, a
-// slice two groups on.
-template <bool KMAJOR, int BK>
+// The 16-deep slice j of a tile.  K-major: 128-byte rows, groups of 8 rows
+// 1024 bytes apart, a slice 32 bytes on.  MN-major: chunks of 64 columns 8 KB
+// apart, groups of 8 k 1024 bytes apart, a slice two groups on.
+template <bool KMAJOR>
 __device__ __forceinline__ uint64_t slice_desc(uint32_t addr, int j) {
-  return KMAJOR ? sdesc_kmajor(addr + j * 32, 16 * BK, BK == 64 ? 2 : 4)
-                : sdesc_mnmajor(addr + j * 2048, 128 * BK, 1024, 2);
+  return KMAJOR ? sdesc_kmajor(addr + j * 32, 1024, 2)
+                : sdesc_mnmajor(addr + j * 2048, kOpBytes / 2, 1024, 2);
 }
 
 // 32 consecutive values of a row, in 32-byte stores; `left` columns remain (a
@@ -148,7 +147,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     bf16_gemm_kernel(const __grid_constant__ Maps<NC> maps, const Params p) {
   using T = typename std::conditional<NC == 1, __nv_bfloat16, float>::type;
   using C = Cfg<NC>;
-  constexpr int kBK = C::kBK, kOpBytes = C::kOpBytes;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -219,8 +217,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           const uint32_t bar = cluster_addr(&full[stage], 0);
 #pragma unroll
           for (int i = 0; i < NC; ++i) {
-            load_tile<AK, kBK>(base + i * kOpBytes, &maps.a[i], bar, m0, kb * kBK);
-            load_tile<BKM, kBK>(base + (NC + i) * kOpBytes, &maps.b[rank][i], bar, n0, kb * kBK);
+            load_tile<AK>(base + i * kOpBytes, &maps.a[i], bar, m0, kb * kBK);
+            load_tile<BKM>(base + (NC + i) * kOpBytes, &maps.b[rank][i], bar, n0, kb * kBK);
           }
           if (++stage == C::kStages) {
             stage = 0;
@@ -277,7 +275,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           if (NC == 1) {
 #pragma unroll
             for (int k = 0; k < kBK / 16; ++k) {
-              mma_f16_pair(d, slice_desc<AK, kBK>(sa, k), slice_desc<BKM, kBK>(sb, k), idesc, accumulate);
+              mma_f16_pair(d, slice_desc<AK>(sa, k), slice_desc<BKM>(sb, k), idesc, accumulate);
               accumulate = 1;
             }
           } else {
@@ -287,8 +285,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             for (int q = 0; q < 6; ++q)
 #pragma unroll
               for (int k = 0; k < kBK / 16; ++k) {
-                mma_f16_pair(d, slice_desc<AK, kBK>(sa + pa[q] * kOpBytes, k),
-                             slice_desc<BKM, kBK>(sb + pb[q] * kOpBytes, k), idesc, accumulate);
+                mma_f16_pair(d, slice_desc<AK>(sa + pa[q] * kOpBytes, k),
+                             slice_desc<BKM>(sb + pb[q] * kOpBytes, k), idesc, accumulate);
                 accumulate = 1;
               }
           }
@@ -526,12 +524,11 @@ Plan plan_of(const Context* ctx, int M, int N, int K, bool gated, int copies) {
   q.tiles_m = (M + kTile - 1) / kTile;
   q.tiles_n = (N + width - 1) / width;
   q.tiles = q.tiles_m * q.tiles_n;
-  const int bk = copies == 3 ? Cfg<3>::kBK : Cfg<1>::kBK;
-  const int num_kb = std::max(1, (K + bk - 1) / bk);
+  const int num_kb = std::max(1, (K + kBK - 1) / kBK);
   const int pairs = std::max(1, ctx->tc_sms() / 2);
   // Split K when whole tiles leave more than half of the pairs idle, into
   // pieces of at least 512 of K (three copies: 128, six times the work).
-  const int least = copies == 3 ? 4 : 8;
+  const int least = copies == 3 ? 2 : 8;
   q.splits = 1;
   if (2 * q.tiles <= pairs) q.splits = std::max(1, std::min(pairs / q.tiles, num_kb / least));
   q.kb_per = (num_kb + q.splits - 1) / q.splits;
@@ -540,22 +537,21 @@ Plan plan_of(const Context* ctx, int M, int N, int K, bool gated, int copies) {
   return q;
 }
 
-bool operand_map(CUtensorMap* m, const Bf16Operand& o, int copy, int rows, int K, int bk) {
+bool operand_map(CUtensorMap* m, const Bf16Operand& o, int copy, int rows, int K) {
   const void* base = static_cast<const __nv_bfloat16*>(o.base) + copy * o.copy;
-  return o.kmajor ? make_tmap_bf16(m, base, K, rows, o.ld * 2, bk, kHalf)
-                  : make_tmap_bf16(m, base, rows, K, o.ld * 2, 64, bk);
+  return o.kmajor ? make_tmap_bf16(m, base, K, rows, o.ld * 2, kBK, kHalf)
+                  : make_tmap_bf16(m, base, rows, K, o.ld * 2, 64, kBK);
 }
 
 template <int NC, bool AK, bool BKM, bool GATED>
 int launch(Context* ctx, const Bf16Gemm& g, cudaStream_t s) {
   using T = typename std::conditional<NC == 1, __nv_bfloat16, float>::type;
   const Plan q = plan_of(ctx, g.M, g.N, g.K, GATED, NC);
-  constexpr int bk = Cfg<NC>::kBK;
   Maps<NC> maps;
   for (int i = 0; i < NC; ++i)
-    if (!operand_map(&maps.a[i], g.a, i, g.M, g.K, bk) ||
-        !operand_map(&maps.b[0][i], g.b, i, g.N, g.K, bk) ||
-        !operand_map(&maps.b[1][i], GATED ? g.b2 : g.b, i, g.N, g.K, bk))
+    if (!operand_map(&maps.a[i], g.a, i, g.M, g.K) ||
+        !operand_map(&maps.b[0][i], g.b, i, g.N, g.K) ||
+        !operand_map(&maps.b[1][i], GATED ? g.b2 : g.b, i, g.N, g.K))
       return kErrUnsupported;
   Params p{};
   p.out = g.out;

@@ -277,7 +277,7 @@ bool make_tmap_3d(CUtensorMap* map, const void* base, const uint64_t dims[3],
                   const uint64_t strides_bytes[2], const uint32_t box[3],
                   CUtensorMapSwizzle swizzle);
 
-// bfloat16; box_inner 64 elements (128-byte swizzle) or 32 (64-byte).
+// bfloat16, 128-byte swizzle: box_inner is 64 elements.
 bool make_tmap_bf16(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer,
                     uint64_t row_stride_bytes, uint32_t box_inner, uint32_t box_outer);
 

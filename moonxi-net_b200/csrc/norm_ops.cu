@@ -105,15 +105,11 @@ __device__ __forceinline__ void row_sum(float (&s)[N], float* buf, int& turn) {
       for (int i = 0; i < N; ++i) b[i * W + (threadIdx.x >> 5)] = s[i];
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      float t = 0.0f;
+    for (int i = 0; i < N; ++i) s[i] = b[i * W + (threadIdx.x & (W - 1))];
 #pragma unroll
-      for (int w = 0; w < W; w += 4) {
-        const float4 q = *reinterpret_cast<const float4*>(b + i * W + w);
-        t += (q.x + q.y) + (q.z + q.w);
-      }
-      s[i] = t;
-    }
+    for (int o = W / 2; o > 0; o >>= 1)
+#pragma unroll
+      for (int i = 0; i < N; ++i) s[i] += __shfl_xor_sync(0xffffffffu, s[i], o);
   }
 }
 
@@ -122,12 +118,14 @@ __device__ __forceinline__ void row_sum(float (&s)[N], float* buf, int& turn) {
 // barrier), and takes them into registers when their turn comes.
 constexpr int kRingBytes = 200 * 1024;  // of an SM, over its blocks
 __host__ __device__ constexpr int block_threads(int tpr) { return tpr == 32 ? 128 : tpr; }
-// 1024 threads an SM, 64 registers each.
-__host__ __device__ constexpr int blocks_per_sm(int tpr) {
-  return 1024 / block_threads(tpr);
+// Blocks an SM is given: 768 threads forward (one tensor), 512 backward (two,
+// and the columns' sums in registers).
+__host__ __device__ constexpr int blocks_per_sm(int tpr, int tensors) {
+  const int n = (tensors == 1 ? 768 : 512) / block_threads(tpr);
+  return n < 1 ? 1 : n;
 }
 __host__ __device__ constexpr int ring_rows(int tpr, int e, int size, int tensors) {
-  const int d = kRingBytes / blocks_per_sm(tpr) / (block_threads(tpr) * e * size * tensors);
+  const int d = kRingBytes / blocks_per_sm(tpr, tensors) / (block_threads(tpr) * e * size * tensors);
   return d < 1 ? 1 : d > 4 ? 4 : d;
 }
 __host__ __device__ constexpr int ring_bytes(int tpr, int e, int size, int tensors, int v) {
@@ -156,14 +154,14 @@ struct NormFwd {
 // consecutive columns.  A block takes rows blockIdx.x, + gridDim.x, ...
 // (TPR = 32: four at a time, one a warp).
 template <typename T, int TPR, int E, int V>
-__global__ void __launch_bounds__(block_threads(TPR), blocks_per_sm(TPR)) norm_fwd_kernel(const NormFwd p) {
+__global__ void __launch_bounds__(block_threads(TPR), blocks_per_sm(TPR, 1)) norm_fwd_kernel(const NormFwd p) {
   constexpr int NV = E / V, D = ring_rows(TPR, E, sizeof(T), 1), BLOCK = block_threads(TPR);
   extern __shared__ uint4 ring[];  // [D][NV][BLOCK]
   __shared__ __align__(16) float buf[TPR > 32 ? 2 * 2 * TPR / 32 : 1];
   const int t = TPR == 32 ? threadIdx.x & 31 : threadIdx.x;
   const int64_t step = TPR == 32 ? gridDim.x * 4ll : gridDim.x;
   int64_t row = TPR == 32 ? blockIdx.x * 4ll + (threadIdx.x >> 5) : blockIdx.x;
-  const float n = static_cast<float>(p.cols);
+  const float inv_n = 1.0f / static_cast<float>(p.cols);
   auto fetch = [&](int64_t r, int slot) {
     if constexpr (V > 1) {
       if (r < p.rows) {
@@ -208,7 +206,7 @@ __global__ void __launch_bounds__(block_threads(TPR), blocks_per_sm(TPR)) norm_f
     fetch(row + D * step, slot);
     slot = slot + 1 == D ? 0 : slot + 1;
     row_sum<TPR>(s, buf, turn);
-    const float mean = s[0] / n;
+    const float mean = s[0] * inv_n;
     // The centred values' own mean is what rounding left of it: it is taken off
     // the values and off the variance, so a mean far above the deviation costs
     // no more than the rounding of x itself.
@@ -223,20 +221,21 @@ __global__ void __launch_bounds__(block_threads(TPR), blocks_per_sm(TPR)) norm_f
           q[1] += v[i][j] * v[i][j];
         }
     row_sum<TPR>(q, buf, turn);
-    const float rest = q[0] / n;
-    const float var = q[1] / n - rest * rest;
-    const float rstd = 1.0f / sqrtf((var < 0.0f ? 0.0f : var) + p.eps);  // NaN stays NaN
+    const float rest = q[0] * inv_n;
+    const float var = q[1] * inv_n - rest * rest;
+    const float rstd = rsqrtf((var < 0.0f ? 0.0f : var) + p.eps);  // NaN stays NaN
     if (t == 0) {
       if (p.mean) p.mean[row] = mean + rest;
       if (p.rstd) p.rstd[row] = rstd;
     }
     T* y = static_cast<T*>(p.y) + row * p.ldy;
+    const float shift = rest * rstd;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = (i * TPR + t) * V;
       if (c < p.cols) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) v[i][j] = (v[i][j] - rest) * rstd * w[i][j] + b[i][j];
+        for (int j = 0; j < V; ++j) v[i][j] = (v[i][j] * rstd - shift) * w[i][j] + b[i][j];
         store_vec<T, V>(y + c, v[i]);
       }
     }
@@ -289,7 +288,7 @@ struct NormBwd {
 // Rows as in norm_fwd_kernel; TPR = 32: the four warps' sums meet in shared
 // memory at the end.
 template <typename T, int TPR, int E, int V>
-__global__ void __launch_bounds__(block_threads(TPR), blocks_per_sm(TPR)) norm_bwd_kernel(const NormBwd p) {
+__global__ void __launch_bounds__(block_threads(TPR), blocks_per_sm(TPR, 2)) norm_bwd_kernel(const NormBwd p) {
   constexpr int NV = E / V, D = ring_rows(TPR, E, sizeof(T), 2), BLOCK = block_threads(TPR);
   extern __shared__ uint4 ring[];  // [D][2][NV][BLOCK]
   __shared__ __align__(16) float buf[TPR > 32 ? 2 * 2 * TPR / 32 : 4 * 32 * E];
@@ -326,8 +325,17 @@ __global__ void __launch_bounds__(block_threads(TPR), blocks_per_sm(TPR)) norm_b
 #pragma unroll
   for (int d = 0; d < D; ++d) fetch(row + d * step, d);
   int slot = 0, turn = 0;
+  float next_mean = 0.0f, next_rstd = 0.0f;  // a row ahead, like the rows
+  if (row < p.rows) {
+    next_mean = __ldg(p.mean + row);
+    next_rstd = __ldg(p.rstd + row);
+  }
   for (; row < p.rows; row += step) {
-    const float mean = __ldg(p.mean + row), rstd = __ldg(p.rstd + row);
+    const float mean = next_mean, rstd = next_rstd;
+    if (row + step < p.rows) {
+      next_mean = __ldg(p.mean + row + step);
+      next_rstd = __ldg(p.rstd + row + step);
+    }
     float xh[NV][V], a[NV][V];
     float s[2] = {0.0f, 0.0f};
     if constexpr (V > 1) cp_async_wait<D - 1>();
@@ -484,7 +492,7 @@ constexpr int kNormRegCols = 16384;
 
 // Blocks of a pass over rows: as many as fit on the SMs at a time.
 int row_blocks(int rows, int cols, int per_sm, int num_sms) {
-  const int at_once = cols <= 256 ? 4 : 1;  // rows of a block
+  const int at_once = cols <= 512 ? 4 : 1;  // rows of a block
   return std::max(1, std::min(per_sm * num_sms, (rows + at_once - 1) / at_once));
 }
 
@@ -495,7 +503,7 @@ cudaError_t run_fwd(const NormFwd& p, int num_sms, cudaStream_t s) {
   static SmemOptIn opt_in;
   cudaError_t e = kBytes > 32768 ? opt_in.ensure(kern, kBytes) : cudaSuccess;
   if (e != cudaSuccess) return e;
-  kern<<<row_blocks(p.rows, p.cols, blocks_per_sm(TPR), num_sms), block_threads(TPR), kBytes,
+  kern<<<row_blocks(p.rows, p.cols, blocks_per_sm(TPR, 1), num_sms), block_threads(TPR), kBytes,
          s>>>(p);
   return cudaGetLastError();
 }
@@ -503,10 +511,11 @@ template <typename T, int V>
 cudaError_t launch_fwd(const NormFwd& p, int num_sms, cudaStream_t s) {
   const int c = p.cols;
   if (c <= 256) return run_fwd<T, 32, 8, V>(p, num_sms, s);
-  if (c <= 1024) return run_fwd<T, 128, 8, V>(p, num_sms, s);
-  if (c <= 2048) return run_fwd<T, 256, 8, V>(p, num_sms, s);
-  if (c <= 4096) return run_fwd<T, 512, 8, V>(p, num_sms, s);
-  if (c <= 8192) return run_fwd<T, 1024, 8, V>(p, num_sms, s);
+  if (c <= 512) return run_fwd<T, 32, 16, V>(p, num_sms, s);
+  if (c <= 1024) return run_fwd<T, 64, 16, V>(p, num_sms, s);
+  if (c <= 2048) return run_fwd<T, 128, 16, V>(p, num_sms, s);
+  if (c <= 4096) return run_fwd<T, 256, 16, V>(p, num_sms, s);
+  if (c <= 8192) return run_fwd<T, 512, 16, V>(p, num_sms, s);
   return run_fwd<T, 1024, 16, V>(p, num_sms, s);
 }
 
@@ -524,18 +533,20 @@ template <typename T, int V>
 cudaError_t launch_bwd(const NormBwd& p, int blocks, cudaStream_t s) {
   const int c = p.cols;
   if (c <= 256) return run_bwd<T, 32, 8, V>(p, blocks, s);
-  if (c <= 1024) return run_bwd<T, 128, 8, V>(p, blocks, s);
-  if (c <= 2048) return run_bwd<T, 256, 8, V>(p, blocks, s);
-  if (c <= 4096) return run_bwd<T, 512, 8, V>(p, blocks, s);
-  if (c <= 8192) return run_bwd<T, 1024, 8, V>(p, blocks, s);
+  if (c <= 512) return run_bwd<T, 32, 16, V>(p, blocks, s);
+  if (c <= 1024) return run_bwd<T, 64, 16, V>(p, blocks, s);
+  if (c <= 2048) return run_bwd<T, 128, 16, V>(p, blocks, s);
+  if (c <= 4096) return run_bwd<T, 256, 16, V>(p, blocks, s);
+  if (c <= 8192) return run_bwd<T, 512, 16, V>(p, blocks, s);
   return run_bwd<T, 1024, 16, V>(p, blocks, s);
 }
 
 // Blocks of the backward pass (rows of partial sums).
 int bwd_blocks(int rows, int cols, int num_sms) {
   if (cols > kNormRegCols) return std::min(64, (rows + 63) / 64);  // row ranges of norm_cols
-  const int tpr = cols <= 1024 ? 128 : cols <= 2048 ? 256 : cols <= 4096 ? 512 : 1024;
-  return row_blocks((rows + 1) / 2, cols, blocks_per_sm(tpr), num_sms);
+  const int tpr = cols <= 512 ? 32 : cols <= 1024 ? 64 : cols <= 2048 ? 128 : cols <= 4096 ? 256
+                : cols <= 8192 ? 512 : 1024;
+  return row_blocks((rows + 1) / 2, cols, blocks_per_sm(tpr, 2), num_sms);
 }
 
 bool aligned16(const void* a) { return (reinterpret_cast<uintptr_t>(a) & 15u) == 0; }
