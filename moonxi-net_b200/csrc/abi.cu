@@ -858,6 +858,7 @@ int gated_args(Context* c, int32_t dtype, int32_t M, int32_t K, int32_t F, int32
   a.act = act;
   a.strict = p == MX_PREC_NPARRAY;
   a.exact = p == MX_PREC_FP32 || a.strict;
+  a.tensor = p == MX_PREC_3XTF32 || p == MX_PREC_TF32;
   return kOk;
 }
 }  // namespace

@@ -1,0 +1,324 @@
+// gated_skinny.cu -- the gated linear layer for a few rows (single tokens).
+//
+// One to four rows read every weight once and do one to four multiply-adds with
+// it: bound by the weights' bytes.  One row of 4096 x 2 x 8192 bfloat16 (134
+// MB, a floor of 20.5 us): 23.3 us here with w [K,2F] and 24.8 us with w
+// [2F,K], 43 us on the tensor-core kernel, whose pipeline has no second tile to
+// hide its start and end behind; four rows 32 and 45 us against 42 and 43.
+// float32: 44 us for one row, a floor of 41.  A warp reads 512 consecutive
+// bytes of a row of w, products and sums stay in float32, and one launch does
+// it all:
+//   w stored [K,2F]: a warp owns 16 bytes of the gate's columns a lane and the
+//     same of the other projection's and walks down K; the eight warps of a
+//     block and the blocks of a cluster split K, and the partial sums meet in
+//     (distributed) shared memory, added in a fixed order;
+//   w stored [2F,K]: a warp owns a pair of rows and the lanes split K.
+#include <algorithm>
+
+#include "gated_act.cuh"
+#include "mx_internal.h"
+#include "mx_ptx.cuh"
+
+namespace mx {
+namespace {
+
+using bf16 = __nv_bfloat16;
+constexpr int kWarps = 8;
+
+struct Skinny {
+  const void* x;
+  const void* w;
+  const void* bias;
+  void* h;
+  float* pre;
+  int M, K, F, act;
+  int k_per;  // [K,2F]: rows of K of one block of a cluster
+};
+
+template <typename T>
+__host__ __device__ constexpr int vec_of() { return 16 / static_cast<int>(sizeof(T)); }
+
+template <typename T, int V>
+__device__ __forceinline__ void unpack(const uint4 r, float (&x)[V]) {
+  const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(T) == 4) {
+      x[i] = __uint_as_float(w[i]);
+    } else {
+      x[2 * i] = __uint_as_float(w[i] << 16);
+      x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  }
+}
+
+// weights are read once: past L1, first out of L2
+__device__ __forceinline__ uint4 stream16(const void* p) {
+  uint4 r;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
+               : "l"(p));
+  return r;
+}
+
+template <typename T>
+__device__ __forceinline__ void finish(const Skinny& p, int m, int f, float g, float u) {
+  if (p.bias) {
+    g += to_f(static_cast<const T*>(p.bias)[f]);
+    u += to_f(static_cast<const T*>(p.bias)[p.F + f]);
+  }
+  if (p.pre) {
+    p.pre[m * 2ll * p.F + f] = g;
+    p.pre[m * 2ll * p.F + p.F + f] = u;
+  }
+  float ga[1] = {g}, ua[1] = {u};
+  gate(p.act, ga, ua);
+  put(static_cast<T*>(p.h) + static_cast<int64_t>(m) * p.F + f, ga[0]);
+}
+
+// w [K,2F].  A cluster owns 32 * V columns of each half; its blocks split K.
+// x of row k in rows m .. of the block's chunk, [k][MT].
+template <int MT>
+__device__ __forceinline__ void load_x(const float* p, float (&x)[MT]) {
+  if constexpr (MT == 1) {
+    x[0] = *p;
+  } else if constexpr (MT == 2) {
+    const float2 v = *reinterpret_cast<const float2*>(p);
+    x[0] = v.x; x[1] = v.y;
+  } else {
+#pragma unroll
+    for (int m = 0; m < MT; m += 4) {
+      const float4 v = *reinterpret_cast<const float4*>(p + m);
+      x[m] = v.x; x[m + 1] = v.y; x[m + 2] = v.z; x[m + 3] = v.w;
+    }
+  }
+}
+
+template <typename T, int MT>
+__global__ void __launch_bounds__(32 * kWarps, 2) skinny_nn_kernel(const Skinny p, int cluster) {
+  constexpr int V = vec_of<T>(), COLS = 32 * V, U = MT == 1 ? 8 : 4;
+  constexpr int kChunk = 1024;  // rows of K whose x a block holds
+  __shared__ __align__(16) float xs[kChunk][MT];
+  __shared__ __align__(16) float red[kWarps][2][COLS];
+  __shared__ __align__(16) float part[MT][2][COLS];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int rank = blockIdx.x % cluster;
+  const int64_t f0 = static_cast<int64_t>(blockIdx.x / cluster) * COLS;
+  const int64_t f = f0 + lane * V;
+  const bool in = f < p.F;  // V divides F: all of a lane's columns or none
+  const T* w = static_cast<const T*>(p.w) + f;
+  const int64_t ld = 2ll * p.F;
+  const int k_end = min(p.K, (rank + 1) * p.k_per);
+  float g[MT][V], u[MT][V];
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int i = 0; i < V; ++i) g[m][i] = u[m][i] = 0.0f;
+  for (int k0 = rank * p.k_per; k0 < k_end; k0 += kChunk) {
+    const int n = min(kChunk, k_end - k0);
+    __syncthreads();
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+      for (int k = threadIdx.x; k < n; k += 32 * kWarps)
+        xs[k][m] = m < p.M ? to_f(static_cast<const T*>(p.x)[static_cast<int64_t>(m) * p.K + k0 + k])
+                           : 0.0f;
+    __syncthreads();
+    if (!in) continue;
+    for (int k = warp * U; k < n; k += kWarps * U) {
+      uint4 a[U], b[U];
+#pragma unroll
+      for (int i = 0; i < U; ++i)
+        if (k + i < n) {
+          const T* row = w + (k0 + k + i) * ld;
+          a[i] = stream16(row);
+          b[i] = stream16(row + p.F);
+        }
+#pragma unroll
+      for (int i = 0; i < U; ++i)
+        if (k + i < n) {
+          float wa[V], wb[V];
+          unpack<T>(a[i], wa);
+          unpack<T>(b[i], wb);
+          float xv[MT];
+          load_x<MT>(xs[k + i], xv);
+#pragma unroll
+          for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+              g[m][j] += xv[m] * wa[j];
+              u[m][j] += xv[m] * wb[j];
+            }
+        }
+    }
+  }
+  // the eight warps' sums, in their order, row by row
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    if (m > 0) __syncthreads();
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      red[warp][0][lane * V + j] = g[m][j];
+      red[warp][1][lane * V + j] = u[m][j];
+    }
+    __syncthreads();
+    for (int c = threadIdx.x; c < 2 * COLS; c += 32 * kWarps) {
+      float s = 0.0f;
+#pragma unroll
+      for (int v = 0; v < kWarps; ++v) s += (&red[v][0][0])[c];
+      (&part[m][0][0])[c] = s;
+    }
+  }
+  // the cluster's blocks each finish a share of the columns
+  if (cluster > 1) cluster_sync();
+  else __syncthreads();
+  const int share = COLS / cluster;
+  for (int i = threadIdx.x; i < share * MT; i += 32 * kWarps) {
+    const int m = i / share, c = rank * share + i % share;
+    if (m >= p.M || f0 + c >= p.F) continue;
+    float gs = 0.0f, us = 0.0f;
+    if (cluster == 1) {
+      gs = part[m][0][c];
+      us = part[m][1][c];
+    } else {
+      for (int r = 0; r < cluster; ++r) {
+        float v;
+        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr(&part[m][0][c], r)));
+        gs += v;
+        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr(&part[m][1][c], r)));
+        us += v;
+      }
+    }
+    finish<T>(p, m, static_cast<int>(f0 + c), gs, us);
+  }
+  if (cluster > 1) cluster_sync();  // no block leaves while its sums are read
+}
+
+// w [2F,K].  A warp makes FW columns of h for all rows, so that x is unpacked
+// once for 2 FW products.
+template <typename T, int MT>
+__global__ void __launch_bounds__(32 * kWarps, 2) skinny_nt_kernel(const Skinny p) {
+  constexpr int V = vec_of<T>(), FW = MT == 1 ? 1 : 2, U = MT == 1 ? 8 : 2;
+  const int lane = threadIdx.x & 31;
+  const int64_t f = (blockIdx.x * static_cast<int64_t>(kWarps) + (threadIdx.x >> 5)) * FW;
+  if (f >= p.F) return;
+  const T* wg[FW];
+  const T* wu[FW];
+#pragma unroll
+  for (int c = 0; c < FW; ++c) {  // past the last column: the last one again
+    const int64_t fc = f + c < p.F ? f + c : p.F - 1;
+    wg[c] = static_cast<const T*>(p.w) + fc * p.K;
+    wu[c] = static_cast<const T*>(p.w) + (fc + p.F) * p.K;
+  }
+  const T* x = static_cast<const T*>(p.x);
+  float g[FW][MT], u[FW][MT];
+#pragma unroll
+  for (int c = 0; c < FW; ++c)
+#pragma unroll
+    for (int m = 0; m < MT; ++m) g[c][m] = u[c][m] = 0.0f;
+  for (int64_t k0 = lane * V; k0 < p.K; k0 += 32 * V * U) {
+    uint4 a[U][FW], b[U][FW];
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+      if (k0 + i * 32 * V < p.K)
+#pragma unroll
+        for (int c = 0; c < FW; ++c) {
+          a[i][c] = stream16(wg[c] + k0 + i * 32 * V);
+          b[i][c] = stream16(wu[c] + k0 + i * 32 * V);
+        }
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int64_t k = k0 + i * 32 * V;
+      if (k < p.K) {
+        float wa[FW][V], wb[FW][V];
+#pragma unroll
+        for (int c = 0; c < FW; ++c) {
+          unpack<T>(a[i][c], wa[c]);
+          unpack<T>(b[i][c], wb[c]);
+        }
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+          if (m < p.M) {
+            float xv[V];
+            unpack<T>(__ldg(reinterpret_cast<const uint4*>(x + static_cast<int64_t>(m) * p.K + k)), xv);
+#pragma unroll
+            for (int c = 0; c < FW; ++c)
+#pragma unroll
+              for (int j = 0; j < V; ++j) {
+                g[c][m] += xv[j] * wa[c][j];
+                u[c][m] += xv[j] * wb[c][j];
+              }
+          }
+      }
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+    for (int c = 0; c < FW; ++c)
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        g[c][m] += __shfl_xor_sync(0xffffffffu, g[c][m], o);
+        u[c][m] += __shfl_xor_sync(0xffffffffu, u[c][m], o);
+      }
+#pragma unroll
+  for (int c = 0; c < FW; ++c)
+#pragma unroll
+    for (int m = 0; m < MT; ++m)  // a lane for each output
+      if (lane == c * MT + m && m < p.M && f + c < p.F)
+        finish<T>(p, m, static_cast<int>(f + c), g[c][m], u[c][m]);
+}
+
+template <typename T, int MT>
+cudaError_t launch(const Context* ctx, Skinny p, bool tw, cudaStream_t s) {
+  if (tw) {
+    constexpr int FW = MT == 1 ? 1 : 2;
+    const unsigned blocks = static_cast<unsigned>((p.F + kWarps * FW - 1) / (kWarps * FW));
+    skinny_nt_kernel<T, MT><<<blocks, 32 * kWarps, 0, s>>>(p);
+    return cudaGetLastError();
+  }
+  constexpr int COLS = 32 * vec_of<T>();
+  const int groups = (p.F + COLS - 1) / COLS;
+  // blocks that share a group's K: about two blocks an SM, at least 64 of K each
+  int cluster = 1;
+  while (cluster < 8 && groups * cluster < 2 * ctx->num_sms && p.K >= 128 * cluster) cluster *= 2;
+  p.k_per = (p.K + cluster - 1) / cluster;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(groups) * cluster);
+  cfg.blockDim = dim3(32 * kWarps);
+  cfg.stream = s;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = cluster;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, skinny_nn_kernel<T, MT>, p, cluster);
+}
+
+template <typename T>
+cudaError_t launch_rows(const Context* ctx, const Skinny& p, bool tw, cudaStream_t s) {
+  if (p.M == 1) return launch<T, 1>(ctx, p, tw, s);
+  if (p.M == 2) return launch<T, 2>(ctx, p, tw, s);
+  return launch<T, 4>(ctx, p, tw, s);
+}
+
+}  // namespace
+
+// Few rows, and 16-byte pieces of w (and, for w [2F,K], of x) that start on 16
+// bytes.
+bool gated_skinny_applies(const GatedArgs& a) {
+  const int v = a.dtype == MX_BF16 ? 8 : 4;
+  return !a.strict && a.M >= 1 && a.M <= 4 && a.K >= 1 && (a.tw ? a.K : a.F) % v == 0 &&
+         (reinterpret_cast<uintptr_t>(a.w) & 15u) == 0 &&
+         (!a.tw || (reinterpret_cast<uintptr_t>(a.x) & 15u) == 0);
+}
+
+int gated_skinny_fwd(Context* ctx, const GatedArgs& a, cudaStream_t s) {
+  const Skinny p{a.x, a.w, a.bias, a.h, a.pre, a.M, a.K, a.F, a.act, 0};
+  const cudaError_t e = a.dtype == MX_BF16 ? launch_rows<bf16>(ctx, p, a.tw != 0, s)
+                                           : launch_rows<float>(ctx, p, a.tw != 0, s);
+  note_launches(1);
+  return cuda_status(e);
+}
+
+}  // namespace mx

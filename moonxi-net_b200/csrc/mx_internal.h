@@ -246,6 +246,7 @@ struct GatedArgs {
   int dtype, M, K, F, tw, act;
   bool exact;   // float32 products on the SIMT kernels
   bool strict;  // ... in NpArray order
+  bool tensor;  // ... on the tensor cores, whatever the shape
   const void* x;
   const void* w;
   const void* bias;
@@ -257,6 +258,9 @@ struct GatedArgs {
   size_t ws_bytes;
 };
 size_t gated_workspace_bytes(const Context* ctx, const GatedArgs& a, bool backward);
+// A few rows (gated_skinny.cu): one launch, no workspace.
+bool gated_skinny_applies(const GatedArgs& a);
+int gated_skinny_fwd(Context* ctx, const GatedArgs& a, cudaStream_t s);
 int gated_fwd(Context* ctx, const GatedArgs& a, cudaStream_t s);
 int gated_bwd(Context* ctx, const GatedArgs& a, cudaStream_t s);
 size_t adamw_scratch_bytes(int count, int clip);
