@@ -430,9 +430,11 @@ uint64_t mx_layer_norm_bwd_scratch_bytes(void* handle, int32_t rows, int32_t col
 /* The gated linear layer: with [g | u] = x[M,K] op(w) + bias[2F],
  * h[M,F] = act(g) * u.  transpose_w = 0: w stored [K,2F]; 1: [2F,K]; the
  * gate's F columns (rows) come first, then the other projection's.  x, w,
- * bias, h: dtype, packed.  bias may be NULL.  pre (may be NULL) receives
- * [g | u] as float32[M,2F] for the backward pass: kept in 32 bits so that the
- * gradients are rounded once.  float32 products are float32-class (relative
+ * bias, h: dtype, packed.  bias may be NULL.  pre (may be NULL, 32-byte
+ * aligned) receives [g | u] for the backward pass as float32[M,2P], P = F
+ * rounded up to a multiple of 8, g in the first F columns of a row and u from
+ * column P on: kept in 32 bits so that the gradients are rounded once, padded
+ * so that its rows are aligned.  float32 products are float32-class (relative
  * error below 1e-6 of the terms' size), on tensor cores where the shape is
  * large; MX_PREC_FP32 on the context or here keeps them on the exact SIMT
  * kernels.  An infinite x or w gives NaN where it meets a float32 tensor-core

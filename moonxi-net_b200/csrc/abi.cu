@@ -876,6 +876,7 @@ MX_EXPORT int32_t mx_gated_linear_fwd(void* handle, int32_t dtype, const void* x
   if (rc != kOk) return rc;
   if (M == 0 || F == 0) return MX_OK;
   if (!h || (K > 0 && (!x || !w))) return MX_ERR_INVALID;
+  if ((reinterpret_cast<uintptr_t>(pre) & 31u) != 0) return MX_ERR_INVALID;
   a.x = x; a.w = w; a.bias = bias; a.h = h; a.pre = pre;
   a.ws = workspace; a.ws_bytes = workspace_bytes;
   const size_t need = gated_workspace_bytes(c, a, false);
@@ -907,6 +908,7 @@ MX_EXPORT int32_t mx_gated_linear_bwd(void* handle, int32_t dtype, const void* d
     dx = dw = nullptr;  // K == 0: the bias alone has a gradient
   }
   if (!dh || !pre || (dx && !w) || (dw && !x)) return MX_ERR_INVALID;
+  if ((reinterpret_cast<uintptr_t>(pre) & 31u) != 0) return MX_ERR_INVALID;
   a.x = x; a.w = w; a.dh = dh; a.pre = const_cast<float*>(pre);
   a.dx = dx; a.dw = dw; a.dbias = dbias;
   a.ws = workspace; a.ws_bytes = workspace_bytes;

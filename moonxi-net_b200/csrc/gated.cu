@@ -69,26 +69,35 @@ __device__ __forceinline__ void load8(const bf16* p, float (&x)[8]) {
 // Copies of a row-major [rows][cols] matrix with rows of ldd elements (a
 // multiple of 8): columns below `split` at 0, the others from `up` on, zeros
 // between.  A thread makes 8 columns.
-template <typename T, int NC, bool VEC>
-__global__ void __launch_bounds__(256) pack_kernel(const T* __restrict__ src, int64_t ld, int rows,
-                                                   int cols, int split, int up,
-                                                   bf16* __restrict__ dst, int64_t ldd,
-                                                   int64_t copy) {
+struct PackJob {
+  const void* src;
+  bf16* dst;
+  int64_t ldd, copy;
+  int rows, cols, split, up;
+  int vec;  // rows start on 16 bytes, and nothing is moved
+};
+struct PackJobs {
+  PackJob job[2];
+};
+template <typename T, int NC>
+__global__ void __launch_bounds__(256) pack_kernel(const __grid_constant__ PackJobs jobs) {
+  const PackJob& p = jobs.job[blockIdx.z];
   const int64_t d = (blockIdx.x * 256ll + threadIdx.x) * 8;
-  if (d >= ldd) return;
-  for (int64_t r = blockIdx.y; r < rows; r += gridDim.y) {
+  if (d >= p.ldd) return;
+  const T* src = static_cast<const T*>(p.src);
+  for (int64_t r = blockIdx.y; r < p.rows; r += gridDim.y) {
     float x[8];
-    if (VEC) {
-      load8(src + r * ld + d, x);
+    if (p.vec) {
+      load8(src + r * p.cols + d, x);
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const int64_t e = d + i;
-        const int64_t c = e < up ? (e < split ? e : cols) : split + (e - up);
-        x[i] = c < cols ? to_f(src[r * ld + c]) : 0.0f;
+        const int64_t c = e < p.up ? (e < p.split ? e : p.cols) : p.split + (e - p.up);
+        x[i] = c < p.cols ? to_f(src[r * p.cols + c]) : 0.0f;
       }
     }
-    store_copies<NC>(x, dst + r * ldd + d, copy);
+    store_copies<NC>(x, p.dst + r * p.ldd + d, p.copy);
   }
 }
 
@@ -99,62 +108,68 @@ struct Dpre {
   int64_t ldo, copy;
   float* part;    // [row blocks][2F], or null
   int rows, F, act, per;  // per: rows of a block
+  int vec;        // dh's rows and the output's halves start on 16 bytes
 };
 
-// A block: 32 * V columns of both halves, `per` rows, its eight warps a row at
-// a time.  V = 8: 16-byte accesses.  Bound by the bytes: with bfloat16 tensors
-// 10 read and 4 written a value of h.
-template <typename T, int OUT, int V>
+// A block: 256 columns of both halves, `per` rows, its eight warps a row at a
+// time, a lane 8 columns.  Bound by the bytes: with bfloat16 tensors 10 read
+// and 4 written a value of h (8192 x 8192: 157 us, 91 % of the copy rate).
+template <typename T, int OUT>
 __global__ void __launch_bounds__(256) dpre_kernel(const Dpre p) {
-  __shared__ float sh[8][32 * V];
+  __shared__ float sh[8][256];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t f = (blockIdx.x * 32ll + lane) * V;
+  const int64_t f = (blockIdx.x * 32ll + lane) * 8, up = (p.F + 7) & ~7ll;
   const int64_t r0 = blockIdx.y * static_cast<int64_t>(p.per);
   const int64_t r1 = r0 + p.per < p.rows ? r0 + p.per : p.rows;
-  float sg[V], su[V];
+  float sg[8], su[8];
 #pragma unroll
-  for (int i = 0; i < V; ++i) sg[i] = su[i] = 0.0f;
+  for (int i = 0; i < 8; ++i) sg[i] = su[i] = 0.0f;
   if (f < p.F) {
+    const int left = static_cast<int>(p.F - f < 8 ? p.F - f : 8);
     for (int64_t r = r0 + warp; r < r1; r += 8) {
       const T* dh = static_cast<const T*>(p.dh) + r * p.F + f;
-      const float* pre = p.pre + r * 2 * p.F + f;
-      float d[V], g[V], u[V];
-      if constexpr (V == 8) {
+      const float* pre = p.pre + r * 2 * up + f;
+      float d[8], g[8], u[8];
+      if (p.vec) {
         load8(dh, d);
-        load8(pre, g);
-        load8(pre + p.F, u);
       } else {
-        d[0] = to_f(*dh);
-        g[0] = pre[0];
-        u[0] = pre[p.F];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) d[i] = i < left ? to_f(dh[i]) : 0.0f;
       }
+      load8(pre, g);  // pre's rows are padded
+      load8(pre + up, u);
       gate_grad(p.act, d, g, u);
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
+      for (int i = 0; i < 8; ++i) {
         sg[i] += g[i];
         su[i] += u[i];
       }
       if constexpr (OUT == 0) {
         float* out = static_cast<float*>(p.out) + r * p.ldo + f;
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          out[i] = g[i];
-          out[p.F + i] = u[i];
-        }
-      } else if constexpr (V == 8) {
-        bf16* out = static_cast<bf16*>(p.out) + r * p.ldo + f;
-        store_copies<OUT>(g, out, p.copy);
-        store_copies<OUT>(u, out + p.F, p.copy);
+        for (int i = 0; i < 8; ++i)
+          if (i < left) {
+            out[i] = g[i];
+            out[p.F + i] = u[i];
+          }
       } else {
         bf16* out = static_cast<bf16*>(p.out) + r * p.ldo + f;
-        float x = g[0], y = u[0];
+        if (p.vec) {
+          store_copies<OUT>(g, out, p.copy);
+          store_copies<OUT>(u, out + p.F, p.copy);
+        } else {
 #pragma unroll
-        for (int c = 0; c < OUT; ++c) {
-          const bf16 a = __float2bfloat16_rn(x), b = __float2bfloat16_rn(y);
-          out[c * p.copy] = a;
-          out[c * p.copy + p.F] = b;
-          x -= __bfloat162float(a);
-          y -= __bfloat162float(b);
+          for (int c = 0; c < OUT; ++c)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const bf16 a = __float2bfloat16_rn(g[i]), b = __float2bfloat16_rn(u[i]);
+              if (i < left) {
+                out[c * p.copy + i] = a;
+                out[c * p.copy + p.F + i] = b;
+              }
+              g[i] -= __bfloat162float(a);
+              u[i] -= __bfloat162float(b);
+            }
         }
       }
     }
@@ -165,10 +180,10 @@ __global__ void __launch_bounds__(256) dpre_kernel(const Dpre p) {
   for (int h = 0; h < 2; ++h) {  // the eight warps' sums, in their order
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < V; ++i) sh[warp][lane * V + i] = h ? su[i] : sg[i];
+    for (int i = 0; i < 8; ++i) sh[warp][lane * 8 + i] = h ? su[i] : sg[i];
     __syncthreads();
-    const int64_t c = blockIdx.x * 32ll * V + threadIdx.x;
-    if (threadIdx.x < 32 * V && c < p.F) {
+    const int64_t c = blockIdx.x * 256ll + threadIdx.x;
+    if (c < p.F) {
       float s = 0.0f;
 #pragma unroll
       for (int w = 0; w < 8; ++w) s += sh[w][threadIdx.x];
@@ -196,26 +211,25 @@ __global__ void __launch_bounds__(256) dbias_kernel(const float* part, T* out, i
   }
 }
 
-// h from a complete [g | u] (the SIMT products); K = 0: [g | u] is the bias.
+// h and pre from the SIMT product's [M][2F] (bias included); without one, K = 0,
+// [g | u] is the bias.
 template <typename T>
-__global__ void __launch_bounds__(256) gate_kernel(const float* pre, T* h, int64_t n, int F,
-                                                   int act) {
+__global__ void __launch_bounds__(256) gate_kernel(const float* gu, const T* bias, float* pre, T* h,
+                                                   int64_t n, int F, int act) {
+  const int64_t up = (F + 7) & ~7ll;
   for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
     const int64_t m = i / F, f = i - m * F;
-    float g[1] = {pre[m * 2 * F + f]}, u[1] = {pre[m * 2 * F + F + f]};
-    gate(act, g, u);
-    put(h + i, g[0]);
-  }
-}
-template <typename T>
-__global__ void __launch_bounds__(256) bias_rows_kernel(const T* bias, float* pre, T* h, int64_t n,
-                                                        int F, int act) {
-  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
-    const int64_t m = i / F, f = i - m * F;
-    float g[1] = {bias ? to_f(bias[f]) : 0.0f}, u[1] = {bias ? to_f(bias[F + f]) : 0.0f};
+    float g[1], u[1];
+    if (gu) {
+      g[0] = gu[m * 2 * F + f];
+      u[0] = gu[m * 2 * F + F + f];
+    } else {
+      g[0] = bias ? to_f(bias[f]) : 0.0f;
+      u[0] = bias ? to_f(bias[F + f]) : 0.0f;
+    }
     if (pre) {
-      pre[m * 2 * F + f] = g[0];
-      pre[m * 2 * F + F + f] = u[0];
+      pre[m * 2 * up + f] = g[0];
+      pre[m * 2 * up + up + f] = u[0];
     }
     gate(act, g, u);
     put(h + i, g[0]);
@@ -271,30 +285,39 @@ Packed packed_of(const GatedArgs& a, const void* src, int rows, int64_t cols, bo
 size_t packed_bytes(const GatedArgs& a, const Packed& p) {
   return p.direct ? 0 : static_cast<size_t>(copies_of(a)) * p.copy * 2;
 }
-// The operand of a matrix: packed into `dst` unless it is read as it is.
-cudaError_t pack(Context* ctx, const GatedArgs& a, const void* src, int rows, int64_t cols,
-                 const Packed& p, bool halves, bf16* dst, cudaStream_t s, Bf16Operand& o) {
-  o.copy = p.copy;
-  o.ld = p.ld;
-  o.base = p.direct ? src : dst;
-  if (p.direct) return cudaSuccess;
-  const int split = static_cast<int>(halves ? cols / 2 : cols);
-  const dim3 grid(static_cast<unsigned>((p.ld / 8 + 255) / 256),
-                  static_cast<unsigned>(std::min(rows, 32768)));
-  const bool vec = cols == p.ld && (!halves || p.up == split) && aligned16(src);
-  const int n = static_cast<int>(cols), up = static_cast<int>(p.up);
-  if (a.dtype == MX_BF16)
-    pack_kernel<bf16, 1, false><<<grid, 256, 0, s>>>(static_cast<const bf16*>(src), cols, rows, n,
-                                                     split, up, dst, p.ld, p.copy);
-  else if (vec)
-    pack_kernel<float, 3, true><<<grid, 256, 0, s>>>(static_cast<const float*>(src), cols, rows,
-                                                     n, split, up, dst, p.ld, p.copy);
-  else
-    pack_kernel<float, 3, false><<<grid, 256, 0, s>>>(static_cast<const float*>(src), cols, rows,
-                                                      n, split, up, dst, p.ld, p.copy);
-  note_launches(1);
-  return cudaGetLastError();
-}
+// The operands of one or two matrices: packed into their places in one launch,
+// unless they are read as they are.
+struct Packing {
+  PackJobs jobs;
+  int count = 0;
+  Bf16Operand add(const void* src, int rows, int64_t cols, const Packed& p, bool halves, bf16* dst) {
+    Bf16Operand o;
+    o.copy = p.copy;
+    o.ld = p.ld;
+    o.base = p.direct ? src : dst;
+    if (p.direct) return o;
+    const int split = static_cast<int>(halves ? cols / 2 : cols);
+    const bool vec = cols == p.ld && (!halves || p.up == split) && aligned16(src);
+    jobs.job[count++] = PackJob{src, dst, p.ld, p.copy, rows, static_cast<int>(cols), split,
+                                static_cast<int>(p.up), vec ? 1 : 0};
+    return o;
+  }
+  cudaError_t run(const GatedArgs& a, cudaStream_t s) {
+    if (count == 0) return cudaSuccess;
+    int64_t ld = 0;
+    int rows = 0;
+    for (int i = 0; i < count; ++i) {
+      ld = std::max(ld, jobs.job[i].ldd);
+      rows = std::max(rows, jobs.job[i].rows);
+    }
+    const dim3 grid(static_cast<unsigned>((ld / 8 + 255) / 256),
+                    static_cast<unsigned>(std::min(rows, 16384)), count);
+    if (a.dtype == MX_BF16) pack_kernel<bf16, 1><<<grid, 256, 0, s>>>(jobs);
+    else pack_kernel<float, 3><<<grid, 256, 0, s>>>(jobs);
+    note_launches(1);
+    return cudaGetLastError();
+  }
+};
 
 // An exact SIMT product on scratch of its own (no workspace or counters of the
 // context, so calls on different streams may overlap).
@@ -335,7 +358,7 @@ struct FwdWork {
   Packed x, w;
   bf16 *xp, *wp;
   float* parts;
-  float* pre;       // SIMT: [g | u] when the caller saves none
+  float* pre;       // SIMT: [g | u]
   void* scratch;
   size_t scratch_bytes, bytes;
 };
@@ -353,7 +376,7 @@ FwdWork fwd_work(const Context* ctx, const GatedArgs& a) {
     w.wp = c.take<bf16>(packed_bytes(a, w.w));
     w.parts = c.take<float>(bf16_gemm_scratch_bytes(ctx, a.M, a.F, a.K, true, copies_of(a)));
   } else {
-    w.pre = a.pre ? a.pre : c.take<float>(static_cast<size_t>(a.M) * 2 * a.F * sizeof(float));
+    w.pre = c.take<float>(static_cast<size_t>(a.M) * 2 * a.F * sizeof(float));
     w.scratch_bytes = simt_scratch(
         ctx, simt_args(a, nullptr, nullptr, nullptr, a.M, a.K, 2 * a.F, 0, a.tw, nullptr));
     w.scratch = c.take<void>(w.scratch_bytes);
@@ -366,8 +389,8 @@ template <typename T>
 int fwd(Context* ctx, const GatedArgs& a, cudaStream_t s) {
   const int64_t n = static_cast<int64_t>(a.M) * a.F;
   if (a.K == 0) {
-    bias_rows_kernel<T><<<grid_for(n, ctx->num_sms), 256, 0, s>>>(
-        static_cast<const T*>(a.bias), a.pre, static_cast<T*>(a.h), n, a.F, a.act);
+    gate_kernel<T><<<grid_for(n, ctx->num_sms), 256, 0, s>>>(
+        nullptr, static_cast<const T*>(a.bias), a.pre, static_cast<T*>(a.h), n, a.F, a.act);
     note_launches(1);
     return cuda_status(cudaGetLastError());
   }
@@ -378,16 +401,17 @@ int fwd(Context* ctx, const GatedArgs& a, cudaStream_t s) {
     const GemmArgs g = simt_args(a, a.x, a.w, w.pre, a.M, a.K, 2 * a.F, 0, a.tw, a.bias);
     const int rc = simt_product(ctx, g, w.scratch, w.scratch_bytes, s);
     if (rc != kOk) return rc;
-    gate_kernel<T><<<grid_for(n, ctx->num_sms), 256, 0, s>>>(w.pre, static_cast<T*>(a.h), n, a.F,
-                                                             a.act);
+    gate_kernel<T><<<grid_for(n, ctx->num_sms), 256, 0, s>>>(w.pre, nullptr, a.pre,
+                                                             static_cast<T*>(a.h), n, a.F, a.act);
     note_launches(1);
     return cuda_status(cudaGetLastError());
   }
   Bf16Gemm g;
-  cudaError_t e = pack(ctx, a, a.x, a.M, a.K, w.x, false, w.xp, s, g.a);
-  if (e == cudaSuccess)
-    e = a.tw ? pack(ctx, a, a.w, 2 * a.F, a.K, w.w, false, w.wp, s, g.b)
-             : pack(ctx, a, a.w, a.K, 2ll * a.F, w.w, true, w.wp, s, g.b);
+  Packing pk;
+  g.a = pk.add(a.x, a.M, a.K, w.x, false, w.xp);
+  g.b = a.tw ? pk.add(a.w, 2 * a.F, a.K, w.w, false, w.wp)
+             : pk.add(a.w, a.K, 2ll * a.F, w.w, true, w.wp);
+  const cudaError_t e = pk.run(a, s);
   if (e != cudaSuccess) return cuda_status(e);
   g.a.kmajor = true;
   g.b.kmajor = a.tw != 0;
@@ -454,12 +478,9 @@ BwdWork bwd_work(const Context* ctx, const GatedArgs& a) {
 }
 
 template <typename T, int OUT>
-void launch_dpre(const Dpre& p, int row_blocks, cudaStream_t s) {
-  const bool vec = p.F % 8 == 0 && aligned16(p.dh) && aligned16(p.pre);
-  const int width = vec ? 256 : 32;
-  const dim3 grid((p.F + width - 1) / width, row_blocks);
-  if (vec) dpre_kernel<T, OUT, 8><<<grid, 256, 0, s>>>(p);
-  else dpre_kernel<T, OUT, 1><<<grid, 256, 0, s>>>(p);
+void launch_dpre(Dpre p, int row_blocks, cudaStream_t s) {
+  p.vec = p.F % 8 == 0 && aligned16(p.dh) ? 1 : 0;
+  dpre_kernel<T, OUT><<<dim3((p.F + 255) / 256, row_blocks), 256, 0, s>>>(p);
   note_launches(1);
 }
 
@@ -469,7 +490,7 @@ int bwd(Context* ctx, const GatedArgs& a, cudaStream_t s) {
   if (w.bytes > a.ws_bytes) return kErrInvalid;
   const bool tensor = tensor_path(a);
   const int F2 = 2 * a.F;
-  const Dpre p{a.dh, a.pre, w.dpre, w.ldp, w.copy, a.dbias ? w.part : nullptr, a.M, a.F, a.act, w.per};
+  const Dpre p{a.dh, a.pre, w.dpre, w.ldp, w.copy, a.dbias ? w.part : nullptr, a.M, a.F, a.act, w.per, 0};
   if (a.dtype == MX_BF16) launch_dpre<bf16, 1>(p, w.row_blocks, s);
   else if (tensor) launch_dpre<float, 3>(p, w.row_blocks, s);
   else launch_dpre<float, 0>(p, w.row_blocks, s);
@@ -493,18 +514,21 @@ int bwd(Context* ctx, const GatedArgs& a, cudaStream_t s) {
                         w.scratch, w.scratch_bytes, s);
     return rc;
   }
-  Bf16Operand d;
+  Bf16Operand d, x, wt;
   d.base = w.dpre;
   d.copy = w.copy;
   d.ld = w.ldp;
+  Packing pk;
+  if (a.dx) wt = a.tw ? pk.add(a.w, F2, a.K, w.w, false, w.wp) : pk.add(a.w, a.K, F2, w.w, false, w.wp);
+  if (a.dw) x = pk.add(a.x, a.M, a.K, w.x, false, w.xp);
+  e = pk.run(a, s);
+  if (e != cudaSuccess) return cuda_status(e);
   Bf16Gemm g;
   g.copies = copies_of(a);
   g.parts = w.parts;
   if (a.dx) {
-    e = a.tw ? pack(ctx, a, a.w, F2, a.K, w.w, false, w.wp, s, g.b)
-             : pack(ctx, a, a.w, a.K, F2, w.w, false, w.wp, s, g.b);
-    if (e != cudaSuccess) return cuda_status(e);
     g.a = d;
+    g.b = wt;
     g.a.kmajor = true;
     g.b.kmajor = !a.tw;
     g.M = a.M; g.N = a.K; g.K = F2;
@@ -513,21 +537,16 @@ int bwd(Context* ctx, const GatedArgs& a, cudaStream_t s) {
     const int rc = bf16_gemm(ctx, g, s);
     if (rc != kOk) return rc;
   }
-  if (a.dw) {
-    Bf16Operand x;
-    e = pack(ctx, a, a.x, a.M, a.K, w.x, false, w.xp, s, x);
-    if (e != cudaSuccess) return cuda_status(e);
-    g.a = a.tw ? d : x;
-    g.b = a.tw ? x : d;
-    g.a.kmajor = g.b.kmajor = false;
-    g.M = a.tw ? F2 : a.K;
-    g.N = a.tw ? a.K : F2;
-    g.K = a.M;
-    g.out = a.dw;
-    g.ldc = g.N;
-    return bf16_gemm(ctx, g, s);
-  }
-  return kOk;
+  if (!a.dw) return kOk;
+  g.a = a.tw ? d : x;
+  g.b = a.tw ? x : d;
+  g.a.kmajor = g.b.kmajor = false;
+  g.M = a.tw ? F2 : a.K;
+  g.N = a.tw ? a.K : F2;
+  g.K = a.M;
+  g.out = a.dw;
+  g.ldc = g.N;
+  return bf16_gemm(ctx, g, s);
 }
 
 }  // namespace

@@ -68,8 +68,9 @@ __device__ __forceinline__ void finish(const Skinny& p, int m, int f, float g, f
     u += to_f(static_cast<const T*>(p.bias)[p.F + f]);
   }
   if (p.pre) {
-    p.pre[m * 2ll * p.F + f] = g;
-    p.pre[m * 2ll * p.F + p.F + f] = u;
+    const int64_t up = (p.F + 7) & ~7ll;  // pre's halves are padded to 8
+    p.pre[m * 2 * up + f] = g;
+    p.pre[m * 2 * up + up + f] = u;
   }
   float ga[1] = {g}, ua[1] = {u};
   gate(p.act, ga, ua);

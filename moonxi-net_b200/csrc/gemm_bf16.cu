@@ -30,8 +30,9 @@
 // columns of a row in 32-byte pieces, whole sectors.  They stay off the shared
 // memory, which the MMAs' operand reads and the TMA writes fill between them: a
 // transpose there took the forward product of 8192 x 4096 x 2 x 8192 from 0.81
-// to 1.6 ms.  Only where rows are not 32-byte aligned do they transpose through
-// padded shared memory, to store whole rows of odd width.  Two accumulators: a tile's epilogue runs
+// to 1.6 ms.  Only where the output's rows are not 16-byte aligned do they
+// transpose through padded shared memory, to store whole rows of odd width
+// (pre and the partial tiles have padded rows).  Two accumulators: a tile's epilogue runs
 // beside the next tile's (three copies: the next stage's) MMAs.
 // Few tiles and a long K: the K range is split over the pairs, fp32 partial
 // tiles go to scratch and a second kernel adds them in order.
@@ -72,7 +73,7 @@ struct Params {
   void* out;
   const void* bias;
   float* pre;
-  float* parts;     // [splits][M][width] when the K range is split
+  float* parts;     // [splits][M][ldp] when the K range is split
   int* status;
   int64_t ldc;
   uint64_t timeout_ns;
@@ -80,7 +81,8 @@ struct Params {
   int tiles_m, tiles_n, tiles;
   int splits, kb_per;  // k-blocks of a split
   int act;
-  int vec;             // 32-byte stores: rows and halves start on 32 bytes
+  int64_t ldp;         // row of parts: pad8(N), gated twice that, like pre
+  int vec;             // bytes of a store to out: 32, 16, or 0 (rows unaligned)
 };
 
 // Bands of 8 tiles of rows, column by column inside a band: the pairs that run
@@ -116,29 +118,38 @@ __device__ __forceinline__ uint64_t slice_desc(uint32_t addr, int j) {
                 : sdesc_mnmajor(addr + j * 2048, kOpBytes / 2, 1024, 2);
 }
 
-// 32 consecutive values of a row, in 32-byte stores; `left` columns remain (a
-// multiple of a store's).
+__device__ __forceinline__ int64_t pad8(int64_t n) { return (n + 7) & ~7ll; }
+
+// 32 consecutive values of a row in stores of BYTES; `left` columns remain, and
+// a store that begins before the last of them may end after it.
+template <int BYTES>
 __device__ __forceinline__ void store_row(float* p, const float (&v)[32], int left) {
 #pragma unroll
-  for (int i = 0; i < 32; i += 8)
+  for (int i = 0; i < 32; i += BYTES / 4)
     if (i < left) {
-      uint32_t r[8];
+      if constexpr (BYTES == 32) {
+        uint32_t r[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) r[j] = __float_as_uint(v[i + j]);
-      st_global_32b(p + i, r);
+        for (int j = 0; j < 8; ++j) r[j] = __float_as_uint(v[i + j]);
+        st_global_32b(p + i, r);
+      } else {
+        *reinterpret_cast<float4*>(p + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+      }
     }
 }
+template <int BYTES>
 __device__ __forceinline__ void store_row(__nv_bfloat16* p, const float (&v)[32], int left) {
 #pragma unroll
-  for (int i = 0; i < 32; i += 16)
+  for (int i = 0; i < 32; i += BYTES / 2)
     if (i < left) {
       uint32_t r[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
+      for (int j = 0; j < BYTES / 4; ++j) {
         const __nv_bfloat162 h = __floats2bfloat162_rn(v[i + 2 * j], v[i + 2 * j + 1]);
         r[j] = *reinterpret_cast<const uint32_t*>(&h);
       }
-      st_global_32b(p + i, r);
+      if constexpr (BYTES == 32) st_global_32b(p + i, r);
+      else *reinterpret_cast<uint4*>(p + i) = make_uint4(r[0], r[1], r[2], r[3]);
     }
 }
 
@@ -323,14 +334,28 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       tmem_ld_32cols(lanes + acc * kTile + col, r);
       tmem_wait_ld();
     };
-    // lane = row -> lane = column: v[i] becomes row i's value of column `lane`
-    auto turn = [&](float (&v)[32]) {
-      __syncwarp();  // the last reads are done
+    // a block of `out`: 32 columns of this warp's rows, lane = row
+    auto store_out = [&](T* out, int64_t row0, int rows, int col0, const float (&v)[32]) {
+      T* dst = out + (row0 + lane) * p.ldc + col0;
+      const int left = p.N - col0;
+      if (p.vec == 32) {
+        if (lane < rows) store_row<32>(dst, v, left);
+      } else if (p.vec == 16) {
+        if (lane < rows) store_row<16>(dst, v, left);
+      } else {
+        // unaligned rows: through shared memory, a row at a time
+        __syncwarp();  // the last block's reads are done
 #pragma unroll
-      for (int i = 0; i < 32; ++i) tw[lane * 33 + i] = v[i];
-      __syncwarp();
-#pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] = tw[i * 33 + lane];
+        for (int i = 0; i < 32; ++i) tw[lane * 33 + i] = v[i];
+        __syncwarp();
+        dst = out + row0 * p.ldc + col0 + lane;
+        if (lane < left)
+#pragma unroll 4
+          for (int i = 0; i < rows; ++i) {
+            put(dst, tw[i * 33 + lane]);
+            dst += p.ldc;
+          }
+      }
     };
     auto wait_acc = [&]() {
       if (!wait_bar(&acc_full[seg & 1], seg >> 1 & 1, abort_flag, p.status, p.timeout_ns, 404))
@@ -389,87 +414,50 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
         }
       };
+      // (one copy: the loops stay rolled, the instruction cache holds one body)
+      const bool mine = lane < rows;
       if constexpr (GATED) {
-        // (one copy: rolled, the registers are loaded inside)
 #pragma unroll(NC == 3 ? 2 : 1)
         for (int q = 0; q < 4; q += 2) {
           const int col0 = tn * kHalf + half * 64 + (q >> 1) * 32;
+          const int left = p.N - col0;
           float g[32], u[32];
           block(q, g);
           block(q + 1, u);
-          const int64_t ld2 = 2ll * p.N;
-          float* pre = p.parts ? p.parts + static_cast<int64_t>(split) * p.M * ld2 : p.pre;
-          T* h = static_cast<T*>(p.out);
-          if (p.vec) {
-            const int64_t row = row0 + lane;
-            if (lane >= rows || col0 >= p.N) continue;
-            if (p.bias && !p.parts) {
+          if (left <= 0) continue;
+          if (p.bias && !p.parts) {
+            const T* bias = static_cast<const T*>(p.bias) + col0;
 #pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if (col0 + i < p.N) {
-                  g[i] += to_f(static_cast<const T*>(p.bias)[col0 + i]);
-                  u[i] += to_f(static_cast<const T*>(p.bias)[p.N + col0 + i]);
-                }
-            }
-            if (pre) {
-              store_row(pre + row * ld2 + col0, g, p.N - col0);
-              store_row(pre + row * ld2 + p.N + col0, u, p.N - col0);
-            }
-            if (!p.parts) {
-              gate(p.act, g, u);
-              store_row(h + row * p.ldc + col0, g, p.N - col0);
-            }
-          } else {
-            turn(g);
-            turn(u);
-            const int col = col0 + lane;
-            const bool in = col < p.N;
-            float bg = 0.0f, bu = 0.0f;
-            if (p.bias && in && !p.parts) {
-              bg = to_f(static_cast<const T*>(p.bias)[col]);
-              bu = to_f(static_cast<const T*>(p.bias)[p.N + col]);
-            }
-#pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              const int64_t row = row0 + i;
-              g[i] += bg;
-              u[i] += bu;
-              if (pre && in && i < rows) {
-                pre[row * ld2 + col] = g[i];
-                pre[row * ld2 + p.N + col] = u[i];
+            for (int i = 0; i < 32; ++i)
+              if (i < left) {
+                g[i] += to_f(bias[i]);
+                u[i] += to_f(bias[p.N + i]);
               }
-            }
-            if (!p.parts) {
-              gate(p.act, g, u);
-#pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if (in && i < rows) put(h + (row0 + i) * p.ldc + col, g[i]);
-            }
+          }
+          float* pre = p.parts ? p.parts + static_cast<int64_t>(split) * p.M * p.ldp : p.pre;
+          if (pre && mine) {
+            pre += static_cast<int64_t>(row0 + lane) * p.ldp + col0;
+            store_row<32>(pre, g, left);
+            store_row<32>(pre + p.ldp / 2, u, left);
+          }
+          if (!p.parts) {
+            gate(p.act, g, u);
+            store_out(static_cast<T*>(p.out), row0, rows, col0, g);
           }
         }
       } else {
-#pragma unroll
+#pragma unroll(NC == 3 ? 4 : 1)
         for (int q = 0; q < 4; ++q) {
           const int col0 = tn * kTile + col_of(q);
           float v[32];
           block(q, v);
-          float* part = p.parts ? p.parts + static_cast<int64_t>(split) * p.M * p.N : nullptr;
-          T* out = static_cast<T*>(p.out);
-          if (p.vec) {
-            const int64_t row = row0 + lane;
-            if (lane >= rows || col0 >= p.N) continue;
-            if (part) store_row(part + row * p.N + col0, v, p.N - col0);
-            else store_row(out + row * p.ldc + col0, v, p.N - col0);
+          if (col0 >= p.N) continue;
+          if (p.parts) {
+            if (mine)
+              store_row<32>(p.parts + (static_cast<int64_t>(split) * p.M + row0 + lane) * p.ldp + col0,
+                            v, p.N - col0);
           } else {
-            turn(v);
-            const int col = col0 + lane;
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (col < p.N && i < rows) {
-                const int64_t row = row0 + i;
-                if (part) part[row * p.N + col] = v[i];
-                else put(out + row * p.ldc + col, v[i]);
-              }
+            store_out(static_cast<T*>(p.out), row0, rows, col0, v);
           }
         }
       }
@@ -487,31 +475,41 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 }
 
 // The sum of a split product's parts, in order; gated: bias and activation too.
+// A thread takes four columns.
 template <typename T, bool GATED>
 __global__ void __launch_bounds__(256) join_kernel(const Params p) {
-  const int64_t width = GATED ? 2ll * p.N : p.N, n = static_cast<int64_t>(p.M) * p.N;
+  const int64_t quads = pad8(p.N) / 4, n = p.M * quads, part = p.M * p.ldp;
   for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
-    const int64_t m = i / p.N, c = i - m * p.N;
-    const float* src = p.parts + m * width + c;
-    float g = 0.0f, u = 0.0f;
+    const int64_t m = i / quads;
+    const int c = static_cast<int>(i - m * quads) * 4;
+    const float* src = p.parts + m * p.ldp + c;
+    float g[4] = {0.0f, 0.0f, 0.0f, 0.0f}, u[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     for (int s = 0; s < p.splits; ++s) {
-      g += src[s * p.M * width];
-      if (GATED) u += src[s * p.M * width + p.N];
+      const float4 a = *reinterpret_cast<const float4*>(src + s * part);
+      g[0] += a.x; g[1] += a.y; g[2] += a.z; g[3] += a.w;
+      if (GATED) {
+        const float4 b = *reinterpret_cast<const float4*>(src + s * part + p.ldp / 2);
+        u[0] += b.x; u[1] += b.y; u[2] += b.z; u[3] += b.w;
+      }
     }
     if (GATED) {
-      if (p.bias) {
-        g += to_f(static_cast<const T*>(p.bias)[c]);
-        u += to_f(static_cast<const T*>(p.bias)[p.N + c]);
-      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (p.bias && c + j < p.N) {
+          g[j] += to_f(static_cast<const T*>(p.bias)[c + j]);
+          u[j] += to_f(static_cast<const T*>(p.bias)[p.N + c + j]);
+        }
       if (p.pre) {
-        p.pre[m * width + c] = g;
-        p.pre[m * width + p.N + c] = u;
+        *reinterpret_cast<float4*>(p.pre + m * p.ldp + c) = make_float4(g[0], g[1], g[2], g[3]);
+        *reinterpret_cast<float4*>(p.pre + m * p.ldp + p.ldp / 2 + c) =
+            make_float4(u[0], u[1], u[2], u[3]);
       }
-      float ga[1] = {g}, ua[1] = {u};
-      gate(p.act, ga, ua);
-      g = ga[0];
+      gate(p.act, g, u);
     }
-    put(static_cast<T*>(p.out) + m * p.ldc + c, g);
+    T* out = static_cast<T*>(p.out) + m * p.ldc + c;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (c + j < p.N) put(out + j, g[j]);
   }
 }
 
@@ -566,9 +564,14 @@ int launch(Context* ctx, const Bf16Gemm& g, cudaStream_t s) {
   p.splits = q.splits; p.kb_per = q.kb_per;
   p.act = g.act;
   if (q.splits > 1 && !g.parts) return kErrInvalid;
-  auto on32 = [](const void* a) { return (reinterpret_cast<uintptr_t>(a) & 31u) == 0; };
-  p.vec = g.N % (32 / sizeof(T)) == 0 && g.ldc % (32 / sizeof(T)) == 0 && on32(g.out) &&
-          on32(g.pre) && on32(p.parts);
+  auto out_on = [&](int bytes) {
+    const int n = bytes / static_cast<int>(sizeof(T));
+    return g.N % n == 0 && g.ldc % n == 0 && (reinterpret_cast<uintptr_t>(g.out) & (bytes - 1)) == 0;
+  };
+  p.vec = out_on(32) ? 32 : out_on(16) ? 16 : 0;
+  p.ldp = ((static_cast<int64_t>(g.N) + 7) & ~7ll) * (GATED ? 2 : 1);
+  if (((reinterpret_cast<uintptr_t>(g.pre) | reinterpret_cast<uintptr_t>(p.parts)) & 31u) != 0)
+    return kErrInvalid;
   auto kern = bf16_gemm_kernel<NC, AK, BKM, GATED>;
   static SmemOptIn opt_in;
   cudaError_t e = opt_in.ensure(kern, Cfg<NC>::kSmem);
@@ -577,7 +580,7 @@ int launch(Context* ctx, const Bf16Gemm& g, cudaStream_t s) {
   note_launches(1);
   e = cudaGetLastError();
   if (e == cudaSuccess && q.splits > 1) {
-    const int64_t n = static_cast<int64_t>(g.M) * g.N;
+    const int64_t n = static_cast<int64_t>(g.M) * (p.ldp / (GATED ? 8 : 4));
     join_kernel<T, GATED><<<static_cast<unsigned>(std::min<int64_t>((n + 255) / 256,
                                                                     ctx->num_sms * 16)),
                             256, 0, s>>>(p);
@@ -602,7 +605,8 @@ int dispatch(Context* ctx, const Bf16Gemm& g, cudaStream_t s) {
 size_t bf16_gemm_scratch_bytes(const Context* ctx, int M, int N, int K, bool gated, int copies) {
   if (M <= 0 || N <= 0 || K <= 0) return 0;
   const Plan q = plan_of(ctx, M, N, K, gated, copies);
-  return q.splits > 1 ? static_cast<size_t>(q.splits) * M * N * (gated ? 2 : 1) * sizeof(float) : 0;
+  const size_t row = (static_cast<size_t>(N) + 7) / 8 * 8 * (gated ? 2 : 1);
+  return q.splits > 1 ? static_cast<size_t>(q.splits) * M * row * sizeof(float) : 0;
 }
 
 // Layouts: A K-major with B of either kind, or both MN-major (not gated).

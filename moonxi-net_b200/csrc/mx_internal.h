@@ -235,9 +235,9 @@ struct Bf16Gemm {
   void* out = nullptr;     // [M][ldc]
   int64_t ldc = 0;
   const void* bias = nullptr;  // gated: [2N], of the output's type
-  float* pre = nullptr;        // gated: float32 [M][2N]
+  float* pre = nullptr;        // gated: float32 [M][2 pad8(N)], 32-byte aligned
   int act = 0;
-  float* parts = nullptr;  // scratch of bf16_gemm_scratch_bytes, 16-byte aligned
+  float* parts = nullptr;  // scratch of bf16_gemm_scratch_bytes, 32-byte aligned
 };
 size_t bf16_gemm_scratch_bytes(const Context* ctx, int M, int N, int K, bool gated, int copies);
 int bf16_gemm(Context* ctx, const Bf16Gemm& g, cudaStream_t s);

@@ -514,6 +514,11 @@ def _gated_shape(x: torch.Tensor, w: torch.Tensor, transpose_w: bool, act: str):
     return dt, dev, M, K, two_f // 2, x.shape[:-1]
 
 
+def _pre_cols(F: int) -> int:
+    """Columns of the saved pre-activations: both halves padded to 8."""
+    return 2 * ((F + 7) // 8 * 8)
+
+
 def gated_linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None,
                  act: str = "silu", transpose_w: bool = False, save: bool = False,
                  out: torch.Tensor | None = None, pre: torch.Tensor | None = None,
@@ -522,7 +527,8 @@ def gated_linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = N
     (mx_gated_linear_fwd).  x: [..., K] float32 or bfloat16; w: [K, 2F]
     (transpose_w=False) or [2F, K], the gate's half first; bias: [2F].  w, bias
     and h are of x's type.  pre, [g | u] in float32 for
-    gated_linear_backward, is None unless `save` (or a buffer) is given."""
+    gated_linear_backward (each half padded to a multiple of 8 columns), is
+    None unless `save` (or a buffer) is given."""
     dt, dev, M, K, F, lead = _gated_shape(x, w, transpose_w, act)
     if bias is not None:
         _check_like(bias, "bias", dev, x.dtype, (2 * F,))
@@ -531,9 +537,9 @@ def gated_linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = N
     else:
         _check_like(out, "out", dev, x.dtype, lead + (F,))
     if pre is not None:
-        _check_like(pre, "pre", dev, torch.float32, lead + (2 * F,))
+        _check_like(pre, "pre", dev, torch.float32, lead + (_pre_cols(F),))
     elif save:
-        pre = _empty(lead + (2 * F,), torch.float32, x.device, stream)
+        pre = _empty(lead + (_pre_cols(F),), torch.float32, x.device, stream)
     L, h, p = _lib.lib(), _handle(ctx, x), _prec(precision)
     nb = L.mx_gated_linear_workspace_bytes(h, dt, M, K, F, transpose_w, p, 0)
     ws = _empty(nb, torch.uint8, x.device, stream) if nb else None
@@ -553,7 +559,7 @@ def gated_linear_backward(grad_out: torch.Tensor, pre: torch.Tensor, x: torch.Te
     (mx_gated_linear_bwd); dbias is None without `want_bias`."""
     dt, dev, M, K, F, lead = _gated_shape(x, w, transpose_w, act)
     _check_like(grad_out, "grad_out", dev, x.dtype, lead + (F,))
-    _check_like(pre, "pre", dev, torch.float32, lead + (2 * F,))
+    _check_like(pre, "pre", dev, torch.float32, lead + (_pre_cols(F),))
     if dx is None:
         dx = _empty(x.shape, x.dtype, x.device, stream)
     else:
