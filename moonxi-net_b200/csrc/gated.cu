@@ -66,41 +66,21 @@ __device__ __forceinline__ void load8(const bf16* p, float (&x)[8]) {
   }
 }
 
-// Copies of a row-major [rows][cols] matrix with rows of ldd elements (a
-// multiple of 8): columns below `split` at 0, the others from `up` on, zeros
-// between.  A thread makes 8 columns.
+// What the products need before they start, in one launch: up to two matrices
+// packed and, for the backward pass, dpre made with dbias's partial sums.
+// Blocks are given to the jobs in turn.
+//
+// Packing: copies of a row-major [rows][cols] matrix with rows of ldd elements
+// (a multiple of 8): columns below `split` at 0, the others from `up` on, zeros
+// between.  A thread makes 8 columns of every by-th row.
 struct PackJob {
   const void* src;
   bf16* dst;
   int64_t ldd, copy;
   int rows, cols, split, up;
-  int vec;  // rows start on 16 bytes, and nothing is moved
+  int vec;     // rows start on 16 bytes, and nothing is moved
+  int bx, by;  // blocks across columns and rows
 };
-struct PackJobs {
-  PackJob job[2];
-};
-template <typename T, int NC>
-__global__ void __launch_bounds__(256) pack_kernel(const __grid_constant__ PackJobs jobs) {
-  const PackJob& p = jobs.job[blockIdx.z];
-  const int64_t d = (blockIdx.x * 256ll + threadIdx.x) * 8;
-  if (d >= p.ldd) return;
-  const T* src = static_cast<const T*>(p.src);
-  for (int64_t r = blockIdx.y; r < p.rows; r += gridDim.y) {
-    float x[8];
-    if (p.vec) {
-      load8(src + r * p.cols + d, x);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int64_t e = d + i;
-        const int64_t c = e < p.up ? (e < p.split ? e : p.cols) : p.split + (e - p.up);
-        x[i] = c < p.cols ? to_f(src[r * p.cols + c]) : 0.0f;
-      }
-    }
-    store_copies<NC>(x, p.dst + r * p.ldd + d, p.copy);
-  }
-}
-
 struct Dpre {
   const void* dh;
   const float* pre;
@@ -109,17 +89,56 @@ struct Dpre {
   float* part;    // [row blocks][2F], or null
   int rows, F, act, per;  // per: rows of a block
   int vec;        // dh's rows and the output's halves start on 16 bytes
+  int bx, by;     // blocks across columns and rows (0: no dpre)
+};
+struct Prep {
+  Dpre dpre;
+  PackJob pack[2];
+  int packs;
 };
 
-// A block: 256 columns of both halves, `per` rows, its eight warps a row at a
+template <typename T, int NC>
+__device__ __forceinline__ void pack_block(const PackJob& p, int block) {
+  const int64_t d = (block % p.bx * 256ll + threadIdx.x) * 8;
+  if (d >= p.ldd) return;
+  const T* src = static_cast<const T*>(p.src);
+  int64_t r = block / p.bx;
+  if (p.vec) {
+    for (; r + p.by < p.rows; r += 2 * p.by) {  // two rows in flight
+      float x[8], y[8];
+      load8(src + r * p.cols + d, x);
+      load8(src + (r + p.by) * p.cols + d, y);
+      store_copies<NC>(x, p.dst + r * p.ldd + d, p.copy);
+      store_copies<NC>(y, p.dst + (r + p.by) * p.ldd + d, p.copy);
+    }
+    if (r < p.rows) {
+      float x[8];
+      load8(src + r * p.cols + d, x);
+      store_copies<NC>(x, p.dst + r * p.ldd + d, p.copy);
+    }
+    return;
+  }
+  for (; r < p.rows; r += p.by) {
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int64_t e = d + i;
+      const int64_t c = e < p.up ? (e < p.split ? e : p.cols) : p.split + (e - p.up);
+      x[i] = c < p.cols ? to_f(src[r * p.cols + c]) : 0.0f;
+    }
+    store_copies<NC>(x, p.dst + r * p.ldd + d, p.copy);
+  }
+}
+
+// dpre: 256 columns of both halves, `per` rows, the eight warps a row at a
 // time, a lane 8 columns.  Bound by the bytes: with bfloat16 tensors 10 read
 // and 4 written a value of h (8192 x 8192: 157 us, 91 % of the copy rate).
 template <typename T, int OUT>
-__global__ void __launch_bounds__(256) dpre_kernel(const Dpre p) {
-  __shared__ float sh[8][256];
+__device__ __forceinline__ void dpre_block(const Dpre& p, int block, float (&sh)[8][256]) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t f = (blockIdx.x * 32ll + lane) * 8, up = (p.F + 7) & ~7ll;
-  const int64_t r0 = blockIdx.y * static_cast<int64_t>(p.per);
+  const int cb = block % p.bx, rb = block / p.bx;
+  const int64_t f = (cb * 32ll + lane) * 8, up = (p.F + 7) & ~7ll;
+  const int64_t r0 = rb * static_cast<int64_t>(p.per);
   const int64_t r1 = r0 + p.per < p.rows ? r0 + p.per : p.rows;
   float sg[8], su[8];
 #pragma unroll
@@ -175,20 +194,38 @@ __global__ void __launch_bounds__(256) dpre_kernel(const Dpre p) {
     }
   }
   if (!p.part) return;
-  float* part = p.part + blockIdx.y * 2ll * p.F;
+  float* part = p.part + rb * 2ll * p.F;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {  // the eight warps' sums, in their order
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < 8; ++i) sh[warp][lane * 8 + i] = h ? su[i] : sg[i];
     __syncthreads();
-    const int64_t c = blockIdx.x * 256ll + threadIdx.x;
+    const int64_t c = cb * 256ll + threadIdx.x;
     if (c < p.F) {
       float s = 0.0f;
 #pragma unroll
       for (int w = 0; w < 8; ++w) s += sh[w][threadIdx.x];
       part[h * static_cast<int64_t>(p.F) + c] = s;
     }
+  }
+}
+
+template <typename T, int NC, bool DPRE>
+__global__ void __launch_bounds__(256) prep_kernel(const __grid_constant__ Prep p) {
+  int block = blockIdx.x;
+  if constexpr (DPRE) {
+    __shared__ float sh[8][256];
+    if (block < p.dpre.bx * p.dpre.by) {
+      dpre_block<T, NC>(p.dpre, block, sh);
+      return;
+    }
+    block -= p.dpre.bx * p.dpre.by;
+  }
+  if constexpr (NC > 0) {
+    const int first = p.packs > 0 ? p.pack[0].bx * p.pack[0].by : 0;
+    if (block < first) pack_block<T, NC>(p.pack[0], block);
+    else if (p.packs > 1) pack_block<T, NC>(p.pack[1], block - first);
   }
 }
 
@@ -285,39 +322,31 @@ Packed packed_of(const GatedArgs& a, const void* src, int rows, int64_t cols, bo
 size_t packed_bytes(const GatedArgs& a, const Packed& p) {
   return p.direct ? 0 : static_cast<size_t>(copies_of(a)) * p.copy * 2;
 }
-// The operands of one or two matrices: packed into their places in one launch,
-// unless they are read as they are.
-struct Packing {
-  PackJobs jobs;
-  int count = 0;
-  Bf16Operand add(const void* src, int rows, int64_t cols, const Packed& p, bool halves, bf16* dst) {
-    Bf16Operand o;
-    o.copy = p.copy;
-    o.ld = p.ld;
-    o.base = p.direct ? src : dst;
-    if (p.direct) return o;
-    const int split = static_cast<int>(halves ? cols / 2 : cols);
-    const bool vec = cols == p.ld && (!halves || p.up == split) && aligned16(src);
-    jobs.job[count++] = PackJob{src, dst, p.ld, p.copy, rows, static_cast<int>(cols), split,
-                                static_cast<int>(p.up), vec ? 1 : 0};
-    return o;
-  }
-  cudaError_t run(const GatedArgs& a, cudaStream_t s) {
-    if (count == 0) return cudaSuccess;
-    int64_t ld = 0;
-    int rows = 0;
-    for (int i = 0; i < count; ++i) {
-      ld = std::max(ld, jobs.job[i].ldd);
-      rows = std::max(rows, jobs.job[i].rows);
-    }
-    const dim3 grid(static_cast<unsigned>((ld / 8 + 255) / 256),
-                    static_cast<unsigned>(std::min(rows, 16384)), count);
-    if (a.dtype == MX_BF16) pack_kernel<bf16, 1><<<grid, 256, 0, s>>>(jobs);
-    else pack_kernel<float, 3><<<grid, 256, 0, s>>>(jobs);
-    note_launches(1);
-    return cudaGetLastError();
-  }
-};
+// Adds a matrix to what a launch packs, unless it is read as it is; its operand.
+Bf16Operand add_pack(Prep& prep, const void* src, int rows, int64_t cols, const Packed& p,
+                     bool halves, bf16* dst) {
+  Bf16Operand o;
+  o.copy = p.copy;
+  o.ld = p.ld;
+  o.base = p.direct ? src : dst;
+  if (p.direct) return o;
+  const int split = static_cast<int>(halves ? cols / 2 : cols);
+  const bool vec = cols == p.ld && (!halves || p.up == split) && aligned16(src);
+  prep.pack[prep.packs++] = PackJob{src, dst, p.ld, p.copy, rows, static_cast<int>(cols), split,
+                                    static_cast<int>(p.up), vec ? 1 : 0,
+                                    static_cast<int>((p.ld / 8 + 255) / 256), std::min((rows + 1) / 2, 2048)};
+  return o;
+}
+// OUT: as in Dpre; without dpre 1 or 3, the copies of a packed matrix.
+template <typename T, int OUT, bool DPRE>
+cudaError_t run_prep(const Prep& p, cudaStream_t s) {
+  int blocks = DPRE ? p.dpre.bx * p.dpre.by : 0;
+  for (int i = 0; i < p.packs; ++i) blocks += p.pack[i].bx * p.pack[i].by;
+  if (blocks == 0) return cudaSuccess;
+  prep_kernel<T, OUT, DPRE><<<blocks, 256, 0, s>>>(p);
+  note_launches(1);
+  return cudaGetLastError();
+}
 
 // An exact SIMT product on scratch of its own (no workspace or counters of the
 // context, so calls on different streams may overlap).
@@ -357,7 +386,8 @@ int simt_product(Context* ctx, const GemmArgs& g, void* scratch, size_t bytes, c
 struct FwdWork {
   Packed x, w;
   bf16 *xp, *wp;
-  float* parts;
+  void* split;      // scratch of a split product
+  size_t split_bytes;
   float* pre;       // SIMT: [g | u]
   void* scratch;
   size_t scratch_bytes, bytes;
@@ -374,7 +404,12 @@ FwdWork fwd_work(const Context* ctx, const GatedArgs& a) {
                : packed_of(a, asked ? off : a.w, a.K, 2ll * a.F, true);
     w.xp = c.take<bf16>(packed_bytes(a, w.x));
     w.wp = c.take<bf16>(packed_bytes(a, w.w));
-    w.parts = c.take<float>(bf16_gemm_scratch_bytes(ctx, a.M, a.F, a.K, true, copies_of(a)));
+    Bf16Gemm g;
+    g.gated = true;
+    g.copies = copies_of(a);
+    g.M = a.M; g.N = a.F; g.K = a.K;
+    w.split_bytes = bf16_gemm_scratch_bytes(ctx, &g, 1);
+    w.split = c.take<void>(w.split_bytes);
   } else {
     w.pre = c.take<float>(static_cast<size_t>(a.M) * 2 * a.F * sizeof(float));
     w.scratch_bytes = simt_scratch(
@@ -407,11 +442,11 @@ int fwd(Context* ctx, const GatedArgs& a, cudaStream_t s) {
     return cuda_status(cudaGetLastError());
   }
   Bf16Gemm g;
-  Packing pk;
-  g.a = pk.add(a.x, a.M, a.K, w.x, false, w.xp);
-  g.b = a.tw ? pk.add(a.w, 2 * a.F, a.K, w.w, false, w.wp)
-             : pk.add(a.w, a.K, 2ll * a.F, w.w, true, w.wp);
-  const cudaError_t e = pk.run(a, s);
+  Prep prep{};
+  g.a = add_pack(prep, a.x, a.M, a.K, w.x, false, w.xp);
+  g.b = a.tw ? add_pack(prep, a.w, 2 * a.F, a.K, w.w, false, w.wp)
+             : add_pack(prep, a.w, a.K, 2ll * a.F, w.w, true, w.wp);
+  const cudaError_t e = run_prep<T, sizeof(T) == 2 ? 1 : 3, false>(prep, s);
   if (e != cudaSuccess) return cuda_status(e);
   g.a.kmajor = true;
   g.b.kmajor = a.tw != 0;
@@ -425,8 +460,7 @@ int fwd(Context* ctx, const GatedArgs& a, cudaStream_t s) {
   g.bias = a.bias;
   g.pre = a.pre;
   g.act = a.act;
-  g.parts = w.parts;
-  return bf16_gemm(ctx, g, s);
+  return bf16_gemm(ctx, &g, 1, w.split, nullptr, s);
 }
 
 struct BwdWork {
@@ -436,10 +470,17 @@ struct BwdWork {
   int64_t ldp, copy;
   float* part;
   int row_blocks, per;
-  float* parts;
+  void* split;      // scratch of split products
+  size_t split_bytes;
   void* scratch;
   size_t scratch_bytes, bytes;
 };
+// The backward products' shapes: dx = dpre op(w)^T, then dw.
+void bwd_shapes(const GatedArgs& a, Bf16Gemm (&g)[2]) {
+  g[0].copies = g[1].copies = copies_of(a);
+  g[0].M = a.M; g[0].N = a.K; g[0].K = 2 * a.F;
+  g[1].M = a.tw ? 2 * a.F : a.K; g[1].N = a.tw ? a.K : 2 * a.F; g[1].K = a.M;
+}
 BwdWork bwd_work(const Context* ctx, const GatedArgs& a) {
   BwdWork w{};
   Carver c{static_cast<uint8_t*>(a.ws)};
@@ -461,9 +502,12 @@ BwdWork bwd_work(const Context* ctx, const GatedArgs& a) {
                : packed_of(a, asked ? off : a.w, a.K, 2ll * a.F, false);
     w.xp = c.take<bf16>(packed_bytes(a, w.x));
     w.wp = c.take<bf16>(packed_bytes(a, w.w));
-    const int m2 = a.tw ? 2 * a.F : a.K, n2 = a.tw ? a.K : 2 * a.F;
-    w.parts = c.take<float>(std::max(bf16_gemm_scratch_bytes(ctx, a.M, a.K, 2 * a.F, false, nc),
-                                     bf16_gemm_scratch_bytes(ctx, m2, n2, a.M, false, nc)));
+    // the larger of what the call's products may need: both, or one of them
+    Bf16Gemm g[2];
+    bwd_shapes(a, g);
+    w.split_bytes = std::max({bf16_gemm_scratch_bytes(ctx, g, 2), bf16_gemm_scratch_bytes(ctx, g, 1),
+                              bf16_gemm_scratch_bytes(ctx, g + 1, 1)});
+    w.split = c.take<void>(w.split_bytes);
   } else {
     w.ldp = 2ll * a.F;
     w.dpre = c.take<void>(static_cast<size_t>(a.M) * w.ldp * sizeof(float));
@@ -477,25 +521,28 @@ BwdWork bwd_work(const Context* ctx, const GatedArgs& a) {
   return w;
 }
 
-template <typename T, int OUT>
-void launch_dpre(Dpre p, int row_blocks, cudaStream_t s) {
-  p.vec = p.F % 8 == 0 && aligned16(p.dh) ? 1 : 0;
-  dpre_kernel<T, OUT><<<dim3((p.F + 255) / 256, row_blocks), 256, 0, s>>>(p);
-  note_launches(1);
-}
-
 template <typename T>
 int bwd(Context* ctx, const GatedArgs& a, cudaStream_t s) {
   const BwdWork w = bwd_work(ctx, a);
   if (w.bytes > a.ws_bytes) return kErrInvalid;
   const bool tensor = tensor_path(a);
   const int F2 = 2 * a.F;
-  const Dpre p{a.dh, a.pre, w.dpre, w.ldp, w.copy, a.dbias ? w.part : nullptr, a.M, a.F, a.act, w.per, 0};
-  if (a.dtype == MX_BF16) launch_dpre<bf16, 1>(p, w.row_blocks, s);
-  else if (tensor) launch_dpre<float, 3>(p, w.row_blocks, s);
-  else launch_dpre<float, 0>(p, w.row_blocks, s);
-  cudaError_t e = cudaGetLastError();
-  if (e == cudaSuccess && a.dbias) {
+  Prep prep{};
+  prep.dpre = Dpre{a.dh, a.pre, w.dpre, w.ldp, w.copy, a.dbias ? w.part : nullptr, a.M, a.F, a.act,
+                   w.per, a.F % 8 == 0 && aligned16(a.dh) ? 1 : 0, (a.F + 255) / 256, w.row_blocks};
+  Bf16Operand x, wt;
+  cudaError_t e;
+  if (!tensor) {
+    e = run_prep<float, 0, true>(prep, s);
+  } else {
+    if (a.dx)
+      wt = a.tw ? add_pack(prep, a.w, F2, a.K, w.w, false, w.wp)
+                : add_pack(prep, a.w, a.K, F2, w.w, false, w.wp);
+    if (a.dw) x = add_pack(prep, a.x, a.M, a.K, w.x, false, w.xp);
+    e = run_prep<T, sizeof(T) == 2 ? 1 : 3, true>(prep, s);
+  }
+  const bool products = tensor && (a.dx || a.dw);
+  if (e == cudaSuccess && a.dbias && !products) {  // else with what follows them
     dbias_kernel<T><<<(F2 + 31) / 32, 256, 0, s>>>(w.part, static_cast<T*>(a.dbias), w.row_blocks, F2);
     note_launches(1);
     e = cudaGetLastError();
@@ -514,39 +561,26 @@ int bwd(Context* ctx, const GatedArgs& a, cudaStream_t s) {
                         w.scratch, w.scratch_bytes, s);
     return rc;
   }
-  Bf16Operand d, x, wt;
+  Bf16Operand d;
   d.base = w.dpre;
   d.copy = w.copy;
   d.ld = w.ldp;
-  Packing pk;
-  if (a.dx) wt = a.tw ? pk.add(a.w, F2, a.K, w.w, false, w.wp) : pk.add(a.w, a.K, F2, w.w, false, w.wp);
-  if (a.dw) x = pk.add(a.x, a.M, a.K, w.x, false, w.xp);
-  e = pk.run(a, s);
-  if (e != cudaSuccess) return cuda_status(e);
-  Bf16Gemm g;
-  g.copies = copies_of(a);
-  g.parts = w.parts;
-  if (a.dx) {
-    g.a = d;
-    g.b = wt;
-    g.a.kmajor = true;
-    g.b.kmajor = !a.tw;
-    g.M = a.M; g.N = a.K; g.K = F2;
-    g.out = a.dx;
-    g.ldc = a.K;
-    const int rc = bf16_gemm(ctx, g, s);
-    if (rc != kOk) return rc;
-  }
-  if (!a.dw) return kOk;
-  g.a = a.tw ? d : x;
-  g.b = a.tw ? x : d;
-  g.a.kmajor = g.b.kmajor = false;
-  g.M = a.tw ? F2 : a.K;
-  g.N = a.tw ? a.K : F2;
-  g.K = a.M;
-  g.out = a.dw;
-  g.ldc = g.N;
-  return bf16_gemm(ctx, g, s);
+  Bf16Gemm g[2];
+  bwd_shapes(a, g);
+  g[0].a = d;
+  g[0].b = wt;
+  g[0].a.kmajor = true;
+  g[0].b.kmajor = !a.tw;
+  g[0].out = a.dx;
+  g[0].ldc = a.K;
+  g[1].a = a.tw ? d : x;
+  g[1].b = a.tw ? x : d;
+  g[1].a.kmajor = g[1].b.kmajor = false;
+  g[1].out = a.dw;
+  g[1].ldc = g[1].N;
+  if (!products) return kOk;
+  const Bf16ColumnSum sum{w.part, a.dbias, w.row_blocks, F2};
+  return bf16_gemm(ctx, a.dx ? g : g + 1, a.dx && a.dw ? 2 : 1, w.split, a.dbias ? &sum : nullptr, s);
 }
 
 }  // namespace

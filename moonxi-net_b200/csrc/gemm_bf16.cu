@@ -23,6 +23,10 @@
 // so an accumulator row holds g and u of the same 128 outputs and the epilogue
 // has both.
 //
+// One launch takes one product or two (a backward pass's dx and dw, which do not
+// need each other): the second's tiles follow the first's, so the two share
+// the waves of tiles and pay one start and one end.
+//
 // Persistent, 320 threads: warp 0 one lane issues TMA loads (128-byte swizzle,
 // both operands in their stored layout, K- or MN-major) into a ring of stages;
 // warp 1 of the even CTA one lane issues the MMAs for the pair; warps 2-9 read
@@ -35,7 +39,10 @@
 // (pre and the partial tiles have padded rows).  Two accumulators: a tile's epilogue runs
 // beside the next tile's (three copies: the next stage's) MMAs.
 // Few tiles and a long K: the K range is split over the pairs, fp32 partial
-// tiles go to scratch and a second kernel adds them in order.
+// tiles go to scratch and a second kernel adds them in order.  (Added up by the
+// last warp to arrive at its part of a tile instead, a product of 33 x 2 x 1000
+// x 784 took 39 us against 12 and 4: few warps, each waiting for one part after
+// the other.)
 // Every mbarrier wait is bounded (mx::wait_bar), as in gemm_tc.cu.
 #include <algorithm>
 #include <type_traits>
@@ -63,45 +70,61 @@ struct Cfg {
 };
 static_assert(Cfg<1>::kSmem <= 232448 && Cfg<3>::kSmem <= 232448, "shared memory of an SM");
 
-template <int NC>
-struct Maps {
-  CUtensorMap a[NC];
-  CUtensorMap b[2][NC];  // by the CTA's rank in the pair
-};
-
-struct Params {
+// One product of a launch.
+struct Problem {
   void* out;
   const void* bias;
   float* pre;
   float* parts;     // [splits][M][ldp] when the K range is split
-  int* status;
   int64_t ldc;
-  uint64_t timeout_ns;
+  int64_t ldp;      // row of parts: pad8(N), gated twice that, like pre
   int M, N, K;
   int tiles_m, tiles_n, tiles;
   int splits, kb_per;  // k-blocks of a split
   int act;
-  int64_t ldp;         // row of parts: pad8(N), gated twice that, like pre
-  int vec;             // bytes of a store to out: 32, 16, or 0 (rows unaligned)
+  int vec;          // bytes of a store to out: 32, 16, or 0 (rows unaligned)
+  int a_kmajor, b_kmajor;
+};
+template <int NC>
+struct Launch {
+  CUtensorMap a[2][NC];     // by problem
+  CUtensorMap b[2][2][NC];  // by problem, by the CTA's rank in the pair
+  Problem p[2];
+  int* status;
+  uint64_t timeout_ns;
+  int jobs0, jobs;          // of the first problem, of both
 };
 
-// Bands of 8 tiles of rows, column by column inside a band: the pairs that run
-// at one time share rows of A and columns of B in L2.
-__device__ __forceinline__ void tile_at(const Params& p, int t, int& tm, int& tn) {
+// Job j: split j / tiles of tile j % tiles of its problem; k-blocks [kb0, kb1).
+struct Job {
+  int q, tm, tn, split, tile, kb0, kb1;
+};
+template <int NC>
+__device__ __forceinline__ Job job_at(const Launch<NC>& L, int j) {
+  Job r;
+  r.q = j >= L.jobs0;
+  if (r.q) j -= L.jobs0;
+  const Problem& p = L.p[r.q];
+  r.split = j / p.tiles;
+  r.tile = j - r.split * p.tiles;
+  // Bands of 8 tiles of rows, column by column inside a band: the pairs that
+  // run at one time share rows of A and columns of B in L2.
   constexpr int G = 8;
-  const int band = t / (G * p.tiles_n);
+  const int band = r.tile / (G * p.tiles_n);
   const int gm = min(G, p.tiles_m - band * G);
-  const int r = t - band * G * p.tiles_n;
-  tm = band * G + r % gm;
-  tn = r / gm;
+  const int i = r.tile - band * G * p.tiles_n;
+  r.tm = band * G + i % gm;
+  r.tn = i / gm;
+  r.kb0 = r.split * p.kb_per;
+  r.kb1 = min((p.K + kBK - 1) / kBK, r.kb0 + p.kb_per);
+  return r;
 }
 
 // A 128 x 64 tile of one copy: one box of 64 k x 128 rows, or two of 64 rows x
 // 64 k.
-template <bool KMAJOR>
-__device__ __forceinline__ void load_tile(uint8_t* dst, const CUtensorMap* map, uint32_t bar,
-                                          int r0, int k0) {
-  if (KMAJOR) {
+__device__ __forceinline__ void load_tile(bool kmajor, uint8_t* dst, const CUtensorMap* map,
+                                          uint32_t bar, int r0, int k0) {
+  if (kmajor) {
     tma_load_2d_pair(dst, map, bar, k0, r0);
   } else {
     tma_load_2d_pair(dst, map, bar, r0, k0);
@@ -109,14 +132,19 @@ __device__ __forceinline__ void load_tile(uint8_t* dst, const CUtensorMap* map, 
   }
 }
 
-// The 16-deep slice j of a tile.  K-major: 128-byte rows, groups of 8 rows
-// 1024 bytes apart, a slice 32 bytes on.  MN-major: chunks of 64 columns 8 KB
-// apart, groups of 8 k 1024 bytes apart, a slice two groups on.
-template <bool KMAJOR>
-__device__ __forceinline__ uint64_t slice_desc(uint32_t addr, int j) {
-  return KMAJOR ? sdesc_kmajor(addr + j * 32, 1024, 2)
-                : sdesc_mnmajor(addr + j * 2048, kOpBytes / 2, 1024, 2);
-}
+// Operand tiles as the MMA reads them.  K-major: 128-byte rows, groups of 8
+// rows 1024 bytes apart, a 16-deep slice 32 bytes on.  MN-major: chunks of 64
+// columns 8 KB apart, groups of 8 k 1024 bytes apart, a slice two groups on.
+struct TileDesc {
+  uint64_t base;   // the descriptor of address 0
+  uint32_t slice;  // bytes from a slice to the next
+  __device__ __forceinline__ explicit TileDesc(bool kmajor)
+      : base(kmajor ? sdesc_kmajor(0, 1024, 2) : sdesc_mnmajor(0, kOpBytes / 2, 1024, 2)),
+        slice(kmajor ? 32 : 2048) {}
+  __device__ __forceinline__ uint64_t at(uint32_t addr, int j) const {
+    return base | static_cast<uint64_t>(((addr + j * slice) & 0x3FFFFu) >> 4);
+  }
+};
 
 __device__ __forceinline__ int64_t pad8(int64_t n) { return (n + 7) & ~7ll; }
 
@@ -153,9 +181,9 @@ __device__ __forceinline__ void store_row(__nv_bfloat16* p, const float (&v)[32]
     }
 }
 
-template <int NC, bool AK, bool BKM, bool GATED>
+template <int NC, bool GATED>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
-    bf16_gemm_kernel(const __grid_constant__ Maps<NC> maps, const Params p) {
+    bf16_gemm_kernel(const __grid_constant__ Launch<NC> L) {
   using T = typename std::conditional<NC == 1, __nv_bfloat16, float>::type;
   using C = Cfg<NC>;
   extern __shared__ uint8_t smem_raw[];
@@ -186,9 +214,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     bar_init(drain, 1);
     *abort_flag = 0;
     fence_barrier_init();
+    const int q = pair >= L.jobs0;  // the first job's operands
     for (int i = 0; i < NC; ++i) {
-      tma_prefetch_desc(&maps.a[i]);
-      tma_prefetch_desc(&maps.b[rank][i]);
+      tma_prefetch_desc(&L.a[q][i]);
+      tma_prefetch_desc(&L.b[q][rank][i]);
     }
   }
   if (warp == 1) {
@@ -200,8 +229,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   cluster_sync();  // both CTAs' barriers exist
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  const int num_kb = (p.K + kBK - 1) / kBK;
-  const int jobs = p.tiles * p.splits;  // job j: split j / tiles of tile j % tiles
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer
@@ -210,14 +237,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       uint32_t phase = 0;
       uint32_t armed = 0, armed_parity = 0;  // bit s: a copy was issued, and its phase
       bool ok = true;
-      for (int j = pair; ok && j < jobs; j += pairs) {
-        int tm, tn;
-        tile_at(p, j % p.tiles, tm, tn);
-        const int kb0 = j / p.tiles * p.kb_per, kb1 = min(num_kb, kb0 + p.kb_per);
-        const int m0 = tm * kTile + rank * kHalf;
-        const int n0 = GATED ? tn * kHalf : tn * kTile + rank * kHalf;
-        for (int kb = kb0; kb < kb1; ++kb) {
-          if (!wait_bar(&empty[stage], phase ^ 1, abort_flag, p.status, p.timeout_ns, 401)) {
+      for (int j = pair; ok && j < L.jobs; j += pairs) {
+        const Job r = job_at(L, j);
+        const bool ak = L.p[r.q].a_kmajor, bk = L.p[r.q].b_kmajor;
+        const int m0 = r.tm * kTile + rank * kHalf;
+        const int n0 = GATED ? r.tn * kHalf : r.tn * kTile + rank * kHalf;
+        for (int kb = r.kb0; kb < r.kb1; ++kb) {
+          if (!wait_bar(&empty[stage], phase ^ 1, abort_flag, L.status, L.timeout_ns, 401)) {
             ok = false;
             break;
           }
@@ -228,8 +254,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           const uint32_t bar = cluster_addr(&full[stage], 0);
 #pragma unroll
           for (int i = 0; i < NC; ++i) {
-            load_tile<AK>(base + i * kOpBytes, &maps.a[i], bar, m0, kb * kBK);
-            load_tile<BKM>(base + (NC + i) * kOpBytes, &maps.b[rank][i], bar, n0, kb * kBK);
+            load_tile(ak, base + i * kOpBytes, &L.a[r.q][i], bar, m0, kb * kBK);
+            load_tile(bk, base + (NC + i) * kOpBytes, &L.b[r.q][rank][i], bar, n0, kb * kBK);
           }
           if (++stage == C::kStages) {
             stage = 0;
@@ -242,7 +268,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       // waits gave up, the odd CTA also lets its own copies finish by time.
       if (rank == 0) {
         for (int s = 0; s < C::kStages; ++s)
-          if (armed >> s & 1) drain_wait(&full[s], armed_parity >> s & 1, p.status, 407);
+          if (armed >> s & 1) drain_wait(&full[s], armed_parity >> s & 1, L.status, 407);
       } else if (!ok || *abort_flag) {
         const uint64_t t0 = globaltimer_ns();
         while (globaltimer_ns() - t0 < 10000000ull) {
@@ -253,29 +279,31 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   } else if (warp == 1) {
     // ---------------------------------------------------------- MMA issuer
     if (lane == 0 && rank == 0) {
-      constexpr uint32_t idesc = idesc_bf16(kTile, kTile, !AK, !BKM);
       int stage = 0;
       uint32_t phase = 0;
       int seg = 0;  // accumulators used so far
       bool ok = true;
       auto take_acc = [&]() {
         const int acc = seg & 1;
-        if (!wait_bar(&acc_empty[acc], (seg >> 1 & 1) ^ 1, abort_flag, p.status, p.timeout_ns, 402))
+        if (!wait_bar(&acc_empty[acc], (seg >> 1 & 1) ^ 1, abort_flag, L.status, L.timeout_ns, 402))
           return false;
         tc_fence_after();
         return true;
       };
-      for (int j = pair; ok && j < jobs; j += pairs) {
-        const int kb0 = j / p.tiles * p.kb_per, kb1 = min(num_kb, kb0 + p.kb_per);
+      for (int j = pair; ok && j < L.jobs; j += pairs) {
+        const Job r = job_at(L, j);
+        const bool ak = L.p[r.q].a_kmajor, bk = L.p[r.q].b_kmajor;
+        const uint32_t idesc = idesc_bf16(kTile, kTile, !ak, !bk);
+        const TileDesc da(ak), db(bk);
         if (NC == 1) ok = take_acc();
         uint32_t accumulate = 0;
-        for (int kb = kb0; ok && kb < kb1; ++kb) {
+        for (int kb = r.kb0; ok && kb < r.kb1; ++kb) {
           if (NC == 3) {
             ok = take_acc();
             if (!ok) break;
             accumulate = 0;
           }
-          if (!wait_bar(&full[stage], phase, abort_flag, p.status, p.timeout_ns, 403)) {
+          if (!wait_bar(&full[stage], phase, abort_flag, L.status, L.timeout_ns, 403)) {
             ok = false;
             break;
           }
@@ -286,7 +314,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           if (NC == 1) {
 #pragma unroll
             for (int k = 0; k < kBK / 16; ++k) {
-              mma_f16_pair(d, slice_desc<AK>(sa, k), slice_desc<BKM>(sb, k), idesc, accumulate);
+              mma_f16_pair(d, da.at(sa, k), db.at(sb, k), idesc, accumulate);
               accumulate = 1;
             }
           } else {
@@ -296,8 +324,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             for (int q = 0; q < 6; ++q)
 #pragma unroll
               for (int k = 0; k < kBK / 16; ++k) {
-                mma_f16_pair(d, slice_desc<AK>(sa + pa[q] * kOpBytes, k),
-                             slice_desc<BKM>(sb + pb[q] * kOpBytes, k), idesc, accumulate);
+                mma_f16_pair(d, da.at(sa + pa[q] * kOpBytes, k), db.at(sb + pb[q] * kOpBytes, k),
+                             idesc, accumulate);
                 accumulate = 1;
               }
           }
@@ -318,7 +346,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         }
       }
       tc_commit_pair(drain);  // every MMA is done before TMEM is released
-      drain_wait(drain, 0, p.status, 408);
+      drain_wait(drain, 0, L.status, 408);
     }
     __syncwarp();
   } else {
@@ -334,31 +362,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       tmem_ld_32cols(lanes + acc * kTile + col, r);
       tmem_wait_ld();
     };
-    // a block of `out`: 32 columns of this warp's rows, lane = row
-    auto store_out = [&](T* out, int64_t row0, int rows, int col0, const float (&v)[32]) {
-      T* dst = out + (row0 + lane) * p.ldc + col0;
-      const int left = p.N - col0;
-      if (p.vec == 32) {
-        if (lane < rows) store_row<32>(dst, v, left);
-      } else if (p.vec == 16) {
-        if (lane < rows) store_row<16>(dst, v, left);
-      } else {
-        // unaligned rows: through shared memory, a row at a time
-        __syncwarp();  // the last block's reads are done
-#pragma unroll
-        for (int i = 0; i < 32; ++i) tw[lane * 33 + i] = v[i];
-        __syncwarp();
-        dst = out + row0 * p.ldc + col0 + lane;
-        if (lane < left)
-#pragma unroll 4
-          for (int i = 0; i < rows; ++i) {
-            put(dst, tw[i * 33 + lane]);
-            dst += p.ldc;
-          }
-      }
-    };
     auto wait_acc = [&]() {
-      if (!wait_bar(&acc_full[seg & 1], seg >> 1 & 1, abort_flag, p.status, p.timeout_ns, 404))
+      if (!wait_bar(&acc_full[seg & 1], seg >> 1 & 1, abort_flag, L.status, L.timeout_ns, 404))
         return false;
       tc_fence_after();
       return true;
@@ -369,63 +374,51 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       if (lane == 0) bar_arrive_cluster(cluster_addr(&acc_empty[seg & 1], 0));
       ++seg;
     };
-    for (int j = pair; ok && j < jobs; j += pairs) {
-      int tm, tn;
-      tile_at(p, j % p.tiles, tm, tn);
-      const int split = j / p.tiles;
-      const int kb0 = split * p.kb_per, kb1 = min(num_kb, kb0 + p.kb_per);
-      const int row0 = tm * kTile + rank * kHalf + group * 32;
+    // where this warp's block q of 32 columns is in the accumulator (gated: the
+    // gate's for even q, the other projection's for odd)
+    auto col_of = [&](int q) {
+      return GATED ? (q & 1) * kHalf + half * 64 + (q >> 1) * 32 : half * kHalf + q * 32;
+    };
+    for (int j = pair; ok && j < L.jobs; j += pairs) {
+      const Job r = job_at(L, j);
+      const Problem& p = L.p[r.q];
+      const int row0 = r.tm * kTile + rank * kHalf + group * 32;
       const int rows = min(32, p.M - row0);  // may be below 1
-      // where this warp's block q of 32 columns is in the accumulator
-      auto col_of = [&](int q) {
-        return GATED ? (q & 1) * kHalf + half * 64 + (q >> 1) * 32 : half * kHalf + q * 32;
-      };
-      float acc[NC == 3 ? 4 : 1][32];
-      if (NC == 3) {
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-#pragma unroll
-          for (int i = 0; i < 32; ++i) acc[q % (NC == 3 ? 4 : 1)][i] = 0.0f;
-        for (int kb = kb0; kb < kb1; ++kb) {
-          ok = wait_acc();
-          if (!ok) break;
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            uint32_t r[32];
-            load32(seg & 1, col_of(q), r);
-#pragma unroll
-            for (int i = 0; i < 32; ++i) acc[q % (NC == 3 ? 4 : 1)][i] += __uint_as_float(r[i]);
-          }
-          free_acc();
-        }
-      } else {
-        ok = wait_acc();
-      }
-      if (!ok) break;
-      // block q of this warp, lane = row
-      auto block = [&](int q, float (&v)[32]) {
-        if (NC == 3) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = acc[q % (NC == 3 ? 4 : 1)][i];
-        } else {
-          uint32_t r[32];
-          load32(seg & 1, col_of(q), r);
-#pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
-        }
-      };
-      // (one copy: the loops stay rolled, the instruction cache holds one body)
       const bool mine = lane < rows;
-      if constexpr (GATED) {
-#pragma unroll(NC == 3 ? 2 : 1)
-        for (int q = 0; q < 4; q += 2) {
-          const int col0 = tn * kHalf + half * 64 + (q >> 1) * 32;
-          const int left = p.N - col0;
-          float g[32], u[32];
-          block(q, g);
-          block(q + 1, u);
-          if (left <= 0) continue;
-          if (p.bias && !p.parts) {
+      const int64_t row = row0 + lane;
+      // the first column of blocks q (and q + 1 when gated) in the output
+      auto out_col = [&](int q) {
+        return GATED ? r.tn * kHalf + half * 64 + (q >> 1) * 32 : r.tn * kTile + col_of(q);
+      };
+      // a block of `out`: 32 columns of this warp's rows, lane = row
+      auto store_out = [&](int col0, const float (&v)[32]) {
+        T* dst = static_cast<T*>(p.out) + row * p.ldc + col0;
+        const int left = p.N - col0;
+        if (p.vec == 32) {
+          if (mine) store_row<32>(dst, v, left);
+        } else if (p.vec == 16) {
+          if (mine) store_row<16>(dst, v, left);
+        } else {
+          // unaligned rows: through shared memory, a row at a time
+          __syncwarp();  // the last block's reads are done
+#pragma unroll
+          for (int i = 0; i < 32; ++i) tw[lane * 33 + i] = v[i];
+          __syncwarp();
+          dst = static_cast<T*>(p.out) + static_cast<int64_t>(row0) * p.ldc + col0 + lane;
+          if (lane < left)
+#pragma unroll 4
+            for (int i = 0; i < rows; ++i) {
+              put(dst, tw[i * 33 + lane]);
+              dst += p.ldc;
+            }
+        }
+      };
+      // a complete block (gated: two) into the outputs
+      auto finish = [&](int q, float (&g)[32], float (&u)[32]) {
+        const int col0 = out_col(q), left = p.N - col0;
+        if (left <= 0) return;
+        if constexpr (GATED) {
+          if (p.bias) {
             const T* bias = static_cast<const T*>(p.bias) + col0;
 #pragma unroll
             for (int i = 0; i < 32; ++i)
@@ -434,34 +427,67 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 u[i] += to_f(bias[p.N + i]);
               }
           }
-          float* pre = p.parts ? p.parts + static_cast<int64_t>(split) * p.M * p.ldp : p.pre;
-          if (pre && mine) {
-            pre += static_cast<int64_t>(row0 + lane) * p.ldp + col0;
+          if (p.pre && mine) {
+            float* pre = p.pre + row * p.ldp + col0;
             store_row<32>(pre, g, left);
             store_row<32>(pre + p.ldp / 2, u, left);
           }
-          if (!p.parts) {
-            gate(p.act, g, u);
-            store_out(static_cast<T*>(p.out), row0, rows, col0, g);
+          gate(p.act, g, u);
+        }
+        store_out(col0, g);
+      };
+      // a block of this split's part
+      auto park = [&](int q, const float (&g)[32], const float (&u)[32]) {
+        const int col0 = out_col(q), left = p.N - col0;
+        if (left <= 0 || !mine) return;
+        float* dst = p.parts + (static_cast<int64_t>(r.split) * p.M + row) * p.ldp + col0;
+        store_row<32>(dst, g, left);
+        if (GATED) store_row<32>(dst + p.ldp / 2, u, left);
+      };
+      constexpr int kStep = GATED ? 2 : 1;
+      if constexpr (NC == 3) {
+        float acc[4][32];
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+          for (int i = 0; i < 32; ++i) acc[q][i] = 0.0f;
+        for (int kb = r.kb0; kb < r.kb1; ++kb) {
+          ok = wait_acc();
+          if (!ok) break;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            uint32_t t[32];
+            load32(seg & 1, col_of(q), t);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) acc[q][i] += __uint_as_float(t[i]);
           }
+          free_acc();
+        }
+        if (!ok) break;
+#pragma unroll
+        for (int q = 0; q < 4; q += kStep) {
+          if (p.splits > 1) park(q, acc[q], acc[(q + 1) & 3]);
+          else finish(q, acc[q], acc[(q + 1) & 3]);
         }
       } else {
-#pragma unroll(NC == 3 ? 4 : 1)
-        for (int q = 0; q < 4; ++q) {
-          const int col0 = tn * kTile + col_of(q);
-          float v[32];
-          block(q, v);
-          if (col0 >= p.N) continue;
-          if (p.parts) {
-            if (mine)
-              store_row<32>(p.parts + (static_cast<int64_t>(split) * p.M + row0 + lane) * p.ldp + col0,
-                            v, p.N - col0);
-          } else {
-            store_out(static_cast<T*>(p.out), row0, rows, col0, v);
-          }
+        ok = wait_acc();
+        if (!ok) break;
+        // (rolled: the instruction cache holds one body)
+#pragma unroll 1
+        for (int q = 0; q < 4; q += kStep) {
+          uint32_t t[32];
+          float g[32], u[32];
+          load32(seg & 1, col_of(q), t);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) g[i] = __uint_as_float(t[i]);
+          if (GATED) load32(seg & 1, col_of(q + 1), t);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) u[i] = GATED ? __uint_as_float(t[i]) : 0.0f;
+          if (p.splits > 1) park(q, g, u);
+          else finish(q, g, u);
         }
+        free_acc();
       }
-      if (NC == 1) free_acc();
     }
   }
 
@@ -474,21 +500,30 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   }
 }
 
-// The sum of a split product's parts, in order; gated: bias and activation too.
-// A thread takes four columns.
+// What follows the products, in one launch: the sums of split products' parts,
+// in order (gated: bias and activation too), four columns a thread; and a
+// column sum over rows of partial sums (dbias), 32 columns a block.
+struct Tail {
+  Problem p[2];
+  int blocks[2];      // of each product's sum (0: not split)
+  const float* part;  // [rows][width]
+  void* sum;
+  int rows, width;
+};
 template <typename T, bool GATED>
-__global__ void __launch_bounds__(256) join_kernel(const Params p) {
+__device__ __forceinline__ void join_block(const Problem& p, int block, int blocks) {
   const int64_t quads = pad8(p.N) / 4, n = p.M * quads, part = p.M * p.ldp;
-  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
+  for (int64_t i = block * 256ll + threadIdx.x; i < n; i += blocks * 256ll) {
     const int64_t m = i / quads;
     const int c = static_cast<int>(i - m * quads) * 4;
     const float* src = p.parts + m * p.ldp + c;
     float g[4] = {0.0f, 0.0f, 0.0f, 0.0f}, u[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
     for (int s = 0; s < p.splits; ++s) {
-      const float4 a = *reinterpret_cast<const float4*>(src + s * part);
+      const float4 a = __ldcg(reinterpret_cast<const float4*>(src + s * part));
       g[0] += a.x; g[1] += a.y; g[2] += a.z; g[3] += a.w;
       if (GATED) {
-        const float4 b = *reinterpret_cast<const float4*>(src + s * part + p.ldp / 2);
+        const float4 b = __ldcg(reinterpret_cast<const float4*>(src + s * part + p.ldp / 2));
         u[0] += b.x; u[1] += b.y; u[2] += b.z; u[3] += b.w;
       }
     }
@@ -512,27 +547,111 @@ __global__ void __launch_bounds__(256) join_kernel(const Params p) {
       if (c + j < p.N) put(out + j, g[j]);
   }
 }
+template <typename T, bool GATED>
+__global__ void __launch_bounds__(256) tail_kernel(const __grid_constant__ Tail t) {
+  int block = blockIdx.x;
+  if (block < t.blocks[0]) {
+    join_block<T, GATED>(t.p[0], block, t.blocks[0]);
+    return;
+  }
+  if constexpr (!GATED) {
+    block -= t.blocks[0];
+    if (block < t.blocks[1]) {
+      join_block<T, false>(t.p[1], block, t.blocks[1]);
+      return;
+    }
+    block -= t.blocks[1];
+    __shared__ float sh[8][33];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t c = block * 32ll + lane;
+    float s = 0.0f;
+    if (c < t.width)
+#pragma unroll 4
+      for (int r = warp; r < t.rows; r += 8) s += t.part[static_cast<int64_t>(r) * t.width + c];
+    sh[warp][lane] = s;
+    __syncthreads();
+    if (warp == 0 && c < t.width) {
+      s = 0.0f;
+      for (int i = 0; i < 8; ++i) s += sh[i][lane];
+      put(static_cast<T*>(t.sum) + c, s);
+    }
+  }
+}
 
 struct Plan {
-  int tiles_m, tiles_n, tiles, splits, kb_per, pairs;
+  int tiles_m = 0, tiles_n = 0, tiles = 0, num_kb = 0, splits = 1, kb_per = 0;
+  size_t part_bytes = 0;
+  int jobs() const { return tiles * splits; }
 };
-Plan plan_of(const Context* ctx, int M, int N, int K, bool gated, int copies) {
-  Plan q;
-  const int width = gated ? kHalf : kTile;
-  q.tiles_m = (M + kTile - 1) / kTile;
-  q.tiles_n = (N + width - 1) / width;
-  q.tiles = q.tiles_m * q.tiles_n;
-  const int num_kb = std::max(1, (K + kBK - 1) / kBK);
+struct Plans {
+  Plan p[2];
+  int pairs = 0;
+  bool split() const { return p[0].splits > 1 || p[1].splits > 1; }
+};
+
+void set_splits(Plan& q, int want) {
+  q.kb_per = (q.num_kb + want - 1) / want;
+  q.splits = (q.num_kb + q.kb_per - 1) / q.kb_per;
+}
+
+// The longest queue of a pair, in k-blocks: jobs go round the pairs, so the
+// queues differ at the pairs where the first product's and all jobs' last
+// rounds end.  A job costs its start and epilogue on top (a copy: six
+// k-blocks, three: one), a split one the partial tile's way through memory too.
+int makespan(const Plans& pl, int pairs, int copies) {
+  const int extra = copies == 3 ? 1 : 6;
+  const int j0 = pl.p[0].jobs(), all = j0 + pl.p[1].jobs();
+  const int c0 = pl.p[0].kb_per + extra * (pl.p[0].splits > 1 ? 2 : 1);
+  const int c1 = pl.p[1].kb_per + extra * (pl.p[1].splits > 1 ? 2 : 1);
+  const int at[3] = {0, j0 % pairs, all % pairs};
+  int worst = 0;
+  for (int c : at) {
+    const int n0 = (j0 - c + pairs - 1) / pairs, n = (all - c + pairs - 1) / pairs;
+    worst = std::max(worst, n0 * c0 + (n - n0) * c1);
+  }
+  return worst;
+}
+
+// Whole tiles where they fill the machine; otherwise the split counts, the
+// longer product's first, with the shortest longest queue.
+Plans plan_of(const Context* ctx, const Bf16Gemm* g, int count) {
+  Plans pl;
+  const int copies = g[0].copies;
   const int pairs = std::max(1, ctx->tc_sms() / 2);
-  // Split K when whole tiles leave more than half of the pairs idle, into
-  // pieces of at least 512 of K (three copies: 128, six times the work).
-  const int least = copies == 3 ? 2 : 8;
-  q.splits = 1;
-  if (2 * q.tiles <= pairs) q.splits = std::max(1, std::min(pairs / q.tiles, num_kb / least));
-  q.kb_per = (num_kb + q.splits - 1) / q.splits;
-  q.splits = (num_kb + q.kb_per - 1) / q.kb_per;
-  q.pairs = std::min(pairs, q.tiles * q.splits);
-  return q;
+  for (int i = 0; i < count; ++i) {
+    Plan& q = pl.p[i];
+    const int width = g[i].gated ? kHalf : kTile;
+    q.tiles_m = (g[i].M + kTile - 1) / kTile;
+    q.tiles_n = (g[i].N + width - 1) / width;
+    q.tiles = q.tiles_m * q.tiles_n;
+    q.num_kb = std::max(1, (g[i].K + kBK - 1) / kBK);
+    q.kb_per = q.num_kb;
+  }
+  const int least = copies == 3 ? 2 : 8;  // k-blocks of a split
+  const int longer = pl.p[1].num_kb > pl.p[0].num_kb ? 1 : 0;
+  if (pl.p[0].tiles + pl.p[1].tiles < 3 * pairs) {
+    for (int n = 0; n < count; ++n) {
+      Plan& q = pl.p[n == 0 ? longer : 1 - longer];
+      int best = 1, cost = makespan(pl, pairs, copies);
+      for (int want = 2; want <= 16 && q.num_kb / want >= least; ++want) {
+        set_splits(q, want);
+        const int c = makespan(pl, pairs, copies);
+        if (c < cost) {
+          best = want;
+          cost = c;
+        }
+      }
+      set_splits(q, best);
+    }
+  }
+  for (int i = 0; i < count; ++i) {
+    Plan& q = pl.p[i];
+    const size_t row = (static_cast<size_t>(g[i].N) + 7) / 8 * 8 * (g[i].gated ? 2 : 1);
+    if (q.splits > 1)
+      q.part_bytes = (static_cast<size_t>(q.splits) * g[i].M * row * sizeof(float) + 255) & ~size_t{255};
+  }
+  pl.pairs = std::min(pairs, pl.p[0].jobs() + pl.p[1].jobs());
+  return pl;
 }
 
 bool operand_map(CUtensorMap* m, const Bf16Operand& o, int copy, int rows, int K) {
@@ -541,79 +660,94 @@ bool operand_map(CUtensorMap* m, const Bf16Operand& o, int copy, int rows, int K
                   : make_tmap_bf16(m, base, rows, K, o.ld * 2, 64, kBK);
 }
 
-template <int NC, bool AK, bool BKM, bool GATED>
-int launch(Context* ctx, const Bf16Gemm& g, cudaStream_t s) {
+template <int NC, bool GATED>
+int launch(Context* ctx, const Bf16Gemm* g, int count, void* scratch, const Bf16ColumnSum* sum,
+           cudaStream_t s) {
   using T = typename std::conditional<NC == 1, __nv_bfloat16, float>::type;
-  const Plan q = plan_of(ctx, g.M, g.N, g.K, GATED, NC);
-  Maps<NC> maps;
-  for (int i = 0; i < NC; ++i)
-    if (!operand_map(&maps.a[i], g.a, i, g.M, g.K) ||
-        !operand_map(&maps.b[0][i], g.b, i, g.N, g.K) ||
-        !operand_map(&maps.b[1][i], GATED ? g.b2 : g.b, i, g.N, g.K))
-      return kErrUnsupported;
-  Params p{};
-  p.out = g.out;
-  p.bias = g.bias;
-  p.pre = g.pre;
-  p.parts = q.splits > 1 ? g.parts : nullptr;
-  p.status = ctx->status;
-  p.ldc = g.ldc;
-  p.timeout_ns = ctx->timeout_ns;
-  p.M = g.M; p.N = g.N; p.K = g.K;
-  p.tiles_m = q.tiles_m; p.tiles_n = q.tiles_n; p.tiles = q.tiles;
-  p.splits = q.splits; p.kb_per = q.kb_per;
-  p.act = g.act;
-  if (q.splits > 1 && !g.parts) return kErrInvalid;
-  auto out_on = [&](int bytes) {
-    const int n = bytes / static_cast<int>(sizeof(T));
-    return g.N % n == 0 && g.ldc % n == 0 && (reinterpret_cast<uintptr_t>(g.out) & (bytes - 1)) == 0;
-  };
-  p.vec = out_on(32) ? 32 : out_on(16) ? 16 : 0;
-  p.ldp = ((static_cast<int64_t>(g.N) + 7) & ~7ll) * (GATED ? 2 : 1);
-  if (((reinterpret_cast<uintptr_t>(g.pre) | reinterpret_cast<uintptr_t>(p.parts)) & 31u) != 0)
+  const Plans pl = plan_of(ctx, g, count);
+  if (pl.split() && (!scratch || (reinterpret_cast<uintptr_t>(scratch) & 255u) != 0))
     return kErrInvalid;
-  auto kern = bf16_gemm_kernel<NC, AK, BKM, GATED>;
+  Launch<NC> L;
+  uint8_t* parts = static_cast<uint8_t*>(scratch);
+  L.p[1] = Problem{};
+  for (int i = 0; i < count; ++i) {
+    for (int c = 0; c < NC; ++c)
+      if (!operand_map(&L.a[i][c], g[i].a, c, g[i].M, g[i].K) ||
+          !operand_map(&L.b[i][0][c], g[i].b, c, g[i].N, g[i].K) ||
+          !operand_map(&L.b[i][1][c], GATED ? g[i].b2 : g[i].b, c, g[i].N, g[i].K))
+        return kErrUnsupported;
+    Problem& p = L.p[i];
+    const Plan& q = pl.p[i];
+    p.out = g[i].out;
+    p.bias = g[i].bias;
+    p.pre = g[i].pre;
+    p.parts = q.splits > 1 ? reinterpret_cast<float*>(parts) : nullptr;
+    parts += q.part_bytes;
+    p.ldc = g[i].ldc;
+    p.ldp = ((static_cast<int64_t>(g[i].N) + 7) & ~7ll) * (GATED ? 2 : 1);
+    p.M = g[i].M; p.N = g[i].N; p.K = g[i].K;
+    p.tiles_m = q.tiles_m; p.tiles_n = q.tiles_n; p.tiles = q.tiles;
+    p.splits = q.splits; p.kb_per = q.kb_per;
+    p.act = g[i].act;
+    p.a_kmajor = g[i].a.kmajor;
+    p.b_kmajor = g[i].b.kmajor;
+    auto out_on = [&](int bytes) {
+      const int n = bytes / static_cast<int>(sizeof(T));
+      return p.N % n == 0 && p.ldc % n == 0 && (reinterpret_cast<uintptr_t>(p.out) & (bytes - 1)) == 0;
+    };
+    p.vec = out_on(32) ? 32 : out_on(16) ? 16 : 0;
+    if ((reinterpret_cast<uintptr_t>(p.pre) & 31u) != 0) return kErrInvalid;
+  }
+  L.status = ctx->status;
+  L.timeout_ns = ctx->timeout_ns;
+  L.jobs0 = pl.p[0].jobs();
+  L.jobs = L.jobs0 + pl.p[1].jobs();
+  auto kern = bf16_gemm_kernel<NC, GATED>;
   static SmemOptIn opt_in;
   cudaError_t e = opt_in.ensure(kern, Cfg<NC>::kSmem);
   if (e != cudaSuccess) return cuda_status(e);
-  kern<<<2 * q.pairs, kThreads, Cfg<NC>::kSmem, s>>>(maps, p);
+  kern<<<2 * pl.pairs, kThreads, Cfg<NC>::kSmem, s>>>(L);
   note_launches(1);
   e = cudaGetLastError();
-  if (e == cudaSuccess && q.splits > 1) {
-    const int64_t n = static_cast<int64_t>(g.M) * (p.ldp / (GATED ? 8 : 4));
-    join_kernel<T, GATED><<<static_cast<unsigned>(std::min<int64_t>((n + 255) / 256,
-                                                                    ctx->num_sms * 16)),
-                            256, 0, s>>>(p);
-    note_launches(1);
-    e = cudaGetLastError();
+  if (e != cudaSuccess || (!pl.split() && !sum)) return cuda_status(e);
+  Tail t{};
+  for (int i = 0; i < 2; ++i) {
+    t.p[i] = L.p[i];
+    if (pl.p[i].splits > 1)
+      t.blocks[i] = static_cast<int>(std::min<int64_t>(
+          (L.p[i].M * (L.p[i].ldp / (GATED ? 8 : 4)) + 255) / 256, ctx->num_sms * 16));
   }
-  return cuda_status(e);
-}
-
-template <int NC>
-int dispatch(Context* ctx, const Bf16Gemm& g, cudaStream_t s) {
-  if (g.gated)
-    return g.b.kmajor ? launch<NC, true, true, true>(ctx, g, s)
-                      : launch<NC, true, false, true>(ctx, g, s);
-  if (!g.a.kmajor) return launch<NC, false, false, false>(ctx, g, s);
-  return g.b.kmajor ? launch<NC, true, true, false>(ctx, g, s)
-                    : launch<NC, true, false, false>(ctx, g, s);
+  int blocks = t.blocks[0] + t.blocks[1];
+  if (sum) {
+    t.part = sum->part;
+    t.sum = sum->out;
+    t.rows = sum->rows;
+    t.width = sum->width;
+    blocks += (sum->width + 31) / 32;
+  }
+  tail_kernel<T, GATED><<<blocks, 256, 0, s>>>(t);
+  note_launches(1);
+  return cuda_status(cudaGetLastError());
 }
 
 }  // namespace
 
-size_t bf16_gemm_scratch_bytes(const Context* ctx, int M, int N, int K, bool gated, int copies) {
-  if (M <= 0 || N <= 0 || K <= 0) return 0;
-  const Plan q = plan_of(ctx, M, N, K, gated, copies);
-  const size_t row = (static_cast<size_t>(N) + 7) / 8 * 8 * (gated ? 2 : 1);
-  return q.splits > 1 ? static_cast<size_t>(q.splits) * M * row * sizeof(float) : 0;
+size_t bf16_gemm_scratch_bytes(const Context* ctx, const Bf16Gemm* g, int count) {
+  const Plans pl = plan_of(ctx, g, count);
+  return pl.p[0].part_bytes + pl.p[1].part_bytes;
 }
 
-// Layouts: A K-major with B of either kind, or both MN-major (not gated).
-int bf16_gemm(Context* ctx, const Bf16Gemm& g, cudaStream_t s) {
-  if (g.M <= 0 || g.N <= 0 || g.K <= 0 || (!g.a.kmajor && (g.b.kmajor || g.gated)))
+int bf16_gemm(Context* ctx, const Bf16Gemm* g, int count, void* scratch, const Bf16ColumnSum* sum,
+              cudaStream_t s) {
+  if (count < 1 || count > 2 || (sum && g[0].gated) || (count == 2 && (g[0].gated || g[1].gated || g[0].copies != g[1].copies)))
     return kErrInvalid;
-  return g.copies == 3 ? dispatch<3>(ctx, g, s) : dispatch<1>(ctx, g, s);
+  for (int i = 0; i < count; ++i)
+    if (g[i].M <= 0 || g[i].N <= 0 || g[i].K <= 0) return kErrInvalid;
+  if (g[0].copies == 3)
+    return g[0].gated ? launch<3, true>(ctx, g, count, scratch, sum, s)
+                      : launch<3, false>(ctx, g, count, scratch, sum, s);
+  return g[0].gated ? launch<1, true>(ctx, g, count, scratch, sum, s)
+                    : launch<1, false>(ctx, g, count, scratch, sum, s);
 }
 
 }  // namespace mx

@@ -237,10 +237,19 @@ struct Bf16Gemm {
   const void* bias = nullptr;  // gated: [2N], of the output's type
   float* pre = nullptr;        // gated: float32 [M][2 pad8(N)], 32-byte aligned
   int act = 0;
-  float* parts = nullptr;  // scratch of bf16_gemm_scratch_bytes, 32-byte aligned
 };
-size_t bf16_gemm_scratch_bytes(const Context* ctx, int M, int N, int K, bool gated, int copies);
-int bf16_gemm(Context* ctx, const Bf16Gemm& g, cudaStream_t s);
+// Column sums of float32 [rows][width] partial sums into out (of the products'
+// output type), made by the launch that follows the products.
+struct Bf16ColumnSum {
+  const float* part;
+  void* out;
+  int rows, width;
+};
+// One product, or two (not gated) in one launch, and what follows them (sum may
+// be NULL; not with a gated product).  scratch: 256-byte aligned.
+size_t bf16_gemm_scratch_bytes(const Context* ctx, const Bf16Gemm* g, int count);
+int bf16_gemm(Context* ctx, const Bf16Gemm* g, int count, void* scratch, const Bf16ColumnSum* sum,
+              cudaStream_t s);
 
 struct GatedArgs {
   int dtype, M, K, F, tw, act;
