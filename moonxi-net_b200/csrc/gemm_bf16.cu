@@ -92,19 +92,64 @@ struct Launch {
   Problem p[2];
   int* status;
   uint64_t timeout_ns;
-  int jobs0, jobs;          // of the first problem, of both
+  int jobs0, jobs1;         // of each problem
+  int fill;                 // see Queue
 };
 
-// Job j: split j / tiles of tile j % tiles of its problem; k-blocks [kb0, kb1).
+// The jobs of a pair, in order.  The first product's go round the pairs; where
+// its last round leaves pairs idle, each of these takes `fill` jobs of the
+// second product, and the rest of them go round again.
+struct Queue {
+  int c, pairs, short0;  // short0: pairs from here on miss the first's last round
+  int q, j, extra;
+  template <int NC>
+  __device__ __forceinline__ void init(const Launch<NC>& L, int pair, int n) {
+    c = pair;
+    pairs = n;
+    short0 = L.jobs0 % n;
+    q = 0;
+    j = c;
+    extra = L.fill > 0 && c >= short0 ? L.fill : 0;
+  }
+  // The next job: its problem and number; false at the end.
+  template <int NC>
+  __device__ __forceinline__ bool next(const Launch<NC>& L, int& problem, int& job) {
+    if (q == 0) {
+      if (j < L.jobs0) {
+        problem = 0;
+        job = j;
+        j += pairs;
+        return true;
+      }
+      q = 1;
+      j = c - short0;  // the fill, then the rounds
+    }
+    problem = 1;
+    if (extra > 0) {
+      job = j;
+      j += pairs - short0;
+      if (--extra == 0) q = 2;
+      return true;
+    }
+    if (q < 3) {
+      j = L.fill * (pairs - short0) + c;
+      q = 3;
+    }
+    job = j;
+    j += pairs;
+    return job < L.jobs1;
+  }
+};
+
+// Job j of problem q: split j / tiles of tile j % tiles; k-blocks [kb0, kb1).
 struct Job {
   int q, tm, tn, split, tile, kb0, kb1;
 };
 template <int NC>
-__device__ __forceinline__ Job job_at(const Launch<NC>& L, int j) {
+__device__ __forceinline__ Job job_at(const Launch<NC>& L, int q, int j) {
   Job r;
-  r.q = j >= L.jobs0;
-  if (r.q) j -= L.jobs0;
-  const Problem& p = L.p[r.q];
+  r.q = q;
+  const Problem& p = L.p[q];
   r.split = j / p.tiles;
   r.tile = j - r.split * p.tiles;
   // Bands of 8 tiles of rows, column by column inside a band: the pairs that
@@ -214,10 +259,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     bar_init(drain, 1);
     *abort_flag = 0;
     fence_barrier_init();
-    const int q = pair >= L.jobs0;  // the first job's operands
     for (int i = 0; i < NC; ++i) {
-      tma_prefetch_desc(&L.a[q][i]);
-      tma_prefetch_desc(&L.b[q][rank][i]);
+      tma_prefetch_desc(&L.a[0][i]);
+      tma_prefetch_desc(&L.b[0][rank][i]);
     }
   }
   if (warp == 1) {
@@ -229,6 +273,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   cluster_sync();  // both CTAs' barriers exist
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  Queue queue;
+  queue.init(L, pair, pairs);
+  int prob, number;
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer
@@ -237,8 +284,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       uint32_t phase = 0;
       uint32_t armed = 0, armed_parity = 0;  // bit s: a copy was issued, and its phase
       bool ok = true;
-      for (int j = pair; ok && j < L.jobs; j += pairs) {
-        const Job r = job_at(L, j);
+      while (ok && queue.next(L, prob, number)) {
+        const Job r = job_at(L, prob, number);
         const bool ak = L.p[r.q].a_kmajor, bk = L.p[r.q].b_kmajor;
         const int m0 = r.tm * kTile + rank * kHalf;
         const int n0 = GATED ? r.tn * kHalf : r.tn * kTile + rank * kHalf;
@@ -290,8 +337,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         tc_fence_after();
         return true;
       };
-      for (int j = pair; ok && j < L.jobs; j += pairs) {
-        const Job r = job_at(L, j);
+      while (ok && queue.next(L, prob, number)) {
+        const Job r = job_at(L, prob, number);
         const bool ak = L.p[r.q].a_kmajor, bk = L.p[r.q].b_kmajor;
         const uint32_t idesc = idesc_bf16(kTile, kTile, !ak, !bk);
         const TileDesc da(ak), db(bk);
@@ -363,10 +410,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       tmem_wait_ld();
     };
     auto wait_acc = [&]() {
-      if (!wait_bar(&acc_full[seg & 1], seg >> 1 & 1, abort_flag, L.status, L.timeout_ns, 404))
-        return false;
+      // one lane polls
+      int got = 0;
+      if (lane == 0)
+        got = wait_bar(&acc_full[seg & 1], seg >> 1 & 1, abort_flag, L.status, L.timeout_ns, 404);
+      got = __shfl_sync(0xffffffffu, got, 0);
       tc_fence_after();
-      return true;
+      return got != 0;
     };
     auto free_acc = [&]() {
       tc_fence_before();
@@ -379,8 +429,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     auto col_of = [&](int q) {
       return GATED ? (q & 1) * kHalf + half * 64 + (q >> 1) * 32 : half * kHalf + q * 32;
     };
-    for (int j = pair; ok && j < L.jobs; j += pairs) {
-      const Job r = job_at(L, j);
+    while (ok && queue.next(L, prob, number)) {
+      const Job r = job_at(L, prob, number);
       const Problem& p = L.p[r.q];
       const int row0 = r.tm * kTile + rank * kHalf + group * 32;
       const int rows = min(32, p.M - row0);  // may be below 1
@@ -594,20 +644,31 @@ void set_splits(Plan& q, int want) {
   q.splits = (q.num_kb + q.kb_per - 1) / q.kb_per;
 }
 
-// The longest queue of a pair, in k-blocks: jobs go round the pairs, so the
-// queues differ at the pairs where the first product's and all jobs' last
-// rounds end.  A job costs its start and epilogue on top (a copy: six
-// k-blocks, three: one), a split one the partial tile's way through memory too.
+// A job's cost in k-blocks: its start and epilogue come on top (one copy: six
+// k-blocks, three: one), for a split one the partial tile's way through memory
+// too.
+int job_cost(const Plan& q, int copies) {
+  return q.kb_per + (copies == 3 ? 1 : 6) * (q.splits > 1 ? 2 : 1);
+}
+// Queue's fill: what the first product's last round leaves to the pairs that
+// miss it.
+int fill_of(const Plans& pl, int pairs, int copies) {
+  const int shorter = pairs - pl.p[0].jobs() % pairs;
+  if (shorter == pairs || pl.p[1].jobs() == 0) return 0;
+  return std::min(job_cost(pl.p[0], copies) / job_cost(pl.p[1], copies), pl.p[1].jobs() / shorter);
+}
+// The longest queue of a pair, in k-blocks; queues differ only where a product's
+// last round ends.
 int makespan(const Plans& pl, int pairs, int copies) {
-  const int extra = copies == 3 ? 1 : 6;
-  const int j0 = pl.p[0].jobs(), all = j0 + pl.p[1].jobs();
-  const int c0 = pl.p[0].kb_per + extra * (pl.p[0].splits > 1 ? 2 : 1);
-  const int c1 = pl.p[1].kb_per + extra * (pl.p[1].splits > 1 ? 2 : 1);
-  const int at[3] = {0, j0 % pairs, all % pairs};
+  const int c0 = job_cost(pl.p[0], copies), c1 = pl.p[1].jobs() > 0 ? job_cost(pl.p[1], copies) : 0;
+  const int j0 = pl.p[0].jobs(), r = j0 % pairs, fill = fill_of(pl, pairs, copies);
+  const int rest = pl.p[1].jobs() - (fill > 0 ? fill * (pairs - r) : 0);
+  const int at[3] = {0, r, rest % pairs};
   int worst = 0;
   for (int c : at) {
-    const int n0 = (j0 - c + pairs - 1) / pairs, n = (all - c + pairs - 1) / pairs;
-    worst = std::max(worst, n0 * c0 + (n - n0) * c1);
+    const int n0 = (j0 - c + pairs - 1) / pairs;
+    const int n1 = (c >= r ? fill : 0) + (rest - c + pairs - 1) / pairs;
+    worst = std::max(worst, n0 * c0 + n1 * c1);
   }
   return worst;
 }
@@ -701,7 +762,8 @@ int launch(Context* ctx, const Bf16Gemm* g, int count, void* scratch, const Bf16
   L.status = ctx->status;
   L.timeout_ns = ctx->timeout_ns;
   L.jobs0 = pl.p[0].jobs();
-  L.jobs = L.jobs0 + pl.p[1].jobs();
+  L.jobs1 = pl.p[1].jobs();
+  L.fill = fill_of(pl, pl.pairs, NC);
   auto kern = bf16_gemm_kernel<NC, GATED>;
   static SmemOptIn opt_in;
   cudaError_t e = opt_in.ensure(kern, Cfg<NC>::kSmem);
