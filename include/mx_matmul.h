@@ -488,7 +488,11 @@ typedef struct mx_adamw_tensor {
  * mx_sgd_momentum_autoclip does (norm_out, device, may be NULL, receives it).
  * 8-bit codes: c stands for sign(c) (c / 127)^2 scale (m) and
  * sqrt(v) = (c / 255)^2 scale; the scale is the largest magnitude of its 256
- * values, NaN if one of them is not finite.  The tensors must not overlap.
+ * values, NaN if one of them is not finite.  Codes are the nearest ones (a v
+ * above zero keeps one above zero; m's codes below 0.5 / (1 - sqrt(beta1)) + 1
+ * are rounded towards zero, so that m dies out with its gradients).  A change
+ * of v against its block's largest by less than half a code a step is lost:
+ * with beta2 above 0.99 the second moments follow only slowly.  The tensors must not overlap.
  * scratch: mx_adamw_scratch_bytes(count, max_grad_norm > 0) bytes, 16-byte
  * aligned (may be NULL without clipping and step_dev). */
 int32_t mx_adamw_step(void* handle, const mx_adamw_tensor* tensors, int32_t count,

@@ -9,7 +9,11 @@
 // largest magnitude among them (top, at least 2^-120).  The first moment is
 // held as signed codes c for (c / 127)^2 top with c's sign, the second as
 // unsigned codes c for sqrt(v) = (c / 255)^2 top; the code is the nearest one
-// in the root.  The square gives values near the largest fine steps (0.8 % of
+// in the root, except that the first moment's codes below 0.5 / (1 -
+// sqrt(b1)) + 1 are rounded towards zero: a step without gradient shrinks
+// such a code by less than half, and the nearest one would keep a value whose
+// gradients have stopped moving for ever (codes up to 9, 0.5 % of the block's
+// largest, for b1 = 0.9).  The square gives values near the largest fine steps (0.8 % of
 // sqrt(v)) and still reaches 1.5e-5 of it; holding sqrt(v) halves the range of
 // exponents that v spans.  A sqrt(v) above zero keeps a code above zero (a
 // vanished v would blow the step up), and since `top` itself is not rounded,
@@ -65,6 +69,7 @@ struct Table {
 
 struct Hyper {
   float b1, omb1, b2, omb2, eps, step_size, inv_root;  // see adamw_one
+  float down;             // 8-bit first moments: codes below it are rounded down
   const float* scalars;   // device: {step_size, inv_root} instead, or null
   const float* norm;      // device: the gradients' norm, or null (no clipping)
   float max_norm;
@@ -204,16 +209,18 @@ __device__ __forceinline__ float block_top(const float (&x)[8]) {
   return __uint_as_float(top >= 0x7f800000u ? 0x7fc00000u : top);
 }
 // The codes: c = round(sqrt(|x| most^2 / top)), rounded by adding 1.5 * 2^23,
-// which leaves it in the low byte.  The root's last bit does not matter here.
+// which leaves it in the low byte; signed ones below `down` are floor(c + 1/64),
+// so that a value that stays as it is keeps its code.  The root's last bit does
+// not matter here.
 template <bool SIGNED>
-__device__ __forceinline__ void encode8(uint8_t* q, float top, bool vec, int left,
+__device__ __forceinline__ void encode8(uint8_t* q, float top, float down, bool vec, int left,
                                         const float (&x)[8]) {
   const float scale = __fdiv_rn(SIGNED ? 16129.0f : 65025.0f, top);
   uint32_t b[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     float c = fast_sqrt(fabsf(x[i]) * scale);
-    if (SIGNED) c = copysignf(c, x[i]);
+    if (SIGNED) c = copysignf(c < down ? fmaxf(c - 0.484375f, 0.0f) : c, x[i]);
     else if (x[i] > 0.0f) c = fmaxf(c, 1.0f);
     b[i] = __float_as_uint(c + 12582912.0f);
   }
@@ -264,8 +271,8 @@ __device__ __forceinline__ void adamw_block(const Tensor& t, const Hyper& h, flo
   if (t.copy) store8(t.copy + at, VEC, left, p);
   if (Q8) {
     const float sm = block_top<true>(m), sv = block_top<false>(root);
-    encode8<true>(static_cast<uint8_t*>(t.m) + at, sm, VEC, left, m);
-    encode8<false>(static_cast<uint8_t*>(t.v) + at, sv, VEC, left, root);
+    encode8<true>(static_cast<uint8_t*>(t.m) + at, sm, h.down, VEC, left, m);
+    encode8<false>(static_cast<uint8_t*>(t.v) + at, sv, 0.0f, VEC, left, root);
     __syncwarp();  // every lane has read the old scales
     if (lane == 0) {
       t.ms[block] = sm;
@@ -501,6 +508,7 @@ int adamw_step(const mx_adamw_tensor* ts, int count, int bits, double lr, double
   h.b2 = static_cast<float>(b2);
   h.omb2 = static_cast<float>(1.0 - b2);
   h.eps = static_cast<float>(eps);
+  h.down = static_cast<float>(0.5 / (1.0 - std::sqrt(b1)) + 1.0);
   const double t = static_cast<double>(step);
   h.step_size = step_dev ? 0.0f : static_cast<float>(lr / (1.0 - std::pow(b1, t)));
   h.inv_root = step_dev ? 0.0f : static_cast<float>(1.0 / std::sqrt(1.0 - std::pow(b2, t)));
