@@ -411,7 +411,8 @@ int32_t mx_layer_norm_fwd(void* handle, int32_t dtype, const void* x, int64_t ld
 /* The gradients of mx_layer_norm_fwd: dx (dtype, rows of lddx), dweight and
  * dbias (float32[cols], sums over the rows in a fixed order).  Any of the
  * three may be NULL.  scratch: mx_layer_norm_bwd_scratch_bytes(handle, rows,
- * cols) bytes, 16-byte aligned, when dweight or dbias is wanted. */
+ * cols) bytes (0 for small problems), 16-byte aligned, when dweight or dbias
+ * is wanted. */
 int32_t mx_layer_norm_bwd(void* handle, int32_t dtype, const void* dy, int64_t lddy,
                           const void* x, int64_t ldx, const float* weight, const float* mean,
                           const float* rstd, void* dx, int64_t lddx, float* dweight,

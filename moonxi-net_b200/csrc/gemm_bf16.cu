@@ -8,9 +8,9 @@
 // 2^-24 of the result), six MMAs for one multiply-add: 1/6 of the bf16 rate.
 // The tensor core truncates its accumulator at every MMA, about 2e-8 of the
 // result each and always towards zero (measured: a 3xTF32 product of K = 1024
-// left in one accumulator is off by 7e-6).  So a stage's six products go from
-// the smallest to the largest, few MMAs meet a full accumulator, and after
-// every stage, 64 of K, the epilogue warps add the accumulator to float32
+// left in one accumulator is off by 7e-6).  So a k-block's six products go
+// from the smallest to the largest, few MMAs meet a full accumulator, and after
+// every k-block, 64 of K, the epilogue warps add the accumulator to float32
 // registers with rounding: 2e-7 for 512 x 1024 x 8192 where SGEMM has 9e-7.
 // (Four stages of 32 of K: 60 us for that product against 45 when every stage
 // is added up, the epilogue's rate, and 48 us and 6e-7 when every second is.)
@@ -28,7 +28,7 @@
 // the waves of tiles and pay one start and one end.
 //
 // Persistent, 320 threads: warp 0 one lane issues TMA loads (128-byte swizzle,
-// both operands in their stored layout, K- or MN-major) into a ring of stages;
+// both operands in their stored layout, K- or MN-major) into a ring of slots;
 // warp 1 of the even CTA one lane issues the MMAs for the pair; warps 2-9 read
 // the accumulator (32 lanes x 32 columns at a time) and store each thread's 32
 // columns of a row in 32-byte pieces, whole sectors.  They stay off the shared
@@ -56,19 +56,20 @@ namespace {
 
 constexpr int kTile = 256;             // rows and columns of a pair's tile
 constexpr int kHalf = 128;             // ... of one CTA's operand tiles
-constexpr int kBK = 64;                // a stage's depth: 128 bytes of bf16
+constexpr int kBK = 64;                // a k-block: 128 bytes of bf16
 constexpr int kOpBytes = kHalf * kBK * 2;  // an operand tile
 constexpr int kThreads = 320;
 constexpr int kTmemCols = 512;
 constexpr int kTrFloats = 32 * 33;     // a warp's transpose buffer
 
-template <int NC>
-struct Cfg {
-  static constexpr int kStages = NC == 3 ? 2 : 6;
-  static constexpr int kStageBytes = 2 * NC * kOpBytes;
-  static constexpr int kSmem = kStages * kStageBytes + 8 * kTrFloats * 4 + 256 + 1024;
-};
-static_assert(Cfg<1>::kSmem <= 232448 && Cfg<3>::kSmem <= 232448, "shared memory of an SM");
+// The ring: a slot holds one copy's tile of A and of B.  Three copies: a
+// k-block takes three slots, from the smallest copy to the largest, which is
+// the order in which the products give them back, so the next k-block but one
+// begins to load after a third of this one's MMAs.
+constexpr int kSlots = 6;
+constexpr int kSlotBytes = 2 * kOpBytes;
+constexpr int kSmem = kSlots * kSlotBytes + 8 * kTrFloats * 4 + 256 + 1024;
+static_assert(kSmem <= 232448, "shared memory of an SM");
 
 // One product of a launch.
 struct Problem {
@@ -230,14 +231,13 @@ template <int NC, bool GATED>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     bf16_gemm_kernel(const __grid_constant__ Launch<NC> L) {
   using T = typename std::conditional<NC == 1, __nv_bfloat16, float>::type;
-  using C = Cfg<NC>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  float* tr = reinterpret_cast<float*>(smem + C::kStages * C::kStageBytes);
+  float* tr = reinterpret_cast<float*>(smem + kSlots * kSlotBytes);
   uint64_t* full = reinterpret_cast<uint64_t*>(tr + 8 * kTrFloats);  // the even CTA's are used
-  uint64_t* empty = full + C::kStages;
-  uint64_t* acc_full = empty + C::kStages;
+  uint64_t* empty = full + kSlots;
+  uint64_t* acc_full = empty + kSlots;
   uint64_t* acc_empty = acc_full + 2;  // the even CTA's are used
   uint64_t* drain = acc_empty + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
@@ -248,7 +248,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < C::kStages; ++s) {
+    for (int s = 0; s < kSlots; ++s) {
       bar_init(&full[s], 1);
       bar_init(&empty[s], 1);
     }
@@ -280,7 +280,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   if (warp == 0) {
     // ------------------------------------------------------------ producer
     if (lane == 0) {
-      int stage = 0;
+      int slot = 0;
       uint32_t phase = 0;
       uint32_t armed = 0, armed_parity = 0;  // bit s: a copy was issued, and its phase
       bool ok = true;
@@ -289,24 +289,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         const bool ak = L.p[r.q].a_kmajor, bk = L.p[r.q].b_kmajor;
         const int m0 = r.tm * kTile + rank * kHalf;
         const int n0 = GATED ? r.tn * kHalf : r.tn * kTile + rank * kHalf;
-        for (int kb = r.kb0; kb < r.kb1; ++kb) {
-          if (!wait_bar(&empty[stage], phase ^ 1, abort_flag, L.status, L.timeout_ns, 401)) {
-            ok = false;
-            break;
-          }
-          uint8_t* base = smem + stage * C::kStageBytes;
-          if (rank == 0) bar_arrive_expect_tx(&full[stage], 2 * C::kStageBytes);
-          armed |= 1u << stage;
-          armed_parity = (armed_parity & ~(1u << stage)) | (phase << stage);
-          const uint32_t bar = cluster_addr(&full[stage], 0);
+        for (int kb = r.kb0; ok && kb < r.kb1; ++kb) {
 #pragma unroll
-          for (int i = 0; i < NC; ++i) {
-            load_tile(ak, base + i * kOpBytes, &L.a[r.q][i], bar, m0, kb * kBK);
-            load_tile(bk, base + (NC + i) * kOpBytes, &L.b[r.q][rank][i], bar, n0, kb * kBK);
-          }
-          if (++stage == C::kStages) {
-            stage = 0;
-            phase ^= 1;
+          for (int i = NC - 1; i >= 0; --i) {
+            if (!wait_bar(&empty[slot], phase ^ 1, abort_flag, L.status, L.timeout_ns, 401)) {
+              ok = false;
+              break;
+            }
+            uint8_t* base = smem + slot * kSlotBytes;
+            if (rank == 0) bar_arrive_expect_tx(&full[slot], 2 * kSlotBytes);
+            armed |= 1u << slot;
+            armed_parity = (armed_parity & ~(1u << slot)) | (phase << slot);
+            const uint32_t bar = cluster_addr(&full[slot], 0);
+            load_tile(ak, base, &L.a[r.q][i], bar, m0, kb * kBK);
+            load_tile(bk, base + kOpBytes, &L.b[r.q][rank][i], bar, n0, kb * kBK);
+            if (++slot == kSlots) {
+              slot = 0;
+              phase ^= 1;
+            }
           }
         }
       }
@@ -314,7 +314,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       // barriers count both CTAs' copies and the pair exits together; when
       // waits gave up, the odd CTA also lets its own copies finish by time.
       if (rank == 0) {
-        for (int s = 0; s < C::kStages; ++s)
+        for (int s = 0; s < kSlots; ++s)
           if (armed >> s & 1) drain_wait(&full[s], armed_parity >> s & 1, L.status, 407);
       } else if (!ok || *abort_flag) {
         const uint64_t t0 = globaltimer_ns();
@@ -326,7 +326,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   } else if (warp == 1) {
     // ---------------------------------------------------------- MMA issuer
     if (lane == 0 && rank == 0) {
-      int stage = 0;
+      int slot = 0;
       uint32_t phase = 0;
       int seg = 0;  // accumulators used so far
       bool ok = true;
@@ -350,39 +350,42 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             if (!ok) break;
             accumulate = 0;
           }
-          if (!wait_bar(&full[stage], phase, abort_flag, L.status, L.timeout_ns, 403)) {
-            ok = false;
-            break;
-          }
+          // the k-block's slots: copy i is in slot + NC - 1 - i (no wrap inside
+          // a k-block, kSlots being a multiple of NC)
+#pragma unroll
+          for (int i = 0; ok && i < NC; ++i)
+            ok = wait_bar(&full[slot + i], phase, abort_flag, L.status, L.timeout_ns, 403);
+          if (!ok) break;
           tc_fence_after();
-          const uint32_t sa = smem_u32(smem + stage * C::kStageBytes);
-          const uint32_t sb = sa + NC * kOpBytes;
+          const uint32_t s0 = smem_u32(smem + slot * kSlotBytes);
           const uint32_t d = tmem_base + (seg & 1) * kTile;
-          if (NC == 1) {
+          auto product = [&](int ca, int cb) {
+            const uint32_t sa = s0 + (NC - 1 - ca) * kSlotBytes;
+            const uint32_t sb = s0 + (NC - 1 - cb) * kSlotBytes + kOpBytes;
 #pragma unroll
             for (int k = 0; k < kBK / 16; ++k) {
               mma_f16_pair(d, da.at(sa, k), db.at(sb, k), idesc, accumulate);
               accumulate = 1;
             }
-          } else {
-            // from the smallest products to the largest
-            constexpr int pa[6] = {2, 1, 0, 1, 0, 0}, pb[6] = {0, 1, 2, 0, 1, 0};
-#pragma unroll
-            for (int q = 0; q < 6; ++q)
-#pragma unroll
-              for (int k = 0; k < kBK / 16; ++k) {
-                mma_f16_pair(d, da.at(sa + pa[q] * kOpBytes, k), db.at(sb + pb[q] * kOpBytes, k),
-                             idesc, accumulate);
-                accumulate = 1;
-              }
+          };
+          if (NC == 3) {  // from the smallest products to the largest
+            product(2, 0);
+            product(0, 2);
+            tc_commit_both(&empty[slot]);
+            product(1, 1);
+            product(1, 0);
+            product(0, 1);
+            tc_commit_both(&empty[slot + 1]);
           }
-          tc_commit_both(&empty[stage]);
+          product(0, 0);
+          tc_commit_both(&empty[slot + NC - 1]);
           if (NC == 3) {
             tc_commit_both(&acc_full[seg & 1]);
             ++seg;
           }
-          if (++stage == C::kStages) {
-            stage = 0;
+          slot += NC;
+          if (slot == kSlots) {
+            slot = 0;
             phase ^= 1;
           }
         }
@@ -766,9 +769,9 @@ int launch(Context* ctx, const Bf16Gemm* g, int count, void* scratch, const Bf16
   L.fill = fill_of(pl, pl.pairs, NC);
   auto kern = bf16_gemm_kernel<NC, GATED>;
   static SmemOptIn opt_in;
-  cudaError_t e = opt_in.ensure(kern, Cfg<NC>::kSmem);
+  cudaError_t e = opt_in.ensure(kern, kSmem);
   if (e != cudaSuccess) return cuda_status(e);
-  kern<<<2 * pl.pairs, kThreads, Cfg<NC>::kSmem, s>>>(L);
+  kern<<<2 * pl.pairs, kThreads, kSmem, s>>>(L);
   note_launches(1);
   e = cudaGetLastError();
   if (e != cudaSuccess || (!pl.split() && !sum)) return cuda_status(e);

@@ -276,7 +276,7 @@ __device__ __forceinline__ uint32_t cluster_addr(const void* p, uint32_t rank) {
   return a;
 }
 __device__ __forceinline__ void bar_arrive_cluster(uint32_t addr) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
 }
 // 2-D tile into this CTA's shared memory, completion counted on a barrier of
 // either CTA of the pair (`bar`: its shared::cluster address).

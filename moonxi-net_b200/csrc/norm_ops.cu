@@ -453,6 +453,89 @@ __global__ void __launch_bounds__(256) norm_cols_kernel(const NormBwd p) {
   out[p.cols + c] = db;
 }
 
+// Small problems in one launch: the first row_blocks blocks make dx, a warp a
+// row, in two passes over it (the second from L1); the others sum 32 columns of
+// dweight and dbias each over all rows, reading x and dy once more, from L2.
+constexpr int kSmallWarps = 16;
+template <typename T, int V>
+__global__ void __launch_bounds__(32 * kSmallWarps) norm_bwd_small_kernel(const NormBwd p, float* dw, float* db,
+                                                             int row_blocks) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (static_cast<int>(blockIdx.x) < row_blocks) {
+    const int64_t row = blockIdx.x * static_cast<int64_t>(kSmallWarps) + warp;
+    if (row >= p.rows) return;
+    const T* x = static_cast<const T*>(p.x) + row * p.ldx;
+    const T* dy = static_cast<const T*>(p.dy) + row * p.lddy;
+    T* dx = static_cast<T*>(p.dx) + row * p.lddx;
+    const float mean = __ldg(p.mean + row), rstd = __ldg(p.rstd + row);
+    float s[2] = {0.0f, 0.0f};
+    int turn = 0;
+#pragma unroll 4
+    for (int c = lane * V; c < p.cols; c += 32 * V) {
+      float xv[V], a[V], w[V];
+      load_vec<T, V>(x + c, xv);
+      load_vec<T, V>(dy + c, a);
+      load_par<V>(p.w, c, w, 1.0f);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        a[j] *= w[j];
+        s[0] += a[j];
+        s[1] += a[j] * ((xv[j] - mean) * rstd);
+      }
+    }
+    row_sum<32>(s, nullptr, turn);
+    const float inv_c = 1.0f / static_cast<float>(p.cols);
+    const float c1 = s[0] * inv_c, c2 = s[1] * inv_c;
+#pragma unroll 4
+    for (int c = lane * V; c < p.cols; c += 32 * V) {
+      float xv[V], a[V], w[V];
+      load_vec<T, V>(x + c, xv);
+      load_vec<T, V>(dy + c, a);
+      load_par<V>(p.w, c, w, 1.0f);
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        a[j] = rstd * (a[j] * w[j] - c1 - (xv[j] - mean) * rstd * c2);
+      store_vec<T, V>(dx + c, a);
+    }
+    return;
+  }
+  __shared__ float sh[2][kSmallWarps][33];
+  const int64_t c = (blockIdx.x - row_blocks) * 32ll + lane;
+  float sw = 0.0f, sb = 0.0f;
+  if (c < p.cols) {
+    const T* dy = static_cast<const T*>(p.dy) + c;
+    const T* x = static_cast<const T*>(p.x) + c;
+    for (int r0 = warp; r0 < p.rows; r0 += 8 * kSmallWarps) {
+      T g[8], xv[8];
+      float mean[8], rstd[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {  // past the last row: the last one, not added
+        const int64_t r = min(r0 + i * kSmallWarps, p.rows - 1);
+        g[i] = dy[r * p.lddy];
+        xv[i] = x[r * p.ldx];
+        mean[i] = p.mean[r];
+        rstd[i] = p.rstd[r];
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (r0 + i * kSmallWarps < p.rows) {
+          sw += to_f(g[i]) * ((to_f(xv[i]) - mean[i]) * rstd[i]);
+          sb += to_f(g[i]);
+        }
+    }
+  }
+  sh[0][warp][lane] = sw;
+  sh[1][warp][lane] = sb;
+  __syncthreads();
+  if (warp < 2 && c < p.cols) {
+    float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kSmallWarps; ++i) s += sh[warp][i][lane];
+    float* out = warp == 0 ? dw : db;
+    if (out) out[c] = s;
+  }
+}
+
 // out[c] = the sum over `blocks` partial rows; column c < cols goes to dw, the
 // rest to db.  A block takes 32 columns, its eight warps an eighth of the rows
 // each; the order is fixed.
@@ -549,12 +632,18 @@ int bwd_blocks(int rows, int cols, int num_sms) {
   return row_blocks((rows + 1) / 2, cols, blocks_per_sm(tpr, 2), num_sms);
 }
 
+// Small enough for norm_bwd_small_kernel, whose columns' blocks walk down all
+// rows and whose warps walk along theirs.  Float32, one launch against two, us:
+// 64 x 257 2.7 / 5.1, 512 x 1024 4.9 / 8.6, 1000 x 257 8.2 / 6.9 (and a launch
+// less for the host, 4 us); 256 x 2048 8.0 / 6.6, 128 x 4096 13.4 / 7.0.
+bool bwd_small(int rows, int cols) { return rows <= 1024 && cols <= 1024; }
+
 bool aligned16(const void* a) { return (reinterpret_cast<uintptr_t>(a) & 15u) == 0; }
 
 }  // namespace
 
 size_t layer_norm_bwd_scratch_bytes(const Context* ctx, int rows, int cols) {
-  if (rows <= 0 || cols <= 0) return 0;
+  if (rows <= 0 || cols <= 0 || bwd_small(rows, cols)) return 0;
   return static_cast<size_t>(bwd_blocks(rows, cols, ctx->num_sms)) * 2 * cols * sizeof(float);
 }
 
@@ -591,14 +680,28 @@ int layer_norm_bwd(Context* ctx, int dtype, const void* dy, int64_t lddy, const 
     if (e == cudaSuccess && db) e = cudaMemsetAsync(db, 0, sizeof(float) * cols, s);
     return cuda_status(e);
   }
+  const int vec = dtype == MX_BF16 ? 8 : 4;
+  const bool v16 = cols % vec == 0 && ldx % vec == 0 && lddy % vec == 0 && aligned16(x) &&
+                   aligned16(dy) && aligned16(w) && (!dx || (lddx % vec == 0 && aligned16(dx)));
+  if (bwd_small(rows, cols)) {
+    const NormBwd p{dy, x, w, mean, rstd, dx, nullptr, lddy, ldx, lddx, rows, cols};
+    const int rb = dx ? (rows + kSmallWarps - 1) / kSmallWarps : 0, grid = rb + (sums ? (cols + 31) / 32 : 0);
+    if (grid == 0) return kOk;
+    if (dtype == MX_BF16) {
+      if (v16) norm_bwd_small_kernel<__nv_bfloat16, 8><<<grid, 32 * kSmallWarps, 0, s>>>(p, dw, db, rb);
+      else norm_bwd_small_kernel<__nv_bfloat16, 1><<<grid, 32 * kSmallWarps, 0, s>>>(p, dw, db, rb);
+    } else {
+      if (v16) norm_bwd_small_kernel<float, 4><<<grid, 32 * kSmallWarps, 0, s>>>(p, dw, db, rb);
+      else norm_bwd_small_kernel<float, 1><<<grid, 32 * kSmallWarps, 0, s>>>(p, dw, db, rb);
+    }
+    note_launches(1);
+    return cuda_status(cudaGetLastError());
+  }
   if (sums && (!scratch || scratch_bytes < layer_norm_bwd_scratch_bytes(ctx, rows, cols)))
     return kErrInvalid;
   const int blocks = bwd_blocks(rows, cols, ctx->num_sms);
   const NormBwd p{dy, x, w, mean, rstd, dx, sums ? static_cast<float*>(scratch) : nullptr,
                   lddy, ldx, lddx, rows, cols};
-  const int vec = dtype == MX_BF16 ? 8 : 4;
-  const bool v16 = cols % vec == 0 && ldx % vec == 0 && lddy % vec == 0 && aligned16(x) &&
-                   aligned16(dy) && aligned16(w) && (!dx || (lddx % vec == 0 && aligned16(dx)));
   cudaError_t e = cudaSuccess;
   if (cols > kNormRegCols) {
     if (dx) {

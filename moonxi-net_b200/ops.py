@@ -486,12 +486,13 @@ def layer_norm_backward(grad_out: torch.Tensor, x: torch.Tensor, weight: torch.T
     else:
         _check_like(dbias, "dbias", dev, f32, (cols,))
     h = _handle(ctx, x)
-    nb = _lib.lib().mx_layer_norm_bwd_scratch_bytes(h, rows, cols)
-    scratch = _empty(nb, torch.uint8, x.device, stream)
-    rc = _lib.lib().mx_layer_norm_bwd(
+    L = _lib.lib()
+    nb = L.mx_layer_norm_bwd_scratch_bytes(h, rows, cols)
+    scratch = _empty(nb, torch.uint8, x.device, stream) if nb else None
+    rc = L.mx_layer_norm_bwd(
         h, dt, grad_out.data_ptr(), lddy, x.data_ptr(), ldx, _ptr(weight), mean.data_ptr(),
         rstd.data_ptr(), dx.data_ptr(), lddx, dweight.data_ptr(), dbias.data_ptr(), rows, cols,
-        scratch.data_ptr(), nb, _launch_stream(dev, stream))
+        _ptr(scratch), nb, _launch_stream(dev, stream))
     check(rc, "mx_layer_norm_bwd")
     return dx, dweight, dbias
 

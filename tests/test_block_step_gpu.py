@@ -89,6 +89,7 @@ def test_gradients_of_the_whole_block(cuda_device, dtype):
     want = -torch.log_softmax(logits, 1).gather(1, labels.long()[:, None]).mean()
     grads = torch.autograd.grad(want, [*leaves.values(), xd])
     tol = 3.1e-3 + (7 * 2.0 ** -8 if dtype is BF16 else 0.0)
+    want = want.detach()
     assert abs(float(loss) - float(want)) <= tol * abs(float(want))
     for k, w in zip([*leaves, "x"], grads):
         g = dx if k == "x" else got[k]

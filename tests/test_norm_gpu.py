@@ -66,7 +66,7 @@ def _all(x, w, b, dy, eps=1e-5, **kw):
 
 
 # the sizes around each kernel's limits: a warp's row, a block's, long rows
-SIZES = [(1, 1), (1, 8), (3, 7), (5, 33), (130, 256), (77, 257), (9, 512), (1000, 513), (4, 1024),
+SIZES = [(1, 1), (1, 8), (1025, 40), (1100, 300), (1024, 511), (1030, 520), (1200, 1000), (3, 7), (5, 33), (130, 256), (77, 257), (9, 512), (1000, 513), (4, 1024),
          (300, 1500), (600, 2048), (333, 2056), (700, 4100), (40, 8192), (19, 10000), (9, 16384),
          (5, 16385), (70, 20000), (2000, 64)]
 
@@ -232,8 +232,12 @@ def test_refusals(cuda_device):
     assert L.mx_layer_norm_fwd(h, 0, p, 63, None, None, p, 64, None, None, 8, 64, 1e-5, None) == bad
     assert L.mx_layer_norm_fwd(h, 0, None, 64, None, None, p, 64, None, None, 8, 64, 1e-5, None) == bad
     assert L.mx_layer_norm_fwd(h, 0, p, 64, None, None, p, 64, None, None, -1, 64, 1e-5, None) == bad
-    need = L.mx_layer_norm_bwd_scratch_bytes(h, 8, 64)
+    assert L.mx_layer_norm_bwd_scratch_bytes(h, 8, 64) == 0
+    x, w, b, dy = _problem(1100, 64, F32)
+    p = x.data_ptr()
+    _, mean, rstd = ops.layer_norm(x, stats=True)
+    need = L.mx_layer_norm_bwd_scratch_bytes(h, 1100, 64)
     args = (h, 0, dy.data_ptr(), 64, p, 64, None, mean.data_ptr(), rstd.data_ptr(), None, 0,
-            w.data_ptr(), None, 8, 64)
+            w.data_ptr(), None, 1100, 64)
     assert L.mx_layer_norm_bwd(*args, p, need - 1, None) == bad
     assert L.mx_layer_norm_bwd(*args, None, need, None) == bad
