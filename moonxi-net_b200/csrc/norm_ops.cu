@@ -354,12 +354,15 @@ __global__ void __launch_bounds__(block_threads(TPR), blocks_per_sm(TPR, 2)) nor
     }
     fetch(row + D * step, slot);
     slot = slot + 1 == D ? 0 : slot + 1;
+    // (x - mean) * rstd in one operation: the product's rounding is that of the
+    // saved mean once more
+    const float shift = -mean * rstd;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
       if ((i * TPR + t) * V < p.cols)
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          xh[i][j] = (xh[i][j] - mean) * rstd;
+          xh[i][j] = fmaf(xh[i][j], rstd, shift);
           dw[i][j] += a[i][j] * xh[i][j];
           db[i][j] += a[i][j];
           a[i][j] *= w[i][j];
@@ -367,7 +370,8 @@ __global__ void __launch_bounds__(block_threads(TPR), blocks_per_sm(TPR, 2)) nor
           s[1] += a[i][j] * xh[i][j];
         }
     row_sum<TPR>(s, buf, turn);
-    const float c1 = s[0] * inv_c, c2 = s[1] * inv_c;
+    // rstd * (a - mean(a) - xhat * mean(a * xhat))
+    const float k1 = -rstd * (s[0] * inv_c), k2 = -rstd * (s[1] * inv_c);
     if (p.dx) {
       T* dx = static_cast<T*>(p.dx) + row * p.lddx;
 #pragma unroll
@@ -375,7 +379,7 @@ __global__ void __launch_bounds__(block_threads(TPR), blocks_per_sm(TPR, 2)) nor
         const int c = (i * TPR + t) * V;
         if (c < p.cols) {
 #pragma unroll
-          for (int j = 0; j < V; ++j) a[i][j] = rstd * (a[i][j] - c1 - xh[i][j] * c2);
+          for (int j = 0; j < V; ++j) a[i][j] = fmaf(a[i][j], rstd, fmaf(xh[i][j], k2, k1));
           store_vec<T, V>(dx + c, a[i]);
         }
       }
@@ -537,31 +541,25 @@ __global__ void __launch_bounds__(32 * kSmallWarps) norm_bwd_small_kernel(const 
 }
 
 // out[c] = the sum over `blocks` partial rows; column c < cols goes to dw, the
-// rest to db.  A block takes 32 columns, its eight warps an eighth of the rows
-// each; the order is fixed.
-__global__ void __launch_bounds__(256) norm_finish_kernel(const float* __restrict__ part,
-                                                          int blocks, int cols, float* dw,
-                                                          float* db) {
-  __shared__ float sh[8][33];
+// rest to db.  A block takes 32 columns, its warps a share of the rows each; the
+// order is fixed.
+constexpr int kFinishWarps = 32;
+__global__ void __launch_bounds__(32 * kFinishWarps) norm_finish_kernel(
+    const float* __restrict__ part, int blocks, int cols, float* dw, float* db) {
+  __shared__ float sh[kFinishWarps][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t width = 2ll * cols, c = blockIdx.x * 32ll + lane;
-  float s0 = 0.0f, s1 = 0.0f, s2 = 0.0f, s3 = 0.0f;
+  float s = 0.0f;
   if (c < width) {
-    int r = warp;
-    for (; r + 24 < blocks; r += 32) {
-      s0 += part[r * width + c];
-      s1 += part[(r + 8) * width + c];
-      s2 += part[(r + 16) * width + c];
-      s3 += part[(r + 24) * width + c];
-    }
-    for (; r < blocks; r += 8) s0 += part[r * width + c];
+#pragma unroll 8
+    for (int r = warp; r < blocks; r += kFinishWarps) s += part[r * width + c];
   }
-  sh[warp][lane] = (s0 + s1) + (s2 + s3);
+  sh[warp][lane] = s;
   __syncthreads();
   if (warp == 0 && c < width) {
-    float s = 0.0f;
+    s = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) s += sh[i][lane];
+    for (int i = 0; i < kFinishWarps; ++i) s += sh[i][lane];
     if (c < cols) {
       if (dw) dw[c] = s;
     } else if (db) {
@@ -725,7 +723,7 @@ int layer_norm_bwd(Context* ctx, int dtype, const void* dy, int64_t lddy, const 
     note_launches(1);
   }
   if (e == cudaSuccess && sums) {
-    norm_finish_kernel<<<static_cast<unsigned>((2ll * cols + 31) / 32), 256, 0, s>>>(static_cast<const float*>(scratch),
+    norm_finish_kernel<<<static_cast<unsigned>((2ll * cols + 31) / 32), 32 * kFinishWarps, 0, s>>>(static_cast<const float*>(scratch),
                                                            blocks, cols, dw, db);
     note_launches(1);
     e = cudaGetLastError();
