@@ -13,6 +13,11 @@
 // The backward pass keeps each thread's columns of dweight and dbias in
 // registers over all the rows of its block; the blocks' partial sums are added
 // in a fixed order by a second, small kernel, so results repeat bit for bit.
+//
+// Measured, with the copy rate of such sizes in mind (64 MB bf16: 5.4 TB/s):
+// 8192 x 4096 bf16 25.3 us forward (134 MB, 5.3 TB/s), 46 us backward (201 MB,
+// 4.4 TB/s; a row's two sums wait for one another, and the registers leave room
+// for two blocks an SM); float32 49 us (5.5 TB/s) and 76 us (5.3 TB/s).
 #include <algorithm>
 
 #include <cuda_bf16.h>
@@ -86,12 +91,15 @@ __device__ __forceinline__ void load_par(const float* p, int c, float (&v)[V], f
 }
 
 // Sums of N values over the TPR threads of a row, given to all of them, in a
-// fixed order.  TPR = 32: the row is a warp's.  Otherwise the block's: `buf`
-// holds two sets of N floats a warp, used in turn, so that one barrier a sum is
-// enough (whoever writes a set again has passed the barrier of the sum between,
-// which its readers reach after reading).
+// fixed order.  TPR = 32: the row is a warp's.  Otherwise the row is the
+// block's, or (rows > 1) that of the block's group-th TPR threads, which have a
+// named barrier of their own.  `buf` holds two sets of N floats a warp of the
+// row, used in turn, so that one barrier a sum is enough (whoever writes a set
+// again has passed the barrier of the sum between, which its readers reach
+// after reading).
 template <int TPR, int N>
-__device__ __forceinline__ void row_sum(float (&s)[N], float* buf, int& turn) {
+__device__ __forceinline__ void row_sum(float (&s)[N], float* buf, int& turn, int rows = 1,
+                                        int group = 0) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1)
 #pragma unroll
@@ -102,8 +110,9 @@ __device__ __forceinline__ void row_sum(float (&s)[N], float* buf, int& turn) {
     turn ^= 1;
     if ((threadIdx.x & 31) == 0)
 #pragma unroll
-      for (int i = 0; i < N; ++i) b[i * W + (threadIdx.x >> 5)] = s[i];
-    __syncthreads();
+      for (int i = 0; i < N; ++i) b[i * W + (threadIdx.x % TPR >> 5)] = s[i];
+    if (rows == 1) __syncthreads();
+    else asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "n"(TPR) : "memory");
 #pragma unroll
     for (int i = 0; i < N; ++i) s[i] = b[i * W + (threadIdx.x & (W - 1))];
 #pragma unroll
@@ -117,25 +126,59 @@ __device__ __forceinline__ void row_sum(float (&s)[N], float* buf, int& turn) {
 // rows to its own places in shared memory (no other thread reads them, so no
 // barrier), and takes them into registers when their turn comes.
 constexpr int kRingBytes = 200 * 1024;  // of an SM, over its blocks
-__host__ __device__ constexpr int block_threads(int tpr) { return tpr == 32 ? 128 : tpr; }
+// Threads of a block: forward a row's (or four rows' of a warp each), backward
+// 256 (or a longer row's), so that few blocks have partial sums to write.
+__host__ __device__ constexpr int block_threads(int tpr, int tensors) {
+  return tensors == 1 ? (tpr == 32 ? 128 : tpr) : tpr < 256 ? 256 : tpr;
+}
 // Blocks an SM is given: 768 threads forward (one tensor), 512 backward (two,
 // and the columns' sums in registers).
 __host__ __device__ constexpr int blocks_per_sm(int tpr, int tensors) {
-  const int n = (tensors == 1 ? 768 : 512) / block_threads(tpr);
+  const int n = (tensors == 1 ? 768 : 512) / block_threads(tpr, tensors);
   return n < 1 ? 1 : n;
 }
 __host__ __device__ constexpr int ring_rows(int tpr, int e, int size, int tensors) {
-  const int d = kRingBytes / blocks_per_sm(tpr, tensors) / (block_threads(tpr) * e * size * tensors);
+  const int d = kRingBytes / blocks_per_sm(tpr, tensors) /
+                (block_threads(tpr, tensors) * e * size * tensors);
   return d < 1 ? 1 : d > 4 ? 4 : d;
 }
 __host__ __device__ constexpr int ring_bytes(int tpr, int e, int size, int tensors, int v) {
-  return v == 1 ? 0 : ring_rows(tpr, e, size, tensors) * block_threads(tpr) * e * size * tensors;
+  return v == 1 ? 0
+                : ring_rows(tpr, e, size, tensors) * block_threads(tpr, tensors) * e * size * tensors;
 }
 __device__ __forceinline__ void copy16(void* dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
                    static_cast<uint32_t>(__cvta_generic_to_shared(dst))),
                "l"(src)
                : "memory");
+}
+
+// Two float32 in a register pair, one instruction for both (fma.rn.f32x2 and
+// its kin): the backward pass has ten operations a value (8192 x 1024 bf16: 13.3
+// us against 14.2 one at a time, 65536 x 256: 21.4 against 23.7).
+using Pair = uint64_t;
+__device__ __forceinline__ Pair pair(float a, float b) {
+  Pair r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpair(Pair p, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p));
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+  Pair r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+  Pair r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+  Pair r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
 }
 
 struct NormFwd {
@@ -154,8 +197,8 @@ struct NormFwd {
 // consecutive columns.  A block takes rows blockIdx.x, + gridDim.x, ...
 // (TPR = 32: four at a time, one a warp).
 template <typename T, int TPR, int E, int V>
-__global__ void __launch_bounds__(block_threads(TPR), blocks_per_sm(TPR, 1)) norm_fwd_kernel(const NormFwd p) {
-  constexpr int NV = E / V, D = ring_rows(TPR, E, sizeof(T), 1), BLOCK = block_threads(TPR);
+__global__ void __launch_bounds__(block_threads(TPR, 1), blocks_per_sm(TPR, 1)) norm_fwd_kernel(const NormFwd p) {
+  constexpr int NV = E / V, D = ring_rows(TPR, E, sizeof(T), 1), BLOCK = block_threads(TPR, 1);
   extern __shared__ uint4 ring[];  // [D][NV][BLOCK]
   __shared__ __align__(16) float buf[TPR > 32 ? 2 * 2 * TPR / 32 : 1];
   const int t = TPR == 32 ? threadIdx.x & 31 : threadIdx.x;
@@ -285,26 +328,37 @@ struct NormBwd {
   int rows, cols;
 };
 
-// Rows as in norm_fwd_kernel; TPR = 32: the four warps' sums meet in shared
-// memory at the end.
+// A block takes ROWS rows at a time, TPR threads each; the rows' sums of dweight
+// and dbias meet in shared memory at the end.
 template <typename T, int TPR, int E, int V>
-__global__ void __launch_bounds__(block_threads(TPR), blocks_per_sm(TPR, 2)) norm_bwd_kernel(const NormBwd p) {
-  constexpr int NV = E / V, D = ring_rows(TPR, E, sizeof(T), 2), BLOCK = block_threads(TPR);
+__global__ void __launch_bounds__(block_threads(TPR, 2), blocks_per_sm(TPR, 2)) norm_bwd_kernel(const NormBwd p) {
+  constexpr int NV = E / V, D = ring_rows(TPR, E, sizeof(T), 2), BLOCK = block_threads(TPR, 2);
+  constexpr int ROWS = BLOCK / TPR;
   extern __shared__ uint4 ring[];  // [D][2][NV][BLOCK]
-  __shared__ __align__(16) float buf[TPR > 32 ? 2 * 2 * TPR / 32 : 4 * 32 * E];
-  const int t = TPR == 32 ? threadIdx.x & 31 : threadIdx.x;
-  const int warp = threadIdx.x >> 5;
+  __shared__ __align__(16) float buf[ROWS > 1 ? BLOCK * E : 2 * 2 * TPR / 32];
+  const int t = threadIdx.x % TPR, group = threadIdx.x / TPR;
+  float* sums = buf + (ROWS > 1 ? group * (2 * 2 * TPR / 32) : 0);
   const float inv_c = 1.0f / static_cast<float>(p.cols);
-  float w[NV][V], dw[NV][V], db[NV][V];
+  // value e = i * V + j of a thread is column (i * TPR + t) * V + j; past the
+  // last column all of it is zero
+  Pair w[E / 2], dw[E / 2], db[E / 2];
+  {
+    float v[NV][V];
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int c = (i * TPR + t) * V;
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * TPR + t) * V;
 #pragma unroll
-    for (int j = 0; j < V; ++j) w[i][j] = dw[i][j] = db[i][j] = 0.0f;
-    if (c < p.cols) load_par<V>(p.w, c, w[i], 1.0f);
+      for (int j = 0; j < V; ++j) v[i][j] = 0.0f;
+      if (c < p.cols) load_par<V>(p.w, c, v[i], 1.0f);
+    }
+#pragma unroll
+    for (int e = 0; e < E; e += 2) {
+      w[e / 2] = pair(v[e / V][e % V], v[(e + 1) / V][(e + 1) % V]);
+      dw[e / 2] = db[e / 2] = pair(0.0f, 0.0f);
+    }
   }
-  const int64_t step = TPR == 32 ? gridDim.x * 4ll : gridDim.x;
-  int64_t row = TPR == 32 ? blockIdx.x * 4ll + warp : blockIdx.x;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * ROWS;
+  int64_t row = static_cast<int64_t>(blockIdx.x) * ROWS + group;
   auto fetch = [&](int64_t r, int slot) {
     if constexpr (V > 1) {
       if (r < p.rows) {
@@ -325,70 +379,92 @@ __global__ void __launch_bounds__(block_threads(TPR), blocks_per_sm(TPR, 2)) nor
 #pragma unroll
   for (int d = 0; d < D; ++d) fetch(row + d * step, d);
   int slot = 0, turn = 0;
-  float next_mean = 0.0f, next_rstd = 0.0f;  // a row ahead, like the rows
-  if (row < p.rows) {
-    next_mean = __ldg(p.mean + row);
-    next_rstd = __ldg(p.rstd + row);
-  }
-  for (; row < p.rows; row += step) {
-    const float mean = next_mean, rstd = next_rstd;
-    if (row + step < p.rows) {
-      next_mean = __ldg(p.mean + row + step);
-      next_rstd = __ldg(p.rstd + row + step);
+  // The rows' statistics, 32 rows of the block at a time, one a lane: a load a
+  // row would be waited for at every row.
+  float lane_mean = 0.0f, lane_rstd = 0.0f;
+  for (int n = 0; row < p.rows; row += step, ++n) {
+    if ((n & 31) == 0) {
+      const int64_t r = row + (threadIdx.x & 31) * step;
+      if (r < p.rows) {
+        lane_mean = __ldg(p.mean + r);
+        lane_rstd = __ldg(p.rstd + r);
+      }
     }
-    float xh[NV][V], a[NV][V];
-    float s[2] = {0.0f, 0.0f};
+    const float mean = __shfl_sync(0xffffffffu, lane_mean, n & 31);
+    const float rstd = __shfl_sync(0xffffffffu, lane_rstd, n & 31);
+    Pair xh[E / 2], a[E / 2];
     if constexpr (V > 1) cp_async_wait<D - 1>();
+    {
+      float xv[NV][V], g[NV][V];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (i * TPR + t) * V;
-      if (c < p.cols) {
-        if constexpr (V > 1) {
-          load_vec<T, V>(reinterpret_cast<const T*>(ring + (slot * 2 * NV + i) * BLOCK + threadIdx.x), xh[i]);
-          load_vec<T, V>(reinterpret_cast<const T*>(ring + (slot * 2 * NV + NV + i) * BLOCK + threadIdx.x), a[i]);
-        } else {
-          load_vec<T, V>(static_cast<const T*>(p.x) + row * p.ldx + c, xh[i]);
-          load_vec<T, V>(static_cast<const T*>(p.dy) + row * p.lddy + c, a[i]);
+      for (int i = 0; i < NV; ++i) {
+        const int c = (i * TPR + t) * V;
+#pragma unroll
+        for (int j = 0; j < V; ++j) xv[i][j] = g[i][j] = 0.0f;
+        if (c < p.cols) {
+          if constexpr (V > 1) {
+            load_vec<T, V>(reinterpret_cast<const T*>(ring + (slot * 2 * NV + i) * BLOCK + threadIdx.x), xv[i]);
+            load_vec<T, V>(reinterpret_cast<const T*>(ring + (slot * 2 * NV + NV + i) * BLOCK + threadIdx.x), g[i]);
+          } else {
+            load_vec<T, V>(static_cast<const T*>(p.x) + row * p.ldx + c, xv[i]);
+            load_vec<T, V>(static_cast<const T*>(p.dy) + row * p.lddy + c, g[i]);
+          }
         }
+      }
+#pragma unroll
+      for (int e = 0; e < E; e += 2) {
+        xh[e / 2] = pair(xv[e / V][e % V], xv[(e + 1) / V][(e + 1) % V]);
+        a[e / 2] = pair(g[e / V][e % V], g[(e + 1) / V][(e + 1) % V]);
       }
     }
     fetch(row + D * step, slot);
     slot = slot + 1 == D ? 0 : slot + 1;
     // (x - mean) * rstd in one operation: the product's rounding is that of the
     // saved mean once more
-    const float shift = -mean * rstd;
+    const Pair r2 = pair(rstd, rstd), shift = pair(-mean * rstd, -mean * rstd);
+    Pair s0 = pair(0.0f, 0.0f), s1 = s0;
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-      if ((i * TPR + t) * V < p.cols)
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          xh[i][j] = fmaf(xh[i][j], rstd, shift);
-          dw[i][j] += a[i][j] * xh[i][j];
-          db[i][j] += a[i][j];
-          a[i][j] *= w[i][j];
-          s[0] += a[i][j];
-          s[1] += a[i][j] * xh[i][j];
-        }
-    row_sum<TPR>(s, buf, turn);
+    for (int e = 0; e < E / 2; ++e) {
+      xh[e] = fma2(xh[e], r2, shift);
+      dw[e] = fma2(a[e], xh[e], dw[e]);
+      db[e] = add2(db[e], a[e]);
+      a[e] = mul2(a[e], w[e]);
+      s0 = add2(s0, a[e]);
+      s1 = fma2(a[e], xh[e], s1);
+    }
+    float s[2], hi[2];
+    unpair(s0, s[0], hi[0]);
+    unpair(s1, s[1], hi[1]);
+    s[0] += hi[0];
+    s[1] += hi[1];
+    row_sum<TPR>(s, sums, turn, ROWS, group);
     // rstd * (a - mean(a) - xhat * mean(a * xhat))
     const float k1 = -rstd * (s[0] * inv_c), k2 = -rstd * (s[1] * inv_c);
     if (p.dx) {
       T* dx = static_cast<T*>(p.dx) + row * p.lddx;
+      const Pair k1p = pair(k1, k1), k2p = pair(k2, k2);
+      float v[NV][V];
+#pragma unroll
+      for (int e = 0; e < E; e += 2)
+        unpair(fma2(a[e / 2], r2, fma2(xh[e / 2], k2p, k1p)), v[e / V][e % V],
+               v[(e + 1) / V][(e + 1) % V]);
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         const int c = (i * TPR + t) * V;
-        if (c < p.cols) {
-#pragma unroll
-          for (int j = 0; j < V; ++j) a[i][j] = fmaf(a[i][j], rstd, fmaf(xh[i][j], k2, k1));
-          store_vec<T, V>(dx + c, a[i]);
-        }
+        if (c < p.cols) store_vec<T, V>(dx + c, v[i]);
       }
     }
   }
+  float dwf[NV][V], dbf[NV][V];
+#pragma unroll
+  for (int e = 0; e < E; e += 2) {
+    unpair(dw[e / 2], dwf[e / V][e % V], dwf[(e + 1) / V][(e + 1) % V]);
+    unpair(db[e / 2], dbf[e / V][e % V], dbf[(e + 1) / V][(e + 1) % V]);
+  }
   if (!p.part) return;
   float* out = p.part + static_cast<int64_t>(blockIdx.x) * 2 * p.cols;
-  if constexpr (TPR == 32) {
-    // the four warps' sums, in their order
+  if constexpr (ROWS > 1) {
+    // the rows' sums, in their order
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       __syncthreads();
@@ -396,10 +472,14 @@ __global__ void __launch_bounds__(block_threads(TPR), blocks_per_sm(TPR, 2)) nor
       for (int i = 0; i < NV; ++i)
 #pragma unroll
         for (int j = 0; j < V; ++j)
-          buf[warp * 32 * E + (i * 32 + t) * V + j] = k ? db[i][j] : dw[i][j];
+          buf[group * TPR * E + (i * TPR + t) * V + j] = k ? dbf[i][j] : dwf[i][j];
       __syncthreads();
-      for (int c = threadIdx.x; c < p.cols; c += 128)
-        out[k * p.cols + c] = (buf[c] + buf[32 * E + c]) + (buf[2 * 32 * E + c] + buf[3 * 32 * E + c]);
+      for (int c = threadIdx.x; c < p.cols; c += BLOCK) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) sum += buf[r * TPR * E + c];
+        out[k * p.cols + c] = sum;
+      }
     }
   } else {
 #pragma unroll
@@ -408,8 +488,8 @@ __global__ void __launch_bounds__(block_threads(TPR), blocks_per_sm(TPR, 2)) nor
       if (c < p.cols)
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          out[c + j] = dw[i][j];
-          out[p.cols + c + j] = db[i][j];
+          out[c + j] = dwf[i][j];
+          out[p.cols + c + j] = dbf[i][j];
         }
     }
   }
@@ -417,7 +497,7 @@ __global__ void __launch_bounds__(block_threads(TPR), blocks_per_sm(TPR, 2)) nor
 
 // Long rows: dx in two passes over the row; the columns' sums are a kernel of
 // their own (norm_cols_kernel), since no block holds a row's columns.
-template <typename T>
+template <typename T, int V>
 __global__ void __launch_bounds__(1024) norm_bwd_long_kernel(const NormBwd p) {
   __shared__ __align__(16) float buf[2 * 2 * 32];
   int turn = 0;
@@ -427,34 +507,61 @@ __global__ void __launch_bounds__(1024) norm_bwd_long_kernel(const NormBwd p) {
   T* dx = static_cast<T*>(p.dx) + row * p.lddx;
   const float mean = p.mean[row], rstd = p.rstd[row];
   float s[2] = {0.0f, 0.0f};
-  for (int c = threadIdx.x; c < p.cols; c += 1024) {
-    const float a = to_f(dy[c]) * (p.w ? p.w[c] : 1.0f);
-    s[0] += a;
-    s[1] += a * ((to_f(x[c]) - mean) * rstd);
+#pragma unroll 2
+  for (int c = threadIdx.x * V; c < p.cols; c += 1024 * V) {
+    float xv[V], a[V], w[V];
+    load_vec<T, V>(x + c, xv);
+    load_vec<T, V>(dy + c, a);
+    load_par<V>(p.w, c, w, 1.0f);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      a[j] *= w[j];
+      s[0] += a[j];
+      s[1] += a[j] * ((xv[j] - mean) * rstd);
+    }
   }
   row_sum<1024>(s, buf, turn);
   const float inv_c = 1.0f / static_cast<float>(p.cols);
   const float c1 = s[0] * inv_c, c2 = s[1] * inv_c;
-  for (int c = threadIdx.x; c < p.cols; c += 1024) {
-    const float a = to_f(dy[c]) * (p.w ? p.w[c] : 1.0f);
-    dx[c] = from_f<T>(rstd * (a - c1 - (to_f(x[c]) - mean) * rstd * c2));
+#pragma unroll 2
+  for (int c = threadIdx.x * V; c < p.cols; c += 1024 * V) {
+    float xv[V], a[V], w[V];
+    load_vec<T, V>(x + c, xv);
+    load_vec<T, V>(dy + c, a);
+    load_par<V>(p.w, c, w, 1.0f);
+#pragma unroll
+    for (int j = 0; j < V; ++j) a[j] = rstd * (a[j] * w[j] - c1 - (xv[j] - mean) * rstd * c2);
+    store_vec<T, V>(dx + c, a);
   }
 }
-template <typename T>
+// A block: 256 * V columns, a range of rows.
+template <typename T, int V>
 __global__ void __launch_bounds__(256) norm_cols_kernel(const NormBwd p) {
-  const int c = blockIdx.x * 256 + threadIdx.x;
+  const int64_t c = (blockIdx.x * 256ll + threadIdx.x) * V;
   if (c >= p.cols) return;
   const int64_t per = (static_cast<int64_t>(p.rows) + gridDim.y - 1) / gridDim.y;
   const int64_t r0 = blockIdx.y * per, r1 = r0 + per < p.rows ? r0 + per : p.rows;
-  float dw = 0.0f, db = 0.0f;
+  float dw[V], db[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) dw[j] = db[j] = 0.0f;
+#pragma unroll 4
   for (int64_t r = r0; r < r1; ++r) {
-    const float g = to_f(static_cast<const T*>(p.dy)[r * p.lddy + c]);
-    dw += g * ((to_f(static_cast<const T*>(p.x)[r * p.ldx + c]) - p.mean[r]) * p.rstd[r]);
-    db += g;
+    float xv[V], g[V];
+    load_vec<T, V>(static_cast<const T*>(p.x) + r * p.ldx + c, xv);
+    load_vec<T, V>(static_cast<const T*>(p.dy) + r * p.lddy + c, g);
+    const float mean = __ldg(p.mean + r), rstd = __ldg(p.rstd + r);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      dw[j] += g[j] * ((xv[j] - mean) * rstd);
+      db[j] += g[j];
+    }
   }
   float* out = p.part + static_cast<int64_t>(blockIdx.y) * 2 * p.cols;
-  out[c] = dw;
-  out[p.cols + c] = db;
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    out[c + j] = dw[j];
+    out[p.cols + c + j] = db[j];
+  }
 }
 
 // Small problems in one launch: the first row_blocks blocks make dx, a warp a
@@ -568,12 +675,13 @@ __global__ void __launch_bounds__(32 * kFinishWarps) norm_finish_kernel(
   }
 }
 
-// Columns up to which a row is held in registers.
-constexpr int kNormRegCols = 16384;
+// Columns up to which a row is held in registers.  (Backward, 2048 x 16384
+// bf16: 137 us with the columns' sums of 1024 threads partly in local memory, 93
+// us in two passes.)
+constexpr int kFwdCols = 16384, kBwdCols = 8192;
 
-// Blocks of a pass over rows: as many as fit on the SMs at a time.
-int row_blocks(int rows, int cols, int per_sm, int num_sms) {
-  const int at_once = cols <= 512 ? 4 : 1;  // rows of a block
+// Blocks of a pass over rows, at_once each: as many as fit on the SMs at a time.
+int row_blocks(int rows, int at_once, int per_sm, int num_sms) {
   return std::max(1, std::min(per_sm * num_sms, (rows + at_once - 1) / at_once));
 }
 
@@ -584,7 +692,8 @@ cudaError_t run_fwd(const NormFwd& p, int num_sms, cudaStream_t s) {
   static SmemOptIn opt_in;
   cudaError_t e = kBytes > 32768 ? opt_in.ensure(kern, kBytes) : cudaSuccess;
   if (e != cudaSuccess) return e;
-  kern<<<row_blocks(p.rows, p.cols, blocks_per_sm(TPR, 1), num_sms), block_threads(TPR), kBytes,
+  const int at_once = block_threads(TPR, 1) / TPR;
+  kern<<<row_blocks(p.rows, at_once, blocks_per_sm(TPR, 1), num_sms), block_threads(TPR, 1), kBytes,
          s>>>(p);
   return cudaGetLastError();
 }
@@ -607,7 +716,7 @@ cudaError_t run_bwd(const NormBwd& p, int blocks, cudaStream_t s) {
   static SmemOptIn opt_in;
   cudaError_t e = kBytes > 32768 ? opt_in.ensure(kern, kBytes) : cudaSuccess;
   if (e != cudaSuccess) return e;
-  kern<<<blocks, block_threads(TPR), kBytes, s>>>(p);
+  kern<<<blocks, block_threads(TPR, 2), kBytes, s>>>(p);
   return cudaGetLastError();
 }
 template <typename T, int V>
@@ -618,16 +727,29 @@ cudaError_t launch_bwd(const NormBwd& p, int blocks, cudaStream_t s) {
   if (c <= 1024) return run_bwd<T, 64, 16, V>(p, blocks, s);
   if (c <= 2048) return run_bwd<T, 128, 16, V>(p, blocks, s);
   if (c <= 4096) return run_bwd<T, 256, 16, V>(p, blocks, s);
-  if (c <= 8192) return run_bwd<T, 512, 16, V>(p, blocks, s);
-  return run_bwd<T, 1024, 16, V>(p, blocks, s);
+  return run_bwd<T, 512, 16, V>(p, blocks, s);
+}
+
+template <typename T, int V>
+cudaError_t launch_long(const NormBwd& p, int blocks, cudaStream_t s) {
+  if (p.dx) {
+    norm_bwd_long_kernel<T, V><<<p.rows, 1024, 0, s>>>(p);
+    note_launches(1);
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+  }
+  if (p.part) {
+    norm_cols_kernel<T, V><<<dim3((p.cols + 256 * V - 1) / (256 * V), blocks), 256, 0, s>>>(p);
+    note_launches(1);
+  }
+  return cudaGetLastError();
 }
 
 // Blocks of the backward pass (rows of partial sums).
 int bwd_blocks(int rows, int cols, int num_sms) {
-  if (cols > kNormRegCols) return std::min(64, (rows + 63) / 64);  // row ranges of norm_cols
-  const int tpr = cols <= 512 ? 32 : cols <= 1024 ? 64 : cols <= 2048 ? 128 : cols <= 4096 ? 256
-                : cols <= 8192 ? 512 : 1024;
-  return row_blocks((rows + 1) / 2, cols, blocks_per_sm(tpr, 2), num_sms);
+  if (cols > kBwdCols) return std::min(64, (rows + 63) / 64);  // row ranges of norm_cols
+  const int tpr = cols <= 512 ? 32 : cols <= 1024 ? 64 : cols <= 2048 ? 128 : cols <= 4096 ? 256 : 512;
+  return row_blocks((rows + 1) / 2, block_threads(tpr, 2) / tpr, blocks_per_sm(tpr, 2), num_sms);
 }
 
 // Small enough for norm_bwd_small_kernel, whose columns' blocks walk down all
@@ -655,7 +777,7 @@ int layer_norm_fwd(Context* ctx, int dtype, const void* x, int64_t ldx, const fl
   const bool v16 = cols % vec == 0 && ldx % vec == 0 && ldy % vec == 0 && aligned16(x) &&
                    aligned16(y) && aligned16(w) && aligned16(b);
   cudaError_t e;
-  if (cols > kNormRegCols) {
+  if (cols > kFwdCols) {
     if (dtype == MX_BF16) norm_fwd_long_kernel<__nv_bfloat16><<<rows, 1024, 0, s>>>(p);
     else norm_fwd_long_kernel<float><<<rows, 1024, 0, s>>>(p);
     e = cudaGetLastError();
@@ -701,20 +823,11 @@ int layer_norm_bwd(Context* ctx, int dtype, const void* dy, int64_t lddy, const 
   const NormBwd p{dy, x, w, mean, rstd, dx, sums ? static_cast<float*>(scratch) : nullptr,
                   lddy, ldx, lddx, rows, cols};
   cudaError_t e = cudaSuccess;
-  if (cols > kNormRegCols) {
-    if (dx) {
-      if (dtype == MX_BF16) norm_bwd_long_kernel<__nv_bfloat16><<<rows, 1024, 0, s>>>(p);
-      else norm_bwd_long_kernel<float><<<rows, 1024, 0, s>>>(p);
-      note_launches(1);
-      e = cudaGetLastError();
-    }
-    if (e == cudaSuccess && sums) {
-      const dim3 grid((cols + 255) / 256, blocks);
-      if (dtype == MX_BF16) norm_cols_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(p);
-      else norm_cols_kernel<float><<<grid, 256, 0, s>>>(p);
-      note_launches(1);
-      e = cudaGetLastError();
-    }
+  if (cols > kBwdCols) {
+    e = dtype == MX_BF16 ? (v16 ? launch_long<__nv_bfloat16, 8>(p, blocks, s)
+                                : launch_long<__nv_bfloat16, 1>(p, blocks, s))
+                         : (v16 ? launch_long<float, 4>(p, blocks, s)
+                                : launch_long<float, 1>(p, blocks, s));
   } else {
     e = dtype == MX_BF16 ? (v16 ? launch_bwd<__nv_bfloat16, 8>(p, blocks, s)
                                 : launch_bwd<__nv_bfloat16, 1>(p, blocks, s))
