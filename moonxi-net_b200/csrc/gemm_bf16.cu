@@ -15,7 +15,8 @@
 // (Four stages of 32 of K: 60 us for that product against 45 when every stage
 // is added up, the epilogue's rate, and 48 us and 6e-7 when every second is.)
 //
-// CTA pairs (cta_group::2): a pair computes a 256 x 256 tile, each CTA holding
+// CTA pairs (cta_group::2): a pair computes a 256 x 256 tile (or two of them, see
+// below), each CTA holding
 // 128 rows of A, 128 columns of B and its 128 x 256 half of the accumulator:
 // 32 KB of loads a CTA for 64 of K where a single CTA's 128 x 256 tile loads
 // 48 KB, which is what keeps the L2 from being the bound.  Gated: the even
@@ -62,14 +63,20 @@ constexpr int kThreads = 320;
 constexpr int kTmemCols = 512;
 constexpr int kTrFloats = 32 * 33;     // a warp's transpose buffer
 
-// The ring: a slot holds one copy's tile of A and of B.  Three copies: a
-// k-block takes three slots, from the smallest copy to the largest, which is
-// the order in which the products give them back, so the next k-block but one
-// begins to load after a third of this one's MMAs.
-constexpr int kSlots = 6;
-constexpr int kSlotBytes = 2 * kOpBytes;
-constexpr int kSmem = kSlots * kSlotBytes + 8 * kTrFloats * 4 + 256 + 1024;
-static_assert(kSmem <= 232448, "shared memory of an SM");
+// The ring.  One copy: a slot is a k-block, SUB tiles of A and one of B.  Three
+// copies: a slot is one copy's tiles of A and B, a k-block takes three slots,
+// from the smallest copy to the largest, which is the order in which the
+// products give them back, so the next k-block but one begins to load after a
+// third of this one's MMAs.
+// VEC (the outputs' rows start on 16 bytes): no transpose buffers.
+template <int NC, bool VEC, int SUB>
+struct Ring {
+  static constexpr int kSlots = SUB == 2 ? 4 : 6;
+  static constexpr int kSlotBytes = (SUB + 1) * kOpBytes;
+  static constexpr int kTranspose = VEC ? 0 : 8 * kTrFloats;
+  static constexpr int kSmem = kSlots * kSlotBytes + kTranspose * 4 + 256 + 1024;
+  static_assert(kSmem <= 232448, "shared memory of an SM");
+};
 
 // One product of a launch.
 struct Problem {
@@ -83,7 +90,7 @@ struct Problem {
   int tiles_m, tiles_n, tiles;
   int splits, kb_per;  // k-blocks of a split
   int act;
-  int vec;          // bytes of a store to out: 32, 16, or 0 (rows unaligned)
+  int vec;          // bytes of a store to out: 32 or 16 (0: rows unaligned, not VEC)
   int a_kmajor, b_kmajor;
 };
 template <int NC>
@@ -95,6 +102,7 @@ struct Launch {
   uint64_t timeout_ns;
   int jobs0, jobs1;         // of each problem
   int fill;                 // see Queue
+  int sub;                  // tiles of 256 rows of a job
 };
 
 // The jobs of a pair, in order.  The first product's go round the pairs; where
@@ -153,9 +161,9 @@ __device__ __forceinline__ Job job_at(const Launch<NC>& L, int q, int j) {
   const Problem& p = L.p[q];
   r.split = j / p.tiles;
   r.tile = j - r.split * p.tiles;
-  // Bands of 8 tiles of rows, column by column inside a band: the pairs that
+  // Bands of tiles of 2048 rows, column by column inside a band: the pairs that
   // run at one time share rows of A and columns of B in L2.
-  constexpr int G = 8;
+  const int G = 8 / L.sub;
   const int band = r.tile / (G * p.tiles_n);
   const int gm = min(G, p.tiles_m - band * G);
   const int i = r.tile - band * G * p.tiles_n;
@@ -227,15 +235,18 @@ __device__ __forceinline__ void store_row(__nv_bfloat16* p, const float (&v)[32]
     }
 }
 
-template <int NC, bool GATED>
+template <int NC, bool GATED, bool VEC, int SUB>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     bf16_gemm_kernel(const __grid_constant__ Launch<NC> L) {
   using T = typename std::conditional<NC == 1, __nv_bfloat16, float>::type;
+  static_assert(NC == 1 || SUB == 1, "three copies' accumulators are added up");
+  constexpr int kSlots = Ring<NC, VEC, SUB>::kSlots, kSlotBytes = Ring<NC, VEC, SUB>::kSlotBytes;
+  constexpr int kB = SUB * kOpBytes;  // B's tile in a slot
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   float* tr = reinterpret_cast<float*>(smem + kSlots * kSlotBytes);
-  uint64_t* full = reinterpret_cast<uint64_t*>(tr + 8 * kTrFloats);  // the even CTA's are used
+  uint64_t* full = reinterpret_cast<uint64_t*>(tr + Ring<NC, VEC, SUB>::kTranspose);  // the even CTA's are used
   uint64_t* empty = full + kSlots;
   uint64_t* acc_full = empty + kSlots;
   uint64_t* acc_empty = acc_full + 2;  // the even CTA's are used
@@ -287,7 +298,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       while (ok && queue.next(L, prob, number)) {
         const Job r = job_at(L, prob, number);
         const bool ak = L.p[r.q].a_kmajor, bk = L.p[r.q].b_kmajor;
-        const int m0 = r.tm * kTile + rank * kHalf;
+        const int m0 = r.tm * SUB * kTile + rank * kHalf;
         const int n0 = GATED ? r.tn * kHalf : r.tn * kTile + rank * kHalf;
         for (int kb = r.kb0; ok && kb < r.kb1; ++kb) {
 #pragma unroll
@@ -301,8 +312,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             armed |= 1u << slot;
             armed_parity = (armed_parity & ~(1u << slot)) | (phase << slot);
             const uint32_t bar = cluster_addr(&full[slot], 0);
-            load_tile(ak, base, &L.a[r.q][i], bar, m0, kb * kBK);
-            load_tile(bk, base + kOpBytes, &L.b[r.q][rank][i], bar, n0, kb * kBK);
+#pragma unroll
+            for (int u = 0; u < SUB; ++u)
+              load_tile(ak, base + u * kOpBytes, &L.a[r.q][i], bar, m0 + u * kTile, kb * kBK);
+            load_tile(bk, base + kB, &L.b[r.q][rank][i], bar, n0, kb * kBK);
             if (++slot == kSlots) {
               slot = 0;
               phase ^= 1;
@@ -330,69 +343,110 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       uint32_t phase = 0;
       int seg = 0;  // accumulators used so far
       bool ok = true;
-      auto take_acc = [&]() {
-        const int acc = seg & 1;
-        if (!wait_bar(&acc_empty[acc], (seg >> 1 & 1) ^ 1, abort_flag, L.status, L.timeout_ns, 402))
+      auto take_acc = [&](int n) {
+        if (!wait_bar(&acc_empty[n & 1], (n >> 1 & 1) ^ 1, abort_flag, L.status, L.timeout_ns, 402))
           return false;
         tc_fence_after();
         return true;
+      };
+      auto wait_slot = [&](int n, uint32_t parity) {
+        if (!wait_bar(&full[n], parity, abort_flag, L.status, L.timeout_ns, 403)) return false;
+        tc_fence_after();
+        return true;
+      };
+      auto advance = [&](int& n, uint32_t& parity, int by) {
+        n += by;
+        if (n == kSlots) {
+          n = 0;
+          parity ^= 1;
+        }
       };
       while (ok && queue.next(L, prob, number)) {
         const Job r = job_at(L, prob, number);
         const bool ak = L.p[r.q].a_kmajor, bk = L.p[r.q].b_kmajor;
         const uint32_t idesc = idesc_bf16(kTile, kTile, !ak, !bk);
         const TileDesc da(ak), db(bk);
-        if (NC == 1) ok = take_acc();
-        uint32_t accumulate = 0;
-        for (int kb = r.kb0; ok && kb < r.kb1; ++kb) {
-          if (NC == 3) {
-            ok = take_acc();
+        // the k-block's product of the operand tiles at sa and sb into
+        // accumulator n
+        auto product = [&](int n, uint32_t sa, uint32_t sb, bool first) {
+          const uint32_t d = tmem_base + (n & 1) * kTile;
+#pragma unroll
+          for (int k = 0; k < kBK / 16; ++k)
+            mma_f16_pair(d, da.at(sa, k), db.at(sb, k), idesc, first && k == 0 ? 0 : 1);
+        };
+        if constexpr (NC == 3) {
+          for (int kb = r.kb0; ok && kb < r.kb1; ++kb) {
+            ok = take_acc(seg);
+            // copy i is in slot + 2 - i (six slots: a k-block does not wrap)
+#pragma unroll
+            for (int i = 0; ok && i < 3; ++i) ok = wait_slot(slot + i, phase);
             if (!ok) break;
-            accumulate = 0;
-          }
-          // the k-block's slots: copy i is in slot + NC - 1 - i (no wrap inside
-          // a k-block, kSlots being a multiple of NC)
-#pragma unroll
-          for (int i = 0; ok && i < NC; ++i)
-            ok = wait_bar(&full[slot + i], phase, abort_flag, L.status, L.timeout_ns, 403);
-          if (!ok) break;
-          tc_fence_after();
-          const uint32_t s0 = smem_u32(smem + slot * kSlotBytes);
-          const uint32_t d = tmem_base + (seg & 1) * kTile;
-          auto product = [&](int ca, int cb) {
-            const uint32_t sa = s0 + (NC - 1 - ca) * kSlotBytes;
-            const uint32_t sb = s0 + (NC - 1 - cb) * kSlotBytes + kOpBytes;
-#pragma unroll
-            for (int k = 0; k < kBK / 16; ++k) {
-              mma_f16_pair(d, da.at(sa, k), db.at(sb, k), idesc, accumulate);
-              accumulate = 1;
-            }
-          };
-          if (NC == 3) {  // from the smallest products to the largest
-            product(2, 0);
-            product(0, 2);
+            const uint32_t s0 = smem_u32(smem + slot * kSlotBytes);
+            auto copies = [&](int ca, int cb, bool first) {
+              product(seg, s0 + (2 - ca) * kSlotBytes, s0 + (2 - cb) * kSlotBytes + kB, first);
+            };
+            // from the smallest products to the largest
+            copies(2, 0, true);
+            copies(0, 2, false);
             tc_commit_both(&empty[slot]);
-            product(1, 1);
-            product(1, 0);
-            product(0, 1);
+            copies(1, 1, false);
+            copies(1, 0, false);
+            copies(0, 1, false);
             tc_commit_both(&empty[slot + 1]);
-          }
-          product(0, 0);
-          tc_commit_both(&empty[slot + NC - 1]);
-          if (NC == 3) {
+            copies(0, 0, false);
+            tc_commit_both(&empty[slot + 2]);
             tc_commit_both(&acc_full[seg & 1]);
             ++seg;
+            advance(slot, phase, 3);
           }
-          slot += NC;
-          if (slot == kSlots) {
-            slot = 0;
-            phase ^= 1;
+        } else if constexpr (SUB == 1) {
+          ok = take_acc(seg);
+          for (int kb = r.kb0; ok && kb < r.kb1; ++kb) {
+            ok = wait_slot(slot, phase);
+            if (!ok) break;
+            const uint32_t sa = smem_u32(smem + slot * kSlotBytes);
+            product(seg, sa, sa + kB, kb == r.kb0);
+            tc_commit_both(&empty[slot]);
+            advance(slot, phase, 1);
           }
-        }
-        if (!ok) break;
-        if (NC == 1) {
+          if (!ok) break;
           tc_commit_both(&acc_full[seg & 1]);
           ++seg;
+        } else {
+          // The first accumulator's products of a ring's worth of k-blocks run
+          // while the epilogue still reads the second.
+          const int ahead = min(kSlots, r.kb1 - r.kb0);
+          ok = take_acc(seg);
+          int n = slot;
+          uint32_t parity = phase;
+          for (int i = 0; ok && i < ahead; ++i) {
+            ok = wait_slot(n, parity);
+            if (!ok) break;
+            const uint32_t sa = smem_u32(smem + n * kSlotBytes);
+            product(seg, sa, sa + kB, i == 0);
+            advance(n, parity, 1);
+          }
+          if (ok && r.kb0 + ahead == r.kb1) tc_commit_both(&acc_full[seg & 1]);
+          ok = ok && take_acc(seg + 1);
+          for (int i = 0; ok && i < ahead; ++i) {
+            const uint32_t sa = smem_u32(smem + slot * kSlotBytes);
+            product(seg + 1, sa + kOpBytes, sa + kB, i == 0);
+            tc_commit_both(&empty[slot]);
+            advance(slot, phase, 1);
+          }
+          for (int kb = r.kb0 + ahead; ok && kb < r.kb1; ++kb) {
+            ok = wait_slot(slot, phase);
+            if (!ok) break;
+            const uint32_t sa = smem_u32(smem + slot * kSlotBytes);
+            product(seg, sa, sa + kB, false);
+            if (kb + 1 == r.kb1) tc_commit_both(&acc_full[seg & 1]);
+            product(seg + 1, sa + kOpBytes, sa + kB, false);
+            tc_commit_both(&empty[slot]);
+            advance(slot, phase, 1);
+          }
+          if (!ok) break;
+          tc_commit_both(&acc_full[(seg + 1) & 1]);
+          seg += 2;
         }
       }
       tc_commit_pair(drain);  // every MMA is done before TMEM is released
@@ -435,7 +489,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     while (ok && queue.next(L, prob, number)) {
       const Job r = job_at(L, prob, number);
       const Problem& p = L.p[r.q];
-      const int row0 = r.tm * kTile + rank * kHalf + group * 32;
+#pragma unroll 1
+      for (int sub = 0; ok && sub < SUB; ++sub) {
+      const int row0 = (r.tm * SUB + sub) * kTile + rank * kHalf + group * 32;
       const int rows = min(32, p.M - row0);  // may be below 1
       const bool mine = lane < rows;
       const int64_t row = row0 + lane;
@@ -447,10 +503,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       auto store_out = [&](int col0, const float (&v)[32]) {
         T* dst = static_cast<T*>(p.out) + row * p.ldc + col0;
         const int left = p.N - col0;
-        if (p.vec == 32) {
-          if (mine) store_row<32>(dst, v, left);
-        } else if (p.vec == 16) {
-          if (mine) store_row<16>(dst, v, left);
+        if (VEC) {
+          if (!mine) return;
+          if (p.vec == 32) store_row<32>(dst, v, left);
+          else store_row<16>(dst, v, left);
         } else {
           // unaligned rows: through shared memory, a row at a time
           __syncwarp();  // the last block's reads are done
@@ -540,6 +596,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           else finish(q, g, u);
         }
         free_acc();
+      }
       }
     }
   }
@@ -638,7 +695,7 @@ struct Plan {
 };
 struct Plans {
   Plan p[2];
-  int pairs = 0;
+  int pairs = 0, sub = 1;
   bool split() const { return p[0].splits > 1 || p[1].splits > 1; }
 };
 
@@ -647,59 +704,71 @@ void set_splits(Plan& q, int want) {
   q.splits = (q.num_kb + q.kb_per - 1) / q.kb_per;
 }
 
-// A job's cost in k-blocks: its start and epilogue come on top (one copy: six
-// k-blocks, three: one), for a split one the partial tile's way through memory
-// too.
-int job_cost(const Plan& q, int copies) {
-  return q.kb_per + (copies == 3 ? 1 : 6) * (q.splits > 1 ? 2 : 1);
+// A job's cost in cycles, as measured: a k-block (one copy, 256 rows: 512
+// cycles of MMAs, which wait for L2; 512 rows: 1024; three copies: 3072), and a
+// start and an epilogue that run beside other jobs' MMAs in part; a split job
+// has the partial tile's way through memory on top.
+int job_cost(const Plan& q, int copies, int sub) {
+  const int kb = copies == 3 ? 3400 : sub == 2 ? 1160 : 700;
+  return q.kb_per * kb + (copies == 3 ? 3400 : sub == 2 ? 7000 : 4200) * (q.splits > 1 ? 2 : 1);
 }
 // Queue's fill: what the first product's last round leaves to the pairs that
 // miss it.
 int fill_of(const Plans& pl, int pairs, int copies) {
   const int shorter = pairs - pl.p[0].jobs() % pairs;
   if (shorter == pairs || pl.p[1].jobs() == 0) return 0;
-  return std::min(job_cost(pl.p[0], copies) / job_cost(pl.p[1], copies), pl.p[1].jobs() / shorter);
+  return std::min(job_cost(pl.p[0], copies, pl.sub) / job_cost(pl.p[1], copies, pl.sub),
+                  pl.p[1].jobs() / shorter);
 }
-// The longest queue of a pair, in k-blocks; queues differ only where a product's
-// last round ends.
-int makespan(const Plans& pl, int pairs, int copies) {
-  const int c0 = job_cost(pl.p[0], copies), c1 = pl.p[1].jobs() > 0 ? job_cost(pl.p[1], copies) : 0;
+// The longest queue of a pair (queues differ only where a product's last round
+// ends), and the launch that adds split products up.
+int64_t makespan(const Plans& pl, int pairs, int copies) {
+  const int c0 = job_cost(pl.p[0], copies, pl.sub);
+  const int c1 = pl.p[1].jobs() > 0 ? job_cost(pl.p[1], copies, pl.sub) : 0;
   const int j0 = pl.p[0].jobs(), r = j0 % pairs, fill = fill_of(pl, pairs, copies);
   const int rest = pl.p[1].jobs() - (fill > 0 ? fill * (pairs - r) : 0);
   const int at[3] = {0, r, rest % pairs};
-  int worst = 0;
+  int64_t worst = 0;
   for (int c : at) {
     const int n0 = (j0 - c + pairs - 1) / pairs;
     const int n1 = (c >= r ? fill : 0) + (rest - c + pairs - 1) / pairs;
-    worst = std::max(worst, n0 * c0 + n1 * c1);
+    worst = std::max(worst, static_cast<int64_t>(n0) * c0 + static_cast<int64_t>(n1) * c1);
   }
-  return worst;
+  return worst + (pl.split() ? 6000 : 0);
 }
 
-// Whole tiles where they fill the machine; otherwise the split counts, the
-// longer product's first, with the shortest longest queue.
-Plans plan_of(const Context* ctx, const Bf16Gemm* g, int count) {
-  Plans pl;
-  const int copies = g[0].copies;
-  const int pairs = std::max(1, ctx->tc_sms() / 2);
+void set_tiles(Plans& pl, const Bf16Gemm* g, int count, int sub) {
+  pl.sub = sub;
   for (int i = 0; i < count; ++i) {
     Plan& q = pl.p[i];
     const int width = g[i].gated ? kHalf : kTile;
-    q.tiles_m = (g[i].M + kTile - 1) / kTile;
+    q.tiles_m = (g[i].M + sub * kTile - 1) / (sub * kTile);
     q.tiles_n = (g[i].N + width - 1) / width;
     q.tiles = q.tiles_m * q.tiles_n;
     q.num_kb = std::max(1, (g[i].K + kBK - 1) / kBK);
     q.kb_per = q.num_kb;
+    q.splits = 1;
   }
+}
+
+// Whole tiles of 256 or (one copy) 512 rows where they fill the machine;
+// otherwise the split counts, the longer product's first, with the shortest
+// longest queue.
+Plans plan_of(const Context* ctx, const Bf16Gemm* g, int count) {
+  Plans pl;
+  const int copies = g[0].copies;
+  const int pairs = std::max(1, ctx->tc_sms() / 2);
+  set_tiles(pl, g, count, 1);
   const int least = copies == 3 ? 2 : 8;  // k-blocks of a split
   const int longer = pl.p[1].num_kb > pl.p[0].num_kb ? 1 : 0;
   if (pl.p[0].tiles + pl.p[1].tiles < 3 * pairs) {
     for (int n = 0; n < count; ++n) {
       Plan& q = pl.p[n == 0 ? longer : 1 - longer];
-      int best = 1, cost = makespan(pl, pairs, copies);
+      int best = 1;
+      int64_t cost = makespan(pl, pairs, copies);
       for (int want = 2; want <= 16 && q.num_kb / want >= least; ++want) {
         set_splits(q, want);
-        const int c = makespan(pl, pairs, copies);
+        const int64_t c = makespan(pl, pairs, copies);
         if (c < cost) {
           best = want;
           cost = c;
@@ -707,6 +776,11 @@ Plans plan_of(const Context* ctx, const Bf16Gemm* g, int count) {
       }
       set_splits(q, best);
     }
+  }
+  if (copies == 1) {
+    Plans tall;
+    set_tiles(tall, g, count, 2);
+    if (makespan(tall, pairs, 1) < makespan(pl, pairs, 1)) pl = tall;
   }
   for (int i = 0; i < count; ++i) {
     Plan& q = pl.p[i];
@@ -767,13 +841,26 @@ int launch(Context* ctx, const Bf16Gemm* g, int count, void* scratch, const Bf16
   L.jobs0 = pl.p[0].jobs();
   L.jobs1 = pl.p[1].jobs();
   L.fill = fill_of(pl, pl.pairs, NC);
-  auto kern = bf16_gemm_kernel<NC, GATED>;
-  static SmemOptIn opt_in;
-  cudaError_t e = opt_in.ensure(kern, kSmem);
-  if (e != cudaSuccess) return cuda_status(e);
-  kern<<<2 * pl.pairs, kThreads, kSmem, s>>>(L);
-  note_launches(1);
-  e = cudaGetLastError();
+  L.sub = pl.sub;
+  auto start = [&](auto kern, int bytes, SmemOptIn& opt_in) {
+    cudaError_t e = opt_in.ensure(kern, bytes);
+    if (e != cudaSuccess) return e;
+    kern<<<2 * pl.pairs, kThreads, bytes, s>>>(L);
+    note_launches(1);
+    return cudaGetLastError();
+  };
+  static SmemOptIn opt_vec, opt_any;
+  const bool vec = L.p[0].vec > 0 && (count == 1 || L.p[1].vec > 0);
+  cudaError_t e;
+  if constexpr (NC == 1) {
+    static SmemOptIn tall_vec, tall_any;
+    if (pl.sub == 2)
+      e = vec ? start(bf16_gemm_kernel<1, GATED, true, 2>, Ring<1, true, 2>::kSmem, tall_vec)
+              : start(bf16_gemm_kernel<1, GATED, false, 2>, Ring<1, false, 2>::kSmem, tall_any);
+  }
+  if (pl.sub == 1)
+    e = vec ? start(bf16_gemm_kernel<NC, GATED, true, 1>, Ring<NC, true, 1>::kSmem, opt_vec)
+            : start(bf16_gemm_kernel<NC, GATED, false, 1>, Ring<NC, false, 1>::kSmem, opt_any);
   if (e != cudaSuccess || (!pl.split() && !sum)) return cuda_status(e);
   Tail t{};
   for (int i = 0; i < 2; ++i) {
