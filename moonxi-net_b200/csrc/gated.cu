@@ -18,6 +18,7 @@
 #include "gated_act.cuh"
 #include "mx_internal.h"
 #include "mx_ptx.cuh"
+#include "mx_unaligned.cuh"
 
 namespace mx {
 namespace {
@@ -63,6 +64,25 @@ __device__ __forceinline__ void load8(const bf16* p, float (&x)[8]) {
   for (int i = 0; i < 4; ++i) {
     x[2 * i] = __uint_as_float(w[i] << 16);
     x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void load8_any(const T* p, const T* lo, const T* hi, float (&x)[8]) {
+  if constexpr (sizeof(T) == 4) {
+    const uint4 a = load16_any(p, lo, hi), b = load16_any(p + 4, lo, hi);
+    x[0] = __uint_as_float(a.x); x[1] = __uint_as_float(a.y);
+    x[2] = __uint_as_float(a.z); x[3] = __uint_as_float(a.w);
+    x[4] = __uint_as_float(b.x); x[5] = __uint_as_float(b.y);
+    x[6] = __uint_as_float(b.z); x[7] = __uint_as_float(b.w);
+  } else {
+    const uint4 r = load16_any(p, lo, hi);
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[2 * i] = __uint_as_float(w[i] << 16);
+      x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
   }
 }
 
@@ -118,14 +138,16 @@ __device__ __forceinline__ void pack_block(const PackJob& p, int block) {
     }
     return;
   }
+  // the source's column of d, and how many of the eight are there
+  const int64_t c = d < p.up ? d : p.split + (d - p.up);
+  const int64_t end = d < p.up ? p.split : p.cols;
+  const int n = static_cast<int>(end - c < 8 ? end - c : 8);
+  const T* hi = src + static_cast<int64_t>(p.rows) * p.cols;
   for (; r < p.rows; r += p.by) {
     float x[8];
+    load8_any(src + r * p.cols + c, src, hi, x);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int64_t e = d + i;
-      const int64_t c = e < p.up ? (e < p.split ? e : p.cols) : p.split + (e - p.up);
-      x[i] = c < p.cols ? to_f(src[r * p.cols + c]) : 0.0f;
-    }
+    for (int i = 0; i < 8; ++i) x[i] = i < n ? x[i] : 0.0f;
     store_copies<NC>(x, p.dst + r * p.ldd + d, p.copy);
   }
 }
@@ -152,8 +174,10 @@ __device__ __forceinline__ void dpre_block(const Dpre& p, int block, float (&sh)
       if (p.vec) {
         load8(dh, d);
       } else {
+        load8_any(dh, static_cast<const T*>(p.dh),
+                  static_cast<const T*>(p.dh) + static_cast<int64_t>(p.rows) * p.F, d);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) d[i] = i < left ? to_f(dh[i]) : 0.0f;
+        for (int i = 0; i < 8; ++i) d[i] = i < left ? d[i] : 0.0f;
       }
       load8(pre, g);  // pre's rows are padded
       load8(pre + up, u);

@@ -120,6 +120,38 @@ def test_against_64_bits(cuda_device, M, K, F, dtype, tw):
     _run_and_check(M, K, F, dtype, tw, act, bias=(M + F) % 2 == 0, seed=M + K)
 
 
+# few rows: lengths on both sides of each of their kernels' widths and splits,
+# rows that start on any element
+@pytest.mark.parametrize("tw", [False, True])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("K,F", [(1, 1), (3, 2), (7, 9), (9, 3), (255, 257), (1025, 1151),
+                                 (2051, 2369), (4099, 127), (130, 4741)])
+def test_few_rows(cuda_device, K, F, dtype, tw):
+    for M in (1, 2, 3, 4):
+        _run_and_check(M, K, F, dtype, tw, ACTS[(M + K) % len(ACTS)], M % 2 == 0, seed=M + F)
+
+
+@pytest.mark.parametrize("tw", [False, True])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_few_rows_at_any_address(cuda_device, dtype, tw):
+    """The products of aligned tensors and of copies that start 1 to 7 elements
+    in, between values that would spoil a sum they get into."""
+    for K, F in ((64, 40), (61, 37), (2048, 24)):
+        for M in (1, 2, 4):
+            x, w, b, _ = _problem(M, K, F, dtype, tw, True, seed=K + M)
+            P = x.double() @ (w.double().t() if tw else w.double()) + b.double()
+            tol = (K + 40) * 2.0 ** -23 * (x.double().abs() @ (w.double().t() if tw else w.double()).abs()
+                                           + b.double().abs())
+            for off in range(8):
+                def moved(t):
+                    buf = torch.full((t.numel() + 16,), math.nan, device="cuda", dtype=dtype)
+                    v = buf[off:off + t.numel()].view(t.shape)
+                    v.copy_(t)
+                    return v
+                _, pre = ops.gated_linear(moved(x), moved(w), moved(b), transpose_w=tw, save=True)
+                _check("pre", _halves(pre, F), P, tol)
+
+
 @pytest.mark.parametrize("act", ACTS)
 @pytest.mark.parametrize("dtype,precision", [(BF16, "default"), (F32, "fp32"), (F32, "3xtf32"),
                                              (F32, "nparray")])
