@@ -176,6 +176,17 @@ __device__ __forceinline__ void store8(__nv_bfloat16* p, bool vec, int left, con
 // first moment, or (SIGNED false) the root of the second.  A byte is made a
 // float32 by putting it under the exponent of 2^23.
 template <bool SIGNED>
+__device__ __forceinline__ void decode_words(const uint32_t (&w)[2], float top, float (&x)[8]) {
+  const float unit = top * (SIGNED ? 1.0f / 16129.0f : 1.0f / 65025.0f);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t word = SIGNED ? w[i >> 2] ^ 0x80808080u : w[i >> 2];
+    const float c = __uint_as_float(__byte_perm(word, 0x4b000000u, 0x7440 + (i & 3))) -
+                    (SIGNED ? 8388736.0f : 8388608.0f);
+    x[i] = c * fabsf(c) * unit;
+  }
+}
+template <bool SIGNED>
 __device__ __forceinline__ void decode8(const uint8_t* q, float top, bool vec, int left,
                                         float (&x)[8]) {
   uint32_t w[2] = {0, 0};
@@ -188,14 +199,7 @@ __device__ __forceinline__ void decode8(const uint8_t* q, float top, bool vec, i
     for (int i = 0; i < 8; ++i)
       if (i < left) w[i >> 2] |= static_cast<uint32_t>(q[i]) << (8 * (i & 3));
   }
-  const float unit = top * (SIGNED ? 1.0f / 16129.0f : 1.0f / 65025.0f);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint32_t word = SIGNED ? w[i >> 2] ^ 0x80808080u : w[i >> 2];
-    const float c = __uint_as_float(__byte_perm(word, 0x4b000000u, 0x7440 + (i & 3))) -
-                    (SIGNED ? 8388736.0f : 8388608.0f);
-    x[i] = c * fabsf(c) * unit;
-  }
+  decode_words<SIGNED>(w, top, x);
 }
 // The warp's largest magnitude, at least 2^-120; NaN if a value is not finite.
 // As integers, magnitudes keep their order, with infinity and NaN above all.
@@ -310,21 +314,49 @@ __global__ void __launch_bounds__(32 * kWarps) adamw_kernel(const __grid_constan
 }
 
 // The values that 8-bit codes stand for, rounded to bf16: the first moment, or
-// (SIGNED false) the second.
+// (SIGNED false) the second.  A warp makes kValues blocks, whose loads are all on
+// their way before the first is used: 3 bytes a value (152M values: @@ us, with
+// one block a warp 115).
+constexpr int kValues = 4;
+template <bool SIGNED>
+__device__ __forceinline__ void store_values(__nv_bfloat16* out, bool vec, int left, float (&x)[8]) {
+  if (!SIGNED)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = __fmul_rn(x[i], x[i]);
+  store8(out, vec, left, x);
+}
 template <bool SIGNED>
 __global__ void __launch_bounds__(32 * kWarps) adamw_values_kernel(const uint8_t* q,
                                                                    const float* scale, int64_t n,
                                                                    __nv_bfloat16* out, bool vec) {
-  const int64_t block = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
-  const int64_t at = block * kQBlock + (threadIdx.x & 31) * 8;
-  if (at >= n) return;
-  const int left = n - at >= 8 ? 8 : static_cast<int>(n - at);
-  float x[8];
-  decode8<SIGNED>(q + at, scale[block], vec, left, x);
-  if (!SIGNED)
+  const int lane = threadIdx.x & 31;
+  const int64_t first = (blockIdx.x * static_cast<int64_t>(kWarps) + (threadIdx.x >> 5)) * kValues;
+  if (vec && (first + kValues) * kQBlock <= n) {
+    uint32_t w[kValues][2];
+    float top[kValues];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = __fmul_rn(x[i], x[i]);
-  store8(out + at, vec, left, x);
+    for (int k = 0; k < kValues; ++k) {
+      const uint2 r = __ldg(reinterpret_cast<const uint2*>(q + (first + k) * kQBlock) + lane);
+      w[k][0] = r.x;
+      w[k][1] = r.y;
+      top[k] = __ldg(scale + first + k);
+    }
+#pragma unroll
+    for (int k = 0; k < kValues; ++k) {
+      float x[8];
+      decode_words<SIGNED>(w[k], top[k], x);
+      store_values<SIGNED>(out + (first + k) * kQBlock + lane * 8, true, 8, x);
+    }
+    return;
+  }
+  for (int k = 0; k < kValues; ++k) {
+    const int64_t at = (first + k) * kQBlock + lane * 8;
+    if (at >= n) return;
+    const int left = n - at >= 8 ? 8 : static_cast<int>(n - at);
+    float x[8];
+    decode8<SIGNED>(q + at, scale[first + k], vec, left, x);
+    store_values<SIGNED>(out + at, vec, left, x);
+  }
 }
 
 // Sum of squares of the gradients of one launch's tensors: block b's sum of
@@ -526,7 +558,8 @@ int adamw_step(const mx_adamw_tensor* ts, int count, int bits, double lr, double
 int adamw_state_values(const void* q, const float* scale, int64_t n, int is_signed, void* out,
                        cudaStream_t s) {
   if (n <= 0) return kOk;
-  const int64_t blocks = (n + kWarps * kQBlock - 1) / (kWarps * kQBlock);
+  constexpr int64_t kEach = static_cast<int64_t>(kWarps) * kValues * kQBlock;
+  const int64_t blocks = (n + kEach - 1) / kEach;
   if (blocks > 0x7fffffff) return kErrUnsupported;
   const bool vec = aligned(q, 8) && aligned(out, 16);
   const uint8_t* c = static_cast<const uint8_t*>(q);

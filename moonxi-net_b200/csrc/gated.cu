@@ -47,6 +47,60 @@ __device__ __forceinline__ void store_copies(const float (&x)[8], bf16* dst, int
   }
 }
 
+// The copies of 8 values a lane of consecutive lanes (`lanes`, from 0 on), of
+// which `left` exist, to a row that starts `shift` elements behind 16 bytes: a
+// lane stores the aligned piece that ends in its own values, with the last ones
+// of the lane before it.  Ends are stored one by one.
+template <int NC>
+__device__ __forceinline__ void store_shifted(float (&x)[8], bf16* dst, int64_t copy, int shift,
+                                              int left, uint32_t lanes) {
+  const int lane = threadIdx.x & 31;
+  const bool next = lane < 31 && (lanes >> (lane + 1) & 1) != 0;
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    uint32_t w[8];  // the lane before's, then its own
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+      w[4 + i] = *reinterpret_cast<const uint32_t*>(&h);
+      if (c + 1 < NC) {
+        x[2 * i] -= __uint_as_float(w[4 + i] << 16);
+        x[2 * i + 1] -= __uint_as_float(w[4 + i] & 0xffff0000u);
+      }
+      w[i] = __shfl_up_sync(lanes, w[4 + i], 1);
+    }
+    bf16* to = dst + c * copy;
+    if (left == 8 && (lane > 0 || shift == 0)) {
+      // elements 8 - shift .. 15 - shift of the sixteen
+      uint32_t v[5];
+      const int word = (8 - shift) >> 1;
+#pragma unroll
+      for (int i = 0; i < 5; ++i) {
+        v[i] = 0;
+#pragma unroll
+        for (int j = 0; j <= 4; ++j)
+          if (word == j && i + j < 8) v[i] = w[i + j];
+      }
+      const uint32_t bits = (shift & 1) * 16;
+      *reinterpret_cast<uint4*>(to - shift) =
+          make_uint4(__funnelshift_r(v[0], v[1], bits), __funnelshift_r(v[1], v[2], bits),
+                     __funnelshift_r(v[2], v[3], bits), __funnelshift_r(v[3], v[4], bits));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {  // the lane before's last and its own first
+        const bool mine = i < 8 ? lane > 0 && i >= 8 - shift : i - 8 < left && i - 8 < 8 - shift;
+        if (mine) to[i - 8] = __ushort_as_bfloat16(static_cast<uint16_t>(w[i >> 1] >> (16 * (i & 1))));
+      }
+    }
+    if (!next) {  // nobody else stores its last
+#pragma unroll
+      for (int i = 1; i < 8; ++i)
+        if (i >= 8 - shift && i < left)
+          to[i] = __ushort_as_bfloat16(static_cast<uint16_t>(w[4 + (i >> 1)] >> (16 * (i & 1))));
+    }
+  }
+}
+
 template <typename T>
 __device__ __forceinline__ void load8(const T* p, float (&x)[8]);
 template <>
@@ -165,6 +219,7 @@ __device__ __forceinline__ void dpre_block(const Dpre& p, int block, float (&sh)
   float sg[8], su[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) sg[i] = su[i] = 0.0f;
+  const uint32_t lanes = __ballot_sync(0xffffffffu, f < p.F);
   if (f < p.F) {
     const int left = static_cast<int>(p.F - f < 8 ? p.F - f : 8);
     for (int64_t r = r0 + warp; r < r1; r += 8) {
@@ -201,18 +256,8 @@ __device__ __forceinline__ void dpre_block(const Dpre& p, int block, float (&sh)
           store_copies<OUT>(g, out, p.copy);
           store_copies<OUT>(u, out + p.F, p.copy);
         } else {
-#pragma unroll
-          for (int c = 0; c < OUT; ++c)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const bf16 a = __float2bfloat16_rn(g[i]), b = __float2bfloat16_rn(u[i]);
-              if (i < left) {
-                out[c * p.copy + i] = a;
-                out[c * p.copy + p.F + i] = b;
-              }
-              g[i] -= __bfloat162float(a);
-              u[i] -= __bfloat162float(b);
-            }
+          store_shifted<OUT>(g, out, p.copy, 0, left, lanes);
+          store_shifted<OUT>(u, out + p.F, p.copy, static_cast<int>(p.F & 7), left, lanes);
         }
       }
     }
@@ -614,7 +659,7 @@ size_t gated_workspace_bytes(const Context* ctx, const GatedArgs& a, bool backwa
   q.ws = nullptr;
   q.x = q.w = nullptr;  // the size does not depend on the tensors' alignment
   q.pre = nullptr;
-  if (!backward && a.K == 0) return 0;
+  if (!backward && (a.K == 0 || gated_skinny_applies(a))) return 0;
   return backward ? bwd_work(ctx, q).bytes : fwd_work(ctx, q).bytes;
 }
 

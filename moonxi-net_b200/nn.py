@@ -772,8 +772,9 @@ class AdamW:
     the global norm, which `norm` then holds after a step.
 
     device_step=True keeps the step number on the device, so that a captured
-    step counts its replays.  state, step_count: the moments and the number of
-    steps of an earlier run (`state`, `step_count`), taken over as they are.
+    step counts its replays (reading `step_count` then waits for the device).
+    state, step_count: the moments and the number of steps of an earlier run
+    (`state`, `step_count`), taken over as they are.
     """
 
     def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
@@ -801,13 +802,18 @@ class AdamW:
         self.lr, self.betas, self.eps = float(lr), (float(betas[0]), float(betas[1])), float(eps)
         self.max_grad_norm, self.state_bits = float(max_grad_norm), int(state_bits)
         self.ctx = ctx
-        self.state = self._fresh_state() if state is None else [tuple(s) for s in state]
+        self.state = tuple(self._fresh_state() if state is None else (tuple(s) for s in state))
         self._check_state()
-        self.step_count = int(step_count)
-        self.step_dev = torch.full((1,), self.step_count, dtype=torch.int32, device=self.device) \
+        self._steps = int(step_count)
+        self.step_dev = torch.full((1,), self._steps, dtype=torch.int32, device=self.device) \
             if device_step else None
         self.norm = torch.zeros(1, device=self.device)
         self._table = (_lib.AdamWTensor * n)()
+        # The table holds addresses: of memory that these keep alive, and, for the
+        # parameters, that every step compares with where they are.
+        self._held = [x.detach() for x in self.params + [c for c in self.copies if c is not None]]
+        self._held += [x.detach() for s in self.state for x in s]
+        self._at = [p.data_ptr() for p in self.params]
         for t, p, c, s, d in zip(self._table, self.params, self.copies, self.state, decay):
             t.param, t.n, t.weight_decay = p.data_ptr(), p.numel(), d
             t.copy_bf16 = None if c is None else c.data_ptr()
@@ -829,6 +835,11 @@ class AdamW:
                  zeros(p.numel(), torch.uint8), zeros(-(-p.numel() // 256), torch.float32))
                 for p in self.params]
 
+    @property
+    def step_count(self) -> int:
+        """Steps taken."""
+        return self._steps if self.step_dev is None else int(self.step_dev.item())
+
     def _check_state(self):
         f32 = torch.float32
         names, types = (("m", "v"), (f32, f32)) if self.state_bits == 32 else \
@@ -846,17 +857,21 @@ class AdamW:
         """One update from `grads`, a tensor for each parameter."""
         if len(grads) != len(self.params):
             raise ValueError(f"{len(grads)} gradients for {len(self.params)} tensors")
-        for i, (t, g) in enumerate(zip(self._table, grads)):
+        for i, (t, p, at, g) in enumerate(zip(self._table, self.params, self._at, grads)):
             kind = ops._check_type(g, f"grads[{i}]")
             if g.numel() != t.n or g.get_device() != self._dev or not g.is_contiguous():
                 raise ValueError(f"grads[{i}] must be contiguous, of {t.n} elements on "
                                  f"{self.device}")
+            if p.data_ptr() != at:
+                raise ValueError(f"params[{i}] was given other memory; make a new AdamW with "
+                                 "`state` and `step_count`")
             t.grad, t.grad_type = g.data_ptr(), kind
         rc = _lib.lib().mx_adamw_step(
             ops._handle(self.ctx, self.params[0]), self._table, len(self.params), self.state_bits,
-            self.lr, self.betas[0], self.betas[1], self.eps, self.step_count + 1,
+            self.lr, self.betas[0], self.betas[1], self.eps, self._steps + 1,
             ops._ptr(self.step_dev), self.max_grad_norm, self.norm.data_ptr(),
             self._scratch.data_ptr(), self._scratch.numel(),
             ops._launch_stream(self._dev, stream))
         ops.check(rc, "mx_adamw_step")
-        self.step_count += 1
+        if self.step_dev is None:
+            self._steps += 1

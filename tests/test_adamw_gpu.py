@@ -382,3 +382,34 @@ def test_refusals(cuda_device):
     assert L.mx_adamw_step(h, t, 1, 32, *args) == bad
     t[0].n = 300
     assert L.mx_adamw_step(h, t, 1, 32, 1e-3, 0.9, 0.99, 1e-8, 1, None, 1.0, None, None, 0, None) == bad
+
+
+def test_memory_that_moved_is_refused(cuda_device):
+    """The optimizer holds addresses: a parameter that was given other memory is
+    an error, and nothing is written to the old."""
+    p, g = torch.ones(300, device="cuda"), torch.ones(300, device="cuda")
+    old = p.detach()
+    opt = nn.AdamW([p], **HYPER)
+    opt.step([g])
+    before = old.clone()
+    p.data = torch.zeros(300, device="cuda")
+    with pytest.raises(ValueError, match="other memory"):
+        opt.step([g])
+    assert torch.equal(old, before) and (p == 0).all() and opt.step_count == 1
+    again = nn.AdamW([p], state=opt.state, step_count=opt.step_count, **HYPER)
+    again.step([g])
+    assert (p != 0).all() and again.step_count == 2
+
+
+def test_step_count_on_the_device_is_the_devices(cuda_device):
+    p, g = torch.ones(300, device="cuda"), torch.ones(300, device="cuda")
+    opt = nn.AdamW([p], device_step=True, step_count=5, **HYPER)
+    opt.step([g])
+    assert opt.step_count == 6
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step([g])
+    assert opt.step_count == 6  # a capture runs nothing
+    for _ in range(3):
+        graph.replay()
+    assert opt.step_count == 9
