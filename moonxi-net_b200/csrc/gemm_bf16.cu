@@ -15,14 +15,23 @@
 // (Four stages of 32 of K: 60 us for that product against 45 when every stage
 // is added up, the epilogue's rate, and 48 us and 6e-7 when every second is.)
 //
-// CTA pairs (cta_group::2): a pair computes a 256 x 256 tile (or two of them, see
-// below), each CTA holding
+// CTA pairs (cta_group::2): a pair computes a 256 x 256 tile, each CTA holding
 // 128 rows of A, 128 columns of B and its 128 x 256 half of the accumulator:
 // 32 KB of loads a CTA for 64 of K where a single CTA's 128 x 256 tile loads
 // 48 KB, which is what keeps the L2 from being the bound.  Gated: the even
 // CTA's 128 columns of B are the gate's, the odd one's the other projection's,
 // so an accumulator row holds g and u of the same 128 outputs and the epilogue
 // has both.
+//
+// One copy's MMAs still wait for the L2 (with half of the loads left out a
+// forward product of 8192 x 4096 x 2 x 8192 took 770 us instead of 939, its
+// gradients 1332 instead of 1708).  So where enough rows are left a job is 512 of
+// them: two tiles of A share one of B, 48 KB a CTA for 1024 cycles of MMAs
+// instead of 64, both accumulators are one job's, and the epilogue of one runs
+// beside the other's last and the next job's first MMAs.  833 and 1473 us.  A
+// short K with a pre-activation to store has more of its epilogue to hide than
+// that: 4096 x 1000 x 2 x 2736 with pre, 62 us in tiles of 256 rows, 71 in 512.
+// The plan's costs decide.
 //
 // One launch takes one product or two (a backward pass's dx and dw, which do not
 // need each other): the second's tiles follow the first's, so the two share
@@ -38,7 +47,7 @@
 // to 1.6 ms.  Only where the output's rows are not 16-byte aligned do they
 // transpose through padded shared memory, to store whole rows of odd width
 // (pre and the partial tiles have padded rows).  Two accumulators: a tile's epilogue runs
-// beside the next tile's (three copies: the next stage's) MMAs.
+// beside the next tile's (three copies: the next k-block's) MMAs.
 // Few tiles and a long K: the K range is split over the pairs, fp32 partial
 // tiles go to scratch and a second kernel adds them in order.  (Added up by the
 // last warp to arrive at its part of a tile instead, a product of 33 x 2 x 1000
@@ -696,6 +705,7 @@ struct Plan {
 struct Plans {
   Plan p[2];
   int pairs = 0, sub = 1;
+  bool vec = true, save = false;  // the outputs' rows start on 16 bytes; pre is stored
   bool split() const { return p[0].splits > 1 || p[1].splits > 1; }
 };
 
@@ -706,25 +716,31 @@ void set_splits(Plan& q, int want) {
 
 // A job's cost in cycles, as measured: a k-block (one copy, 256 rows: 512
 // cycles of MMAs, which wait for L2; 512 rows: 1024; three copies: 3072), and a
-// start and an epilogue that run beside other jobs' MMAs in part; a split job
+// start and an epilogue, which runs beside the next job's MMAs (512 rows: only
+// beside a ring's worth of them, so what it stores counts for more); a split job
 // has the partial tile's way through memory on top.
-int job_cost(const Plan& q, int copies, int sub) {
-  const int kb = copies == 3 ? 3400 : sub == 2 ? 1160 : 700;
-  return q.kb_per * kb + (copies == 3 ? 3400 : sub == 2 ? 7000 : 4200) * (q.splits > 1 ? 2 : 1);
+int job_cost(const Plans& pl, int i, int copies) {
+  const Plan& q = pl.p[i];
+  const bool tall = pl.sub == 2;
+  const int kb = copies == 3 ? 3400 : tall ? 1160 : 700;
+  int ends = copies == 3 ? 3400 : tall ? 7000 : 4200;
+  if (copies == 1 && pl.save) ends += tall ? 13000 : 3800;
+  if (copies == 1 && !pl.vec) ends += tall ? 14000 : 5000;
+  return q.kb_per * kb + ends * (q.splits > 1 ? 2 : 1);
 }
 // Queue's fill: what the first product's last round leaves to the pairs that
 // miss it.
 int fill_of(const Plans& pl, int pairs, int copies) {
   const int shorter = pairs - pl.p[0].jobs() % pairs;
   if (shorter == pairs || pl.p[1].jobs() == 0) return 0;
-  return std::min(job_cost(pl.p[0], copies, pl.sub) / job_cost(pl.p[1], copies, pl.sub),
+  return std::min(job_cost(pl, 0, copies) / job_cost(pl, 1, copies),
                   pl.p[1].jobs() / shorter);
 }
 // The longest queue of a pair (queues differ only where a product's last round
 // ends), and the launch that adds split products up.
 int64_t makespan(const Plans& pl, int pairs, int copies) {
-  const int c0 = job_cost(pl.p[0], copies, pl.sub);
-  const int c1 = pl.p[1].jobs() > 0 ? job_cost(pl.p[1], copies, pl.sub) : 0;
+  const int c0 = job_cost(pl, 0, copies);
+  const int c1 = pl.p[1].jobs() > 0 ? job_cost(pl, 1, copies) : 0;
   const int j0 = pl.p[0].jobs(), r = j0 % pairs, fill = fill_of(pl, pairs, copies);
   const int rest = pl.p[1].jobs() - (fill > 0 ? fill * (pairs - r) : 0);
   const int at[3] = {0, r, rest % pairs};
@@ -751,9 +767,9 @@ void set_tiles(Plans& pl, const Bf16Gemm* g, int count, int sub) {
   }
 }
 
-// Whole tiles of 256 or (one copy) 512 rows where they fill the machine;
-// otherwise the split counts, the longer product's first, with the shortest
-// longest queue.
+// Tiles of 256 rows: whole ones where they fill the machine; otherwise the
+// split counts, the longer product's first, with the shortest longest queue.
+// Sizes alone decide, and with them the scratch.
 Plans plan_of(const Context* ctx, const Bf16Gemm* g, int count) {
   Plans pl;
   const int copies = g[0].copies;
@@ -777,11 +793,6 @@ Plans plan_of(const Context* ctx, const Bf16Gemm* g, int count) {
       set_splits(q, best);
     }
   }
-  if (copies == 1) {
-    Plans tall;
-    set_tiles(tall, g, count, 2);
-    if (makespan(tall, pairs, 1) < makespan(pl, pairs, 1)) pl = tall;
-  }
   for (int i = 0; i < count; ++i) {
     Plan& q = pl.p[i];
     const size_t row = (static_cast<size_t>(g[i].N) + 7) / 8 * 8 * (g[i].gated ? 2 : 1);
@@ -790,6 +801,23 @@ Plans plan_of(const Context* ctx, const Bf16Gemm* g, int count) {
   }
   pl.pairs = std::min(pairs, pl.p[0].jobs() + pl.p[1].jobs());
   return pl;
+}
+
+// The plan of a launch: tiles of 512 rows (one copy, no scratch) where those are
+// sooner done.  vec: the outputs' rows start on 16 bytes; save: pre is stored.
+Plans launch_plan(const Context* ctx, const Bf16Gemm* g, int count, bool vec, bool save) {
+  Plans pl = plan_of(ctx, g, count);
+  pl.vec = vec;
+  pl.save = save;
+  if (g[0].copies != 1) return pl;
+  const int pairs = std::max(1, ctx->tc_sms() / 2);
+  Plans tall;
+  tall.vec = vec;
+  tall.save = save;
+  set_tiles(tall, g, count, 2);
+  if (makespan(tall, pairs, 1) >= makespan(pl, pairs, 1)) return pl;
+  tall.pairs = std::min(pairs, tall.p[0].jobs() + tall.p[1].jobs());
+  return tall;
 }
 
 bool operand_map(CUtensorMap* m, const Bf16Operand& o, int copy, int rows, int K) {
@@ -802,7 +830,12 @@ template <int NC, bool GATED>
 int launch(Context* ctx, const Bf16Gemm* g, int count, void* scratch, const Bf16ColumnSum* sum,
            cudaStream_t s) {
   using T = typename std::conditional<NC == 1, __nv_bfloat16, float>::type;
-  const Plans pl = plan_of(ctx, g, count);
+  auto out_on = [&](const Bf16Gemm& q, int bytes) {
+    const int n = bytes / static_cast<int>(sizeof(T));
+    return q.N % n == 0 && q.ldc % n == 0 && (reinterpret_cast<uintptr_t>(q.out) & (bytes - 1)) == 0;
+  };
+  const bool vec = out_on(g[0], 16) && (count == 1 || out_on(g[1], 16));
+  const Plans pl = launch_plan(ctx, g, count, vec, GATED && g[0].pre);
   if (pl.split() && (!scratch || (reinterpret_cast<uintptr_t>(scratch) & 255u) != 0))
     return kErrInvalid;
   Launch<NC> L;
@@ -829,11 +862,7 @@ int launch(Context* ctx, const Bf16Gemm* g, int count, void* scratch, const Bf16
     p.act = g[i].act;
     p.a_kmajor = g[i].a.kmajor;
     p.b_kmajor = g[i].b.kmajor;
-    auto out_on = [&](int bytes) {
-      const int n = bytes / static_cast<int>(sizeof(T));
-      return p.N % n == 0 && p.ldc % n == 0 && (reinterpret_cast<uintptr_t>(p.out) & (bytes - 1)) == 0;
-    };
-    p.vec = out_on(32) ? 32 : out_on(16) ? 16 : 0;
+    p.vec = out_on(g[i], 32) ? 32 : out_on(g[i], 16) ? 16 : 0;
     if ((reinterpret_cast<uintptr_t>(p.pre) & 31u) != 0) return kErrInvalid;
   }
   L.status = ctx->status;
@@ -850,7 +879,6 @@ int launch(Context* ctx, const Bf16Gemm* g, int count, void* scratch, const Bf16
     return cudaGetLastError();
   };
   static SmemOptIn opt_vec, opt_any;
-  const bool vec = L.p[0].vec > 0 && (count == 1 || L.p[1].vec > 0);
   cudaError_t e;
   if constexpr (NC == 1) {
     static SmemOptIn tall_vec, tall_any;

@@ -120,6 +120,25 @@ def test_against_64_bits(cuda_device, M, K, F, dtype, tw):
     _run_and_check(M, K, F, dtype, tw, act, bias=(M + F) % 2 == 0, seed=M + K)
 
 
+@pytest.mark.parametrize("tw", [False, True])
+@pytest.mark.parametrize("K,F", [(1024, 4096), (1000, 4099)])
+def test_many_tiles(cuda_device, K, F, tw):
+    """Rows for several of a pair's larger tiles, the last one in part; with and
+    without pre, which the choice of tiles depends on."""
+    M = 2125
+    _run_and_check(M, K, F, BF16, tw, "silu", not tw, seed=K)
+    x, w, b, _ = _problem(M, K, F, BF16, tw, not tw, seed=K)
+    h, pre = ops.gated_linear(x, w, b, transpose_w=tw)
+    assert pre is None
+    P = x.double() @ (w.double().t() if tw else w.double()) + (b.double() if b is not None else 0)
+    E = (K / 16 + 40) * 2.0 ** -23 * (x.double().abs() @ (w.t() if tw else w).double().abs()
+                                     + (b.double().abs() if b is not None else 0))
+    g, u, eg, eu = P[:, :F], P[:, F:], E[:, :F], E[:, F:]
+    a = _act("silu", g)[0]
+    ea = 1.2 * eg + 32 * U * g.abs().clamp_min(1)
+    _check("h", h, a * u, ea * u.abs() + a.abs() * eu + ea * eu + 2 * U * (a * u).abs())
+
+
 # few rows: lengths on both sides of each of their kernels' widths and splits,
 # rows that start on any element
 @pytest.mark.parametrize("tw", [False, True])
