@@ -210,7 +210,7 @@ __device__ __forceinline__ void pack_block(const PackJob& p, int block) {
 // time, a lane 8 columns.  Bound by the bytes: with bfloat16 tensors 10 read
 // and 4 written a value of h (8192 x 8192: 157 us, 91 % of the copy rate).
 template <typename T, int OUT>
-__device__ __forceinline__ void dpre_block(const Dpre& p, int block, float (&sh)[8][256]) {
+__device__ __forceinline__ void dpre_block(const Dpre& p, int block, float (&sh)[8][8][33]) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int cb = block % p.bx, rb = block / p.bx;
   const int64_t f = (cb * 32ll + lane) * 8, up = (p.F + 7) & ~7ll;
@@ -268,13 +268,13 @@ __device__ __forceinline__ void dpre_block(const Dpre& p, int block, float (&sh)
   for (int h = 0; h < 2; ++h) {  // the eight warps' sums, in their order
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 8; ++i) sh[warp][lane * 8 + i] = h ? su[i] : sg[i];
+    for (int i = 0; i < 8; ++i) sh[warp][i][lane] = h ? su[i] : sg[i];
     __syncthreads();
     const int64_t c = cb * 256ll + threadIdx.x;
     if (c < p.F) {
       float s = 0.0f;
 #pragma unroll
-      for (int w = 0; w < 8; ++w) s += sh[w][threadIdx.x];
+      for (int w = 0; w < 8; ++w) s += sh[w][threadIdx.x & 7][threadIdx.x >> 3];
       part[h * static_cast<int64_t>(p.F) + c] = s;
     }
   }
@@ -284,7 +284,7 @@ template <typename T, int NC, bool DPRE>
 __global__ void __launch_bounds__(256) prep_kernel(const __grid_constant__ Prep p) {
   int block = blockIdx.x;
   if constexpr (DPRE) {
-    __shared__ float sh[8][256];
+    __shared__ float sh[8][8][33];
     if (block < p.dpre.bx * p.dpre.by) {
       dpre_block<T, NC>(p.dpre, block, sh);
       return;
