@@ -282,6 +282,7 @@ __device__ __forceinline__ void dpre_block(const Dpre& p, int block, float (&sh)
 
 template <typename T, int NC, bool DPRE>
 __global__ void __launch_bounds__(256) prep_kernel(const __grid_constant__ Prep p) {
+  grid_trigger();
   int block = blockIdx.x;
   if constexpr (DPRE) {
     __shared__ float sh[8][8][33];
@@ -529,7 +530,7 @@ int fwd(Context* ctx, const GatedArgs& a, cudaStream_t s) {
   g.bias = a.bias;
   g.pre = a.pre;
   g.act = a.act;
-  return bf16_gemm(ctx, &g, 1, w.split, nullptr, s);
+  return bf16_gemm(ctx, &g, 1, w.split, nullptr, prep.packs > 0, s);
 }
 
 struct BwdWork {
@@ -553,9 +554,11 @@ void bwd_shapes(const GatedArgs& a, Bf16Gemm (&g)[2]) {
 BwdWork bwd_work(const Context* ctx, const GatedArgs& a) {
   BwdWork w{};
   Carver c{static_cast<uint8_t*>(a.ws)};
-  // rows of a block of dpre_kernel: at least 16, and four blocks an SM at most
+  // rows of a block of dpre's: at least 16, and one round of three blocks an SM
+  // (1000 x 2736: 12.1 us, in two or three rounds 13.5; 4096 x 2736: 37.0, 38.7 and
+  // 40.9; 8192 x 8192: 174 and 171)
   const int col_blocks = (a.F + 255) / 256;
-  const int want = std::max(1, 8 * ctx->num_sms / col_blocks);
+  const int want = std::max(1, 3 * ctx->num_sms / col_blocks);
   w.per = std::max(16, (a.M + want - 1) / want);
   w.row_blocks = (a.M + w.per - 1) / w.per;
   w.part = c.take<float>(static_cast<size_t>(w.row_blocks) * 2 * a.F * sizeof(float));
@@ -649,7 +652,7 @@ int bwd(Context* ctx, const GatedArgs& a, cudaStream_t s) {
   g[1].ldc = g[1].N;
   if (!products) return kOk;
   const Bf16ColumnSum sum{w.part, a.dbias, w.row_blocks, F2};
-  return bf16_gemm(ctx, a.dx ? g : g + 1, a.dx && a.dw ? 2 : 1, w.split, a.dbias ? &sum : nullptr, s);
+  return bf16_gemm(ctx, a.dx ? g : g + 1, a.dx && a.dw ? 2 : 1, w.split, a.dbias ? &sum : nullptr, true, s);
 }
 
 }  // namespace

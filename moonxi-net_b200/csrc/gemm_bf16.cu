@@ -293,6 +293,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   cluster_sync();  // both CTAs' barriers exist
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  grid_trigger();
+  grid_wait();
   Queue queue;
   queue.init(L, pair, pairs);
   int prob, number;
@@ -668,6 +670,7 @@ __device__ __forceinline__ void join_block(const Problem& p, int block, int bloc
 }
 template <typename T, bool GATED>
 __global__ void __launch_bounds__(256) tail_kernel(const __grid_constant__ Tail t) {
+  grid_wait();
   int block = blockIdx.x;
   if (block < t.blocks[0]) {
     join_block<T, GATED>(t.p[0], block, t.blocks[0]);
@@ -828,7 +831,7 @@ bool operand_map(CUtensorMap* m, const Bf16Operand& o, int copy, int rows, int K
 
 template <int NC, bool GATED>
 int launch(Context* ctx, const Bf16Gemm* g, int count, void* scratch, const Bf16ColumnSum* sum,
-           cudaStream_t s) {
+           bool after, cudaStream_t s) {
   using T = typename std::conditional<NC == 1, __nv_bfloat16, float>::type;
   auto out_on = [&](const Bf16Gemm& q, int bytes) {
     const int n = bytes / static_cast<int>(sizeof(T));
@@ -874,9 +877,8 @@ int launch(Context* ctx, const Bf16Gemm* g, int count, void* scratch, const Bf16
   auto start = [&](auto kern, int bytes, SmemOptIn& opt_in) {
     cudaError_t e = opt_in.ensure(kern, bytes);
     if (e != cudaSuccess) return e;
-    kern<<<2 * pl.pairs, kThreads, bytes, s>>>(L);
     note_launches(1);
-    return cudaGetLastError();
+    return launch_after(kern, 2 * pl.pairs, kThreads, bytes, s, after, L);
   };
   static SmemOptIn opt_vec, opt_any;
   cudaError_t e;
@@ -905,9 +907,8 @@ int launch(Context* ctx, const Bf16Gemm* g, int count, void* scratch, const Bf16
     t.width = sum->width;
     blocks += (sum->width + 31) / 32;
   }
-  tail_kernel<T, GATED><<<blocks, 256, 0, s>>>(t);
   note_launches(1);
-  return cuda_status(cudaGetLastError());
+  return cuda_status(launch_after(tail_kernel<T, GATED>, blocks, 256, 0, s, true, t));
 }
 
 }  // namespace
@@ -918,16 +919,16 @@ size_t bf16_gemm_scratch_bytes(const Context* ctx, const Bf16Gemm* g, int count)
 }
 
 int bf16_gemm(Context* ctx, const Bf16Gemm* g, int count, void* scratch, const Bf16ColumnSum* sum,
-              cudaStream_t s) {
+              bool after, cudaStream_t s) {
   if (count < 1 || count > 2 || (sum && g[0].gated) || (count == 2 && (g[0].gated || g[1].gated || g[0].copies != g[1].copies)))
     return kErrInvalid;
   for (int i = 0; i < count; ++i)
     if (g[i].M <= 0 || g[i].N <= 0 || g[i].K <= 0) return kErrInvalid;
   if (g[0].copies == 3)
-    return g[0].gated ? launch<3, true>(ctx, g, count, scratch, sum, s)
-                      : launch<3, false>(ctx, g, count, scratch, sum, s);
-  return g[0].gated ? launch<1, true>(ctx, g, count, scratch, sum, s)
-                    : launch<1, false>(ctx, g, count, scratch, sum, s);
+    return g[0].gated ? launch<3, true>(ctx, g, count, scratch, sum, after, s)
+                      : launch<3, false>(ctx, g, count, scratch, sum, after, s);
+  return g[0].gated ? launch<1, true>(ctx, g, count, scratch, sum, after, s)
+                    : launch<1, false>(ctx, g, count, scratch, sum, after, s);
 }
 
 }  // namespace mx

@@ -254,6 +254,18 @@ __device__ __forceinline__ void st_global_32b(void* p, const uint32_t (&r)[8]) {
                : "memory");
 }
 
+// ------------------------------------------- a launch that follows another
+// Programmatic dependent launch (launch_after): the second kernel's blocks come
+// onto SMs as the first one's leave them, set themselves up and wait here until
+// the first is complete and what it wrote can be read, by TMA too.
+__device__ __forceinline__ void grid_wait() {
+  asm volatile("griddepcontrol.wait;\n\tfence.proxy.async.global;" ::: "memory");
+}
+// The first kernel's: once every block has passed this, the second may come.
+__device__ __forceinline__ void grid_trigger() {
+  asm volatile("griddepcontrol.launch_dependents;");
+}
+
 // ------------------------------------------------- CTA pairs (cta_group::2)
 // Two CTAs of a cluster work on one tile: each holds half of A's rows and half
 // of B's columns in its shared memory and half of the accumulator's rows in

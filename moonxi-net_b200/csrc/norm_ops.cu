@@ -336,6 +336,7 @@ __global__ void __launch_bounds__(block_threads(TPR, 2), blocks_per_sm(TPR, 2)) 
   constexpr int ROWS = BLOCK / TPR;
   extern __shared__ uint4 ring[];  // [D][2][NV][BLOCK]
   __shared__ __align__(16) float buf[ROWS > 1 ? BLOCK * E : 2 * 2 * TPR / 32];
+  grid_trigger();
   const int t = threadIdx.x % TPR, group = threadIdx.x / TPR;
   float* sums = buf + (ROWS > 1 ? group * (2 * 2 * TPR / 32) : 0);
   const float inv_c = 1.0f / static_cast<float>(p.cols);
@@ -537,6 +538,7 @@ __global__ void __launch_bounds__(1024) norm_bwd_long_kernel(const NormBwd p) {
 // A block: 256 * V columns, a range of rows.
 template <typename T, int V>
 __global__ void __launch_bounds__(256) norm_cols_kernel(const NormBwd p) {
+  grid_trigger();
   const int64_t c = (blockIdx.x * 256ll + threadIdx.x) * V;
   if (c >= p.cols) return;
   const int64_t per = (static_cast<int64_t>(p.rows) + gridDim.y - 1) / gridDim.y;
@@ -657,6 +659,7 @@ __global__ void __launch_bounds__(32 * kFinishWarps) norm_finish_kernel(
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t width = 2ll * cols, c = blockIdx.x * 32ll + lane;
   float s = 0.0f;
+  grid_wait();
   if (c < width) {
 #pragma unroll 8
     for (int r = warp; r < blocks; r += kFinishWarps) s += part[r * width + c];
@@ -836,10 +839,10 @@ int layer_norm_bwd(Context* ctx, int dtype, const void* dy, int64_t lddy, const 
     note_launches(1);
   }
   if (e == cudaSuccess && sums) {
-    norm_finish_kernel<<<static_cast<unsigned>((2ll * cols + 31) / 32), 32 * kFinishWarps, 0, s>>>(static_cast<const float*>(scratch),
-                                                           blocks, cols, dw, db);
     note_launches(1);
-    e = cudaGetLastError();
+    e = launch_after(norm_finish_kernel, static_cast<unsigned>((2ll * cols + 31) / 32),
+                     32 * kFinishWarps, 0, s, true, static_cast<const float*>(scratch), blocks, cols,
+                     dw, db);
   }
   return cuda_status(e);
 }
