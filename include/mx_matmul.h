@@ -398,6 +398,7 @@ int32_t mx_sgd_momentum_clip(void* handle, float* params, const float* grads, fl
  * on such a context the gated layer's float32 products run in NpArray order. */
 #define MX_F32 0
 #define MX_BF16 1
+/* Sizes (rows, columns, M, K, 2F) above 0x7fff0000 are MX_ERR_UNSUPPORTED. */
 
 /* y = (x - mean) * rstd * weight + bias over the last dimension, with
  * mean = sum(x) / cols and rstd = 1 / sqrt(sum((x - mean)^2) / cols + eps).

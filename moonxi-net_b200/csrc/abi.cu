@@ -804,6 +804,9 @@ MX_EXPORT int32_t mx_sgd_momentum_autoclip(void* handle, float* params, const fl
 // ------------------------- layer norm, the gated linear layer, AdamW
 namespace {
 bool known_type(int32_t dtype) { return dtype == MX_F32 || dtype == MX_BF16; }
+// The largest size that the kernels' 32-bit column counters step past without
+// wrapping.
+constexpr int32_t kMaxSize = 0x7fff0000;
 }  // namespace
 
 MX_EXPORT int32_t mx_layer_norm_fwd(void* handle, int32_t dtype, const void* x, int64_t ldx,
@@ -815,6 +818,7 @@ MX_EXPORT int32_t mx_layer_norm_fwd(void* handle, int32_t dtype, const void* x, 
   if (!c) return MX_ERR_NO_DEVICE;
   if (!known_type(dtype) || rows < 0 || cols < 1 || ldx < cols || ldy < cols || !(eps >= 0.0f))
     return MX_ERR_INVALID;
+  if (rows > kMaxSize || cols > kMaxSize) return MX_ERR_UNSUPPORTED;
   if (rows > 0 && (!x || !y)) return MX_ERR_INVALID;
   cudaStream_t s = pick_stream(c, stream);
   return finish(c, layer_norm_fwd(c, dtype, x, ldx, weight, bias, y, ldy, mean, rstd, rows, cols,
@@ -832,6 +836,7 @@ MX_EXPORT int32_t mx_layer_norm_bwd(void* handle, int32_t dtype, const void* dy,
   if (!known_type(dtype) || rows < 0 || cols < 1 || ldx < cols || lddy < cols ||
       (dx && lddx < cols))
     return MX_ERR_INVALID;
+  if (rows > kMaxSize || cols > kMaxSize) return MX_ERR_UNSUPPORTED;
   if (rows > 0 && (!dy || !x || !mean || !rstd)) return MX_ERR_INVALID;
   cudaStream_t s = pick_stream(c, stream);
   return finish(c, layer_norm_bwd(c, dtype, dy, lddy, x, ldx, weight, mean, rstd, dx, lddx,
@@ -840,7 +845,8 @@ MX_EXPORT int32_t mx_layer_norm_bwd(void* handle, int32_t dtype, const void* dy,
 
 MX_EXPORT uint64_t mx_layer_norm_bwd_scratch_bytes(void* handle, int32_t rows, int32_t cols) {
   Scoped scope(handle);
-  return scope.c ? layer_norm_bwd_scratch_bytes(scope.c, rows, cols) : 0;
+  if (!scope.c || rows > kMaxSize || cols > kMaxSize) return 0;
+  return layer_norm_bwd_scratch_bytes(scope.c, rows, cols);
 }
 
 namespace {
@@ -848,7 +854,8 @@ namespace {
 int gated_args(Context* c, int32_t dtype, int32_t M, int32_t K, int32_t F, int32_t transpose_w,
                int32_t act, int32_t precision, GatedArgs& a) {
   a = GatedArgs{};
-  if (!known_type(dtype) || M < 0 || K < 0 || F < 0 || F > 0x3fffffff) return MX_ERR_INVALID;
+  if (!known_type(dtype) || M < 0 || K < 0 || F < 0) return MX_ERR_INVALID;
+  if (M > kMaxSize || K > kMaxSize || F > kMaxSize / 2) return MX_ERR_UNSUPPORTED;
   if (act < MX_ACT_SILU || act > MX_ACT_SIGMOID) return MX_ERR_INVALID;
   if (precision < MX_PREC_DEFAULT || precision > MX_PREC_NPARRAY) return MX_ERR_INVALID;
   const int p = precision == MX_PREC_DEFAULT ? c->precision : precision;

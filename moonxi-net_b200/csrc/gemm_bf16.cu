@@ -722,28 +722,28 @@ void set_splits(Plan& q, int want) {
 // start and an epilogue, which runs beside the next job's MMAs (512 rows: only
 // beside a ring's worth of them, so what it stores counts for more); a split job
 // has the partial tile's way through memory on top.
-int job_cost(const Plans& pl, int i, int copies) {
+int64_t job_cost(const Plans& pl, int i, int copies) {
   const Plan& q = pl.p[i];
   const bool tall = pl.sub == 2;
   const int kb = copies == 3 ? 3400 : tall ? 1160 : 700;
   int ends = copies == 3 ? 3400 : tall ? 7000 : 4200;
   if (copies == 1 && pl.save) ends += tall ? 13000 : 3800;
   if (copies == 1 && !pl.vec) ends += tall ? 14000 : 5000;
-  return q.kb_per * kb + ends * (q.splits > 1 ? 2 : 1);
+  return static_cast<int64_t>(q.kb_per) * kb + ends * (q.splits > 1 ? 2 : 1);
 }
 // Queue's fill: what the first product's last round leaves to the pairs that
 // miss it.
 int fill_of(const Plans& pl, int pairs, int copies) {
   const int shorter = pairs - pl.p[0].jobs() % pairs;
   if (shorter == pairs || pl.p[1].jobs() == 0) return 0;
-  return std::min(job_cost(pl, 0, copies) / job_cost(pl, 1, copies),
-                  pl.p[1].jobs() / shorter);
+  return static_cast<int>(std::min<int64_t>(job_cost(pl, 0, copies) / job_cost(pl, 1, copies),
+                                            pl.p[1].jobs() / shorter));
 }
 // The longest queue of a pair (queues differ only where a product's last round
 // ends), and the launch that adds split products up.
 int64_t makespan(const Plans& pl, int pairs, int copies) {
-  const int c0 = job_cost(pl, 0, copies);
-  const int c1 = pl.p[1].jobs() > 0 ? job_cost(pl, 1, copies) : 0;
+  const int64_t c0 = job_cost(pl, 0, copies);
+  const int64_t c1 = pl.p[1].jobs() > 0 ? job_cost(pl, 1, copies) : 0;
   const int j0 = pl.p[0].jobs(), r = j0 % pairs, fill = fill_of(pl, pairs, copies);
   const int rest = pl.p[1].jobs() - (fill > 0 ? fill * (pairs - r) : 0);
   const int at[3] = {0, r, rest % pairs};
@@ -751,7 +751,7 @@ int64_t makespan(const Plans& pl, int pairs, int copies) {
   for (int c : at) {
     const int n0 = (j0 - c + pairs - 1) / pairs;
     const int n1 = (c >= r ? fill : 0) + (rest - c + pairs - 1) / pairs;
-    worst = std::max(worst, static_cast<int64_t>(n0) * c0 + static_cast<int64_t>(n1) * c1);
+    worst = std::max(worst, n0 * c0 + n1 * c1);
   }
   return worst + (pl.split() ? 6000 : 0);
 }

@@ -813,6 +813,12 @@ class AdamW:
         # parameters, that every step compares with where they are.
         self._held = [x.detach() for x in self.params + [c for c in self.copies if c is not None]]
         self._held += [x.detach() for s in self.state for x in s]
+        end = -1
+        for a, b in sorted((x.data_ptr(), x.data_ptr() + x.numel() * x.element_size())
+                           for x in self._held if x.numel()):
+            if a < end:
+                raise ValueError("params, copies and state must not share memory")
+            end = b
         self._at = [p.data_ptr() for p in self.params]
         for t, p, c, s, d in zip(self._table, self.params, self.copies, self.state, decay):
             t.param, t.n, t.weight_decay = p.data_ptr(), p.numel(), d
@@ -866,6 +872,9 @@ class AdamW:
                 raise ValueError(f"params[{i}] was given other memory; make a new AdamW with "
                                  "`state` and `step_count`")
             t.grad, t.grad_type = g.data_ptr(), kind
+        if stream is not None and not torch.cuda.is_current_stream_capturing():
+            self._scratch.record_stream(stream)
+            self.norm.record_stream(stream)
         rc = _lib.lib().mx_adamw_step(
             ops._handle(self.ctx, self.params[0]), self._table, len(self.params), self.state_bits,
             self.lr, self.betas[0], self.betas[1], self.eps, self._steps + 1,

@@ -417,12 +417,33 @@ def _empty_like(t, stream):
         return torch.empty_like(t)
 
 
+_MAX_SIZE = 0x7FFF0000  # of a dimension
+
+
+def _apart(out: torch.Tensor, name: str, *others) -> None:
+    """An output that the caller gives does not share memory with what the call
+    reads or writes beside it.  (Of tensors with gaps between their rows only
+    those that begin at the same place are known to.)"""
+    a = out.data_ptr()
+    end = a + out.numel() * out.element_size()
+    for t in others:
+        if t is None:
+            continue
+        b = t.data_ptr()
+        dense = out.is_contiguous() and t.is_contiguous()
+        if out.numel() and t.numel() and (
+                a == b or dense and a < b + t.numel() * t.element_size() and b < end):
+            raise ValueError(f"{name} must not share memory with another argument")
+
+
 def _rows(t: torch.Tensor, name: str) -> tuple[int, int, int]:
     """(rows, columns, row stride) of a tensor seen as rows of its last
     dimension: contiguous, or 2-D with contiguous rows."""
     if t.dim() < 1 or t.shape[-1] < 1:
         raise ValueError(f"{name} needs a last dimension of at least 1")
     cols = t.shape[-1]
+    if cols > _MAX_SIZE or t.numel() > _MAX_SIZE * cols:
+        raise ValueError(f"{name} has more than {_MAX_SIZE} rows or columns")
     if t.is_contiguous():
         return t.numel() // cols, cols, cols
     if t.dim() == 2 and t.stride(1) == 1 and t.stride(0) >= cols:
@@ -456,6 +477,7 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None,
         ldy = cols
     else:
         ldy = _like_rows(out, "out", x, "x")
+        _apart(out, "out", x, weight, bias)
     mean = rstd = None
     if stats:
         mean = _empty(rows, torch.float32, x.device, stream)
@@ -487,15 +509,18 @@ def layer_norm_backward(grad_out: torch.Tensor, x: torch.Tensor, weight: torch.T
         lddx = cols
     else:
         lddx = _like_rows(dx, "dx", x, "x")
+        _apart(dx, "dx", grad_out, x, weight, mean, rstd, dweight, dbias)
     if dweight is None:
         dweight = _empty(cols, f32, x.device, stream) if weight is None else \
             _empty_like(weight, stream)
     else:
         _check_like(dweight, "dweight", dev, f32, (cols,))
+        _apart(dweight, "dweight", grad_out, x, weight, mean, rstd, dbias)
     if dbias is None:
         dbias = _empty_like(dweight, stream)
     else:
         _check_like(dbias, "dbias", dev, f32, (cols,))
+        _apart(dbias, "dbias", grad_out, x, weight, mean, rstd)
     h = _handle(ctx, x)
     L = _lib.lib()
     nb = L.mx_layer_norm_bwd_scratch_bytes(h, rows, cols)
@@ -523,6 +548,8 @@ def _gated_shape(x: torch.Tensor, w: torch.Tensor, transpose_w: bool, act: str):
     if two_f % 2 or w.shape[1 if transpose_w else 0] != K:
         raise ValueError(f"w has shape {tuple(w.shape)}, needs "
                          f"{('[2F, %d]' if transpose_w else '[%d, 2F]') % K}")
+    if max(M, K, two_f) > _MAX_SIZE:
+        raise ValueError(f"x and w have a dimension above {_MAX_SIZE}")
     return dt, dev, M, K, two_f // 2, x.shape[:-1]
 
 
@@ -548,8 +575,10 @@ def gated_linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = N
         out = _empty(lead + (F,), x.dtype, x.device, stream)
     else:
         _check_like(out, "out", dev, x.dtype, lead + (F,))
+        _apart(out, "out", x, w, bias, pre)
     if pre is not None:
         _check_like(pre, "pre", dev, torch.float32, lead + (_pre_cols(F),))
+        _apart(pre, "pre", x, w, bias)
     elif save:
         pre = _empty(lead + (_pre_cols(F),), torch.float32, x.device, stream)
     L, h, p = _lib.lib(), _handle(ctx, x), _prec(precision)
@@ -576,12 +605,15 @@ def gated_linear_backward(grad_out: torch.Tensor, pre: torch.Tensor, x: torch.Te
         dx = _empty_like(x, stream)
     else:
         _check_like(dx, "dx", dev, x.dtype, x.shape)
+        _apart(dx, "dx", grad_out, pre, x, w, dw, dbias)
     if dw is None:
         dw = _empty_like(w, stream)
     else:
         _check_like(dw, "dw", dev, x.dtype, w.shape)
+        _apart(dw, "dw", grad_out, pre, x, w, dbias)
     if dbias is not None:
         _check_like(dbias, "dbias", dev, x.dtype, (2 * F,))
+        _apart(dbias, "dbias", grad_out, pre, x, w)
     elif want_bias:
         dbias = _empty(2 * F, x.dtype, x.device, stream)
     L, h, p = _lib.lib(), _handle(ctx, x), _prec(precision)
@@ -611,6 +643,7 @@ def adamw_state_values(codes: torch.Tensor, scale: torch.Tensor, out: torch.Tens
         out = _empty(codes.shape, torch.bfloat16, codes.device, stream)
     else:
         _check_like(out, "out", dev, torch.bfloat16, codes.shape)
+        _apart(out, "out", codes, scale)
     rc = _lib.lib().mx_adamw_state_values(
         _handle(ctx, codes), codes.data_ptr(), scale.data_ptr(), n, codes.dtype is torch.uint8,
         out.data_ptr(), _launch_stream(dev, stream))

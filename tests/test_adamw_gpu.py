@@ -413,3 +413,29 @@ def test_step_count_on_the_device_is_the_devices(cuda_device):
     for _ in range(3):
         graph.replay()
     assert opt.step_count == 9
+
+
+def test_shared_memory_is_refused(cuda_device):
+    p = torch.ones(600, device="cuda")
+    with pytest.raises(ValueError, match="share memory"):
+        nn.AdamW([p, p])
+    with pytest.raises(ValueError, match="share memory"):
+        nn.AdamW([p[:400], p[300:]])
+    m = torch.zeros(600, device="cuda")
+    with pytest.raises(ValueError, match="share memory"):
+        nn.AdamW([p], state=[(m, m)])
+    nn.AdamW([p[:300], p[300:]]).step([torch.ones(300, device="cuda")] * 2)
+
+
+def test_step_on_another_stream(cuda_device):
+    p = torch.ones(5000, device="cuda")
+    ref = p.clone()
+    g = torch.linspace(-1, 1, 5000, device="cuda")
+    s = torch.cuda.Stream()
+    a = nn.AdamW([p], max_grad_norm=0.5, **HYPER)
+    s.wait_stream(torch.cuda.current_stream())
+    a.step([g], stream=s)
+    torch.cuda.current_stream().wait_stream(s)
+    b = nn.AdamW([ref], max_grad_norm=0.5, **HYPER)
+    b.step([g])
+    assert torch.equal(p, ref) and torch.equal(a.norm, b.norm)

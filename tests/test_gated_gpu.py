@@ -437,3 +437,42 @@ def test_refusals(cuda_device):
                                  0, None, 0, None) == bad  # pre off 32 bytes
     assert L.mx_gated_linear_fwd(hd, 1, None, p[1], None, p[2], None, 8, 32, 24, 0, 0, 0, None, 0,
                                  None) == bad
+
+
+def test_shared_memory_and_sizes_are_refused(cuda_device):
+    x, w, b, dh = _problem(8, 24, 24, BF16, False, True)
+    h, pre = ops.gated_linear(x, w, b, save=True)
+    with pytest.raises(ValueError, match="share memory"):
+        ops.gated_linear(x, w, b, out=x)
+    with pytest.raises(ValueError, match="share memory"):
+        ops.gated_linear_backward(dh, pre, x, w, dx=x)
+    with pytest.raises(ValueError, match="share memory"):
+        ops.gated_linear_backward(dh, pre, x, w, dw=w)
+    both = torch.empty(2 * 8 * 24, device="cuda", dtype=BF16)  # out and x overlap in part
+    with pytest.raises(ValueError, match="share memory"):
+        ops.gated_linear(both[:192].view(8, 24), w, b, out=both[100:292].view(8, 24))
+    ops.gated_linear(both[:192].view(8, 24), w, b, out=both[192:].view(8, 24))
+    L, hd = _lib.lib(), ops.context(0)
+    p = [t.data_ptr() for t in (x, w, h)]
+    for m, k, f in ((2 ** 31 - 1, 24, 24), (8, 2 ** 31 - 1, 24), (8, 24, 2 ** 30 - 1)):
+        assert L.mx_gated_linear_fwd(hd, 1, p[0], p[1], None, p[2], None, m, k, f, 0, 0, 0, None, 0,
+                                     None) == _lib.MX_ERR_UNSUPPORTED
+        assert L.mx_gated_linear_workspace_bytes(hd, 1, m, k, f, 0, 0, 0) == 0
+
+
+def test_long_and_thin(cuda_device):
+    """A product over 42 million rows, whose whole cost in cycles passes 31 bits."""
+    M, K, F = 42_000_001, 8, 8
+    x = torch.full((M, K), 0.5, device="cuda")
+    w = torch.zeros(K, 2 * F, device="cuda")
+    b = torch.ones(2 * F, device="cuda")
+    h, pre = ops.gated_linear(x, w, b, act="relu", save=True)
+    assert (h == 1).all()
+    dx, dw, db = ops.gated_linear_backward(h.mul_(0.25), pre, x, w, act="relu")
+    assert (dx == 0).all()
+    # dpre = 0.25 everywhere: dw = M / 8, db = M / 4, all of whose terms have one
+    # sign: M / 64 rounded sums of k-blocks of at most 24 truncations, and sums of
+    # no more terms than that for db
+    tol = M / 64 * U + 24 * 2 * U
+    assert ((dw.double() / (M / 8) - 1).abs() <= tol).all()
+    assert ((db.double() / (M / 4) - 1).abs() <= tol).all()

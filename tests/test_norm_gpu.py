@@ -241,3 +241,28 @@ def test_refusals(cuda_device):
             w.data_ptr(), None, 1100, 64)
     assert L.mx_layer_norm_bwd(*args, p, need - 1, None) == bad
     assert L.mx_layer_norm_bwd(*args, None, need, None) == bad
+
+
+def test_shared_memory_and_sizes_are_refused(cuda_device):
+    x, w, b, dy = _problem(8, 64, F32)
+    _, mean, rstd = ops.layer_norm(x, stats=True)
+    with pytest.raises(ValueError, match="share memory"):
+        ops.layer_norm(x, w, b, out=x)
+    with pytest.raises(ValueError, match="share memory"):
+        ops.layer_norm_backward(dy, x, w, mean, rstd, dx=dy)
+    with pytest.raises(ValueError, match="share memory"):
+        ops.layer_norm_backward(dy, x, w, mean, rstd, dweight=w)
+    one = torch.empty(64, device="cuda")
+    with pytest.raises(ValueError, match="share memory"):
+        ops.layer_norm_backward(dy, x, w, mean, rstd, dweight=one, dbias=one)
+    # halves of the same rows do not
+    both = torch.randn(8, 128, device="cuda")
+    ref = ops.layer_norm(both[:, 64:].contiguous(), w, b)[0]
+    ops.layer_norm(both[:, 64:], w, b, out=both[:, :64])
+    assert torch.equal(both[:, :64], ref)
+    L, h, p = _lib.lib(), ops.context(0), x.data_ptr()
+    top = 2 ** 31 - 1
+    for rows, cols in ((1, top), (top, 1)):
+        assert L.mx_layer_norm_fwd(h, 0, p, cols, None, None, p, cols, None, None, rows, cols, 1e-5,
+                                   None) == _lib.MX_ERR_UNSUPPORTED
+        assert L.mx_layer_norm_bwd_scratch_bytes(h, rows, cols) == 0
