@@ -55,6 +55,7 @@
 // the other.)
 // Every mbarrier wait is bounded (mx::wait_bar), as in gemm_tc.cu.
 #include <algorithm>
+#include <array>
 #include <type_traits>
 
 #include "gated_act.cuh"
@@ -773,10 +774,9 @@ void set_tiles(Plans& pl, const Bf16Gemm* g, int count, int sub) {
 // Tiles of 256 rows: whole ones where they fill the machine; otherwise the
 // split counts, the longer product's first, with the shortest longest queue.
 // Sizes alone decide, and with them the scratch.
-Plans plan_of(const Context* ctx, const Bf16Gemm* g, int count) {
+Plans make_plan(const Bf16Gemm* g, int count, int pairs) {
   Plans pl;
   const int copies = g[0].copies;
-  const int pairs = std::max(1, ctx->tc_sms() / 2);
   set_tiles(pl, g, count, 1);
   const int least = copies == 3 ? 2 : 8;  // k-blocks of a split
   const int longer = pl.p[1].num_kb > pl.p[0].num_kb ? 1 : 0;
@@ -804,6 +804,28 @@ Plans plan_of(const Context* ctx, const Bf16Gemm* g, int count) {
   }
   pl.pairs = std::min(pairs, pl.p[0].jobs() + pl.p[1].jobs());
   return pl;
+}
+
+// A plan depends on nothing but its key.  A backward call asks for the same few
+// plans eleven times (its workspace's size, the check of it, the launch), which
+// took 3 us of the host's 28 for 33 x 784 x 2 x 1000.
+Plans plan_of(const Context* ctx, const Bf16Gemm* g, int count) {
+  using Key = std::array<int, 10>;
+  struct Entry {
+    Key key{};
+    Plans plans;
+  };
+  static thread_local Entry kept[8];
+  static thread_local unsigned turn = 0;
+  const int pairs = std::max(1, ctx->tc_sms() / 2);
+  const Bf16Gemm& h = g[count - 1];
+  const Key key{pairs, count, g[0].copies, g[0].gated, g[0].M, g[0].N, g[0].K, h.M, h.N, h.K};
+  for (const Entry& e : kept)
+    if (e.key == key) return e.plans;
+  Entry& e = kept[turn++ % 8];
+  e.plans = make_plan(g, count, pairs);
+  e.key = key;
+  return e.plans;
 }
 
 // The plan of a launch: tiles of 512 rows (one copy, no scratch) where those are
@@ -848,8 +870,9 @@ int launch(Context* ctx, const Bf16Gemm* g, int count, void* scratch, const Bf16
     for (int c = 0; c < NC; ++c)
       if (!operand_map(&L.a[i][c], g[i].a, c, g[i].M, g[i].K) ||
           !operand_map(&L.b[i][0][c], g[i].b, c, g[i].N, g[i].K) ||
-          !operand_map(&L.b[i][1][c], GATED ? g[i].b2 : g[i].b, c, g[i].N, g[i].K))
+          (GATED && !operand_map(&L.b[i][1][c], g[i].b2, c, g[i].N, g[i].K)))
         return kErrUnsupported;
+    if (!GATED) std::copy(L.b[i][0], L.b[i][0] + NC, L.b[i][1]);
     Problem& p = L.p[i];
     const Plan& q = pl.p[i];
     p.out = g[i].out;

@@ -1,8 +1,9 @@
 """Device ops of the matmul path, called through the C ABI.
 
 torch is used only for device memory and streams: every function here takes
-CUDA tensors (float32; the layer norm, gated layer and AdamW also bfloat16), passes their raw pointers and the current torch stream
-to ``libmxgemm.so`` and lets the library's kernels do the work.
+CUDA tensors (float32; the layer norm, gated layer and AdamW also bfloat16),
+passes their raw pointers and the current torch stream to ``libmxgemm.so`` and
+lets the library's kernels do the work.
 """
 from __future__ import annotations
 
@@ -400,13 +401,14 @@ def _launch_stream(device: int, stream) -> int:
         torch._C._cuda_getCurrentRawStream(device)
 
 
-def _empty(shape, dtype, device, stream):
-    """Memory for a call on `stream` (None: the current one), allocated on that
-    stream, so that it is not handed on before the call is done with it."""
+def _empty(shape, dtype, t, stream):
+    """Memory on t's device for a call on `stream` (None: the current one),
+    allocated on that stream, so that it is not handed on before the call is
+    done with it.  (new_empty costs the host a quarter less than empty.)"""
     if stream is None:
-        return torch.empty(shape, dtype=dtype, device=device)
+        return t.new_empty(shape, dtype=dtype)
     with torch.cuda.stream(stream):
-        return torch.empty(shape, dtype=dtype, device=device)
+        return t.new_empty(shape, dtype=dtype)
 
 
 def _empty_like(t, stream):
@@ -473,14 +475,14 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None,
         if t is not None:
             _check_like(t, name, dev, torch.float32, (cols,))
     if out is None:
-        out = _empty_like(x, stream) if ldx == cols else _empty(x.shape, x.dtype, x.device, stream)
+        out = _empty_like(x, stream) if ldx == cols else _empty(x.shape, x.dtype, x, stream)
         ldy = cols
     else:
         ldy = _like_rows(out, "out", x, "x")
         _apart(out, "out", x, weight, bias)
     mean = rstd = None
     if stats:
-        mean = _empty(rows, torch.float32, x.device, stream)
+        mean = _empty(rows, torch.float32, x, stream)
         rstd = _empty_like(mean, stream)
     rc = _lib.lib().mx_layer_norm_fwd(
         _handle(ctx, x), dt, x.data_ptr(), ldx, _ptr(weight), _ptr(bias), out.data_ptr(), ldy,
@@ -505,13 +507,13 @@ def layer_norm_backward(grad_out: torch.Tensor, x: torch.Tensor, weight: torch.T
     _check_like(mean, "mean", dev, f32, (rows,))
     _check_like(rstd, "rstd", dev, f32, (rows,))
     if dx is None:
-        dx = _empty_like(x, stream) if ldx == cols else _empty(x.shape, x.dtype, x.device, stream)
+        dx = _empty_like(x, stream) if ldx == cols else _empty(x.shape, x.dtype, x, stream)
         lddx = cols
     else:
         lddx = _like_rows(dx, "dx", x, "x")
         _apart(dx, "dx", grad_out, x, weight, mean, rstd, dweight, dbias)
     if dweight is None:
-        dweight = _empty(cols, f32, x.device, stream) if weight is None else \
+        dweight = _empty(cols, f32, x, stream) if weight is None else \
             _empty_like(weight, stream)
     else:
         _check_like(dweight, "dweight", dev, f32, (cols,))
@@ -524,7 +526,7 @@ def layer_norm_backward(grad_out: torch.Tensor, x: torch.Tensor, weight: torch.T
     h = _handle(ctx, x)
     L = _lib.lib()
     nb = L.mx_layer_norm_bwd_scratch_bytes(h, rows, cols)
-    scratch = _empty(nb, torch.uint8, x.device, stream) if nb else None
+    scratch = _empty(nb, torch.uint8, x, stream) if nb else None
     rc = L.mx_layer_norm_bwd(
         h, dt, grad_out.data_ptr(), lddy, x.data_ptr(), ldx, _ptr(weight), mean.data_ptr(),
         rstd.data_ptr(), dx.data_ptr(), lddx, dweight.data_ptr(), dbias.data_ptr(), rows, cols,
@@ -572,7 +574,7 @@ def gated_linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = N
     if bias is not None:
         _check_like(bias, "bias", dev, x.dtype, (2 * F,))
     if out is None:
-        out = _empty(lead + (F,), x.dtype, x.device, stream)
+        out = _empty(lead + (F,), x.dtype, x, stream)
     else:
         _check_like(out, "out", dev, x.dtype, lead + (F,))
         _apart(out, "out", x, w, bias, pre)
@@ -580,10 +582,10 @@ def gated_linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = N
         _check_like(pre, "pre", dev, torch.float32, lead + (_pre_cols(F),))
         _apart(pre, "pre", x, w, bias)
     elif save:
-        pre = _empty(lead + (_pre_cols(F),), torch.float32, x.device, stream)
+        pre = _empty(lead + (_pre_cols(F),), torch.float32, x, stream)
     L, h, p = _lib.lib(), _handle(ctx, x), _prec(precision)
     nb = L.mx_gated_linear_workspace_bytes(h, dt, M, K, F, transpose_w, p, 0)
-    ws = _empty(nb, torch.uint8, x.device, stream) if nb else None
+    ws = _empty(nb, torch.uint8, x, stream) if nb else None
     rc = L.mx_gated_linear_fwd(
         h, dt, x.data_ptr(), w.data_ptr(), _ptr(bias), out.data_ptr(), _ptr(pre), M, K, F,
         transpose_w, _lib.ACTIVATIONS[act], p, _ptr(ws), nb, _launch_stream(dev, stream))
@@ -615,10 +617,10 @@ def gated_linear_backward(grad_out: torch.Tensor, pre: torch.Tensor, x: torch.Te
         _check_like(dbias, "dbias", dev, x.dtype, (2 * F,))
         _apart(dbias, "dbias", grad_out, pre, x, w)
     elif want_bias:
-        dbias = _empty(2 * F, x.dtype, x.device, stream)
+        dbias = _empty(2 * F, x.dtype, x, stream)
     L, h, p = _lib.lib(), _handle(ctx, x), _prec(precision)
     nb = L.mx_gated_linear_workspace_bytes(h, dt, M, K, F, transpose_w, p, 1)
-    ws = _empty(nb, torch.uint8, x.device, stream) if nb else None
+    ws = _empty(nb, torch.uint8, x, stream) if nb else None
     rc = L.mx_gated_linear_bwd(
         h, dt, grad_out.data_ptr(), pre.data_ptr(), x.data_ptr(), w.data_ptr(), dx.data_ptr(),
         dw.data_ptr(), _ptr(dbias), M, K, F, transpose_w, _lib.ACTIVATIONS[act], p, _ptr(ws), nb,
@@ -640,7 +642,7 @@ def adamw_state_values(codes: torch.Tensor, scale: torch.Tensor, out: torch.Tens
     _check_like(codes, "codes", dev, codes.dtype)
     _check_like(scale, "scale", dev, torch.float32, (-(-n // 256),))
     if out is None:
-        out = _empty(codes.shape, torch.bfloat16, codes.device, stream)
+        out = _empty(codes.shape, torch.bfloat16, codes, stream)
     else:
         _check_like(out, "out", dev, torch.bfloat16, codes.shape)
         _apart(out, "out", codes, scale)
