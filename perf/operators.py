@@ -127,29 +127,25 @@ def prepare(case, seed):
     m, v = flat(3e-4) * size, (flat(1e-3) * size).square() + torch.where(live, size.square() * 1e-8, zero)
     if case["bits"] == 32:
         return {**st, "m": m, "v": v}
-    st["m"], st["m_scale"] = _encode(m, True)
-    st["v"], st["v_scale"] = _encode(v.sqrt(), False)
+    st["m"], st["m_scale"] = _encode(m)
+    st["v"], st["v_scale"] = _encode(v.sqrt())
     return st
 
 
-def _encode(x, signed):
-    """8-bit codes of blocks of values and each block's largest magnitude, `top`: a code c stands for (c / 127)^2 top with
-    its sign, or without signs for (c / 255)^2 top.  The nearest code by the root; without signs, what is above zero
-    stays above zero."""
+def _encode(x):
+    """8-bit floating-point values (4 exponent bits, 3 of mantissa) and one power of two for each block, which takes
+    the block's largest value into [128, 256).  A value above zero stays above zero."""
     x = x.view(-1, BLOCK)
-    top = x.abs().amax(1, keepdim=True).clamp(min=2.0 ** -120)
-    root = torch.sqrt(x.abs() * (1 / top))
-    if signed:
-        c = torch.copysign(torch.round(root * 127), x).to(torch.int8)
-    else:
-        c = torch.where(x > 0, torch.round(root * 255).clamp(min=1), 0.0).to(torch.uint8)
-    return c.view(-1), top.view(-1)
+    top = x.abs().amax(1, keepdim=True).clamp(min=2.0 ** -119)
+    scale = (top.view(torch.int32) & 0x7F800000).view(torch.float32) * 2.0 ** -7
+    y = x / scale
+    y = torch.where((y > 0) & (y < 2.0 ** -9), 2.0 ** -9, y)
+    y = torch.where((y < 0) & (y > -(2.0 ** -9)), -(2.0 ** -9), y)
+    return y.to(torch.float8_e4m3fn).view(-1), scale.view(-1)
 
 
-def _decode(c, top, most):
-    c = c.view(-1, BLOCK).to(top.dtype)
-    r = c * (1 / most)
-    return ((r * r.abs()) * top.view(-1, 1)).view(-1)
+def _decode(q, scale):
+    return (q.float().view(-1, BLOCK) * scale.view(-1, 1)).view(-1)
 
 
 def _act(name, g):
@@ -228,20 +224,16 @@ def _gated(st):
 
 def _adamw(st):
     c = st["case"]
-    # what is held in 8 bits comes back as the values that it stands for
-    out = {"p": st["p"], "m": st["m"], "v": st["v"], "copy": st["copy"]}
+    keys = ("p", "m", "v", "copy") if c["bits"] == 32 else ("p", "m", "m_scale", "v", "v_scale", "copy")
     if own:
         if "opt" not in st:
             st["opt"], st["grads"] = _optimizer(st)
         st["opt"].step(st["grads"])
-        if c["bits"] == 8:
-            from moonxi_net_b200 import ops
-            out["m"], out["v"] = (ops.adamw_state_values(st[k], st[k + "_scale"]) for k in ("m", "v"))
-        return out
+        return {k: st[k] for k in keys}
     st["step"] += 1
     p, g = st["p"], st["g"].float()
-    m = st["m"] if c["bits"] == 32 else _decode(st["m"], st["m_scale"], 127)
-    v = st["v"] if c["bits"] == 32 else _decode(st["v"], st["v_scale"], 255).square()
+    m = st["m"] if c["bits"] == 32 else _decode(st["m"], st["m_scale"])
+    v = st["v"] if c["bits"] == 32 else _decode(st["v"], st["v_scale"]).square()
     m = m * BETA1 + g * (1 - BETA1)
     v = v * BETA2 + (g * g) * (1 - BETA2)
     root = torch.sqrt(v)
@@ -251,15 +243,13 @@ def _adamw(st):
         st["m"].copy_(m)
         st["v"].copy_(v)
     else:
-        for key, x, most in (("m", m, 127), ("v", root, 255)):
-            q, top = _encode(x, key == "m")
+        for key, x in (("m", m), ("v", root)):
+            q, scale = _encode(x)
             st[key].copy_(q)
-            st[key + "_scale"].copy_(top)
-            x = _decode(q, top, most)
-            out[key] = (x if key == "m" else x.square()).to(torch.bfloat16)
+            st[key + "_scale"].copy_(scale)
     if st["copy"] is not None:
         st["copy"].copy_(p)
-    return out
+    return {k: st[k] for k in keys}
 
 
 def _optimizer(st):
@@ -295,8 +285,7 @@ def work(case):
             return {"bytes": x + w + h + bias, "flops": 4 * m * d * f}
         return {"bytes": 2 * x + 2 * w + 2 * h + 2 * bias, "flops": 12 * m * d * f}
     n = sum(math.prod(s) for s in _shapes(case))
-    # parameters in and out, gradients, both moments in and out; 8-bit ones come back as bf16 values too
-    per = 8 + (4 if case["grad"] == "f32" else 2) + (16 if case["bits"] == 32 else 4 + 16 / BLOCK + 4)
+    per = 8 + (4 if case["grad"] == "f32" else 2) + (16 if case["bits"] == 32 else 4 + 16 / BLOCK)
     return {"bytes": n * (per + (2 if case["kind"] == "block" else 0)), "flops": 15 * n}
 
 
@@ -327,18 +316,13 @@ def exact(case, seed):
     t = st["step"] + 1
     p, g, m, v = (st[k].double() for k in ("p", "g", "m", "v"))
     if case["bits"] == 8:
-        m, v = (t.view(-1, BLOCK) * t.abs().view(-1, BLOCK) * top.double().view(-1, 1) / most ** 2
-                for t, top, most in ((m, st["m_scale"], 127), (v, st["v_scale"], 255)))
-        m, v = m.flatten(), v.flatten() ** 2
+        m = m * st["m_scale"].double().repeat_interleave(BLOCK)
+        v = (v * st["v_scale"].double().repeat_interleave(BLOCK)) ** 2
     m, v = torch.lerp(g, m, BETA1), torch.lerp(g ** 2, v, BETA2)
     p = p - LR * DECAY * p
     p = p - LR * (m / (1 - BETA1 ** t)) / (torch.sqrt(v / (1 - BETA2 ** t)) + ADAM_EPS)
-    if case["bits"] == 8:
-        def nearest(x, most, least):  # the value that x is held as
-            top = x.abs().view(-1, BLOCK).amax(1).clamp(min=2.0 ** -120).repeat_interleave(BLOCK)
-            c = ((x.abs() / top).sqrt() * most).round()
-            c = torch.where(x.abs() > 0, c.clamp(min=least), 0.0)
-            return x.sign() * (c / most) ** 2 * top
-
-        m, v = nearest(m, 127, 0), nearest(v.sqrt(), 255, 1) ** 2
-    return {"p": p, "m": m, "v": v, "copy": p if case["kind"] == "block" else None}
+    copy = p if case["kind"] == "block" else None
+    if case["bits"] == 32:
+        return {"p": p, "m": m, "v": v, "copy": copy}
+    # which of two neighbours an 8-bit value or a scale becomes is decided in 32 bits: no value in 64
+    return {"p": p, "m": None, "m_scale": None, "v": None, "v_scale": None, "copy": copy}
