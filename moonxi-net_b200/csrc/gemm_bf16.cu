@@ -473,8 +473,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     float* tw = tr + (warp - 2) * kTrFloats;
     int seg = 0;
     bool ok = true;
-    // 32 columns of this warp's rows in accumulator `acc`
+    // 32 columns of this warp's rows in accumulator `acc`.  The lanes part where
+    // rows end and where an activation branches; the load wants them together.
     auto load32 = [&](int acc, int col, uint32_t (&r)[32]) {
+      __syncwarp();
       tmem_ld_32cols(lanes + acc * kTile + col, r);
       tmem_wait_ld();
     };

@@ -275,9 +275,11 @@ __device__ __forceinline__ uint32_t cluster_rank() {
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
   return r;
 }
-// Both CTAs of the pair arrive, then wait for each other.  Every wait before
-// it is bounded, so both always reach it.
+// All threads of the cluster arrive, then wait for each other.  Every wait
+// before it is bounded, so all of them reach it; a warp's lanes arrive together,
+// whatever loops or branches they come from.
 __device__ __forceinline__ void cluster_sync() {
+  __syncwarp();
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::
                    : "memory");
 }
