@@ -212,18 +212,20 @@ __device__ __forceinline__ float block_top(const float (&x)[8]) {
   top = __reduce_max_sync(0xffffffffu, top);
   return __uint_as_float(top >= 0x7f800000u ? 0x7fc00000u : top);
 }
-// The codes: c = round(sqrt(|x| most^2 / top)), rounded by adding 1.5 * 2^23,
+// The codes: c = round(sqrt(|x| / top) most), rounded by adding 1.5 * 2^23,
 // which leaves it in the low byte; signed ones below `down` are floor(c + 1/64),
 // so that a value that stays as it is keeps its code.  The root's last bit does
-// not matter here.
+// not matter here.  (most^2 / top would pass float32 from a top of 2^-112 down,
+// and infinity times a zero is no zero; 1 / top is at most 2^120.)
 template <bool SIGNED>
 __device__ __forceinline__ void encode8(uint8_t* q, float top, float down, bool vec, int left,
                                         const float (&x)[8]) {
-  const float scale = __fdiv_rn(SIGNED ? 16129.0f : 65025.0f, top);
+  constexpr float kMost = SIGNED ? 127.0f : 255.0f;
+  const float inv = __fdiv_rn(1.0f, top);
   uint32_t b[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    float c = fast_sqrt(fabsf(x[i]) * scale);
+    float c = fast_sqrt(fabsf(x[i]) * inv) * kMost;
     if (SIGNED) c = copysignf(c < down ? fmaxf(c - 0.484375f, 0.0f) : c, x[i]);
     else if (x[i] > 0.0f) c = fmaxf(c, 1.0f);
     b[i] = __float_as_uint(c + 12582912.0f);
