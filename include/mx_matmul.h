@@ -464,9 +464,9 @@ uint64_t mx_gated_linear_workspace_bytes(void* handle, int32_t dtype, int32_t M,
 
 /* One tensor of mx_adamw_step.  param: float32, updated in place; grad:
  * float32 or bfloat16 (grad_type); m, v: the moments, float32[n], or with
- * 8-bit states int8[n] and uint8[n] with one float32 scale for each 256
- * values in m_scale and v_scale (ceil(n / 256) floats each; zeros are a fresh
- * state).  copy_bf16 (may be NULL) receives the new values as bfloat16. */
+ * 8-bit states int8[n] and uint8[n] (MX_ADAMW_E4M3: float8 e4m3[n] both) with one
+ * float32 scale for each 256 values in m_scale and v_scale (ceil(n / 256) floats
+ * each; zeros are a fresh state).  copy_bf16 (may be NULL) receives the new values as bfloat16. */
 typedef struct mx_adamw_tensor {
   float* param;
   const void* grad;
@@ -480,11 +480,13 @@ typedef struct mx_adamw_tensor {
   int32_t grad_type;
 } mx_adamw_tensor;
 
+#define MX_ADAMW_E4M3 0x100
+
 /* One AdamW step over `count` tensors (host array) in one launch:
  *   g' = clip * g,  m = beta1 m + (1 - beta1) g',  v = beta2 v + (1 - beta2) g'^2,
  *   p = (1 - lr weight_decay) p
  *       - lr / (1 - beta1^t) m / (sqrt(v) / sqrt(1 - beta2^t) + eps).
- * state_bits: 32 or 8.  t = step (>= 1), or, with step_dev (device int32), the
+ * state_bits: 32, 8, or 8 | MX_ADAMW_E4M3.  t = step (>= 1), or, with step_dev (device int32), the
  * incremented *step_dev, so that a captured call counts its replays.
  * max_grad_norm > 0 clips by the norm over all the tensors' gradients as
  * mx_sgd_momentum_autoclip does (norm_out, device, may be NULL, receives it).
@@ -494,7 +496,12 @@ typedef struct mx_adamw_tensor {
  * above zero keeps one above zero; m's codes below 0.5 / (1 - sqrt(beta1)) + 1
  * are rounded towards zero, so that m dies out with its gradients).  A change
  * of v against its block's largest by less than half a code a step is lost:
- * with beta2 above 0.99 the second moments follow only slowly.  The tensors must not overlap.
+ * with beta2 above 0.99 the second moments follow only slowly.
+ * MX_ADAMW_E4M3: m and sqrt(v) are the nearest e4m3 value (what is not zero stays
+ * above zero) times the scale, a power of two that takes the largest of its 256
+ * magnitudes (at least 2^-119) into [128, 256), infinite if one of them is not
+ * finite; the step is that of 32-bit states, bit for bit.
+ * The tensors must not overlap.
  * scratch: mx_adamw_scratch_bytes(count, max_grad_norm > 0) bytes, 16-byte
  * aligned (may be NULL without clipping and step_dev). */
 int32_t mx_adamw_step(void* handle, const mx_adamw_tensor* tensors, int32_t count,

@@ -37,6 +37,7 @@ PRECISIONS = {"default": PREC_DEFAULT, "auto": PREC_AUTO, "fp32": PREC_FP32,
 # element types and activations of the layer norm, gated layer and AdamW calls
 F32 = 0
 BF16 = 1
+ADAMW_E4M3 = 0x100  # with 8-bit states: the moments are float8_e4m3fn values
 ACTIVATIONS = {"silu": 0, "gelu": 1, "gelu_tanh": 2, "relu": 3, "sigmoid": 4}
 
 _vp = ctypes.c_void_p

@@ -1,5 +1,5 @@
 // adamw.cu -- one AdamW step over many tensors in one launch, its two moments
-// held in float32 or in 8 bits.
+// held in float32 or in 8 bits, as square-root codes or as floating-point values.
 //
 //   g' = clip * g                         clip = max_norm / ||g|| when above it
 //   m  = b1 m + (1 - b1) g',   v = b2 v + (1 - b2) g'^2
@@ -22,6 +22,14 @@
 // uses this step's float32 moments, before they are rounded.  A moment that is
 // not finite makes its block's scale, and so the whole block, NaN.
 //
+// 8-bit floating-point states (e4m3, three bits of mantissa): m and sqrt(v) as
+// such values times a power of two, the same for 256 of them, which takes the
+// largest magnitude (at least 2^-119) into [128, 256).  The nearest value is kept;
+// what is not zero stays above zero (2^-9 before the power of two).  A factor
+// that is infinite marks a block with a moment that is not finite.  The step is
+// that of 32-bit states, bit for bit the one of elementwise float32 operations,
+// since a value near the middle of two falls by its last bit.
+//
 // Bound by the bytes: 28 B a value with float32 gradients and states, 16 B
 // with 8-bit states (14 B with bf16 gradients).  A warp takes 256 values,
 // 8 a lane in 16-byte accesses, so an 8-bit block is one warp's and its
@@ -30,6 +38,7 @@
 #include <cmath>
 
 #include <cuda_bf16.h>
+#include <cuda_fp8.h>
 
 #include "../../include/mx_matmul.h"
 #include "mx_internal.h"
@@ -44,6 +53,9 @@ constexpr int kPerWarp = 1;            // 256-value blocks of a warp
 constexpr int kChunk = kPerWarp * kWarps * kQBlock;  // values of one block
 
 enum : uint32_t { kGradBf16 = 1, kVec = 2 };
+
+// How the moments are held.
+enum Kind { kF32, kRoot, kE4m3 };
 
 struct Tensor {
   float* p;
@@ -98,15 +110,15 @@ __device__ __forceinline__ float fast_rcp(float x) {
   return r;
 }
 
-// The new m, v and p of one value; returns sqrt(v).  32-bit moments: every
-// operation rounded by itself, as the elementwise form of the step computes
-// it.  8-bit moments: fused, with the approximate root and quotient (2 units in
+// The new m, v and p of one value; returns sqrt(v).  32-bit and e4m3 moments:
+// every operation rounded by itself, as the elementwise form of the step computes
+// it.  Root codes: fused, with the approximate root and quotient (2 units in
 // the last place), which the exact ones' instructions would bind: 0.82 ms
 // against 0.49 ms of bytes for 201 M values.
-template <bool Q8>
+template <Kind KIND>
 __device__ __forceinline__ float adamw_one(float& p, float g, float& m, float& v, float keep,
                                            const Hyper& h) {
-  if constexpr (Q8) {
+  if constexpr (KIND == kRoot) {
     m = fmaf(m, h.b1, g * h.omb1);
     v = fmaf(v, h.b2, g * g * h.omb2);
     const float root = fast_sqrt(v);
@@ -186,10 +198,9 @@ __device__ __forceinline__ void decode_words(const uint32_t (&w)[2], float top, 
     x[i] = c * fabsf(c) * unit;
   }
 }
-template <bool SIGNED>
-__device__ __forceinline__ void decode8(const uint8_t* q, float top, bool vec, int left,
-                                        float (&x)[8]) {
-  uint32_t w[2] = {0, 0};
+// 8 bytes of a lane, those past `left` not touched (read as zeros).
+__device__ __forceinline__ void load_bytes8(const uint8_t* q, bool vec, int left, uint32_t (&w)[2]) {
+  w[0] = w[1] = 0;
   if (vec && left >= 8) {
     const uint2 r = *reinterpret_cast<const uint2*>(q);
     w[0] = r.x;
@@ -199,6 +210,21 @@ __device__ __forceinline__ void decode8(const uint8_t* q, float top, bool vec, i
     for (int i = 0; i < 8; ++i)
       if (i < left) w[i >> 2] |= static_cast<uint32_t>(q[i]) << (8 * (i & 3));
   }
+}
+__device__ __forceinline__ void store_bytes8(uint8_t* q, bool vec, int left, const uint32_t (&w)[2]) {
+  if (vec && left >= 8) {
+    *reinterpret_cast<uint2*>(q) = make_uint2(w[0], w[1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < left) q[i] = static_cast<uint8_t>(w[i >> 2] >> (8 * (i & 3)));
+  }
+}
+template <bool SIGNED>
+__device__ __forceinline__ void decode8(const uint8_t* q, float top, bool vec, int left,
+                                        float (&x)[8]) {
+  uint32_t w[2];
+  load_bytes8(q, vec, left, w);
   decode_words<SIGNED>(w, top, x);
 }
 // The warp's largest magnitude, at least 2^-120; NaN if a value is not finite.
@@ -235,18 +261,53 @@ __device__ __forceinline__ void encode8(uint8_t* q, float top, float down, bool 
   for (int i = 0; i < 2; ++i)
     w[i] = __byte_perm(__byte_perm(b[4 * i], b[4 * i + 1], 0x0040),
                        __byte_perm(b[4 * i + 2], b[4 * i + 3], 0x0040), 0x5410);
-  if (vec && left >= 8) {
-    *reinterpret_cast<uint2*>(q) = make_uint2(w[0], w[1]);
-  } else {
+  store_bytes8(q, vec, left, w);
+}
+
+// The power of two that takes the warp's largest magnitude, at least 2^-119, into
+// [128, 256); infinity if a value is not finite.
+__device__ __forceinline__ float block_power(const float (&x)[8]) {
+  uint32_t top = 0x04000000u;  // 2^-119
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i < left) q[i] = static_cast<uint8_t>(w[i >> 2] >> (8 * (i & 3)));
+  for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+  top = __reduce_max_sync(0xffffffffu, top) & 0x7f800000u;
+  return __uint_as_float(top == 0x7f800000u ? top : top - (7u << 23));
+}
+// What 8 e4m3 values times `power` stand for (exact).
+__device__ __forceinline__ void decode8_e4m3(const uint8_t* q, float power, bool vec, int left,
+                                             float (&x)[8]) {
+  uint32_t w[2];
+  load_bytes8(q, vec, left, w);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __half2 h(__nv_cvt_fp8x2_to_halfraw2(
+        static_cast<__nv_fp8x2_storage_t>(w[i >> 1] >> (16 * (i & 1))), __NV_E4M3));
+    const float2 f = __half22float2(h);
+    x[2 * i] = f.x * power;
+    x[2 * i + 1] = f.y * power;
   }
+}
+__device__ __forceinline__ void encode8_e4m3(uint8_t* q, float power, bool vec, int left,
+                                             const float (&x)[8]) {
+  const float inv = __fdiv_rn(1.0f, power);  // exact; 0 where power is infinite
+  float y[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    y[i] = x[i] * inv;
+    if (y[i] != 0.0f && fabsf(y[i]) < 0.001953125f) y[i] = copysignf(0.001953125f, y[i]);
+  }
+  uint32_t w[2] = {0, 0};
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    w[i >> 1] |= static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(
+                     make_float2(y[2 * i], y[2 * i + 1]), __NV_SATFINITE, __NV_E4M3))
+                 << (16 * (i & 1));
+  store_bytes8(q, vec, left, w);
 }
 
 // The step of 256 values, a warp's; VEC: all of them are there, 16-byte
 // aligned (8-bit states 8-byte).
-template <bool Q8, bool VEC>
+template <Kind KIND, bool VEC>
 __device__ __forceinline__ void adamw_block(const Tensor& t, const Hyper& h, float clip,
                                             int64_t block) {
   const int lane = threadIdx.x & 31;
@@ -257,9 +318,16 @@ __device__ __forceinline__ void adamw_block(const Tensor& t, const Hyper& h, flo
   load8(t.p + at, VEC, left, p);
   if (t.flags & kGradBf16) load8(static_cast<const __nv_bfloat16*>(t.g) + at, VEC, left, g);
   else load8(static_cast<const float*>(t.g) + at, VEC, left, g);
-  if (Q8) {
-    decode8<true>(static_cast<const uint8_t*>(t.m) + at, t.ms[block], VEC, left, m);
-    decode8<false>(static_cast<const uint8_t*>(t.v) + at, t.vs[block], VEC, left, v);
+  if constexpr (KIND != kF32) {
+    const uint8_t* mq = static_cast<const uint8_t*>(t.m) + at;
+    const uint8_t* vq = static_cast<const uint8_t*>(t.v) + at;
+    if constexpr (KIND == kRoot) {
+      decode8<true>(mq, t.ms[block], VEC, left, m);
+      decode8<false>(vq, t.vs[block], VEC, left, v);
+    } else {
+      decode8_e4m3(mq, t.ms[block], VEC, left, m);
+      decode8_e4m3(vq, t.vs[block], VEC, left, v);
+    }
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = __fmul_rn(v[i], v[i]);
   } else {
@@ -272,13 +340,24 @@ __device__ __forceinline__ void adamw_block(const Tensor& t, const Hyper& h, flo
   }
   float root[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) root[i] = adamw_one<Q8>(p[i], g[i], m[i], v[i], t.keep, h);
+  for (int i = 0; i < 8; ++i) root[i] = adamw_one<KIND>(p[i], g[i], m[i], v[i], t.keep, h);
   store8(t.p + at, VEC, left, p);
   if (t.copy) store8(t.copy + at, VEC, left, p);
-  if (Q8) {
-    const float sm = block_top<true>(m), sv = block_top<false>(root);
-    encode8<true>(static_cast<uint8_t*>(t.m) + at, sm, h.down, VEC, left, m);
-    encode8<false>(static_cast<uint8_t*>(t.v) + at, sv, 0.0f, VEC, left, root);
+  if constexpr (KIND != kF32) {
+    uint8_t* mq = static_cast<uint8_t*>(t.m) + at;
+    uint8_t* vq = static_cast<uint8_t*>(t.v) + at;
+    float sm, sv;
+    if constexpr (KIND == kRoot) {
+      sm = block_top<true>(m);
+      sv = block_top<false>(root);
+      encode8<true>(mq, sm, h.down, VEC, left, m);
+      encode8<false>(vq, sv, 0.0f, VEC, left, root);
+    } else {
+      sm = block_power(m);
+      sv = block_power(root);
+      encode8_e4m3(mq, sm, VEC, left, m);
+      encode8_e4m3(vq, sv, VEC, left, root);
+    }
     __syncwarp();  // every lane has read the old scales
     if (lane == 0) {
       t.ms[block] = sm;
@@ -290,7 +369,7 @@ __device__ __forceinline__ void adamw_block(const Tensor& t, const Hyper& h, flo
   }
 }
 
-template <int CAP, bool Q8>
+template <int CAP, Kind KIND>
 __global__ void __launch_bounds__(32 * kWarps) adamw_kernel(const __grid_constant__ Table<CAP> tb,
                                                             const Hyper hy) {
   const int ti = find_tensor(tb, blockIdx.x);
@@ -310,8 +389,8 @@ __global__ void __launch_bounds__(32 * kWarps) adamw_kernel(const __grid_constan
   for (int k = 0; k < kPerWarp; ++k) {
     const int64_t block = first + k * kWarps;
     if (block * kQBlock >= t.n) return;  // the whole warp
-    if ((t.flags & kVec) && (block + 1) * kQBlock <= t.n) adamw_block<Q8, true>(t, h, clip, block);
-    else adamw_block<Q8, false>(t, h, clip, block);
+    if ((t.flags & kVec) && (block + 1) * kQBlock <= t.n) adamw_block<KIND, true>(t, h, clip, block);
+    else adamw_block<KIND, false>(t, h, clip, block);
   }
 }
 
@@ -450,7 +529,7 @@ void fill(Table<CAP>& tb, const mx_adamw_tensor* ts, int count, int bits, double
     t.copy = static_cast<__nv_bfloat16*>(a.copy_bf16);
     t.n = a.n;
     t.keep = static_cast<float>(1.0 - lr * a.weight_decay);
-    const unsigned sa = bits == 8 ? 8 : 16;
+    const unsigned sa = bits & 8 ? 8 : 16;
     t.flags = (a.grad_type == MX_BF16 ? kGradBf16 : 0u) |
               (aligned(a.param, 16) && aligned(a.grad, 16) && aligned(a.m, sa) &&
                        aligned(a.v, sa) && aligned(a.copy_bf16, 16)
@@ -480,10 +559,10 @@ cudaError_t launch_step(const mx_adamw_tensor* ts, int count, int bits, double l
   fill(tb, ts, count, bits, lr);
   const int64_t chunks = tb.first[tb.count];
   if (chunks == 0) return cudaSuccess;
-  if (bits == 8)
-    adamw_kernel<CAP, true><<<static_cast<unsigned>(chunks), 32 * kWarps, 0, s>>>(tb, h);
-  else
-    adamw_kernel<CAP, false><<<static_cast<unsigned>(chunks), 32 * kWarps, 0, s>>>(tb, h);
+  const unsigned grid = static_cast<unsigned>(chunks);
+  if (bits & MX_ADAMW_E4M3) adamw_kernel<CAP, kE4m3><<<grid, 32 * kWarps, 0, s>>>(tb, h);
+  else if (bits & 8) adamw_kernel<CAP, kRoot><<<grid, 32 * kWarps, 0, s>>>(tb, h);
+  else adamw_kernel<CAP, kF32><<<grid, 32 * kWarps, 0, s>>>(tb, h);
   note_launches(1);
   return cudaGetLastError();
 }
@@ -508,7 +587,7 @@ int adamw_check(const mx_adamw_tensor* ts, int count, int bits) {
     if (a.n < 0 || (a.grad_type != MX_F32 && a.grad_type != MX_BF16)) return kErrInvalid;
     if (a.n == 0) continue;
     if (!a.param || !a.grad || !a.m || !a.v) return kErrInvalid;
-    if (bits == 8 && (!a.m_scale || !a.v_scale)) return kErrInvalid;
+    if ((bits & 8) && (!a.m_scale || !a.v_scale)) return kErrInvalid;
     chunks += chunks_of(a.n);
     if (chunks > 0x7fffffff) return kErrUnsupported;  // blocks of one launch
   }

@@ -766,7 +766,8 @@ class AdamW:
     params: contiguous float32 CUDA tensors of one device, updated in place.
     Gradients may be float32 or bfloat16, tensor by tensor.  state_bits = 32
     keeps both moments in float32, 8 in one byte each with a float32 scale for
-    every 256 values.  copies: bfloat16 tensors (or None) that receive the new
+    every 256 values: int8 and uint8 codes of their roots, or, where `state` has
+    them (zeros are a fresh state), float8_e4m3fn values.  copies: bfloat16 tensors (or None) that receive the new
     values, for layers that compute in bfloat16.  weight_decay: one number, or
     one for each tensor (0 for norms and biases).  max_grad_norm > 0 clips by
     the global norm, which `norm` then holds after a step.
@@ -850,6 +851,11 @@ class AdamW:
         f32 = torch.float32
         names, types = (("m", "v"), (f32, f32)) if self.state_bits == 32 else \
             (("m", "m_scale", "v", "v_scale"), (torch.int8, f32, torch.uint8, f32))
+        self._kind = self.state_bits
+        if self.state_bits == 8 and getattr(next(iter(self.state[0]), None), "dtype", None) is \
+                torch.float8_e4m3fn:
+            types = (torch.float8_e4m3fn, f32) * 2
+            self._kind |= _lib.ADAMW_E4M3
         for i, (s, p) in enumerate(zip(self.state, self.params)):
             if len(s) != len(names):
                 raise ValueError(f"state[{i}] needs {names}")
@@ -876,7 +882,7 @@ class AdamW:
             self._scratch.record_stream(stream)
             self.norm.record_stream(stream)
         rc = _lib.lib().mx_adamw_step(
-            ops._handle(self.ctx, self.params[0]), self._table, len(self.params), self.state_bits,
+            ops._handle(self.ctx, self.params[0]), self._table, len(self.params), self._kind,
             self.lr, self.betas[0], self.betas[1], self.eps, self._steps + 1,
             ops._ptr(self.step_dev), self.max_grad_norm, self.norm.data_ptr(),
             self._scratch.data_ptr(), self._scratch.numel(),
