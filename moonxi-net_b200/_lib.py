@@ -38,6 +38,7 @@ PRECISIONS = {"default": PREC_DEFAULT, "auto": PREC_AUTO, "fp32": PREC_FP32,
 F32 = 0
 BF16 = 1
 ADAMW_E4M3 = 0x100  # with 8-bit states: the moments are float8_e4m3fn values
+ADAMW_DITHER = 0x200  # with 8-bit states: rounded up or down, right on the average
 ACTIVATIONS = {"silu": 0, "gelu": 1, "gelu_tanh": 2, "relu": 3, "sigmoid": 4}
 
 _vp = ctypes.c_void_p

@@ -944,7 +944,7 @@ MX_EXPORT int32_t mx_adamw_step(void* handle, const mx_adamw_tensor* tensors, in
   Context* c = scope.c;
   if (!c) return MX_ERR_NO_DEVICE;
   if (count < 0 || (count > 0 && !tensors) ||
-      (state_bits != 32 && state_bits != 8 && state_bits != (8 | MX_ADAMW_E4M3)))
+      (state_bits != 32 && (state_bits & ~(MX_ADAMW_E4M3 | MX_ADAMW_DITHER)) != 8))
     return MX_ERR_INVALID;
   if (!(beta1 >= 0.0 && beta1 < 1.0) || !(beta2 >= 0.0 && beta2 < 1.0) || !(eps >= 0.0))
     return MX_ERR_INVALID;

@@ -17,15 +17,28 @@
 // sqrt(v)) and still reaches 1.5e-5 of it; holding sqrt(v) halves the range of
 // exponents that v spans.  A sqrt(v) above zero keeps a code above zero (a
 // vanished v would blow the step up), and since `top` itself is not rounded,
-// moments that decay together decay exactly.  What is lost is a change of one
-// value against its block's largest by less than half a step.  The step itself
+// moments that decay together decay exactly.  The step itself
 // uses this step's float32 moments, before they are rounded.  A moment that is
 // not finite makes its block's scale, and so the whole block, NaN.
+//
+// Nearest codes lose a change of one value against its block's largest by less
+// than half a step.  Without gradient no v code below 0.5 / (1 - b2^(1/4)) falls (39
+// of 255 for b2 = 0.95, 66 for 0.97, all of them for 0.999), and a first moment
+// under a constant gradient settles at 0.23, 0.33 and 0.38 of its true value where
+// that is 0.4, 0.9 and 1.6 % of the block's largest, at 0.65 to 0.74 where it is 2
+// to 5 % (b1 = 0.9; rounded to nearest 0.45, 0.50, 0.60).  So there is a
+// second rounding, DITHER: up or down by a number made from the step and the
+// value's place, with the chance that makes the stored moment (m, and v itself)
+// right on the average.  It follows at any decay rates, at the price of noise: a
+// v of code c is off by a deviation of sqrt(2 / c) or so for b2 = 0.999.  Small m
+// then need no rounding towards zero: they die out by chance.
 //
 // 8-bit floating-point states (e4m3, three bits of mantissa): m and sqrt(v) as
 // such values times a power of two, the same for 256 of them, which takes the
 // largest magnitude (at least 2^-119) into [128, 256).  The nearest value is kept;
-// what is not zero stays above zero (2^-9 before the power of two).  A factor
+// what is not zero stays above zero (2^-9 before the power of two).  Neighbours are
+// up to 1/8 apart, so that a nearest v never falls where sqrt(b2) is above 31/32;
+// DITHER is there for these states too (and keeps v alone above zero).  A factor
 // that is infinite marks a block with a moment that is not finite.  The step is
 // that of 32-bit states, bit for bit the one of elementwise float32 operations,
 // since a value near the middle of two falls by its last bit.
@@ -82,7 +95,8 @@ struct Table {
 struct Hyper {
   float b1, omb1, b2, omb2, eps, step_size, inv_root;  // see adamw_one
   float down;             // 8-bit first moments: codes below it are rounded down
-  const float* scalars;   // device: {step_size, inv_root} instead, or null
+  uint32_t step;          // of the dither
+  const float* scalars;   // device: {step_size, inv_root, step} instead, or null
   const float* norm;      // device: the gradients' norm, or null (no clipping)
   float max_norm;
 };
@@ -131,6 +145,20 @@ __device__ __forceinline__ float adamw_one(float& p, float g, float& m, float& v
   const float denom = __fadd_rn(__fmul_rn(root, h.inv_root), h.eps);
   p = __fsub_rn(__fmul_rn(p, keep), __fdiv_rn(__fmul_rn(m, h.step_size), denom));
   return root;
+}
+
+// 32 bits for the dither from a step and a place: multiplications by 2^32 over the
+// golden ratio, and shifts that bring the upper bits down.  (Means, variances and
+// the correlations between places, steps and both halves are those of random
+// numbers to within 3 deviations of 2^20 places and 40 steps.)
+__device__ __forceinline__ uint32_t scatter(uint32_t x) {
+  x = (x ^ (x >> 16)) * 0x9e3779b1u;
+  x = (x ^ (x >> 15)) * 0x9e3779b1u;
+  return x ^ (x >> 16);
+}
+// Whether 16 of them are below the chance p.
+__device__ __forceinline__ bool below(uint32_t bits, float p) {
+  return static_cast<float>(bits & 0xffffu) + 0.5f < p * 65536.0f;
 }
 
 // 8 values of a lane, those past `left` not touched.
@@ -243,16 +271,25 @@ __device__ __forceinline__ float block_top(const float (&x)[8]) {
 // so that a value that stays as it is keeps its code.  The root's last bit does
 // not matter here.  (most^2 / top would pass float32 from a top of 2^-112 down,
 // and infinity times a zero is no zero; 1 / top is at most 2^120.)
-template <bool SIGNED>
+// DITHER: the two codes k and k + 1 around c stand for k^2 and (k + 1)^2 (m), or k^4
+// and (k + 1)^4 (v).
+template <bool SIGNED, bool DITHER>
 __device__ __forceinline__ void encode8(uint8_t* q, float top, float down, bool vec, int left,
-                                        const float (&x)[8]) {
+                                        const float (&x)[8], const uint32_t (&bits)[8]) {
   constexpr float kMost = SIGNED ? 127.0f : 255.0f;
   const float inv = __fdiv_rn(1.0f, top);
   uint32_t b[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     float c = fast_sqrt(fabsf(x[i]) * inv) * kMost;
-    if (SIGNED) c = copysignf(c < down ? fmaxf(c - 0.484375f, 0.0f) : c, x[i]);
+    if constexpr (DITHER) {
+      const float k = fminf(floorf(c), kMost - 1.0f);  // the largest is the last code
+      const float a = SIGNED ? c * c : c * c * c * c, lo = SIGNED ? k * k : k * k * k * k;
+      const float k1 = k + 1.0f, hi = SIGNED ? k1 * k1 : k1 * k1 * k1 * k1;
+      c = below(bits[i] >> (SIGNED ? 0 : 16), __fdividef(a - lo, hi - lo)) ? k1 : k;
+      if (SIGNED) c = copysignf(c, x[i]);
+      else if (x[i] > 0.0f) c = fmaxf(c, 1.0f);
+    } else if (SIGNED) c = copysignf(c < down ? fmaxf(c - 0.484375f, 0.0f) : c, x[i]);
     else if (x[i] > 0.0f) c = fmaxf(c, 1.0f);
     b[i] = __float_as_uint(c + 12582912.0f);
   }
@@ -287,14 +324,31 @@ __device__ __forceinline__ void decode8_e4m3(const uint8_t* q, float power, bool
     x[2 * i + 1] = f.y * power;
   }
 }
+// DITHER: the two values around y, q apart, are chosen between for m itself, or
+// (SIGNED false) for the square that sqrt(v) stands for.
+template <bool SIGNED, bool DITHER>
 __device__ __forceinline__ void encode8_e4m3(uint8_t* q, float power, bool vec, int left,
-                                             const float (&x)[8]) {
+                                             const float (&x)[8], const uint32_t (&bits)[8]) {
   const float inv = __fdiv_rn(1.0f, power);  // exact; 0 where power is infinite
   float y[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     y[i] = x[i] * inv;
-    if (y[i] != 0.0f && fabsf(y[i]) < 0.001953125f) y[i] = copysignf(0.001953125f, y[i]);
+    if constexpr (DITHER) {
+      const float a = fabsf(y[i]);
+      if (a < 256.0f) {  // else it is not finite
+        const uint32_t w = __float_as_uint(a);
+        const bool normal = a >= 0.015625f;  // 2^-6
+        const float step = normal ? __uint_as_float((w & 0x7f800000u) - (3u << 23)) : 0.001953125f;
+        const float lo = normal ? __uint_as_float(w & 0xfff00000u) : floorf(a * 512.0f) * 0.001953125f;
+        const float rest = a - lo;
+        const float p = SIGNED ? __fdividef(rest, step)
+                               : __fdividef(rest * (a + lo), step * (2.0f * lo + step));
+        float r = below(bits[i] >> (SIGNED ? 0 : 16), p) ? lo + step : lo;
+        if (!SIGNED && a > 0.0f) r = fmaxf(r, 0.001953125f);
+        y[i] = copysignf(r, y[i]);
+      }
+    } else if (y[i] != 0.0f && fabsf(y[i]) < 0.001953125f) y[i] = copysignf(0.001953125f, y[i]);
   }
   uint32_t w[2] = {0, 0};
 #pragma unroll
@@ -307,7 +361,7 @@ __device__ __forceinline__ void encode8_e4m3(uint8_t* q, float power, bool vec, 
 
 // The step of 256 values, a warp's; VEC: all of them are there, 16-byte
 // aligned (8-bit states 8-byte).
-template <Kind KIND, bool VEC>
+template <Kind KIND, bool DITHER, bool VEC>
 __device__ __forceinline__ void adamw_block(const Tensor& t, const Hyper& h, float clip,
                                             int64_t block) {
   const int lane = threadIdx.x & 31;
@@ -347,16 +401,23 @@ __device__ __forceinline__ void adamw_block(const Tensor& t, const Hyper& h, flo
     uint8_t* mq = static_cast<uint8_t*>(t.m) + at;
     uint8_t* vq = static_cast<uint8_t*>(t.v) + at;
     float sm, sv;
+    uint32_t bits[8] = {};
+    if constexpr (DITHER) {
+      const uint32_t key = scatter(h.step * 0x9e3779b9u + 1u);
+      const uint32_t place = (blockIdx.x * kWarps + (threadIdx.x >> 5)) * kQBlock + lane * 8;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) bits[i] = scatter((place + i) ^ key);
+    }
     if constexpr (KIND == kRoot) {
       sm = block_top<true>(m);
       sv = block_top<false>(root);
-      encode8<true>(mq, sm, h.down, VEC, left, m);
-      encode8<false>(vq, sv, 0.0f, VEC, left, root);
+      encode8<true, DITHER>(mq, sm, h.down, VEC, left, m, bits);
+      encode8<false, DITHER>(vq, sv, 0.0f, VEC, left, root, bits);
     } else {
       sm = block_power(m);
       sv = block_power(root);
-      encode8_e4m3(mq, sm, VEC, left, m);
-      encode8_e4m3(vq, sv, VEC, left, root);
+      encode8_e4m3<true, DITHER>(mq, sm, VEC, left, m, bits);
+      encode8_e4m3<false, DITHER>(vq, sv, VEC, left, root, bits);
     }
     __syncwarp();  // every lane has read the old scales
     if (lane == 0) {
@@ -369,7 +430,7 @@ __device__ __forceinline__ void adamw_block(const Tensor& t, const Hyper& h, flo
   }
 }
 
-template <int CAP, Kind KIND>
+template <int CAP, Kind KIND, bool DITHER>
 __global__ void __launch_bounds__(32 * kWarps) adamw_kernel(const __grid_constant__ Table<CAP> tb,
                                                             const Hyper hy) {
   const int ti = find_tensor(tb, blockIdx.x);
@@ -378,6 +439,7 @@ __global__ void __launch_bounds__(32 * kWarps) adamw_kernel(const __grid_constan
   if (h.scalars) {
     h.step_size = h.scalars[0];
     h.inv_root = h.scalars[1];
+    h.step = __float_as_uint(h.scalars[2]);
   }
   float clip = 1.0f;
   if (h.norm) {
@@ -389,8 +451,8 @@ __global__ void __launch_bounds__(32 * kWarps) adamw_kernel(const __grid_constan
   for (int k = 0; k < kPerWarp; ++k) {
     const int64_t block = first + k * kWarps;
     if (block * kQBlock >= t.n) return;  // the whole warp
-    if ((t.flags & kVec) && (block + 1) * kQBlock <= t.n) adamw_block<KIND, true>(t, h, clip, block);
-    else adamw_block<KIND, false>(t, h, clip, block);
+    if ((t.flags & kVec) && (block + 1) * kQBlock <= t.n) adamw_block<KIND, DITHER, true>(t, h, clip, block);
+    else adamw_block<KIND, DITHER, false>(t, h, clip, block);
   }
 }
 
@@ -503,6 +565,7 @@ __global__ void __launch_bounds__(256) adamw_prelude_kernel(const float* part, i
     *step = t;
     scalars[0] = static_cast<float>(lr / (1.0 - pow(b1, static_cast<double>(t))));
     scalars[1] = static_cast<float>(1.0 / sqrt(1.0 - pow(b2, static_cast<double>(t))));
+    scalars[2] = __uint_as_float(static_cast<uint32_t>(t));
   }
 }
 
@@ -560,9 +623,13 @@ cudaError_t launch_step(const mx_adamw_tensor* ts, int count, int bits, double l
   const int64_t chunks = tb.first[tb.count];
   if (chunks == 0) return cudaSuccess;
   const unsigned grid = static_cast<unsigned>(chunks);
-  if (bits & MX_ADAMW_E4M3) adamw_kernel<CAP, kE4m3><<<grid, 32 * kWarps, 0, s>>>(tb, h);
-  else if (bits & 8) adamw_kernel<CAP, kRoot><<<grid, 32 * kWarps, 0, s>>>(tb, h);
-  else adamw_kernel<CAP, kF32><<<grid, 32 * kWarps, 0, s>>>(tb, h);
+  auto kern = adamw_kernel<CAP, kF32, false>;
+  const bool dither = (bits & MX_ADAMW_DITHER) != 0;
+  if (bits & MX_ADAMW_E4M3)
+    kern = dither ? adamw_kernel<CAP, kE4m3, true> : adamw_kernel<CAP, kE4m3, false>;
+  else if (bits & 8)
+    kern = dither ? adamw_kernel<CAP, kRoot, true> : adamw_kernel<CAP, kRoot, false>;
+  kern<<<grid, 32 * kWarps, 0, s>>>(tb, h);
   note_launches(1);
   return cudaGetLastError();
 }
@@ -597,7 +664,7 @@ int adamw_check(const mx_adamw_tensor* ts, int count, int bits) {
 int adamw_step(const mx_adamw_tensor* ts, int count, int bits, double lr, double b1, double b2,
                double eps, int64_t step, int32_t* step_dev, double max_norm, float* norm_out,
                void* scratch, cudaStream_t s) {
-  float* sc = static_cast<float*>(scratch);  // [0] norm, [1..2] scalars, [4..] partial sums
+  float* sc = static_cast<float*>(scratch);  // [0] norm, [1..3] scalars, [4..] partial sums
   float* part = sc + 4;
   const bool clip = max_norm > 0.0;
   int parts = 0;
@@ -623,6 +690,7 @@ int adamw_step(const mx_adamw_tensor* ts, int count, int bits, double lr, double
   h.omb2 = static_cast<float>(1.0 - b2);
   h.eps = static_cast<float>(eps);
   h.down = static_cast<float>(0.5 / (1.0 - std::sqrt(b1)) + 1.0);
+  h.step = static_cast<uint32_t>(step);
   const double t = static_cast<double>(step);
   h.step_size = step_dev ? 0.0f : static_cast<float>(lr / (1.0 - std::pow(b1, t)));
   h.inv_root = step_dev ? 0.0f : static_cast<float>(1.0 / std::sqrt(1.0 - std::pow(b2, t)));

@@ -30,6 +30,8 @@ communicator), on a gloo group through torch.distributed.
 """
 from __future__ import annotations
 
+import warnings
+
 import numpy as np
 import torch
 
@@ -767,7 +769,11 @@ class AdamW:
     Gradients may be float32 or bfloat16, tensor by tensor.  state_bits = 32
     keeps both moments in float32, 8 in one byte each with a float32 scale for
     every 256 values: int8 and uint8 codes of their roots, or, where `state` has
-    them (zeros are a fresh state), float8_e4m3fn values.  copies: bfloat16 tensors (or None) that receive the new
+    them (zeros are a fresh state), float8_e4m3fn values.  rounding: how 8-bit
+    moments are: "nearest", which is for decay rates that change a moment by more
+    than half a code a step, or "dither", up or down by a number made from the
+    step and the value's place, so that they are right on the average; by default
+    nearest where betas are at most (0.9, 0.97).  copies: bfloat16 tensors (or None) that receive the new
     values, for layers that compute in bfloat16.  weight_decay: one number, or
     one for each tensor (0 for norms and biases).  max_grad_norm > 0 clips by
     the global norm, which `norm` then holds after a step.
@@ -780,12 +786,14 @@ class AdamW:
 
     def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
                  weight_decay=0.01, max_grad_norm: float = 0.0, state_bits: int = 32, copies=None,
-                 device_step: bool = False, state=None, step_count: int = 0, ctx=None):
+                 device_step: bool = False, state=None, step_count: int = 0, rounding=None, ctx=None):
         self.params = list(params)
         if not self.params:
             raise ValueError("AdamW needs at least one tensor")
         if state_bits not in (8, 32):
             raise ValueError(f"state_bits must be 8 or 32, got {state_bits}")
+        if rounding not in ((None, "nearest", "dither") if state_bits == 8 else (None,)):
+            raise ValueError(f"rounding must be 'nearest' or 'dither', for 8-bit states, got {rounding!r}")
         n = len(self.params)
         ops._check_type(self.params[0], "params[0]")
         self.device = self.params[0].device
@@ -805,6 +813,14 @@ class AdamW:
         self.ctx = ctx
         self.state = tuple(self._fresh_state() if state is None else (tuple(s) for s in state))
         self._check_state()
+        # Nearest codes of v above 66 of 255 (7 % of a block's largest root) still
+        # fall at 0.97, none at 0.999; m's codes above 10 of 127 at 0.9.
+        if rounding == "dither" or (rounding is None and state_bits == 8 and
+                                    (self.betas[0] > 0.9 or self.betas[1] > 0.97)):
+            self._kind |= _lib.ADAMW_DITHER
+        elif rounding is None and self._kind & _lib.ADAMW_E4M3 and self.betas[1] > (31 / 32) ** 2:
+            warnings.warn(f"second moments held as nearest float8 values never fall with beta2 = "
+                          f"{self.betas[1]}: pass rounding='dither' (or 'nearest')", stacklevel=2)
         self._steps = int(step_count)
         self.step_dev = torch.full((1,), self._steps, dtype=torch.int32, device=self.device) \
             if device_step else None
