@@ -401,7 +401,10 @@ __global__ void __launch_bounds__(block_threads(TPR, 2), blocks_per_sm(TPR, 2)) 
       for (int i = 0; i < NV; ++i) {
         const int c = (i * TPR + t) * V;
 #pragma unroll
-        for (int j = 0; j < V; ++j) xv[i][j] = g[i][j] = 0.0f;
+        for (int j = 0; j < V; ++j) {
+          xv[i][j] = mean;  // past the last column: xhat is zero
+          g[i][j] = 0.0f;
+        }
         if (c < p.cols) {
           if constexpr (V > 1) {
             load_vec<T, V>(reinterpret_cast<const T*>(ring + (slot * 2 * NV + i) * BLOCK + threadIdx.x), xv[i]);
@@ -420,13 +423,14 @@ __global__ void __launch_bounds__(block_threads(TPR, 2), blocks_per_sm(TPR, 2)) 
     }
     fetch(row + D * step, slot);
     slot = slot + 1 == D ? 0 : slot + 1;
-    // (x - mean) * rstd in one operation: the product's rounding is that of the
-    // saved mean once more
-    const Pair r2 = pair(rstd, rstd), shift = pair(-mean * rstd, -mean * rstd);
+    // (x - mean) * rstd, and not x * rstd - mean * rstd in one operation: that
+    // would round mean * rstd, which is all there is in a row without deviation,
+    // and overflow where this does not
+    const Pair r2 = pair(rstd, rstd), shift = pair(-mean, -mean);
     Pair s0 = pair(0.0f, 0.0f), s1 = s0;
 #pragma unroll
     for (int e = 0; e < E / 2; ++e) {
-      xh[e] = fma2(xh[e], r2, shift);
+      xh[e] = mul2(add2(xh[e], shift), r2);
       dw[e] = fma2(a[e], xh[e], dw[e]);
       db[e] = add2(db[e], a[e]);
       a[e] = mul2(a[e], w[e]);
