@@ -30,6 +30,7 @@ communicator), on a gloo group through torch.distributed.
 """
 from __future__ import annotations
 
+import contextlib
 import warnings
 
 import numpy as np
@@ -779,7 +780,8 @@ class AdamW:
     the global norm, which `norm` then holds after a step.
 
     device_step=True keeps the step number on the device, so that a captured
-    step counts its replays (reading `step_count` then waits for the device).
+    step counts its replays (reading `step_count` then waits for the device);
+    without it a step refuses to be captured.
     state, step_count: the moments and the number of steps of an earlier run
     (`state`, `step_count`), taken over as they are.
     """
@@ -885,6 +887,11 @@ class AdamW:
         """One update from `grads`, a tensor for each parameter."""
         if len(grads) != len(self.params):
             raise ValueError(f"{len(grads)} gradients for {len(self.params)} tensors")
+        with contextlib.nullcontext() if stream is None else torch.cuda.stream(stream):
+            capturing = torch.cuda.is_current_stream_capturing()
+        if capturing and self.step_dev is None:
+            raise RuntimeError("a step that is captured needs device_step=True: every replay "
+                               "would take the same step number")
         for i, (t, p, at, g) in enumerate(zip(self._table, self.params, self._at, grads)):
             kind = ops._check_type(g, f"grads[{i}]")
             if g.numel() != t.n or g.get_device() != self._dev or not g.is_contiguous():
@@ -894,7 +901,7 @@ class AdamW:
                 raise ValueError(f"params[{i}] was given other memory; make a new AdamW with "
                                  "`state` and `step_count`")
             t.grad, t.grad_type = g.data_ptr(), kind
-        if stream is not None and not torch.cuda.is_current_stream_capturing():
+        if stream is not None and not capturing:
             self._scratch.record_stream(stream)
             self.norm.record_stream(stream)
         rc = _lib.lib().mx_adamw_step(
