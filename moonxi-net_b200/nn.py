@@ -829,7 +829,7 @@ class AdamW:
         self.norm = torch.zeros(1, device=self.device)
         self._table = (_lib.AdamWTensor * n)()
         # The table holds addresses: of memory that these keep alive, and, for the
-        # parameters, that every step compares with where they are.
+        # parameters and copies, that every step compares with where they are.
         self._held = [x.detach() for x in self.params + [c for c in self.copies if c is not None]]
         self._held += [x.detach() for s in self.state for x in s]
         end = -1
@@ -839,6 +839,7 @@ class AdamW:
                 raise ValueError("params, copies and state must not share memory")
             end = b
         self._at = [p.data_ptr() for p in self.params]
+        self._copies_at = [(i, c, c.data_ptr()) for i, c in enumerate(self.copies) if c is not None]
         for t, p, c, s, d in zip(self._table, self.params, self.copies, self.state, decay):
             t.param, t.n, t.weight_decay = p.data_ptr(), p.numel(), d
             t.copy_bf16 = None if c is None else c.data_ptr()
@@ -901,6 +902,10 @@ class AdamW:
                 raise ValueError(f"params[{i}] was given other memory; make a new AdamW with "
                                  "`state` and `step_count`")
             t.grad, t.grad_type = g.data_ptr(), kind
+        for i, c, at in self._copies_at:
+            if c.data_ptr() != at:
+                raise ValueError(f"copies[{i}] was given other memory; make a new AdamW with "
+                                 "`state` and `step_count`")
         if stream is not None and not capturing:
             self._scratch.record_stream(stream)
             self.norm.record_stream(stream)

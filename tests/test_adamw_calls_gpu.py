@@ -30,3 +30,18 @@ def test_a_captured_step_needs_its_number_on_the_device(cuda_device):
     assert opt.step_count == 1
     opt.step([g])
     assert opt.step_count == 2
+
+
+def test_copies_that_moved_are_refused(cuda_device):
+    """A bfloat16 copy that was given other memory would go stale while the old
+    memory is written."""
+    p, g = torch.ones(300, device="cuda"), torch.ones(300, device="cuda")
+    c = torch.zeros(300, device="cuda", dtype=BF16)
+    old = c.detach()
+    opt = nn.AdamW([p, p.clone()], copies=[None, c])
+    opt.step([g, g])
+    before = old.clone(), p.clone()
+    c.data = torch.zeros(300, device="cuda", dtype=BF16)
+    with pytest.raises(ValueError, match="copies\\[1\\] was given other memory"):
+        opt.step([g, g])
+    assert torch.equal(old, before[0]) and torch.equal(p, before[1]) and opt.step_count == 1
