@@ -422,19 +422,35 @@ def _empty_like(t, stream):
 _MAX_SIZE = 0x7FFF0000  # of a dimension
 
 
+def _span(t: torch.Tensor) -> tuple[int, int, int, int]:
+    """(address, bytes of a row, bytes from a row to the next, rows) of a
+    contiguous tensor (one row) or a 2-D one with contiguous rows."""
+    size = t.element_size()
+    if t.is_contiguous():
+        return t.data_ptr(), t.numel() * size, t.numel() * size, 1
+    return t.data_ptr(), t.shape[1] * size, t.stride(0) * size, t.shape[0]
+
+
 def _apart(out: torch.Tensor, name: str, *others) -> None:
     """An output that the caller gives does not share memory with what the call
-    reads or writes beside it.  (Of tensors with gaps between their rows only
-    those that begin at the same place are known to.)"""
-    a = out.data_ptr()
-    end = a + out.numel() * out.element_size()
+    reads or writes beside it; rows may lie between another tensor's rows."""
+    if not out.numel():
+        return
+    a, la, pa, na = _span(out)
     for t in others:
-        if t is None:
+        if t is None or not t.numel():
             continue
-        b = t.data_ptr()
-        dense = out.is_contiguous() and t.is_contiguous()
-        if out.numel() and t.numel() and (
-                a == b or dense and a < b + t.numel() * t.element_size() and b < end):
+        b, lb, pb, nb = _span(t)
+        if b >= a + (na - 1) * pa + la or a >= b + (nb - 1) * pb + lb:
+            continue
+        if pa == pb and na > 1 and nb > 1:
+            clear = la <= (b - a) % pa <= pa - lb
+        else:  # row j of t ends behind a row of out's start and starts before its end
+            start = a - b + torch.arange(na) * pa
+            first = ((start - lb).div(pb, rounding_mode="floor") + 1).clamp(min=0)
+            last = -((-(start + la)).div(pb, rounding_mode="floor")) - 1
+            clear = not (first <= last.clamp(max=nb - 1)).any()
+        if not clear:
             raise ValueError(f"{name} must not share memory with another argument")
 
 
