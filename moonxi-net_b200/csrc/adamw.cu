@@ -46,7 +46,9 @@
 // Bound by the bytes: 28 B a value with float32 gradients and states, 16 B
 // with 8-bit states (14 B with bf16 gradients).  A warp takes 256 values,
 // 8 a lane in 16-byte accesses, so an 8-bit block is one warp's and its
-// maximum five shuffles.
+// maximum one warp reduction.  201 M values with bf16 gradients and copies, 16 B each,
+// a floor of 492 us: codes 544, e4m3 587; rounded by DITHER, whose numbers and
+// neighbours then bound the step, 684 and 792.
 #include <algorithm>
 #include <cmath>
 
@@ -127,8 +129,8 @@ __device__ __forceinline__ float fast_rcp(float x) {
 // The new m, v and p of one value; returns sqrt(v).  32-bit and e4m3 moments:
 // every operation rounded by itself, as the elementwise form of the step computes
 // it.  Root codes: fused, with the approximate root and quotient (2 units in
-// the last place), which the exact ones' instructions would bind: 0.82 ms
-// against 0.49 ms of bytes for 201 M values.
+// the last place, far below what the codes round away): 544 us for 201 M values
+// against 590 with exact ones, 492 of bytes.
 template <Kind KIND>
 __device__ __forceinline__ float adamw_one(float& p, float g, float& m, float& v, float keep,
                                            const Hyper& h) {
@@ -156,9 +158,9 @@ __device__ __forceinline__ uint32_t scatter(uint32_t x) {
   x = (x ^ (x >> 15)) * 0x9e3779b1u;
   return x ^ (x >> 16);
 }
-// Whether 16 of them are below the chance p.
-__device__ __forceinline__ bool below(uint32_t bits, float p) {
-  return static_cast<float>(bits & 0xffffu) + 0.5f < p * 65536.0f;
+// Whether 16 of them are below the chance part / whole.
+__device__ __forceinline__ bool below(uint32_t bits, float part, float whole) {
+  return (static_cast<float>(bits & 0xffffu) + 0.5f) * whole < part * 65536.0f;
 }
 
 // 8 values of a lane, those past `left` not touched.
@@ -286,7 +288,7 @@ __device__ __forceinline__ void encode8(uint8_t* q, float top, float down, bool 
       const float k = fminf(floorf(c), kMost - 1.0f);  // the largest is the last code
       const float a = SIGNED ? c * c : c * c * c * c, lo = SIGNED ? k * k : k * k * k * k;
       const float k1 = k + 1.0f, hi = SIGNED ? k1 * k1 : k1 * k1 * k1 * k1;
-      c = below(bits[i] >> (SIGNED ? 0 : 16), __fdividef(a - lo, hi - lo)) ? k1 : k;
+      c = below(bits[i] >> (SIGNED ? 0 : 16), a - lo, hi - lo) ? k1 : k;
       if (SIGNED) c = copysignf(c, x[i]);
       else if (x[i] > 0.0f) c = fmaxf(c, 1.0f);
     } else if (SIGNED) c = copysignf(c < down ? fmaxf(c - 0.484375f, 0.0f) : c, x[i]);
@@ -342,9 +344,9 @@ __device__ __forceinline__ void encode8_e4m3(uint8_t* q, float power, bool vec, 
         const float step = normal ? __uint_as_float((w & 0x7f800000u) - (3u << 23)) : 0.001953125f;
         const float lo = normal ? __uint_as_float(w & 0xfff00000u) : floorf(a * 512.0f) * 0.001953125f;
         const float rest = a - lo;
-        const float p = SIGNED ? __fdividef(rest, step)
-                               : __fdividef(rest * (a + lo), step * (2.0f * lo + step));
-        float r = below(bits[i] >> (SIGNED ? 0 : 16), p) ? lo + step : lo;
+        const bool up = SIGNED ? below(bits[i], rest, step)
+                               : below(bits[i] >> 16, rest * (a + lo), step * (2.0f * lo + step));
+        float r = up ? lo + step : lo;
         if (!SIGNED && a > 0.0f) r = fmaxf(r, 0.001953125f);
         y[i] = copysignf(r, y[i]);
       }
