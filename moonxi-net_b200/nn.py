@@ -30,7 +30,6 @@ communicator), on a gloo group through torch.distributed.
 """
 from __future__ import annotations
 
-import contextlib
 import warnings
 
 import numpy as np
@@ -888,13 +887,18 @@ class AdamW:
         """One update from `grads`, a tensor for each parameter."""
         if len(grads) != len(self.params):
             raise ValueError(f"{len(grads)} gradients for {len(self.params)} tensors")
-        with contextlib.nullcontext() if stream is None else torch.cuda.stream(stream):
+        if stream is None:
             capturing = torch.cuda.is_current_stream_capturing()
+        else:
+            with torch.cuda.stream(stream):
+                capturing = torch.cuda.is_current_stream_capturing()
         if capturing and self.step_dev is None:
             raise RuntimeError("a step that is captured needs device_step=True: every replay "
                                "would take the same step number")
         for i, (t, p, at, g) in enumerate(zip(self._table, self.params, self._at, grads)):
-            kind = ops._check_type(g, f"grads[{i}]")
+            kind = ops._DTYPES.get(g.dtype) if isinstance(g, torch.Tensor) and g.is_cuda else None
+            if kind is None:
+                ops._check_type(g, f"grads[{i}]")  # says what is wrong
             if g.numel() != t.n or g.get_device() != self._dev or not g.is_contiguous():
                 raise ValueError(f"grads[{i}] must be contiguous, of {t.n} elements on "
                                  f"{self.device}")
