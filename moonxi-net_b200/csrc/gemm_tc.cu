@@ -396,6 +396,7 @@ __device__ __forceinline__ float4 store_quad(const TcParams& p, int row, int col
 }
 
 __device__ __forceinline__ void epilogue_bar() {
+  __syncwarp();  // the barrier is an instruction of whole warps
   asm volatile("bar.sync 1, 128;" ::: "memory");  // the four epilogue warps
 }
 

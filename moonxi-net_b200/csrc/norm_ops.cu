@@ -117,8 +117,12 @@ __device__ __forceinline__ void row_sum(float (&s)[N], float* buf, int& turn, in
     if ((threadIdx.x & 31) == 0)
 #pragma unroll
       for (int i = 0; i < N; ++i) b[i * W + (threadIdx.x % TPR >> 5)] = s[i];
-    if (rows == 1) __syncthreads();
-    else asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "n"(TPR) : "memory");
+    if (rows == 1) {
+      __syncthreads();
+    } else {
+      __syncwarp();  // the barrier is an instruction of whole warps
+      asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "n"(TPR) : "memory");
+    }
 #pragma unroll
     for (int i = 0; i < N; ++i) s[i] = b[i * W + (threadIdx.x & (W - 1))];
 #pragma unroll

@@ -14,6 +14,17 @@ def _sources():
             yield os.path.basename(path), f.read().splitlines()
 
 
+def test_lanes_meet_before_a_named_barrier():
+    """bar.sync is barrier.sync.aligned: one instruction of all 32 lanes, too."""
+    checked = 0
+    for name, lines in _sources():
+        for i, line in enumerate(lines):
+            if '"bar.sync' in line.split("//")[0]:
+                checked += 1
+                assert any("__syncwarp()" in x for x in lines[max(0, i - 4):i]), (name, i + 1)
+    assert checked >= 2
+
+
 def test_lanes_meet_before_a_warps_collective_instructions():
     """A TMEM load and a cluster barrier (.aligned) are one instruction of all 32
     lanes.  Their lanes part in the loops and branches before them (rows past the
