@@ -439,8 +439,8 @@ uint64_t mx_layer_norm_bwd_scratch_bytes(void* handle, int32_t rows, int32_t col
  * so that its rows are aligned.  float32 products are float32-class (relative
  * error below 1e-6 of the terms' size), on tensor cores where the shape is
  * large; MX_PREC_FP32 on the context or here keeps them on the exact SIMT
- * kernels.  An infinite x or w gives NaN where it meets a float32 tensor-core
- * product.  workspace: mx_gated_linear_workspace_bytes(...) bytes, 256-byte
+ * kernels.  An infinite x or w, or one above 3.39e38, gives NaN where it meets a
+ * float32 tensor-core product.  workspace: mx_gated_linear_workspace_bytes(...) bytes, 256-byte
  * aligned, not shared with an overlapping call. */
 int32_t mx_gated_linear_fwd(void* handle, int32_t dtype, const void* x, const void* w,
                             const void* bias, void* h, float* pre, int32_t M, int32_t K,
@@ -457,7 +457,8 @@ int32_t mx_gated_linear_bwd(void* handle, int32_t dtype, const void* dh, const f
                             int32_t M, int32_t K, int32_t F, int32_t transpose_w, int32_t act,
                             int32_t precision, void* workspace, uint64_t workspace_bytes,
                             void* stream);
-/* Workspace of the forward (backward = 0) or backward (1) call of a shape. */
+/* Workspace of the forward (backward = 0) or backward (1) call of a shape, with
+ * room for tensors that start on any element. */
 uint64_t mx_gated_linear_workspace_bytes(void* handle, int32_t dtype, int32_t M, int32_t K,
                                          int32_t F, int32_t transpose_w, int32_t precision,
                                          int32_t backward);

@@ -787,7 +787,7 @@ class AdamW:
 
     def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
                  weight_decay=0.01, max_grad_norm: float = 0.0, state_bits: int = 32, copies=None,
-                 device_step: bool = False, state=None, step_count: int = 0, rounding=None, ctx=None):
+                 device_step: bool = False, state=None, step_count: int = 0, ctx=None, rounding=None):
         self.params = list(params)
         if not self.params:
             raise ValueError("AdamW needs at least one tensor")

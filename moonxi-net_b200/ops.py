@@ -445,11 +445,12 @@ def _apart(out: torch.Tensor, name: str, *others) -> None:
             continue
         if pa == pb and na > 1 and nb > 1:
             clear = la <= (b - a) % pa <= pa - lb
-        else:  # row j of t ends behind a row of out's start and starts before its end
-            start = a - b + torch.arange(na) * pa
-            first = ((start - lb).div(pb, rounding_mode="floor") + 1).clamp(min=0)
-            last = -((-(start + la)).div(pb, rounding_mode="floor")) - 1
-            clear = not (first <= last.clamp(max=nb - 1)).any()
+        else:  # row j ends behind another's row's start and starts before its end
+            few, many = sorted(((a, la, pa, na), (b, lb, pb, nb)), key=lambda r: r[3])
+            start = few[0] - many[0] + torch.arange(few[3]) * few[2]
+            first = ((start - many[1]).div(many[2], rounding_mode="floor") + 1).clamp(min=0)
+            last = -((-(start + few[1])).div(many[2], rounding_mode="floor")) - 1
+            clear = not (first <= last.clamp(max=many[3] - 1)).any()
         if not clear:
             raise ValueError(f"{name} must not share memory with another argument")
 

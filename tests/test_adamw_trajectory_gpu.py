@@ -156,3 +156,37 @@ def test_rounding_is_an_argument(cuda_device):
         nn.AdamW([g], rounding="dither")
     with pytest.warns(UserWarning, match="never fall"):
         nn.AdamW([g], state_bits=8, betas=(0.9, 0.95), state=_state("float8", 2560))
+
+
+@pytest.mark.parametrize("kind", ["codes", "float8"])
+def test_zero_and_not_finite_values(cuda_device, kind):
+    """Rounded up or down, zero stays zero, in blocks of zeros and in others; what
+    is not finite reaches its block and no further."""
+    n = 256 * 5
+    g = torch.zeros(n, device="cuda")
+    g[256:512:2] = torch.randn(128, device="cuda", generator=torch.Generator("cuda").manual_seed(1))
+    g[512:768] = 2.0 ** -100
+    p = torch.zeros(n, device="cuda")
+    opt = nn.AdamW([p], state_bits=8, state=_state(kind, n), weight_decay=0.0)
+    for _ in range(5):
+        opt.step([g])
+    m, v = _decode(opt.state[0])
+    zero = g == 0
+    assert (m[zero] == 0).all() and (v[zero] == 0).all() and (p[zero] == 0).all()
+    assert (m[256:512:2] != 0).all() and (v[256:512:2] > 0).all()
+    before = [x.clone() for x in opt.state[0]]
+    for bad in (math.inf, -math.inf, math.nan):
+        state = [tuple(x.clone() for x in before)]
+        other = nn.AdamW([p.clone()], state_bits=8, state=state, step_count=5, weight_decay=0.0)
+        good = nn.AdamW([p.clone()], state_bits=8, state=[tuple(x.clone() for x in before)], step_count=5,
+                        weight_decay=0.0)
+        g2 = g.clone()
+        g2[300] = bad
+        other.step([g2])
+        good.step([g])
+        keep = torch.arange(n, device="cuda") // 256 != 1
+        (ma, va), (mb, vb) = _decode(other.state[0]), _decode(good.state[0])
+        assert torch.equal(ma[keep], mb[keep]) and torch.equal(va[keep], vb[keep])
+        ok = torch.arange(n, device="cuda") != 300
+        assert torch.equal(other.params[0][ok], good.params[0][ok]) and other.params[0][300].isnan()
+        assert not ma[300].isfinite() and not va[300].isfinite()
